@@ -551,6 +551,155 @@ LLMR_API int llmr_flash_attention_pc(llmr_context* ctx, const void* q, const voi
                                      const llmr_flash_attention_params* pc);
 
 /* ---------------------------------------------------------------------------
+ * Batches of requests of the text path (the text encoder and text model beside
+ * the DiT): the requests' tokens lie one request after the other in packed
+ * rows, row t of request s for seq_offsets[s] <= t < seq_offsets[s + 1], and
+ * keys and values are either the same rows (a prompt of its own) or the pages
+ * of a cache. A step is llmr_paged_plan, the QKV projection, llmr_qkv_tokens,
+ * attention, the output projection.
+ *
+ * Lengths, offsets, tables and slots are int32 arrays in device memory: nothing
+ * here reads them on the host, so a captured step replays with other lengths.
+ * What the host cannot check the kernels keep in bounds: offsets are taken
+ * within [0, n_tokens], a page outside [0, n_pages) or past the table's columns
+ * is a page of keys nobody sees, a slot outside the cache stores nothing. Rows
+ * that belong to no request (a batch padded to a captured size) are left as they
+ * are. None of these calls allocates.
+ * ------------------------------------------------------------------------- */
+
+/* Most requests of one llmr_paged_plan or llmr_paged_attention call. */
+#define LLMR_MAX_SEQS 4096u
+
+typedef struct llmr_prompt_attention_params {
+    uint32_t head_dim;       /* 64 or 128 */
+    uint32_t n_heads;        /* query heads, a multiple of n_kv_heads */
+    uint32_t n_kv_heads;     /* query head h reads key/value head h / (n_heads / n_kv_heads) */
+    uint32_t n_tokens;       /* rows of q, k, v and out */
+    uint32_t n_seqs;
+    uint32_t q_stride;       /* elements from one token to the next, and from one */
+    uint32_t q_head_stride;  /* head to the next: multiples of 8, so that rows */
+    uint32_t kv_stride;      /* [n_tokens, heads, head_dim], columns of a wider */
+    uint32_t kv_head_stride; /* row and [heads, n_tokens, head_dim] are all taken */
+    uint32_t out_stride;     /* elements from one row of out to the next, a multiple of 8 */
+    float scale;             /* softmax scale, 1/sqrt(head_dim) */
+} llmr_prompt_attention_params;
+
+/* Causal attention of packed prompts, grouped heads:
+ *   out[t, h*D + d] = sum_j softmax_j(scale * <q[t, h], k[j, h / G]>) * v[j, h / G][d]
+ * over j = the first row of t's request .. t, G = n_heads / n_kv_heads. q, k, v
+ * and out of type F16 or BF16, 16-byte aligned; seq_offsets [n_seqs + 1],
+ * nondecreasing (a request may have no rows). Scores, the running maximum and
+ * sum and the accumulated rows are f32; the softmax weights are rounded to
+ * `type` for the products with v, and the sums that divide are of the rounded
+ * weights. A key or value row changes no row of out that does not see it,
+ * whatever it holds (infinities and NaN too). Of the reference's
+ * attention_prefill (dependencies/llm_text.c3l/shaders/llm.slang), for a whole
+ * batch of prompts in one launch. */
+LLMR_API int llmr_prompt_attention(llmr_context* ctx, const void* q, const void* k, const void* v, uint32_t type,
+                                   void* out, const int32_t* seq_offsets, const llmr_prompt_attention_params* params);
+
+typedef struct llmr_paged_plan_params {
+    uint32_t n_seqs;    /* <= LLMR_MAX_SEQS */
+    uint32_t n_tokens;  /* rows of slots and positions: at least the new tokens' sum */
+    uint32_t page_size; /* tokens of a page: 16, 32, 64, 128 or 256 */
+    uint32_t max_pages; /* columns of block_table */
+    uint32_t n_free;    /* entries free_pages has room for */
+} llmr_paged_plan_params;
+
+/* Pages and slots of one step, from the requests' lengths. Request s holds
+ * past_len[s] cached tokens and gets new_len[s] more (negative lengths count as
+ * 0; their sums stay under 2^31):
+ *   seq_offsets[s]  = sum of new_len[0 .. s-1]             (n_seqs + 1 entries)
+ *   kv_len[s]       = past_len[s] + new_len[s]
+ *   block_table     [n_seqs, max_pages]: the pages past_len[s] fills are there
+ *                   already; the ones it needs more are taken from the end of
+ *                   free_pages[0 .. *free_count), in the requests' order, and
+ *                   written behind them. No other entry is touched.
+ *   positions[t]    = t's position in its request, slots[t] = page * page_size
+ *                   + position % page_size, for the new tokens t in packed order
+ *                   (0 and -1 for the rows behind them)
+ *   pages[0]        = pages left in free_pages, pages[1] = pages that were lacking
+ * A page that is lacking, or past max_pages, is entered (where the table has room)
+ * as -1, and its tokens get slot -1: llmr_qkv_tokens stores nothing there. To give
+ * pages back, write them at free_pages[pages[0] ..] and raise the count. An
+ * output array may not overlap another array. */
+LLMR_API int llmr_paged_plan(llmr_context* ctx, const int32_t* past_len, const int32_t* new_len,
+                             const int32_t* free_pages, const int32_t* free_count, int32_t* block_table,
+                             int32_t* seq_offsets, int32_t* kv_len, int32_t* slots, int32_t* positions,
+                             int32_t* pages, const llmr_paged_plan_params* params);
+
+typedef struct llmr_qkv_tokens_params {
+    uint32_t head_dim;    /* 64 or 128 */
+    uint32_t n_heads;
+    uint32_t n_kv_heads;  /* n_heads % n_kv_heads == 0 */
+    uint32_t n_tokens;
+    uint32_t qkv_stride;  /* elements from one f32 row to the next, a multiple of 4 */
+    uint32_t q_stride;    /* elements from one token of q to the next, a multiple of 8 */
+    uint32_t out_type;    /* F16 or BF16: q, k and v */
+    uint32_t kv_stride;   /* without slots: elements from one token of k and v to the next */
+    uint32_t page_size;   /* with slots: 16, 32, 64, 128 or 256 */
+    uint32_t n_pages;     /* with slots: pages of the cache */
+    uint32_t n_positions; /* rows of the rotation tables */
+    uint32_t rope_halves; /* pairs of a rotation: 0 (2j, 2j + 1), 1 (j, j + head_dim / 2) */
+    float eps;
+} llmr_qkv_tokens_params;
+
+/* Rows of a QKV projection with grouped heads -> query rows, and key and value
+ * rows at their place. qkv f32: row r holds Q (n_heads * D) | K (n_kv_heads * D) |
+ * V (n_kv_heads * D). Per head of Q and K: x *= (1 / sqrt(sum x^2 / D + eps)) *
+ * norm (q_norm, k_norm [D], each may be NULL), then the pair (x0, x1) of column j
+ * of the tables [n_positions, D / 2] -> (x0 c - x1 s, x0 s + x1 c) at row
+ * positions[r] (NULL: r; taken within the tables). rope_cos and rope_sin NULL: no
+ * rotation. q [n_tokens, n_heads, D] at row stride q_stride. With slots, k and v
+ * are caches [n_pages, n_kv_heads, page_size, D] and row r goes to token slots[r] %
+ * page_size of page slots[r] / page_size, nowhere where the slot is outside the
+ * cache (-1); the slots of a call are distinct. Without, they are rows [n_tokens,
+ * n_kv_heads, D] at stride kv_stride, as llmr_prompt_attention reads them. f32
+ * arithmetic in llmr_qkv_heads' order, rounded once to out_type. */
+LLMR_API int llmr_qkv_tokens(llmr_context* ctx, const float* qkv, const float* q_norm, const float* k_norm,
+                             const float* rope_cos, const float* rope_sin, const int32_t* positions,
+                             const int32_t* slots, void* q, void* k, void* v, const llmr_qkv_tokens_params* params);
+
+typedef struct llmr_paged_attention_params {
+    uint32_t head_dim;   /* 64 or 128 */
+    uint32_t n_heads;    /* query heads, a multiple of n_kv_heads */
+    uint32_t n_kv_heads;
+    uint32_t n_tokens;   /* rows of q and out */
+    uint32_t n_seqs;     /* <= LLMR_MAX_SEQS */
+    uint32_t max_new;    /* no request has more new tokens than this (1: single tokens);
+                            rows of a request past it are not computed */
+    uint32_t page_size;  /* 16, 32, 64, 128 or 256 */
+    uint32_t n_pages;    /* pages of the caches */
+    uint32_t max_pages;  /* columns of block_table */
+    uint32_t q_stride;   /* elements from one token of q to the next, a multiple of 8 */
+    uint32_t out_stride; /* elements from one row of out to the next, a multiple of 8 */
+    float scale;
+} llmr_paged_attention_params;
+
+/* Attention of the requests' new tokens over a paged cache, causal, grouped heads.
+ * Request s has n = seq_offsets[s + 1] - seq_offsets[s] new tokens, the last n of
+ * its kv_len[s] cached ones (llmr_qkv_tokens has stored them): its i-th new token
+ * sees the keys j <= kv_len[s] - n + i, key j being token j % page_size of page
+ * block_table[s, j / page_size] in k_cache and v_cache [n_pages, n_kv_heads,
+ * page_size, D]. Keys on a page outside the cache are seen by nobody; a row that
+ * sees no key is 0. q [n_tokens, n_heads, D], out [n_tokens, n_heads * D], caches
+ * of type F16 or BF16, 16-byte aligned. Arithmetic as llmr_prompt_attention's.
+ * scratch: device memory of at least llmr_paged_attention_scratch_bytes, 16-byte
+ * aligned, the caller's: two calls that may overlap, captured ones too, take one
+ * each. It holds nothing between calls. Of the reference's attention_split and
+ * attention_combine (dependencies/llm_text.c3l/shaders/llm.slang), for a batch and
+ * over pages. */
+LLMR_API int llmr_paged_attention(llmr_context* ctx, const void* q, const void* k_cache, const void* v_cache,
+                                  uint32_t type, void* out, const int32_t* seq_offsets, const int32_t* kv_len,
+                                  const int32_t* block_table, void* scratch, size_t scratch_bytes,
+                                  const llmr_paged_attention_params* params);
+
+/* Bytes of the scratch of an llmr_paged_attention call on this context's device with
+ * these params (0 where the call needs none or would refuse them). Lengths do not
+ * matter: it holds for every replay of a captured call. */
+LLMR_API size_t llmr_paged_attention_scratch_bytes(llmr_context* ctx, const llmr_paged_attention_params* params);
+
+/* ---------------------------------------------------------------------------
  * Block glue: the row reductions and elementwise ops the DiT blocks run
  * between the GEMMs and attention. Each replaces a chain of the reference's
  * dispatches over one tensor with one pass, and writes its result directly in

@@ -1013,3 +1013,240 @@ int llmr_synth_q4k(llmr_context* ctx, void* out, uint64_t n_rows, uint32_t in_di
 }
 
 }  // extern "C"
+
+// --- batches of requests --------------------------------------------------------
+
+namespace {
+
+bool is_16bit(uint32_t t) { return t == LLMR_GGML_F16 || t == LLMR_GGML_BF16; }
+
+int check_heads(uint32_t head_dim, uint32_t n_heads, uint32_t n_kv_heads) {
+    if (head_dim != 64 && head_dim != 128)
+        return fail(LLMR_ERR_INVALID_ARG, "head_dim must be 64 or 128 (got %u)", head_dim);
+    if (n_heads == 0 || n_heads > 1024 || n_kv_heads == 0 || n_heads % n_kv_heads)
+        return fail(LLMR_ERR_INVALID_ARG, "n_heads must be in [1, 1024] and a multiple of n_kv_heads (got %u, %u)",
+                    n_heads, n_kv_heads);
+    return LLMR_OK;
+}
+
+int check_16(const void* p, const char* what) {
+    if (!p) return fail(LLMR_ERR_INVALID_ARG, "null %s pointer", what);
+    if (!aligned(p, 16)) return fail(LLMR_ERR_INVALID_ARG, "%s pointer must be 16-byte aligned", what);
+    return LLMR_OK;
+}
+
+int check_ints(const void* p, const char* what) {
+    if (!p) return fail(LLMR_ERR_INVALID_ARG, "null %s pointer", what);
+    if (!aligned(p, 4)) return fail(LLMR_ERR_INVALID_ARG, "%s pointer must be 4-byte aligned", what);
+    return LLMR_OK;
+}
+
+// Rows of 16-bit elements read or written in 16-byte vectors.
+int check_stride8(uint32_t stride, uint64_t width, const char* what) {
+    if (stride % 8 || stride < width)
+        return fail(LLMR_ERR_INVALID_ARG, "%s must be a multiple of 8 and >= %llu (got %u)", what,
+                    (unsigned long long)width, stride);
+    return LLMR_OK;
+}
+
+int check_scale(float scale) {
+    if (!(scale > 0.0f) || !std::isfinite(scale * 1.4426950408889634f))
+        return fail(LLMR_ERR_INVALID_ARG, "scale must be positive and finite");
+    return LLMR_OK;
+}
+
+// 4 .. 8 for pages of 16 .. 256 tokens; 0 after an error.
+uint32_t page_log2(uint32_t page_size) {
+    for (uint32_t b = 4; b <= 8; b++)
+        if (page_size == 1u << b) return b;
+    fail(LLMR_ERR_INVALID_ARG, "page_size must be 16, 32, 64, 128 or 256 (got %u)", page_size);
+    return 0;
+}
+
+int check_seqs(uint32_t n_seqs, uint32_t n_tokens) {
+    if (n_seqs > LLMR_MAX_SEQS)
+        return fail(LLMR_ERR_INVALID_ARG, "n_seqs must be <= %u (got %u)", LLMR_MAX_SEQS, n_seqs);
+    if (n_tokens > 0x7fffffffu) return fail(LLMR_ERR_INVALID_ARG, "n_tokens too large (%u)", n_tokens);
+    return LLMR_OK;
+}
+
+bool overlap(const void* a, uint64_t an, const void* b, uint64_t bn) {
+    return an && bn && (uintptr_t)a < (uintptr_t)b + bn && (uintptr_t)b < (uintptr_t)a + an;
+}
+
+int check_paged_attention(const llmr_paged_attention_params* p) {
+    if (!p) return fail(LLMR_ERR_INVALID_ARG, "null params");
+    if (int r = check_heads(p->head_dim, p->n_heads, p->n_kv_heads)) return r;
+    if (int r = check_seqs(p->n_seqs, p->n_tokens)) return r;
+    if (!page_log2(p->page_size)) return LLMR_ERR_INVALID_ARG;
+    if ((uint64_t)p->max_pages * p->page_size > 0x7fffffffull || (uint64_t)p->n_pages * p->page_size > 0x7fffffffull)
+        return fail(LLMR_ERR_INVALID_ARG, "max_pages and n_pages times page_size must be < 2^31");
+    if (int r = check_scale(p->scale)) return r;
+    return LLMR_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int llmr_prompt_attention(llmr_context* ctx, const void* q, const void* k, const void* v, uint32_t type, void* out,
+                          const int32_t* seq_offsets, const llmr_prompt_attention_params* p) {
+    if (int r = check_ctx(ctx)) return r;
+    if (!p) return fail(LLMR_ERR_INVALID_ARG, "null params");
+    if (!is_16bit(type)) return fail(LLMR_ERR_UNSUPPORTED, "type %u not supported (F16=1, BF16=30)", type);
+    if (int r = check_heads(p->head_dim, p->n_heads, p->n_kv_heads)) return r;
+    if (p->n_tokens > 0x7fffffffu) return fail(LLMR_ERR_INVALID_ARG, "n_tokens too large (%u)", p->n_tokens);
+    if (int r = check_scale(p->scale)) return r;
+    if (p->n_tokens == 0 || p->n_seqs == 0) return ok();
+    if (int r = check_16(q, "q")) return r;
+    if (int r = check_16(k, "k")) return r;
+    if (int r = check_16(v, "v")) return r;
+    if (int r = check_16(out, "out")) return r;
+    if (int r = check_ints(seq_offsets, "seq_offsets")) return r;
+    if (int r = check_stride8(p->q_stride, p->head_dim, "q_stride")) return r;
+    if (int r = check_stride8(p->q_head_stride, p->head_dim, "q_head_stride")) return r;
+    if (int r = check_stride8(p->kv_stride, p->head_dim, "kv_stride")) return r;
+    if (int r = check_stride8(p->kv_head_stride, p->head_dim, "kv_head_stride")) return r;
+    if (int r = check_stride8(p->out_stride, (uint64_t)p->n_heads * p->head_dim, "out_stride")) return r;
+    if ((uint64_t)p->n_tokens * p->n_heads > 0x7fffffffull)
+        return fail(LLMR_ERR_INVALID_ARG, "n_tokens * n_heads must be < 2^31");
+    llmr::SeqAttnArgs a{};
+    a.q = q, a.k = k, a.v = v, a.out = out, a.offsets = seq_offsets;
+    a.n_heads = p->n_heads, a.n_kv_heads = p->n_kv_heads, a.n_tokens = p->n_tokens, a.n_seqs = p->n_seqs;
+    a.q_stride = p->q_stride, a.q_head_stride = p->q_head_stride;
+    a.kv_stride = p->kv_stride, a.kv_head_stride = p->kv_head_stride, a.out_stride = p->out_stride;
+    a.scale_log2 = p->scale * 1.4426950408889634f;
+    return launched(llmr::launch_prompt_attention(a, type, p->head_dim, ctx->cur), "prompt_attention");
+}
+
+int llmr_paged_plan(llmr_context* ctx, const int32_t* past_len, const int32_t* new_len, const int32_t* free_pages,
+                    const int32_t* free_count, int32_t* block_table, int32_t* seq_offsets, int32_t* kv_len,
+                    int32_t* slots, int32_t* positions, int32_t* pages, const llmr_paged_plan_params* p) {
+    if (int r = check_ctx(ctx)) return r;
+    if (!p) return fail(LLMR_ERR_INVALID_ARG, "null params");
+    if (int r = check_seqs(p->n_seqs, p->n_tokens)) return r;
+    const uint32_t log2 = page_log2(p->page_size);
+    if (!log2) return LLMR_ERR_INVALID_ARG;
+    if ((uint64_t)p->max_pages * p->page_size > 0x7fffffffull || p->n_free > 0x7fffffffu ||
+        (uint64_t)p->n_seqs * p->max_pages > 0x7fffffffull)
+        return fail(LLMR_ERR_INVALID_ARG, "max_pages * page_size, n_seqs * max_pages and n_free must be < 2^31");
+    struct {
+        const void* p;
+        uint64_t n;
+        const char* what;
+    } arr[] = {{past_len, p->n_seqs, "past_len"}, {new_len, p->n_seqs, "new_len"},
+               {free_pages, p->n_free, "free_pages"}, {free_count, 1, "free_count"},
+               {block_table, (uint64_t)p->n_seqs * p->max_pages, "block_table"}, {seq_offsets, p->n_seqs + 1ull, "seq_offsets"},
+               {kv_len, p->n_seqs, "kv_len"}, {slots, p->n_tokens, "slots"}, {positions, p->n_tokens, "positions"},
+               {pages, 2, "pages"}};
+    constexpr int kIn = 4, kAll = 10;  // the inputs come first
+    for (auto& x : arr)
+        if (x.n)
+            if (int r = check_ints(x.p, x.what)) return r;
+    for (int i = kIn; i < kAll; i++)
+        for (int j = 0; j < i; j++)
+            if (overlap(arr[i].p, 4 * arr[i].n, arr[j].p, 4 * arr[j].n))
+                return fail(LLMR_ERR_INVALID_ARG, "%s overlaps %s", arr[i].what, arr[j].what);
+    llmr::PagedPlanArgs a{past_len, new_len, free_pages, free_count, block_table, seq_offsets, kv_len, slots,
+                          positions, pages, p->n_seqs, p->n_tokens, log2, p->max_pages, p->n_free};
+    return launched(llmr::launch_paged_plan(a, ctx->cur), "paged_plan");
+}
+
+int llmr_qkv_tokens(llmr_context* ctx, const float* qkv, const float* q_norm, const float* k_norm,
+                    const float* rope_cos, const float* rope_sin, const int32_t* positions, const int32_t* slots,
+                    void* q, void* k, void* v, const llmr_qkv_tokens_params* p) {
+    if (int r = check_ctx(ctx)) return r;
+    if (!p) return fail(LLMR_ERR_INVALID_ARG, "null params");
+    if (!is_16bit(p->out_type))
+        return fail(LLMR_ERR_UNSUPPORTED, "output type %u not supported (F16=1, BF16=30)", p->out_type);
+    if (int r = check_heads(p->head_dim, p->n_heads, p->n_kv_heads)) return r;
+    if (!(p->eps >= 0.0f) || !std::isfinite(p->eps)) return fail(LLMR_ERR_INVALID_ARG, "eps must be finite and >= 0");
+    if (p->n_tokens > 0x7fffffffu) return fail(LLMR_ERR_INVALID_ARG, "n_tokens too large (%u)", p->n_tokens);
+    if (p->rope_halves > 1) return fail(LLMR_ERR_INVALID_ARG, "rope_halves must be 0 or 1");
+    if ((rope_cos == nullptr) != (rope_sin == nullptr))
+        return fail(LLMR_ERR_INVALID_ARG, "rope_cos and rope_sin must both be given or both be null");
+    if (p->n_tokens == 0) return ok();
+    const uint64_t D = p->head_dim, width = (p->n_heads + 2ull * p->n_kv_heads) * D;
+    if (int r = check_16(qkv, "qkv")) return r;
+    if (p->qkv_stride % 4 || p->qkv_stride < width)
+        return fail(LLMR_ERR_INVALID_ARG, "qkv_stride must be a multiple of 4 and >= %llu (got %u)",
+                    (unsigned long long)width, p->qkv_stride);
+    if (int r = check_vec(q_norm, "q_norm", false)) return r;
+    if (int r = check_vec(k_norm, "k_norm", false)) return r;
+    if (int r = check_vec(rope_cos, "rope_cos", false)) return r;
+    if (int r = check_vec(rope_sin, "rope_sin", false)) return r;
+    if (int r = check_16(q, "q")) return r;
+    if (int r = check_16(k, "k")) return r;
+    if (int r = check_16(v, "v")) return r;
+    if (int r = check_stride8(p->q_stride, p->n_heads * D, "q_stride")) return r;
+    if (rope_cos) {
+        if (p->n_positions == 0 || p->n_positions > 0x7fffffffu)
+            return fail(LLMR_ERR_INVALID_ARG, "n_positions must be in [1, 2^31)");
+        if (!positions && p->n_tokens > p->n_positions)
+            return fail(LLMR_ERR_INVALID_ARG, "n_tokens %u > n_positions %u without positions", p->n_tokens,
+                        p->n_positions);
+        if (positions)
+            if (int r = check_ints(positions, "positions")) return r;
+    }
+    uint32_t log2 = 0;
+    if (slots) {
+        if (int r = check_ints(slots, "slots")) return r;
+        if (!(log2 = page_log2(p->page_size))) return LLMR_ERR_INVALID_ARG;
+        if ((uint64_t)p->n_pages * p->page_size > 0x7fffffffull)
+            return fail(LLMR_ERR_INVALID_ARG, "n_pages * page_size must be < 2^31");
+    } else if (int r = check_stride8(p->kv_stride, p->n_kv_heads * D, "kv_stride")) {
+        return r;
+    }
+    llmr::QkvTokensArgs a{qkv, q_norm, k_norm, rope_cos, rope_sin, rope_cos ? positions : nullptr, slots, q, k, v,
+                          p->n_heads, p->n_kv_heads, p->n_tokens, p->qkv_stride, p->q_stride, p->kv_stride, log2,
+                          p->n_pages, p->n_positions, p->eps};
+    return launched(llmr::launch_qkv_tokens(a, p->head_dim, p->out_type, p->rope_halves != 0, ctx->cur), "qkv_tokens");
+}
+
+size_t llmr_paged_attention_scratch_bytes(llmr_context* ctx, const llmr_paged_attention_params* p) {
+    if (check_ctx(ctx) || check_paged_attention(p)) return 0;
+    if (p->n_tokens == 0 || p->n_seqs == 0 || p->max_new == 0) return 0;
+    return llmr::paged_attention_scratch_bytes(p->head_dim, p->n_heads, p->n_kv_heads, p->n_tokens, p->n_seqs,
+                                               p->max_new, ctx->num_cus);
+}
+
+int llmr_paged_attention(llmr_context* ctx, const void* q, const void* k_cache, const void* v_cache, uint32_t type,
+                         void* out, const int32_t* seq_offsets, const int32_t* kv_len, const int32_t* block_table,
+                         void* scratch, size_t scratch_bytes, const llmr_paged_attention_params* p) {
+    if (int r = check_ctx(ctx)) return r;
+    if (int r = check_paged_attention(p)) return r;
+    if (!is_16bit(type)) return fail(LLMR_ERR_UNSUPPORTED, "type %u not supported (F16=1, BF16=30)", type);
+    if (p->n_tokens == 0 || p->n_seqs == 0 || p->max_new == 0) return ok();
+    if (int r = check_16(q, "q")) return r;
+    if (int r = check_16(out, "out")) return r;
+    if (p->n_pages) {
+        if (int r = check_16(k_cache, "k_cache")) return r;
+        if (int r = check_16(v_cache, "v_cache")) return r;
+    }
+    if (int r = check_ints(seq_offsets, "seq_offsets")) return r;
+    if (int r = check_ints(kv_len, "kv_len")) return r;
+    if (p->max_pages)
+        if (int r = check_ints(block_table, "block_table")) return r;
+    if (int r = check_stride8(p->q_stride, (uint64_t)p->n_heads * p->head_dim, "q_stride")) return r;
+    if (int r = check_stride8(p->out_stride, (uint64_t)p->n_heads * p->head_dim, "out_stride")) return r;
+    if ((uint64_t)p->n_tokens * p->n_heads > 0x7fffffffull)
+        return fail(LLMR_ERR_INVALID_ARG, "n_tokens * n_heads must be < 2^31");
+    const size_t need = llmr::paged_attention_scratch_bytes(p->head_dim, p->n_heads, p->n_kv_heads, p->n_tokens,
+                                                            p->n_seqs, p->max_new, ctx->num_cus);
+    if (need) {
+        if (int r = check_16(scratch, "scratch")) return r;
+        if (scratch_bytes < need)
+            return fail(LLMR_ERR_INVALID_ARG, "scratch holds %zu bytes, needs %zu", scratch_bytes, need);
+    }
+    llmr::SeqAttnArgs a{};
+    a.q = q, a.k = k_cache, a.v = v_cache, a.out = out, a.offsets = seq_offsets, a.kv_len = kv_len;
+    a.table = block_table;
+    a.n_heads = p->n_heads, a.n_kv_heads = p->n_kv_heads, a.n_tokens = p->n_tokens, a.n_seqs = p->n_seqs;
+    a.q_stride = p->q_stride, a.q_head_stride = p->head_dim, a.out_stride = p->out_stride;
+    a.page_log2 = page_log2(p->page_size), a.n_pages = p->n_pages, a.max_pages = p->max_pages, a.max_new = p->max_new;
+    a.scale_log2 = p->scale * 1.4426950408889634f;
+    return launched(llmr::launch_paged_attention(a, type, p->head_dim, ctx->num_cus, scratch, ctx->cur),
+                    "paged_attention");
+}
+
+}  // extern "C"

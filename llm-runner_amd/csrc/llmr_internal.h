@@ -196,6 +196,59 @@ hipError_t launch_flash_attention(const void* q, const void* k, const void* v, u
                                   void* o, uint32_t otype, uint32_t ostride, uint32_t n_heads, uint32_t seq_len,
                                   float scale, void* ws, hipStream_t st);
 
+// Batches of requests (seq_attn.hip, paged.hip). Strides are in elements;
+// lengths, offsets, tables and slots are device memory the kernels bounds-check.
+struct SeqAttnArgs {
+    const void* q;
+    const void* k;            // packed rows, or the pages [n_pages, n_kv_heads, 1 << page_log2, dim]
+    const void* v;
+    void* out;
+    const int32_t* offsets;   // [n_seqs + 1]
+    const int32_t* kv_len;    // paged: [n_seqs]
+    const int32_t* table;     // paged: [n_seqs, max_pages]
+    uint32_t n_heads, n_kv_heads, n_tokens, n_seqs;
+    uint32_t q_stride, q_head_stride, kv_stride, kv_head_stride, out_stride;
+    uint32_t page_log2, n_pages, max_pages, max_new;
+    float scale_log2;         // softmax scale * log2(e)
+};
+constexpr uint32_t kMaxSeqs = 4096;
+hipError_t launch_prompt_attention(const SeqAttnArgs& a, uint32_t type, uint32_t dim, hipStream_t st);
+size_t paged_attention_scratch_bytes(uint32_t dim, uint32_t n_heads, uint32_t n_kv_heads, uint32_t n_tokens,
+                                     uint32_t n_seqs, uint32_t max_new, int num_cus);
+hipError_t launch_paged_attention(const SeqAttnArgs& a, uint32_t type, uint32_t dim, int num_cus, void* scratch,
+                                  hipStream_t st);
+
+struct PagedPlanArgs {
+    const int32_t* past_len;
+    const int32_t* new_len;
+    const int32_t* free_pages;
+    const int32_t* free_count;
+    int32_t* block_table;
+    int32_t* seq_offsets;
+    int32_t* kv_len;
+    int32_t* slots;
+    int32_t* positions;
+    int32_t* pages;
+    uint32_t n_seqs, n_tokens, page_log2, max_pages, n_free;
+};
+hipError_t launch_paged_plan(const PagedPlanArgs& a, hipStream_t st);
+
+struct QkvTokensArgs {
+    const float* qkv;
+    const float* q_norm;      // [dim] or null
+    const float* k_norm;
+    const float* rope_cos;    // [n_positions, dim / 2] or null
+    const float* rope_sin;
+    const int32_t* positions; // [n_tokens] or null: the row
+    const int32_t* slots;     // [n_tokens], or null: k and v are rows at kv_stride
+    void* q;
+    void* k;
+    void* v;
+    uint32_t n_heads, n_kv_heads, n_tokens, qkv_stride, q_stride, kv_stride, page_log2, n_pages, n_positions;
+    float eps;
+};
+hipError_t launch_qkv_tokens(const QkvTokensArgs& a, uint32_t dim, uint32_t otype, bool halves, hipStream_t st);
+
 // --- block glue (glue.hip). Strides are in elements; the C-ABI layer checks
 // that every vector access is aligned (dims, strides and column offsets % 4,
 // pointers 16-byte aligned) and that dims fit the kernels' register rows.

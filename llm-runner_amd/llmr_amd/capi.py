@@ -100,6 +100,36 @@ class Lora(ctypes.Structure):
     _fields_ = [("a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("rank", ctypes.c_uint32),
                 ("scale", ctypes.c_float)]
 
+
+class PromptAttentionParams(ctypes.Structure):
+    """llmr_prompt_attention_params."""
+    _fields_ = [(n, ctypes.c_uint32) for n in (
+        "head_dim", "n_heads", "n_kv_heads", "n_tokens", "n_seqs", "q_stride", "q_head_stride", "kv_stride",
+        "kv_head_stride", "out_stride")] + [("scale", ctypes.c_float)]
+
+
+class PagedPlanParams(ctypes.Structure):
+    """llmr_paged_plan_params."""
+    _fields_ = [(n, ctypes.c_uint32) for n in ("n_seqs", "n_tokens", "page_size", "max_pages", "n_free")]
+
+
+class QkvTokensParams(ctypes.Structure):
+    """llmr_qkv_tokens_params."""
+    _fields_ = [(n, ctypes.c_uint32) for n in (
+        "head_dim", "n_heads", "n_kv_heads", "n_tokens", "qkv_stride", "q_stride", "out_type", "kv_stride",
+        "page_size", "n_pages", "n_positions", "rope_halves")] + [("eps", ctypes.c_float)]
+
+
+class PagedAttentionParams(ctypes.Structure):
+    """llmr_paged_attention_params."""
+    _fields_ = [(n, ctypes.c_uint32) for n in (
+        "head_dim", "n_heads", "n_kv_heads", "n_tokens", "n_seqs", "max_new", "page_size", "n_pages", "max_pages",
+        "q_stride", "out_stride")] + [("scale", ctypes.c_float)]
+
+
+# Most requests of one paged_plan or paged_attention call (LLMR_MAX_SEQS).
+MAX_SEQS = 4096
+
 _vp = ctypes.c_void_p
 _u32 = ctypes.c_uint32
 _SIGS = {
@@ -162,6 +192,13 @@ _SIGS = {
     "llmr_batch_matmul_lora": (ctypes.c_int, [_vp, _vp, _u32, _vp, _u32, _vp, _u32, _u32, _u32, _u32, _vp, _vp,
                                               _u32, _u32, _u32]),
     "llmr_q8_lora_merge": (ctypes.c_int, [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, ctypes.c_float]),
+    "llmr_prompt_attention": (ctypes.c_int, [_vp, _vp, _vp, _vp, _u32, _vp, _vp,
+                                             ctypes.POINTER(PromptAttentionParams)]),
+    "llmr_paged_plan": (ctypes.c_int, [_vp] * 11 + [ctypes.POINTER(PagedPlanParams)]),
+    "llmr_qkv_tokens": (ctypes.c_int, [_vp] * 11 + [ctypes.POINTER(QkvTokensParams)]),
+    "llmr_paged_attention": (ctypes.c_int, [_vp, _vp, _vp, _vp, _u32, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t,
+                                            ctypes.POINTER(PagedAttentionParams)]),
+    "llmr_paged_attention_scratch_bytes": (ctypes.c_size_t, [_vp, ctypes.POINTER(PagedAttentionParams)]),
     "llmr_gguf_open": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(_vp)]),
     "llmr_gguf_close": (ctypes.c_int, [_vp]),
     "llmr_gguf_info": (ctypes.c_int, [_vp, ctypes.POINTER(_u32), ctypes.POINTER(ctypes.c_uint64),
@@ -217,6 +254,7 @@ class Context:
     """One device + one in-order stream (createContext, lib/vulkan/context.c3:73)."""
 
     def __init__(self, device: int = 0):
+        self.device = device
         self._h = _vp()
         check(lib().llmr_create_context(device, ctypes.byref(self._h)))
 
@@ -378,3 +416,26 @@ class Context:
                       rank: int, scale: float) -> None:
         check(lib().llmr_q8_lora_merge(self._h, w_ptr, a_ptr, b_ptr, in_dim, b_rows, dst_row_offset, rank,
                                        float(scale)))
+
+    # --- batches of requests (pointers are device addresses, params a structure) ---
+
+    def prompt_attention(self, q, k, v, type_, out, seq_offsets, params: PromptAttentionParams) -> None:
+        check(lib().llmr_prompt_attention(self._h, q, k, v, type_, out, seq_offsets, params))
+
+    def paged_plan(self, past_len, new_len, free_pages, free_count, block_table, seq_offsets, kv_len, slots,
+                   positions, pages, params: PagedPlanParams) -> None:
+        check(lib().llmr_paged_plan(self._h, past_len, new_len, free_pages, free_count, block_table, seq_offsets,
+                                    kv_len, slots, positions, pages, params))
+
+    def qkv_tokens(self, qkv, q_norm, k_norm, rope_cos, rope_sin, positions, slots, q, k, v,
+                   params: QkvTokensParams) -> None:
+        check(lib().llmr_qkv_tokens(self._h, qkv, q_norm, k_norm, rope_cos, rope_sin, positions, slots, q, k, v,
+                                    params))
+
+    def paged_attention(self, q, k_cache, v_cache, type_, out, seq_offsets, kv_len, block_table, scratch,
+                        scratch_bytes, params: PagedAttentionParams) -> None:
+        check(lib().llmr_paged_attention(self._h, q, k_cache, v_cache, type_, out, seq_offsets, kv_len, block_table,
+                                         scratch, scratch_bytes, params))
+
+    def paged_attention_scratch_bytes(self, params: PagedAttentionParams) -> int:
+        return lib().llmr_paged_attention_scratch_bytes(self._h, params)

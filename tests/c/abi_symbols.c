@@ -53,6 +53,11 @@ static const struct {
     {"llmr_gguf_load_tensor", (void (*)(void))(uintptr_t)llmr_gguf_load_tensor},
     {"llmr_lora_correction", (void (*)(void))(uintptr_t)llmr_lora_correction},
     {"llmr_batch_matmul_lora", (void (*)(void))(uintptr_t)llmr_batch_matmul_lora},
+    {"llmr_prompt_attention", (void (*)(void))(uintptr_t)llmr_prompt_attention},
+    {"llmr_paged_plan", (void (*)(void))(uintptr_t)llmr_paged_plan},
+    {"llmr_qkv_tokens", (void (*)(void))(uintptr_t)llmr_qkv_tokens},
+    {"llmr_paged_attention", (void (*)(void))(uintptr_t)llmr_paged_attention},
+    {"llmr_paged_attention_scratch_bytes", (void (*)(void))(uintptr_t)llmr_paged_attention_scratch_bytes},
     {"llmr_q8_lora_merge", (void (*)(void))(uintptr_t)llmr_q8_lora_merge},
     {"llmr_flash_attention", (void (*)(void))(uintptr_t)llmr_flash_attention},
     {"llmr_flash_attention_pc", (void (*)(void))(uintptr_t)llmr_flash_attention_pc},

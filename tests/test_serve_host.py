@@ -1,0 +1,65 @@
+"""The batch operators' refusals that need no device: the C entry points without a context, and the Python front
+end's checks of shapes and types (before anything is issued)."""
+import ctypes
+
+import pytest
+import torch
+
+from llmr_amd import capi, serve
+
+F16 = torch.float16
+
+
+def test_entry_points_refuse_a_null_context():
+    L = capi.lib()
+    for name, n in (("llmr_prompt_attention", 7), ("llmr_paged_plan", 11), ("llmr_qkv_tokens", 11),
+                    ("llmr_paged_attention", 10)):
+        args = [None] * n
+        if name == "llmr_prompt_attention":
+            args = [None, 16, 16, 16, 1, 16, 16]
+        elif name == "llmr_paged_attention":
+            args = [None, 16, 16, 16, 1, 16, 16, 16, 16, 16, 0]
+        assert getattr(L, name)(*args, None) == capi.LLMR_ERR_INVALID_ARG
+        assert "context" in capi.last_error()
+    assert L.llmr_paged_attention_scratch_bytes(None, None) == 0
+
+
+def test_params_have_the_headers_fields():
+    """Every params structure has the header's fields in the header's order."""
+    import re
+    text = open(capi.HEADER_PATH).read()
+    for cls, name in ((capi.PromptAttentionParams, "prompt_attention"), (capi.PagedPlanParams, "paged_plan"),
+                      (capi.QkvTokensParams, "qkv_tokens"), (capi.PagedAttentionParams, "paged_attention")):
+        body = re.search(r"typedef struct llmr_%s_params \{(.*?)\} llmr_%s_params;" % (name, name), text, re.S).group(1)
+        fields = re.findall(r"(uint32_t|float)\s+(\w+);", re.sub(r"/\*.*?\*/", "", body, flags=re.S))
+        types = {"uint32_t": ctypes.c_uint32, "float": ctypes.c_float}
+        assert [(n, types[t]) for t, n in fields] == cls._fields_
+    assert "LLMR_MAX_SEQS %du" % capi.MAX_SEQS in text
+
+
+def test_tensors_have_to_be_on_the_device():
+    q, k = torch.zeros(4, 2, 64, dtype=F16), torch.zeros(4, 1, 64, dtype=F16)
+    off = torch.tensor([0, 4], dtype=torch.int32)
+    for bad in (dict(q=q.float()), dict(q=q[0]), dict(k=k[:3]), dict(seq_offsets=off.long()),
+                dict(out=torch.zeros(4, 64, dtype=F16))):
+        with pytest.raises(ValueError):
+            serve.prompt_attention(**{**dict(q=q, k=k, v=k.clone(), seq_offsets=off), **bad})
+
+
+def test_shapes_are_checked():
+    i32 = lambda n: torch.zeros(n, dtype=torch.int32)  # noqa: E731
+    b = serve.PagedBatch.empty(2, 5, "cpu")
+    with pytest.raises(ValueError, match="one per request"):
+        serve.paged_plan(i32(2), i32(3), i32(4), i32(1), i32(4).view(2, 2), 16, b)
+    with pytest.raises(ValueError, match="PagedBatch"):
+        serve.paged_plan(i32(3), i32(3), i32(4), i32(1), i32(6).view(3, 2), 16, b)
+    with pytest.raises(ValueError, match="int32"):
+        serve.paged_plan(i32(2), i32(2).long(), i32(4), i32(1), i32(4).view(2, 2), 16, b)
+    cache = torch.zeros(3, 1, 16, 64, dtype=F16)
+    q = torch.zeros(4, 2, 64, dtype=F16)
+    with pytest.raises(ValueError, match="one per request"):
+        serve.paged_attention(q, cache, cache.clone(), i32(4), i32(2), i32(4).view(2, 2), 1)
+    with pytest.raises(ValueError, match="dtype"):
+        serve.paged_attention(q, cache, cache.float(), i32(3), i32(2), i32(4).view(2, 2), 1)
+    with pytest.raises(ValueError, match="qkv"):
+        serve.qkv_tokens(torch.zeros(4, 3 * 64), q, q[:, :1], q[:, :1])
