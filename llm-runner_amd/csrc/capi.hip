@@ -1206,8 +1206,7 @@ int llmr_qkv_tokens(llmr_context* ctx, const float* qkv, const float* q_norm, co
 size_t llmr_paged_attention_scratch_bytes(llmr_context* ctx, const llmr_paged_attention_params* p) {
     if (check_ctx(ctx) || check_paged_attention(p)) return 0;
     if (p->n_tokens == 0 || p->n_seqs == 0 || p->max_new == 0) return 0;
-    return llmr::paged_attention_scratch_bytes(p->head_dim, p->n_heads, p->n_kv_heads, p->n_tokens, p->n_seqs,
-                                               p->max_new, ctx->num_cus);
+    return llmr::paged_attention_scratch_bytes(p->head_dim, p->n_heads, p->n_kv_heads, p->max_new, ctx->num_cus);
 }
 
 int llmr_paged_attention(llmr_context* ctx, const void* q, const void* k_cache, const void* v_cache, uint32_t type,
@@ -1231,8 +1230,8 @@ int llmr_paged_attention(llmr_context* ctx, const void* q, const void* k_cache, 
     if (int r = check_stride8(p->out_stride, (uint64_t)p->n_heads * p->head_dim, "out_stride")) return r;
     if ((uint64_t)p->n_tokens * p->n_heads > 0x7fffffffull)
         return fail(LLMR_ERR_INVALID_ARG, "n_tokens * n_heads must be < 2^31");
-    const size_t need = llmr::paged_attention_scratch_bytes(p->head_dim, p->n_heads, p->n_kv_heads, p->n_tokens,
-                                                            p->n_seqs, p->max_new, ctx->num_cus);
+    const size_t need =
+        llmr::paged_attention_scratch_bytes(p->head_dim, p->n_heads, p->n_kv_heads, p->max_new, ctx->num_cus);
     if (need) {
         if (int r = check_16(scratch, "scratch")) return r;
         if (scratch_bytes < need)

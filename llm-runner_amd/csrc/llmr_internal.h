@@ -213,8 +213,7 @@ struct SeqAttnArgs {
 };
 constexpr uint32_t kMaxSeqs = 4096;
 hipError_t launch_prompt_attention(const SeqAttnArgs& a, uint32_t type, uint32_t dim, hipStream_t st);
-size_t paged_attention_scratch_bytes(uint32_t dim, uint32_t n_heads, uint32_t n_kv_heads, uint32_t n_tokens,
-                                     uint32_t n_seqs, uint32_t max_new, int num_cus);
+size_t paged_attention_scratch_bytes(uint32_t dim, uint32_t n_heads, uint32_t n_kv_heads, uint32_t max_new, int num_cus);
 hipError_t launch_paged_attention(const SeqAttnArgs& a, uint32_t type, uint32_t dim, int num_cus, void* scratch,
                                   hipStream_t st);
 

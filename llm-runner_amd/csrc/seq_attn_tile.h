@@ -1,0 +1,502 @@
+// seq_attn_tile.h - the matrix-core body of causal attention over packed rows
+// (seq_attn.hip): 32 * NW rows of one key/value head per workgroup.
+//
+// A row is one query head of one token: the G query heads of a key/value head
+// lie side by side (row = token * G + head in group), so a workgroup's 256 rows
+// are 64 tokens at G = 4 and one tile of keys serves all of a group's heads;
+// with heads apart a workgroup would reach over 256 tokens and pass four
+// diagonal tiles of keys, half of each hidden, instead of one. Rows are numbered
+// through the whole batch: a workgroup that reaches over the end of one request
+// into the next takes the keys of both and masks each row to its own request, so
+// short prompts share workgroups instead of leaving them part-filled.
+//
+// S^T = K Q^T (32 keys x 32 rows an MFMA; Q in registers as the B operand), then
+// O^T += V^T P^T with P^T straight from the score registers. K and V tiles of 64
+// keys come by DMA into LDS rings of four and three slots, V row-major, read by
+// transposing reads. The scores start from -m_ref (a row's reference maximum),
+// so that p = exp2(c (s - m_ref)) is one multiplication and one exp2; m_ref is
+// raised lazily, when a maximum exceeds it by more than 2^8 in p. Scores,
+// maxima, sums and O are f32; P is rounded to the input type for its MFMA (bf16
+// or fp16, half a step 2^-8 or 2^-11 of each weight).
+//
+// fp16 weights carry a factor 2^7, which the division takes out again: weights
+// below 2^-14 of the reference would lose bits, now below 2^-21, and the lazy
+// maximum's 2^8 above it is 2^15, within fp16.
+#pragma once
+
+#include "llmr_device.h"
+#include "llmr_internal.h"
+
+namespace llmr {
+namespace seqattn {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) s16x8 lds_s16x8;
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+
+template <uint32_t T>
+__device__ __forceinline__ f32x16 mfma32(s16x8 a, s16x8 b, f32x16 c) {
+    if constexpr (T == kGgmlBF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                      0, 0);
+}
+template <uint32_t T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (T == kGgmlBF16) return pack_bf16x2(a, b);
+    else return pack_f16x2(a, b);
+}
+// The two halves of a dword as f32.
+template <uint32_t T>
+__device__ __forceinline__ float lo_f32(uint32_t w) {
+    if constexpr (T == kGgmlBF16) return __uint_as_float(w << 16);
+    else return (float)__builtin_bit_cast(f16x2, w).x;
+}
+template <uint32_t T>
+__device__ __forceinline__ float hi_f32(uint32_t w) {
+    if constexpr (T == kGgmlBF16) return __uint_as_float(w & 0xffff0000u);
+    else return (float)__builtin_bit_cast(f16x2, w).y;
+}
+// A dword's halves with 0 in the place of infinities and NaN.
+template <uint32_t T>
+__device__ __forceinline__ uint32_t finite2(uint32_t w) {
+    constexpr uint32_t E = T == kGgmlBF16 ? 0x7f80u : 0x7c00u;
+    return w & (((w & E) == E ? 0u : 0xffffu) | ((w & (E << 16)) == (E << 16) ? 0u : 0xffff0000u));
+}
+// Whether either half of a dword is an infinity or NaN.
+template <uint32_t T>
+__device__ __forceinline__ bool nonfinite2(uint32_t w) {
+    constexpr uint32_t E = T == kGgmlBF16 ? 0x7f80u : 0x7c00u;
+    return (w & E) == E || (w & (E << 16)) == (E << 16);
+}
+
+template <uint32_t T>
+__device__ __forceinline__ bool nonfinite4(u32x4 w) {
+    return nonfinite2<T>(w.x) || nonfinite2<T>(w.y) || nonfinite2<T>(w.z) || nonfinite2<T>(w.w);
+}
+template <uint32_t T>
+__device__ __forceinline__ u32x4 finite4(u32x4 w) {
+    return u32x4{finite2<T>(w.x), finite2<T>(w.y), finite2<T>(w.z), finite2<T>(w.w)};
+}
+
+__device__ __forceinline__ float xhalf_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float xhalf_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ int wave_imin(int v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
+    return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int wave_imax(int v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
+    return __builtin_amdgcn_readfirstlane(v);
+}
+
+// Where a 16-byte chunk of key r lies within its row in an LDS slot: chunk c at
+// c ^ swizzle(r). K: a fragment read's 16 lanes (16 keys, one chunk) touch 16
+// distinct places of the 256 bytes the banks cover (a row of 256 bytes, or two
+// rows of 128). V: a transposing read's 8 keys x 4 chunks lie evenly, two a place.
+template <uint32_t D>
+__device__ __forceinline__ uint32_t kswz(uint32_t r) {
+    return D == 128u ? r & 15u : (r >> 1) & 7u;
+}
+template <uint32_t D>
+__device__ __forceinline__ uint32_t vswz(uint32_t r) {
+    return D == 128u ? ((r & 3u) << 2) | ((r >> 2) & 1u) : (((r >> 1) & 1u) << 2) | ((r >> 2) & 1u);
+}
+
+constexpr uint32_t kKeys = 64;  // keys of a tile
+
+template <uint32_t D>
+constexpr uint32_t tile_bytes() { return kKeys * D * 2u; }
+// LDS of a workgroup: four K and three V slots, then three words of its own; the
+// epilogue stages 32 rows a wave in the rings.
+template <uint32_t D>
+constexpr uint32_t lds_bytes() { return 7u * tile_bytes<D>() + 16u; }
+
+// The rows, keys and masks of a workgroup. Keys are counted from the first one the
+// workgroup takes; a lane's row sees the keys j with (uint32_t)(j - jlo) <= span
+// (no row: none).
+struct RowsOfLane {
+    uint32_t jlo, span;
+    const uint8_t* q;  // the row's first byte (some row's, for a lane that has none)
+    uint64_t out;      // element offset of the row in `out`
+    bool live;
+};
+
+// One workgroup: its rows over n_keys keys. Source: where key tiles come from,
+//   rsrc_t tile(const void* base, t, i): descriptor of DMA instruction i of tile t
+//     (its lanes' keys past the request, or on no page, read as zero), and
+//   uint32_t voffset(r, chunk): byte offset of chunk of the tile's key r in it, and
+//   const uint8_t* row(base, j): key j < n_keys's row (null: on no page).
+template <uint32_t T, uint32_t D, uint32_t NW, typename Source>
+__device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, const Source& src, uint32_t n_keys,
+                                          const RowsOfLane& row, uint32_t lo_max, uint32_t hi_min) {
+    constexpr uint32_t ROW = D * 2u, TILE = tile_bytes<D>();
+    constexpr int NF = D / 8;                       // K fragments of a tile, and V fragments
+    constexpr int CH = D / 32;                      // 32-dim blocks of a row
+    constexpr uint32_t RPI = 1024u / ROW;           // keys a DMA instruction fills (64 lanes x 16 bytes)
+    constexpr uint32_t DI = kKeys / RPI / NW;       // DMA instructions per tile and wave
+    constexpr uint32_t CPR = ROW / 16u;             // 16-byte chunks of a key row
+    constexpr float OFF = T == kGgmlF16 ? 7.0f : 0.0f;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t l32 = lane & 31u, kh = lane >> 5;
+    const float c = a.scale_log2, grow_by = 8.0f / c;
+    uint32_t* const wave_lohi = (uint32_t*)(lds + 7u * TILE);  // lo_max, hi_min over the workgroup
+    uint32_t* const any_bad = wave_lohi + 2;                    // a masked tile's V has an infinity or NaN
+
+    // Q fragments (B operand): row l32, dims 32 ch + 16 kh + 8 st ..
+    s16x8 qf[CH][2];
+#pragma unroll
+    for (int ch = 0; ch < CH; ch++)
+#pragma unroll
+        for (int st = 0; st < 2; st++) qf[ch][st] = *(const s16x8*)(row.q + 64u * ch + 32u * kh + 16u * st);
+
+    if (tid == 0) {
+        wave_lohi[0] = 0;
+        wave_lohi[1] = 0xffffffffu;
+        *any_bad = 0;
+    }
+
+    // instruction i of wave w fills the keys RPI (DI w + i) + lane / CPR of a slot,
+    // the lane's chunk landing at lane % CPR of its key's row
+    uint32_t kvo[DI], vvo[DI];
+#pragma unroll
+    for (int i = 0; i < (int)DI; i++) {
+        const uint32_t r = RPI * (DI * wave + i) + lane / CPR, p = lane % CPR;
+        kvo[i] = src.voffset(r, p ^ kswz<D>(r));
+        vvo[i] = src.voffset(r, p ^ vswz<D>(r));
+    }
+    auto dma = [&](const void* base, const uint32_t (&vo)[DI], uint32_t t, uint32_t slot) {
+        uint8_t* dst = lds + slot * TILE + wave * (DI * 1024u);
+#pragma unroll
+        for (int i = 0; i < (int)DI; i++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(src.tile(base, t, wave * DI + i), (lds_void*)(dst + 1024u * i), 16,
+                                                     vo[i], 0, 0, 0);
+    };
+
+    // K fragment: keys 32 kb + l32, chunk 4 ch + 2 kh + st. V^T fragment (transposing
+    // reads): lane (group g, index j) addresses key 4 (g / 2) + j / 4 (+ R), dims
+    // 32 dt + 16 (g % 2) + 4 (j % 4) .. + 3.
+    uint32_t kfo[CH][2], vto[CH];
+    {
+        const uint32_t g = lane >> 4, j = lane & 15u, kr = 4u * (g >> 1) + (j >> 2);
+        const uint32_t x = 2u * (g & 1u) + ((j & 3u) >> 1), half = j & 1u;
+#pragma unroll
+        for (int ch = 0; ch < CH; ch++) {
+#pragma unroll
+            for (int st = 0; st < 2; st++)
+                kfo[ch][st] = l32 * ROW + (((4u * ch + 2u * kh + st) ^ kswz<D>(l32)) << 4);
+            vto[ch] = kr * ROW + (((4u * ch + x) ^ vswz<D>(kr)) << 4) + 8u * half;
+        }
+    }
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)lds;
+    // fragment addresses in registers of their own: every read of a tile is then one of
+    // them plus an immediate
+    auto kaddr = [&](uint32_t slot, uint32_t (&ka)[CH][2]) {
+#pragma unroll
+        for (int ch = 0; ch < CH; ch++)
+#pragma unroll
+            for (int st = 0; st < 2; st++) {
+                ka[ch][st] = lds0 + slot * TILE + kfo[ch][st];
+                asm("" : "+v"(ka[ch][st]));
+            }
+    };
+    auto vaddr = [&](uint32_t slot, uint32_t (&va)[CH]) {
+#pragma unroll
+        for (int dt = 0; dt < CH; dt++) {
+            va[dt] = lds0 + (4u + slot) * TILE + vto[dt];
+            asm("" : "+v"(va[dt]));
+        }
+    };
+    auto kfrag = [&](const uint32_t (&ka)[CH][2], int f) -> s16x8 {
+        const int k = f % (NF / 2);
+        return *(const lds_s16x8*)(uintptr_t)(ka[k / 2][k % 2] + 32u * (uint32_t)(f / (NF / 2)) * ROW);
+    };
+    auto vfrag = [&](const uint32_t (&va)[CH], int f) -> s16x8 {
+        const uint32_t R = 32u * (uint32_t)(f / (NF / 2)) + 16u * (uint32_t)((f % (NF / 2)) / CH);
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(va[f % CH] + R * ROW));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(va[f % CH] + (R + 8u) * ROW));
+        return s16x8{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    };
+
+    f32x16 o[CH];
+#pragma unroll
+    for (int dt = 0; dt < CH; dt++) o[dt] = f32x16{};
+    float m_ref = 0.0f, l_i = 0.0f;
+    uint64_t seen = 0;  // lanes whose m_ref is a maximum of theirs
+
+    const uint32_t n_tiles = (n_keys + kKeys - 1u) / kKeys;
+    // tiles [full0, full1) are seen whole by every row of the wave
+    const uint32_t full0 = (lo_max + kKeys - 1u) / kKeys, full1 = (hi_min + 1u) / kKeys;
+    auto masked = [&](uint32_t t) { return t < full0 || t >= full1; };
+
+    // scores of the keys a row does not see to -inf
+    auto mask = [&](f32x16& h0, f32x16& h1, uint32_t t) {
+        const uint32_t rel = t * kKeys + 4u * kh - row.jlo;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const uint32_t k = rel + 8u * (i >> 2) + (i & 3);
+            h0[i] = k <= row.span ? h0[i] : -INFINITY;
+            h1[i] = k + 32u <= row.span ? h1[i] : -INFINITY;
+        }
+    };
+    auto rescale = [&](uint64_t grow, float mx, f32x16& n0, f32x16& n1) {
+        if (grow != 0) {
+            const bool fresh = ((seen >> lane) & 1u) == 0;
+            const float d = fresh ? (mx > -INFINITY ? mx : 0.0f) : fmaxf(mx, 0.0f);
+            const float alpha = fresh ? 0.0f : __builtin_amdgcn_exp2f(-d * c);
+            m_ref += d;
+            l_i *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < CH; dt++) o[dt] *= alpha;
+            n0 -= d;
+            n1 -= d;
+        }
+    };
+    // P of score pair `item` (keys 2 (item % 8), + 1 of half h) into dword item of p
+    auto exp_pair = [&](const f32x16& h, int item, uint32_t (&p)[16], float& rs) {
+        const int i = 2 * (item % 8);
+        const float e0 = __builtin_amdgcn_exp2f(fmaf(h[i], c, OFF));
+        const float e1 = __builtin_amdgcn_exp2f(fmaf(h[i + 1], c, OFF));
+        p[item] = pack2<T>(e0, e1);
+        rs += e0 + e1;
+    };
+    auto pfrag = [&](const uint32_t (&p)[16], int kb, int cc) -> s16x8 {
+        const int b = 8 * kb + 4 * cc;
+        return __builtin_bit_cast(s16x8, u32x4{p[b], p[b + 1], p[b + 2], p[b + 3]});
+    };
+
+    // Infinities and NaN in V rows that some row of the workgroup does not see: its
+    // weight there is 0, and 0 times them is NaN. Where a tile is masked they are set to 0
+    // in LDS before anyone reads it; the rows that do see them, with a weight above 0, get
+    // them from memory after the last tile.
+    uint32_t wg_full0 = 0, wg_full1 = 0;
+    auto wg_masked = [&](uint32_t t) { return t < wg_full0 || t >= wg_full1; };
+    auto clean_v = [&](uint32_t t, uint32_t slot) {
+        uint8_t* const vt = lds + (4u + slot) * TILE;
+#pragma unroll
+        for (uint32_t b = 0; b < TILE / (NW * 1024u); b++) {
+            u32x4* const at = (u32x4*)(vt + (b * NW + wave) * 1024u + lane * 16u);
+            const u32x4 w = *at;
+            const bool n = nonfinite4<T>(w);
+            if (__builtin_amdgcn_ballot_w64(n) != 0) {
+                if (n) {
+                    // (past the last key: whatever LDS held)
+                    if (t * kKeys + (b * NW + wave) * RPI + lane / CPR < n_keys) *any_bad = 1u;
+                    *at = finite4<T>(w);
+                }
+            }
+        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));  // lgkmcnt(0), the DMAs go on
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    auto add_bad = [&](uint32_t t) {
+        const uint32_t j = t * kKeys + lane;
+        bool n = false;
+        if (j < n_keys) {
+            const uint8_t* const vr = src.row(a.v, j);
+            for (uint32_t b = 0; vr && b < CPR; b++) {
+                const u32x4 w = *(const u32x4*)(vr + 16u * b);
+                n = n || nonfinite4<T>(w);
+            }
+        }
+        for (uint64_t bad = __builtin_amdgcn_ballot_w64(n); bad != 0; bad &= bad - 1u) {
+            const uint32_t key = t * kKeys + (uint32_t)__builtin_ctzll(bad);  // < n_keys: a lane found it there
+            const bool sees = key - row.jlo <= row.span;
+            const uint8_t* const vr = src.row(a.v, key);
+#pragma unroll
+            for (int dt = 0; dt < CH; dt++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const u32x2 v = *(const u32x2*)(vr + 64u * dt + 16u * g + 8u * kh);
+                    const float x[4] = {lo_f32<T>(v.x), hi_f32<T>(v.x), lo_f32<T>(v.y), hi_f32<T>(v.y)};
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        o[dt][4 * g + e] += (int)sees & (int)!(fabsf(x[e]) < INFINITY) ? x[e] : 0.0f;
+                }
+        }
+    };
+
+    // prologue: K(0) V(0) K(1) K(2) V(1) K(3) in flight; S(0) and its maximum
+    dma(a.k, kvo, 0, 0);
+    dma(a.v, vvo, 0, 4);
+    dma(a.k, kvo, 1, 1);
+    dma(a.k, kvo, 2, 2);
+    dma(a.v, vvo, 1, 5);
+    dma(a.k, kvo, 3, 3);
+    LLMR_STAGE_BARRIER(5 * DI);  // K(0) has landed
+    if (lane == 0) {
+        atomicMax(&wave_lohi[0], lo_max);
+        atomicMin(&wave_lohi[1], hi_min);
+    }
+    f32x16 h0, h1, h2;
+    {
+        uint32_t ka[CH][2];
+        kaddr(0, ka);
+        static_for<0, NF>([&](auto F) {
+            constexpr int f = F, kb = f / (NF / 2), k = f % (NF / 2);
+            f32x16& s = kb == 0 ? h0 : h1;
+            s = mfma32<T>(kfrag(ka, f), qf[k / 2][k % 2], k == 0 ? f32x16{} : s);
+        });
+        if (masked(0)) mask(h0, h1, 0);
+        float m = h0[0];
+#pragma unroll
+        for (int i = 0; i < 16; i++) m = fmaxf(fmaxf(m, h0[i]), h1[i]);
+        m = xhalf_max(m);
+        seen = __builtin_amdgcn_ballot_w64(m > -INFINITY);
+        m_ref = m > -INFINITY ? m : 0.0f;
+        h0 -= m_ref;
+        h1 -= m_ref;
+    }
+    LLMR_STAGE_BARRIER(2 * DI);  // K(1), K(2), V(0) have landed; every wave is done with K(0)
+    wg_full0 = (__builtin_amdgcn_readfirstlane(wave_lohi[0]) + kKeys - 1u) / kKeys;
+    wg_full1 = (__builtin_amdgcn_readfirstlane(wave_lohi[1]) + 1u) / kKeys;
+
+    constexpr int PF = 3;  // fragments in flight ahead of their MFMAs
+    uint32_t ka[CH][2];    // K(t+1)'s fragment addresses
+    s16x8 kf[PF + 1];      // its fragments in flight: the first PF are read before the tile starts
+    kaddr(1, ka);
+    static_for<0, PF>([&](auto F) { kf[F] = kfrag(ka, F); });
+
+    // One tile t: S(t) in (c0, c1), S(t+1) = K(t+1) Q^T to (n0, c0). K(t+1) is in K slot
+    // (t+1) % 4, V(t) in V slot vs; K(t+4) is DMAed to K slot t % 4 and V(t+2) to V slot vd.
+    // The MFMAs are issued in a fixed order with the vector work spread between them: the
+    // exponentials of S(t)'s first half before c0 is written again, those of the second
+    // half by the time its accumulation starts, the maximum of S(t+1) under the first
+    // accumulations, the first fragment reads of K(t+2) under the last ones.
+    auto tile = [&](f32x16& c0, f32x16& c1, f32x16& n0, uint32_t t, uint32_t vs, uint32_t vd) {
+        dma(a.k, kvo, t + 4u, t & 3u);
+        dma(a.v, vvo, t + 2u, 4u + vd);
+        if (wg_masked(t)) clean_v(t, vs);
+        const bool mask_next = masked(t + 1u);
+        uint32_t va[CH], p[16];
+        vaddr(vs, va);
+        s16x8 vf[PF + 1];
+        float rs = 0.0f, mt = -INFINITY, mx = 0.0f;
+        uint64_t grow = 0, any = 0;
+        static_for<0, 2 * NF>([&](auto J) {
+            constexpr int j = J;
+            if constexpr (j < NF) {
+                constexpr int f = j, kb = f / (NF / 2), k = f % (NF / 2);
+                if constexpr (f + PF < NF) kf[(f + PF) % (PF + 1)] = kfrag(ka, f + PF);
+                f32x16& s = kb == 0 ? n0 : c0;
+                s = mfma32<T>(kf[f % (PF + 1)], qf[k / 2][k % 2], k == 0 ? f32x16{} - m_ref : s);
+            } else {
+                constexpr int f = j - NF, kb = f / (NF / 2), cc = (f % (NF / 2)) / CH, dt = f % CH;
+                if constexpr (f + PF < NF) vf[(f + PF) % (PF + 1)] = vfrag(va, f + PF);
+                o[dt] = mfma32<T>(vf[f % (PF + 1)], pfrag(p, kb, cc), o[dt]);
+            }
+            if constexpr (j >= NF - PF && j < NF) vf[j - (NF - PF)] = vfrag(va, j - (NF - PF));
+            // first half: 8 pairs over NF / 2 steps; second half: 8 over the next NF
+            if constexpr (j < NF / 2)
+                static_for<0, 16 / NF>([&](auto E) { exp_pair(c0, j * (16 / NF) + E, p, rs); });
+            if constexpr (j >= NF / 2 && j < NF + NF / 2 && (NF == 8 || j % 2 == 0))
+                exp_pair(c1, 8 + (j - NF / 2) / (NF / 8), p, rs);
+            if constexpr (j == NF - 1) {
+                if (mask_next) mask(n0, c0, t + 1u);
+            }
+            if constexpr (j >= NF && j < NF + NF / 2)
+                static_for<0, 16 / NF>([&](auto E) {  // 4 scores of 32 at a time
+                    constexpr int k = (j - NF) * (16 / NF) + E, i = 4 * (k % 4);
+                    const f32x16& s = k < 4 ? n0 : c0;
+                    mt = fmaxf(fmaxf(mt, s[i]), s[i + 1]);
+                    mt = fmaxf(fmaxf(mt, s[i + 2]), s[i + 3]);
+                });
+            if constexpr (j == NF + NF / 2) mx = xhalf_max(mt);
+            if constexpr (j == NF + NF / 2 + 1) {
+                any = __builtin_amdgcn_ballot_w64(mx > -INFINITY);
+                grow = __builtin_amdgcn_ballot_w64(mx > grow_by) | (any & ~seen);
+            }
+            if constexpr (j == NF + NF / 2 + 2) kaddr((t + 2u) & 3u, ka);
+            // K(t+2): this tile's successor starts with it
+            if constexpr (NF == 16 && j >= NF + NF / 2 + 3 && j < NF + NF / 2 + 3 + PF)
+                kf[j - (NF + NF / 2 + 3)] = kfrag(ka, j - (NF + NF / 2 + 3));
+            if constexpr (NF == 8 && j == 2 * NF - 1) static_for<0, PF>([&](auto F) { kf[F] = kfrag(ka, F); });
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        l_i += rs;
+        rescale(grow, mx, n0, c0);
+        seen |= any;
+        LLMR_STAGE_BARRIER(2 * DI);
+    };
+
+    // V(t) is in V slot t % 3; the score halves rotate with period 3: S(t) in (h0, h1),
+    // (h2, h0), (h1, h2)
+    uint32_t t = 0, r0 = 0;
+    auto step = [&](f32x16& c0, f32x16& c1, f32x16& n0) {
+        const uint32_t r1 = r0 == 2u ? 0u : r0 + 1u, r2 = r0 == 0u ? 2u : r0 - 1u;
+        tile(c0, c1, n0, t, r0, r2);
+        t++;
+        r0 = r1;
+    };
+    while (t + 4u <= n_tiles) {
+        step(h0, h1, h2);
+        step(h2, h0, h1);
+        step(h1, h2, h0);
+    }
+    while (t + 1u < n_tiles) {
+        step(h0, h1, h2);
+        h1 = h0;
+        h0 = h2;
+    }
+    {   // last tile: S(n-1) is in (h0, h1), V(n-1) in V slot r0
+        uint32_t va[CH], p[16];
+        if (wg_masked(t)) clean_v(t, r0);
+        float rs = 0.0f;
+        static_for<0, 8>([&](auto I) { exp_pair(h0, I, p, rs); });
+        static_for<8, 16>([&](auto I) { exp_pair(h1, I, p, rs); });
+        l_i += rs;
+        vaddr(r0, va);
+        static_for<0, NF>([&](auto F) {
+            constexpr int f = F, kb = f / (NF / 2), cc = (f % (NF / 2)) / CH, dt = f % CH;
+            o[dt] = mfma32<T>(vfrag(va, f), pfrag(p, kb, cc), o[dt]);
+        });
+    }
+    LLMR_WAIT_VMCNT(0);  // no DMA may still be writing LDS when the rows are staged in it
+    __syncthreads();
+    if (__builtin_amdgcn_readfirstlane(*any_bad) != 0)
+        for (t = 0; t < n_tiles; t++)
+            if (wg_masked(t)) add_bad(t);
+
+    // O = O^T / l through LDS, so that a store writes whole rows: lane l32 holds the dims
+    // 32 dt + 8 g + 4 kh .. + 3 of its row; row r's chunk q lies at q ^ (r % CPR)
+    uint8_t* const ot = lds + wave * (32u * ROW);
+    const float inv_l = 1.0f / xhalf_sum(l_i);
+#pragma unroll
+    for (int dt = 0; dt < CH; dt++)
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+            *(u32x2*)(ot + l32 * ROW + (((4u * dt + g) ^ (l32 % CPR)) << 4) + 8u * kh) =
+                u32x2{pack2<T>(o[dt][4 * g] * inv_l, o[dt][4 * g + 1] * inv_l),
+                      pack2<T>(o[dt][4 * g + 2] * inv_l, o[dt][4 * g + 3] * inv_l)};
+    // the wave reads back only what it wrote: its LDS operations run in order
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (uint32_t i = 0; i < 32u / RPI; i++) {
+        const uint32_t r = RPI * i + lane / CPR, q = lane % CPR;
+        const u32x4 v = *(const u32x4*)(ot + r * ROW + ((q ^ (r % CPR)) << 4));
+        const uint64_t at = ((uint64_t)(uint32_t)__shfl((int)(row.out >> 32), (int)r, 64) << 32) |
+                            (uint32_t)__shfl((int)(uint32_t)row.out, (int)r, 64);
+        if (__shfl((int)row.live, (int)r, 64)) *(u32x4*)((uint16_t*)a.out + at + 8u * q) = v;
+    }
+}
+
+}  // namespace seqattn
+}  // namespace llmr

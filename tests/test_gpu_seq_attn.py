@@ -70,6 +70,10 @@ def _near(a, b, v, what):
     assert worst <= 6.2 * u * vmax, (what, worst)
 
 
+def _say(*a):
+    print(*a, flush=True)
+
+
 def _prompt_case(dev, dtype, D, H, Hk, lens, pad=0, seed=0, layout="tokens", qstd=1.5, shift=0.0):
     g = torch.Generator(device=dev).manual_seed(seed)
     T = sum(lens) + pad
@@ -182,6 +186,7 @@ def test_prompt_attention_unseen_values_do_not_matter(dev, dtype, bad):
     lens = [40, 150, 70]
     for where in ("k", "v"):
         for row in (0, 39, 45, 189, 190, 200, 259):
+            _say(f"{bad} in {where} row {row}")
             q, k, v, at, off = _prompt_case(dev, dtype, 128, 4, 2, lens, seed=12)
             clean = serve.prompt_attention(q, k, v, off).clone()
             (k if where == "k" else v)[row, 1, 5] = bad
@@ -387,6 +392,7 @@ def test_paged_attention_unseen_values_do_not_matter(dev, dtype, new, row):
     past = 97 if new == 3 else 96
     for where in (0, 1):
         for bad in (math.nan, math.inf):
+            _say(f"{bad} in {'kv'[where]}, {new} new")
             q, kc, vc, rows, at, off, kvl, table, kv = _paged_case(dev, dtype, 128, 8, 2, 16, [past, 60], [new, 1], seed=5)
             clean = serve.paged_attention(q, kc, vc, off, kvl, table, new).clone()
             page = int(table[0, row // 16])
