@@ -12,115 +12,15 @@
 namespace llmr {
 namespace {
 
-template <uint32_t T>
-__device__ __forceinline__ float widen(uint16_t x) {
-    if constexpr (T == kGgmlBF16) return __uint_as_float((uint32_t)x << 16);
-    else return (float)__builtin_bit_cast(_Float16, x);
-}
-template <uint32_t T>
-__device__ __forceinline__ uint16_t narrow(float x) {
-    if constexpr (T == kGgmlBF16) return __builtin_bit_cast(uint16_t, (__bf16)x);
-    else return __builtin_bit_cast(uint16_t, (_Float16)x);
-}
-
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
-}
-__device__ __forceinline__ float wave_add(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
-}
-
-// One wave per (row, query head): 64 keys a step, a lane one key's score, then
-// D / 64 dims of the row.
-template <uint32_t T, uint32_t D, bool PAGED>
-__global__ void __launch_bounds__(256) seq_attn_rows(SeqAttnArgs a) {
-    __shared__ float qs[4][D];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const uint32_t t = blockIdx.x * 4u + wave, head = blockIdx.y;
-    if (t >= a.n_tokens) return;
-    uint32_t lo = 0, hi = a.n_seqs;  // the first request that ends behind row t
-    while (lo < hi) {
-        const uint32_t mid = (lo + hi) / 2u;
-        if (a.offsets[mid + 1u] > (int32_t)t) hi = mid;
-        else lo = mid + 1u;
-    }
-    if (lo == a.n_seqs) return;
-    const int32_t first = a.offsets[lo];
-    if (first < 0 || first > (int32_t)t) return;
-    const uint32_t i = t - (uint32_t)first;
-    if (PAGED && i >= a.max_new) return;
-    const uint32_t kvh = head / (a.n_heads / a.n_kv_heads);
-    int64_t keys;  // seen by this row
-    if constexpr (PAGED) {
-        const int64_t n = min(a.offsets[lo + 1u], (int32_t)a.n_tokens) - first;
-        keys = (int64_t)a.kv_len[lo] - n + i + 1;
-        keys = min(keys, (int64_t)a.max_pages << a.page_log2);
-    } else {
-        keys = i + 1;
-    }
-    const uint16_t* qr = (const uint16_t*)a.q + (size_t)t * a.q_stride + (size_t)head * a.q_head_stride;
-    for (uint32_t d = lane; d < D; d += 64u) qs[wave][d] = widen<T>(qr[d]);
-    __builtin_amdgcn_wave_barrier();
-    float m = -INFINITY, l = 0.0f, o[D / 64u] = {};
-    bool sees = false;  // any key: a row that sees none is 0
-    for (int64_t k0 = 0; k0 < keys; k0 += 64) {
-        const int64_t j = k0 + lane;
-        size_t row = 0;
-        bool seen = j < keys;
-        if (seen) {
-            if constexpr (PAGED) {
-                const int32_t page = a.table[(size_t)lo * a.max_pages + (uint32_t)(j >> a.page_log2)];
-                seen = page >= 0 && (uint32_t)page < a.n_pages;
-                row = ((((size_t)(uint32_t)page * a.n_kv_heads + kvh) << a.page_log2) +
-                       ((uint32_t)j & ((1u << a.page_log2) - 1u))) * D;
-            } else {
-                row = (size_t)(first + (uint32_t)j) * a.kv_stride + (size_t)kvh * a.kv_head_stride;
-            }
-        }
-        float s = -INFINITY;
-        if (seen) {
-            float acc = 0.0f;
-            const uint16_t* kr = (const uint16_t*)a.k + row;
-            for (uint32_t d = 0; d < D; d++) acc = fmaf(qs[wave][d], widen<T>(kr[d]), acc);
-            s = acc;
-        }
-        const uint64_t any = __builtin_amdgcn_ballot_w64(seen);
-        if (any == 0) continue;
-        sees = true;
-        // NaN scores go into the row by way of exp2
-        const float mx = fmaxf(m, wave_max(s));
-        const float mu = mx == -INFINITY ? 0.0f : mx;
-        const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mu) * a.scale_log2);
-        const float p = seen ? widen<T>(narrow<T>(__builtin_amdgcn_exp2f((s - mu) * a.scale_log2))) : 0.0f;
-        m = mx;
-        l = l * alpha + wave_add(p);
-#pragma unroll
-        for (uint32_t x = 0; x < D / 64u; x++) o[x] *= alpha;
-        for (uint32_t b = 0; b < 64u; b++) {
-            if (!((any >> b) & 1u)) continue;
-            const float pb = __shfl(p, (int)b, 64);
-            const size_t rb = ((size_t)__shfl((int)(row >> 32), (int)b, 64) << 32) |
-                              (uint32_t)__shfl((int)(uint32_t)row, (int)b, 64);
-            const uint16_t* vr = (const uint16_t*)a.v + rb;
-#pragma unroll
-            for (uint32_t x = 0; x < D / 64u; x++) o[x] = fmaf(pb, widen<T>(vr[lane + 64u * x]), o[x]);
-        }
-    }
-    uint16_t* dst = (uint16_t*)a.out + (size_t)t * a.out_stride + (size_t)head * D;
-#pragma unroll
-    for (uint32_t x = 0; x < D / 64u; x++) dst[lane + 64u * x] = narrow<T>(sees ? o[x] / l : 0.0f);
-}
-
 // Keys in packed rows: a tile's descriptor starts at its first key and ends with the
 // workgroup's last.
 struct PackedKeys {
+    static constexpr bool kStages = false;
     uint64_t first;    // element offset of key 0 of the key/value head
     uint32_t stride2;  // bytes between keys
     uint32_t n_keys;
+    __device__ __forceinline__ uint32_t stage(uint32_t, uint32_t n) { return n; }
+    __device__ __forceinline__ uint32_t page(uint32_t) const { return 0; }
     __device__ __forceinline__ rsrc_t tile(const void* base, uint32_t t, uint32_t) const {
         // a saturating subtraction, not a comparison and a difference: from the latter's
         // difference for K(t+4) hipcc took n_keys >= 64 (t+4) as given and left V(t+2) without
@@ -133,6 +33,8 @@ struct PackedKeys {
             (int)__builtin_amdgcn_readfirstlane(left * stride2), 0x00020000);
     }
     __device__ __forceinline__ uint32_t voffset(uint32_t r, uint32_t chunk) const { return r * stride2 + (chunk << 4); }
+    __device__ __forceinline__ bool holes() const { return false; }
+    __device__ __forceinline__ uint32_t groups(uint32_t) const { return 15u; }
     __device__ __forceinline__ const uint8_t* row(const void* base, uint32_t j) const {
         return (const uint8_t*)base + 2u * first + (uint64_t)j * stride2;
     }
@@ -169,7 +71,7 @@ __global__ void __launch_bounds__(64 * NW, 1) prompt_attn_tiles(SeqAttnArgs a) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const uint32_t r = min(row0 + 32u * wave + (lane & 31u), rows - 1u);
     const uint32_t tok = r / G, head = kvh * G + r % G;
-    seqattn::RowsOfLane row;
+    seqattn::RowOfLane row;
     row.live = row0 + 32u * wave + (lane & 31u) < rows;
     int32_t start = start0;
     if ((int32_t)tok >= end0) {
@@ -178,14 +80,16 @@ __global__ void __launch_bounds__(64 * NW, 1) prompt_attn_tiles(SeqAttnArgs a) {
     }
     row.live = row.live && start <= (int32_t)tok;
     const uint32_t lo = (uint32_t)max(start, 0);
-    row.jlo = row.live ? (lo > kv0 ? lo - kv0 : 0u) : 0x80000000u;
+    row.jlo = row.live ? (lo > kv0 ? lo - kv0 : 0u) : seqattn::kNoKeys;
     row.span = row.live ? tok - kv0 - row.jlo : 0u;
     row.q = (const uint8_t*)a.q + 2u * ((uint64_t)tok * a.q_stride + (uint64_t)head * a.q_head_stride);
-    row.out = (uint64_t)tok * a.out_stride + head * D;
     const uint32_t lo_max = (uint32_t)seqattn::wave_imax(row.live ? (int)row.jlo : 0);
-    const uint32_t hi_min = (uint32_t)seqattn::wave_imin(row.live ? (int)(tok - kv0) : 0x7fffffff);
-    const PackedKeys src{(uint64_t)kv0 * a.kv_stride + (uint64_t)kvh * a.kv_head_stride, a.kv_stride * 2u, t1 + 1u - kv0};
-    seqattn::tile_rows<T, D, NW>(a, lds, src, t1 + 1u - kv0, row, lo_max, hi_min);
+    const int hi_min = seqattn::wave_imin(row.live ? (int)(tok - kv0) : 0x7ffffffe);
+    PackedKeys src{(uint64_t)kv0 * a.kv_stride + (uint64_t)kvh * a.kv_head_stride, a.kv_stride * 2u, t1 + 1u - kv0};
+    seqattn::tile_rows<T, D, NW>(a, lds, src, t1 + 1u - kv0, row, lo_max, hi_min, nullptr, [&]() {
+        const uint32_t x = min(row0 + 32u * wave + (lane & 31u), rows - 1u);
+        return (uint64_t)(x / G) * a.out_stride + (kvh * G + x % G) * D;
+    });
 }
 
 template <uint32_t T, uint32_t D, uint32_t NW>
@@ -195,17 +99,223 @@ hipError_t launch_tiles(const SeqAttnArgs& a, hipStream_t st) {
     return hipGetLastError();
 }
 
-template <bool PAGED>
-hipError_t launch(const SeqAttnArgs& a, uint32_t type, uint32_t dim, hipStream_t st) {
-    const dim3 grid((a.n_tokens + 3u) / 4u, a.n_heads), block(256);
-    if (type == kGgmlBF16) {
-        if (dim == 128u) hipLaunchKernelGGL((seq_attn_rows<kGgmlBF16, 128, PAGED>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((seq_attn_rows<kGgmlBF16, 64, PAGED>), grid, block, 0, st, a);
-    } else {
-        if (dim == 128u) hipLaunchKernelGGL((seq_attn_rows<kGgmlF16, 128, PAGED>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((seq_attn_rows<kGgmlF16, 64, PAGED>), grid, block, 0, st, a);
+
+
+using seqattn::PagedRequest;
+constexpr uint32_t kBlockRows = 256;  // rows of a workgroup of paged_attn_tiles
+constexpr uint32_t kPageCap = 8192;   // pages staged at a time: 2040 tiles of the smallest pages
+constexpr uint32_t kStageTiles = 2040;
+
+// Keys in the pages of a cache: fragment tiles of 64 keys from key0 on. The request's pages
+// lie in LDS, kStageTiles tiles of them at a time, checked (~0: none).
+template <uint32_t ROW>
+struct PagedKeys {
+    static constexpr bool kStages = true;
+    const int32_t* table;  // the request's row of the table
+    uint32_t* pages;       // LDS: [kPageCap], then a word: some page is none
+    uint32_t key0, n_keys, kvh, n_kv_heads, n_pages, log2, wave;
+    uint32_t end = 0, page0 = 0;  // tiles below `end` are staged; the table's column of pages[0]
+    bool none = false;
+    __device__ __forceinline__ uint32_t stage(uint32_t t, uint32_t n) {
+        end = min(n, t + kStageTiles);
+        page0 = (key0 + t * seqattn::kKeys) >> log2;
+        const uint32_t last = (key0 + min(n_keys, end * seqattn::kKeys) - 1u) >> log2;
+        for (uint32_t i = threadIdx.x; page0 + i <= last; i += blockDim.x) {
+            const uint32_t p = (uint32_t)table[page0 + i];
+            pages[i] = p < n_pages ? p : ~0u;
+            if (p >= n_pages) pages[kPageCap] = 1u;
+        }
+        return end;
     }
-    return hipGetLastError();
+    __device__ __forceinline__ void staged() { none = __builtin_amdgcn_readfirstlane(pages[kPageCap]) != 0; }
+    __device__ __forceinline__ uint32_t page_of(uint32_t k) const {  // of the fragment's key k
+        const uint32_t top = min(n_keys, end * seqattn::kKeys);
+        const uint32_t p = pages[((key0 + min(k, top - 1u)) >> log2) - page0];
+        return k < top ? p : ~0u;
+    }
+    // the wave's keys of a tile: 8 wave .. + 7, on one page
+    __device__ __forceinline__ uint32_t page(uint32_t t) const { return page_of(t * seqattn::kKeys + 8u * wave); }
+    __device__ __forceinline__ rsrc_t tile(const void* base, uint32_t t, uint32_t page) const {
+        const uint32_t k = t * seqattn::kKeys + 8u * wave, in = (key0 + k) & ((1u << log2) - 1u);
+        const uint32_t left = page == ~0u ? 0u : min(__builtin_elementwise_sub_sat(n_keys, k), 8u);
+        const uint64_t off = ((((uint64_t)(page == ~0u ? 0u : page) * n_kv_heads + kvh) << log2) + in) * ROW;
+        return __builtin_amdgcn_make_buffer_rsrc((uint8_t*)const_cast<void*>(base) + off, (short)0,
+                                                 (int)__builtin_amdgcn_readfirstlane(left * ROW), 0x00020000);
+    }
+    __device__ __forceinline__ uint32_t voffset(uint32_t r, uint32_t chunk) const { return (r & 7u) * ROW + (chunk << 4); }
+    __device__ __forceinline__ bool holes() const { return none; }
+    __device__ __forceinline__ uint32_t groups(uint32_t t) const {
+        uint32_t on = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; i++)
+            on |= (uint32_t)__builtin_amdgcn_readfirstlane(page_of(t * seqattn::kKeys + 16u * i)) != ~0u ? 1u << i : 0u;
+        return on;
+    }
+    __device__ __forceinline__ const uint8_t* row(const void* base, uint32_t j) const {
+        const uint32_t p = (uint32_t)table[(key0 + j) >> log2];
+        if (p >= n_pages) return nullptr;
+        return (const uint8_t*)base +
+               ((((uint64_t)p * n_kv_heads + kvh) << log2) + ((key0 + j) & ((1u << log2) - 1u))) * ROW;
+    }
+};
+
+// Row blocks of a request, and the keys and 64-key tiles of one (a tile at least: its rows are
+// written).
+__device__ __forceinline__ uint32_t blocks_of(const PagedRequest& rq, uint32_t G) {
+    return (uint32_t)(((uint64_t)rq.rows * G + kBlockRows - 1u) / kBlockRows);
+}
+__device__ __forceinline__ uint32_t block_keys(const SeqAttnArgs& a, const PagedRequest& rq, uint32_t G, uint32_t b) {
+    const uint32_t last = (uint32_t)(min((uint64_t)rq.rows * G, (uint64_t)(b + 1u) * kBlockRows) - 1u) / G;
+    const int64_t cap = (int64_t)a.max_pages << a.page_log2;
+    return (uint32_t)min(max((int64_t)rq.pos0 + last + 1, (int64_t)0), cap);
+}
+__device__ __forceinline__ uint32_t block_tiles(const SeqAttnArgs& a, const PagedRequest& rq, uint32_t G, uint32_t b) {
+    return max((block_keys(a, rq, G, b) + seqattn::kKeys - 1u) / seqattn::kKeys, 1u);
+}
+__device__ __forceinline__ uint64_t request_tiles(const SeqAttnArgs& a, const PagedRequest& rq, uint32_t G) {
+    uint64_t n = 0;
+    for (uint32_t b = 0; b < blocks_of(rq, G); b++) n += block_tiles(a, rq, G, b);
+    return n;
+}
+// Tiles before request `upto` (of one key/value head), by one wave.
+__device__ __forceinline__ uint64_t tiles_before(const SeqAttnArgs& a, uint32_t G, uint32_t upto, uint32_t lane) {
+    uint64_t sum = 0;
+    for (uint32_t s = lane; s < upto; s += 64u) sum += request_tiles(a, seqattn::paged_request(a, s), G);
+    return seqattn::uniform64(seqattn::shfl64(seqattn::wave_scan(sum, lane), 63));
+}
+
+template <uint32_t D>
+constexpr size_t tile_part_floats() { return kBlockRows * (D + 2u); }
+
+// Attention over a paged cache for requests of any number of new tokens: the tiles of all
+// (request, key/value head, block of 256 rows) make one line that the workgroups, one a CU,
+// share evenly, as paged_attn_few's waves do; parts of a block that several workgroups take
+// go to scratch, at most two a workgroup, and paged_attn_tiles_join joins them.
+template <uint32_t T, uint32_t D>
+__device__ __forceinline__ void paged_tiles(const SeqAttnArgs& a, uint8_t* lds, float* __restrict__ scratch) {
+    constexpr uint32_t NW = 8, ROW = D * 2u;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t G = a.n_heads / a.n_kv_heads;
+    uint32_t* const pages = (uint32_t*)(lds + seqattn::lds_bytes<D>());
+
+    const uint64_t w = tiles_before(a, G, a.n_seqs, lane) * a.n_kv_heads;
+    const uint32_t n = (uint32_t)min((uint64_t)gridDim.x, w);  // every workgroup has a tile
+    if (blockIdx.x >= n) return;
+    uint64_t at = seqattn::part_begin(blockIdx.x, w, n);
+    const uint64_t end = seqattn::part_begin(blockIdx.x + 1u, w, n);
+    uint32_t s = 0;     // the last request whose tiles begin at or before `at`
+    uint64_t base = 0;  // tiles (all heads) before it
+    for (uint32_t s0 = 0; s0 < a.n_seqs; s0 += 64u) {
+        const uint64_t u = s0 + lane < a.n_seqs ? request_tiles(a, seqattn::paged_request(a, s0 + lane), G) * a.n_kv_heads : 0;
+        const uint64_t inc = seqattn::wave_scan(u, lane);
+        const uint64_t here = __builtin_amdgcn_ballot_w64(base + inc > at);
+        if (here != 0) {
+            const int l = __builtin_ctzll(here);
+            s = s0 + (uint32_t)l;
+            base += seqattn::uniform64(seqattn::shfl64(inc - u, l));
+            break;
+        }
+        base += seqattn::uniform64(seqattn::shfl64(inc, 63));
+    }
+
+    while (at < end) {
+        const PagedRequest rq = seqattn::paged_request(a, s);
+        const uint64_t per_head = request_tiles(a, rq, G), all = per_head * a.n_kv_heads;
+        if (all == 0 || at >= base + all) {
+            base += all;
+            s++;
+            continue;
+        }
+        const uint32_t kvh = (uint32_t)((at - base) / per_head);
+        uint64_t x = (at - base) % per_head;
+        uint32_t b = 0, tiles;
+        while (x >= (tiles = block_tiles(a, rq, G, b))) {
+            x -= tiles;
+            b++;
+        }
+        const uint32_t t0 = (uint32_t)x, t1 = (uint32_t)min((uint64_t)tiles, x + (end - at));
+        const uint32_t keys = block_keys(a, rq, G, b), key0 = t0 * seqattn::kKeys;
+        const uint32_t n_keys = min(keys, t1 * seqattn::kKeys) - min(keys, key0);
+
+        const uint32_t rows = rq.rows * G, row0 = b * kBlockRows;
+        const auto out_at = [&]() {
+            const uint32_t r = min(row0 + 32u * wave + (lane & 31u), rows - 1u);
+            return (uint64_t)(rq.first + r / G) * a.out_stride + (kvh * G + r % G) * D;
+        };
+        const uint32_t r = min(row0 + 32u * wave + (lane & 31u), rows - 1u), i = r / G;
+        seqattn::RowOfLane row;
+        row.live = row0 + 32u * wave + (lane & 31u) < rows;
+        const int64_t pos = (int64_t)rq.pos0 + i - key0;  // last key it sees, of this part
+        const bool any = row.live && pos >= 0;
+        row.jlo = any ? 0u : seqattn::kNoKeys;
+        row.span = any ? (uint32_t)min(pos, (int64_t)0x7ffffffe) : 0u;
+        row.q = (const uint8_t*)a.q + 2u * ((uint64_t)(rq.first + i) * a.q_stride + (uint64_t)(kvh * G + r % G) * a.q_head_stride);
+        const int hi_min = seqattn::wave_imin(row.live ? (any ? (int)row.span : -1) : 0x7ffffffe);
+
+        // (the workgroup's last part is done with LDS)
+        __syncthreads();
+        if (tid == 0) pages[kPageCap] = 0;
+        __syncthreads();
+        PagedKeys<ROW> src{a.table + (size_t)s * a.max_pages, pages, key0, n_keys, kvh, a.n_kv_heads, a.n_pages,
+                           a.page_log2, wave};
+        float* const part = t0 == 0 && t1 == tiles
+                                ? nullptr
+                                : scratch + (2u * blockIdx.x + (t0 == 0 ? 1u : 0u)) * tile_part_floats<D>();
+        seqattn::tile_rows<T, D, NW>(a, lds, src, n_keys, row, 0u, hi_min, part, out_at);
+        at += t1 - t0;
+    }
+}
+
+template <uint32_t T, uint32_t D>
+__global__ void __launch_bounds__(512, 1) paged_attn_tiles(SeqAttnArgs a, float* __restrict__ scratch) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[seqattn::lds_bytes<D>() + 4u * (kPageCap + 4u)];
+    paged_tiles<T, D>(a, lds, scratch);
+}
+
+// Joins the parts of a row block that more than one workgroup took, in their order, 32 rows a
+// workgroup. n_wgs: the grid of paged_attn_tiles.
+template <uint32_t T, uint32_t D>
+__global__ void __launch_bounds__(256) paged_attn_tiles_join(SeqAttnArgs a, const float* __restrict__ scratch,
+                                                             uint32_t n_wgs) {
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, kvh = blockIdx.y, row0 = 32u * blockIdx.z;
+    const uint32_t G = a.n_heads / a.n_kv_heads;
+    // the blockIdx.x-th row block of the batch
+    uint32_t s = a.n_seqs, b = 0;
+    uint64_t before = 0;
+    for (uint32_t s0 = 0; s0 < a.n_seqs; s0 += 64u) {
+        const uint64_t u = s0 + lane < a.n_seqs ? blocks_of(seqattn::paged_request(a, s0 + lane), G) : 0;
+        const uint64_t inc = seqattn::wave_scan(u, lane);
+        const uint64_t here = __builtin_amdgcn_ballot_w64(before + inc > blockIdx.x);
+        if (here != 0) {
+            const int l = __builtin_ctzll(here);
+            s = s0 + (uint32_t)l;
+            b = blockIdx.x - (uint32_t)(before + seqattn::uniform64(seqattn::shfl64(inc - u, l)));
+            break;
+        }
+        before += seqattn::uniform64(seqattn::shfl64(inc, 63));
+    }
+    if (s == a.n_seqs) return;
+    const PagedRequest rq = seqattn::paged_request(a, s);
+    const uint32_t tiles = block_tiles(a, rq, G, b), rows = min(rq.rows * G - b * kBlockRows, kBlockRows);
+    if (tiles <= 1u || row0 >= rows) return;
+    const uint64_t w = tiles_before(a, G, a.n_seqs, lane) * a.n_kv_heads;
+    uint64_t begin = tiles_before(a, G, s, lane) * a.n_kv_heads + kvh * request_tiles(a, rq, G);
+    for (uint32_t i = 0; i < b; i++) begin += block_tiles(a, rq, G, i);
+    const uint32_t n = (uint32_t)min((uint64_t)n_wgs, w);
+    const uint32_t g0 = seqattn::part_of(begin, w, n), g1 = seqattn::part_of(begin + tiles - 1u, w, n);
+    if (g0 == g1) return;
+    for (uint32_t e = tid; e < 32u * (D / 4u); e += 256u) {
+        const uint32_t x = row0 + e / (D / 4u), d = 4u * (e % (D / 4u));
+        if (x >= rows) break;
+        f32x4 v;
+        const bool sees = seqattn::join_row(
+            g0, g1, a.scale_log2,
+            [&](uint32_t g) { return scratch + (2u * g + (g == g0 ? 1u : 0u)) * tile_part_floats<D>(); }, kBlockRows, D, x, d, v);
+        const uint32_t r = b * kBlockRows + x;
+        uint16_t* const dst = (uint16_t*)a.out + (size_t)(rq.first + r / G) * a.out_stride + (kvh * G + r % G) * D + d;
+        *(u32x2*)dst = sees ? u32x2{seqattn::pack2<T>(v.x, v.y), seqattn::pack2<T>(v.z, v.w)} : u32x2{0u, 0u};
+    }
 }
 
 }  // namespace
@@ -215,6 +325,7 @@ hipError_t launch_prompt_attention(const SeqAttnArgs& a, uint32_t type, uint32_t
         return dim == 128u ? launch_tiles<kGgmlBF16, 128, 8>(a, st) : launch_tiles<kGgmlBF16, 64, 8>(a, st);
     return dim == 128u ? launch_tiles<kGgmlF16, 128, 8>(a, st) : launch_tiles<kGgmlF16, 64, 8>(a, st);
 }
+
 // Row blocks of 16 of the kernel for few rows that holds max_new tokens of a group; 0: more rows.
 static uint32_t few_blocks(uint32_t n_heads, uint32_t n_kv_heads, uint32_t max_new) {
     const uint64_t rows = (uint64_t)max_new * (n_heads / n_kv_heads);
@@ -222,8 +333,23 @@ static uint32_t few_blocks(uint32_t n_heads, uint32_t n_kv_heads, uint32_t max_n
 }
 constexpr uint32_t kFewPerCu = 4;  // waves a CU: their rings fill its LDS
 
+template <uint32_t T, uint32_t D>
+static hipError_t launch_paged_tiles(const SeqAttnArgs& a, int num_cus, float* scratch, hipStream_t st) {
+    const uint32_t n = (uint32_t)num_cus, G = a.n_heads / a.n_kv_heads;
+    hipLaunchKernelGGL((paged_attn_tiles<T, D>), dim3(n), dim3(512), 0, st, a, scratch);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    // row blocks there can be: a request of r rows has (r + 255) / 256, and r > 0
+    const uint64_t rows = (uint64_t)a.n_tokens * G, full = rows / kBlockRows;
+    const uint32_t blocks = (uint32_t)(full + (a.n_seqs < rows ? a.n_seqs : rows));
+    hipLaunchKernelGGL((paged_attn_tiles_join<T, D>), dim3(blocks, a.n_kv_heads, kBlockRows / 32u), dim3(256), 0, st, a,
+                       scratch, n);
+    return hipGetLastError();
+}
+
 size_t paged_attention_scratch_bytes(uint32_t dim, uint32_t n_heads, uint32_t n_kv_heads, uint32_t max_new, int num_cus) {
     const uint32_t nr = few_blocks(n_heads, n_kv_heads, max_new);
+    if (nr == 0) return (size_t)2u * num_cus * kBlockRows * (dim + 2u) * sizeof(float);
     return (size_t)2u * kFewPerCu * num_cus * 16u * nr * (dim + 2u) * sizeof(float);
 }
 
@@ -240,12 +366,13 @@ static hipError_t launch_few(const SeqAttnArgs& a, int num_cus, float* scratch, 
 hipError_t launch_paged_attention(const SeqAttnArgs& a, uint32_t type, uint32_t dim, int num_cus, void* scratch,
                                   hipStream_t st) {
     const uint32_t nr = few_blocks(a.n_heads, a.n_kv_heads, a.max_new);
-    if (nr == 0) return launch<true>(a, type, dim, st);
     float* const p = (float*)scratch;
     auto go = [&](auto t, auto d) {
         constexpr uint32_t T = decltype(t)::value, D = decltype(d)::value;
-        return nr == 1u ? launch_few<T, D, 1>(a, num_cus, p, st)
-                        : nr == 2u ? launch_few<T, D, 2>(a, num_cus, p, st) : launch_few<T, D, 4>(a, num_cus, p, st);
+        return nr == 0u ? launch_paged_tiles<T, D>(a, num_cus, p, st)
+               : nr == 1u ? launch_few<T, D, 1>(a, num_cus, p, st)
+               : nr == 2u ? launch_few<T, D, 2>(a, num_cus, p, st)
+                          : launch_few<T, D, 4>(a, num_cus, p, st);
     };
     using BF16 = std::integral_constant<uint32_t, kGgmlBF16>;
     using F16 = std::integral_constant<uint32_t, kGgmlF16>;

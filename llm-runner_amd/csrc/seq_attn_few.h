@@ -395,6 +395,32 @@ __global__ void __launch_bounds__(64, 1) paged_attn_few(SeqAttnArgs a, float* __
     few_rows<T, D, NR>(a, lds, scratch);
 }
 
+// One row's dims d .. d + 3 of the parts g0 .. g1, in their order, divided by the sum; false:
+// the row sees no key. part(g): O[rows][D], m[rows], l[rows] of part g.
+template <typename Part>
+__device__ __forceinline__ bool join_row(uint32_t g0, uint32_t g1, float c, const Part& part, uint32_t rows, uint32_t D,
+                                         uint32_t x, uint32_t d, f32x4& out) {
+    f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;
+    bool sees = false;
+    for (uint32_t g = g0; g <= g1; g++) {
+        const float* const p = part(g);
+        const float pm = p[rows * D + x], pl = p[rows * (D + 1u) + x];
+        const f32x4 po = *(const f32x4*)(p + x * D + d);
+        if (pl == -1.0f) continue;  // no key of this part is seen
+        const float mx = fmaxf(m, pm);
+        // (a part whose scores are all -inf has m = -inf and sums of 0 or NaN)
+        const float fo = !sees || m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mx) * c);
+        const float fp = pm == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((pm - mx) * c);
+        o = o * fo + po * fp;
+        l = l * fo + pl * fp;
+        m = mx;
+        sees = true;
+    }
+    out = o * (1.0f / l);
+    return sees;
+}
+
 // Joins the parts of a (request, key/value head) pair that more than one wave took, in
 // their order. waves: the grid of paged_attn_few.
 template <uint32_t T, uint32_t D, uint32_t NR>
@@ -411,24 +437,11 @@ __global__ void __launch_bounds__(256) paged_attn_join(SeqAttnArgs a, const floa
     if (g0 == g1) return;
     for (uint32_t e = tid; e < rq.rows * G * (D / 4u); e += 256u) {
         const uint32_t x = e / (D / 4u), d = 4u * (e % (D / 4u));
-        f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
-        float m = -INFINITY, l = 0.0f;
-        bool sees = false;
-        for (uint32_t g = g0; g <= g1; g++) {
-            const float* const part = scratch + (size_t)(2u * g + (g == g0 ? 1u : 0u)) * part_floats<D, NR>();
-            const float pm = part[16u * NR * D + x], pl = part[16u * NR * (D + 1u) + x];
-            const f32x4 po = *(const f32x4*)(part + x * D + d);
-            if (pl == -1.0f) continue;  // no key of this part is seen
-            const float mx = fmaxf(m, pm);
-            // (a part whose scores are all -inf has m = -inf and sums of 0 or NaN)
-            const float fo = !sees || m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mx) * a.scale_log2);
-            const float fp = pm == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((pm - mx) * a.scale_log2);
-            o = o * fo + po * fp;
-            l = l * fo + pl * fp;
-            m = mx;
-            sees = true;
-        }
-        const f32x4 v = o * (1.0f / l);
+        f32x4 v;
+        const bool sees = join_row(
+            g0, g1, a.scale_log2,
+            [&](uint32_t g) { return scratch + (size_t)(2u * g + (g == g0 ? 1u : 0u)) * part_floats<D, NR>(); }, 16u * NR, D,
+            x, d, v);
         uint16_t* const dst = (uint16_t*)a.out + (size_t)(rq.first + x / G) * a.out_stride + (kvh * G + x % G) * D + d;
         *(u32x2*)dst = sees ? u32x2{pack2<T>(v.x, v.y), pack2<T>(v.z, v.w)} : u32x2{0u, 0u};
     }

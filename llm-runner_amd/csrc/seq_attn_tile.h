@@ -125,24 +125,33 @@ constexpr uint32_t tile_bytes() { return kKeys * D * 2u; }
 template <uint32_t D>
 constexpr uint32_t lds_bytes() { return 7u * tile_bytes<D>() + 16u; }
 
-// The rows, keys and masks of a workgroup. Keys are counted from the first one the
-// workgroup takes; a lane's row sees the keys j with (uint32_t)(j - jlo) <= span
-// (no row: none).
-struct RowsOfLane {
+// A lane's row. Keys are counted from the first one the workgroup takes; the row sees the
+// keys j with (uint32_t)(j - jlo) <= span (jlo = kNoKeys, span = 0: none).
+constexpr uint32_t kNoKeys = 0x80000000u;
+struct RowOfLane {
     uint32_t jlo, span;
     const uint8_t* q;  // the row's first byte (some row's, for a lane that has none)
-    uint64_t out;      // element offset of the row in `out`
-    bool live;
+    bool live;         // the lane has a row
 };
 
-// One workgroup: its rows over n_keys keys. Source: where key tiles come from,
-//   rsrc_t tile(const void* base, t, i): descriptor of DMA instruction i of tile t
-//     (its lanes' keys past the request, or on no page, read as zero), and
-//   uint32_t voffset(r, chunk): byte offset of chunk of the tile's key r in it, and
+// One workgroup: its rows over n_keys keys, into `out`, or, where part is given, as a part
+// to be joined with others: O[32 NW][D] f32, then m, then l (l = -1: the row sees no key of
+// the part). lo_max, hi_min: over the wave's rows, the last key that comes before one and
+// the first that comes behind one, less 1. Source: where keys come from,
+//   uint32_t stage(t, n): tiles [t, its result) of n are made ready; kStages: a barrier and
+//     staged() come before the first is asked for;
+//   uint32_t page(t): of the wave's keys of tile t (read where lgkmcnt(0) is waited for);
+//   rsrc_t tile(base, t, page): the wave's keys of tile t; keys past n_keys, on no page or of
+//     no tile that is staged read as zero, or as whatever LDS held;
+//   uint32_t voffset(r, chunk): byte offset of a chunk of the tile's key r in it;
+//   bool holes(): some staged page is none; uint32_t groups(t): bit i: the keys 16 i .. of
+//     tile t have a page;
 //   const uint8_t* row(base, j): key j < n_keys's row (null: on no page).
-template <uint32_t T, uint32_t D, uint32_t NW, typename Source>
-__device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, const Source& src, uint32_t n_keys,
-                                          const RowsOfLane& row, uint32_t lo_max, uint32_t hi_min) {
+// out_at(): element offset of the lane's row in `out`.
+template <uint32_t T, uint32_t D, uint32_t NW, typename Source, typename OutAt>
+__device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, Source& src, uint32_t n_keys,
+                                          const RowOfLane& row, uint32_t lo_max, int hi_min, float* part,
+                                          const OutAt& out_at) {
     constexpr uint32_t ROW = D * 2u, TILE = tile_bytes<D>();
     constexpr int NF = D / 8;                       // K fragments of a tile, and V fragments
     constexpr int CH = D / 32;                      // 32-dim blocks of a row
@@ -166,7 +175,7 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, co
 
     if (tid == 0) {
         wave_lohi[0] = 0;
-        wave_lohi[1] = 0xffffffffu;
+        wave_lohi[1] = 0x7fffffffu;
         *any_bad = 0;
     }
 
@@ -179,12 +188,12 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, co
         kvo[i] = src.voffset(r, p ^ kswz<D>(r));
         vvo[i] = src.voffset(r, p ^ vswz<D>(r));
     }
-    auto dma = [&](const void* base, const uint32_t (&vo)[DI], uint32_t t, uint32_t slot) {
+    auto dma = [&](const void* base, const uint32_t (&vo)[DI], uint32_t t, uint32_t page, uint32_t slot) {
+        const rsrc_t r = src.tile(base, t, page);
         uint8_t* dst = lds + slot * TILE + wave * (DI * 1024u);
 #pragma unroll
         for (int i = 0; i < (int)DI; i++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(src.tile(base, t, wave * DI + i), (lds_void*)(dst + 1024u * i), 16,
-                                                     vo[i], 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(dst + 1024u * i), 16, vo[i], 0, 0, 0);
     };
 
     // K fragment: keys 32 kb + l32, chunk 4 ch + 2 kh + st. V^T fragment (transposing
@@ -240,8 +249,9 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, co
 
     const uint32_t n_tiles = (n_keys + kKeys - 1u) / kKeys;
     // tiles [full0, full1) are seen whole by every row of the wave
-    const uint32_t full0 = (lo_max + kKeys - 1u) / kKeys, full1 = (hi_min + 1u) / kKeys;
-    auto masked = [&](uint32_t t) { return t < full0 || t >= full1; };
+    const uint32_t full0 = (lo_max + kKeys - 1u) / kKeys, full1 = (uint32_t)(hi_min + 1) / kKeys;
+    auto masked = [&](uint32_t t) { return t < full0 || t >= full1 || src.holes(); };
+    bool sees = false;  // a key
 
     // scores of the keys a row does not see to -inf
     auto mask = [&](f32x16& h0, f32x16& h1, uint32_t t) {
@@ -251,6 +261,17 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, co
             const uint32_t k = rel + 8u * (i >> 2) + (i & 3);
             h0[i] = k <= row.span ? h0[i] : -INFINITY;
             h1[i] = k + 32u <= row.span ? h1[i] : -INFINITY;
+        }
+        if (src.holes()) {
+            const uint32_t on = src.groups(t);
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const uint32_t k = rel + 8u * (i >> 2) + (i & 3);
+                const bool p0 = (on >> (i >> 3)) & 1u, p1 = (on >> (2 + (i >> 3))) & 1u;
+                h0[i] = p0 ? h0[i] : -INFINITY;
+                h1[i] = p1 ? h1[i] : -INFINITY;
+                sees = sees || (p0 && k <= row.span) || (p1 && k + 32u <= row.span);
+            }
         }
     };
     auto rescale = [&](uint64_t grow, float mx, f32x16& n0, f32x16& n1) {
@@ -284,7 +305,7 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, co
     // in LDS before anyone reads it; the rows that do see them, with a weight above 0, get
     // them from memory after the last tile.
     uint32_t wg_full0 = 0, wg_full1 = 0;
-    auto wg_masked = [&](uint32_t t) { return t < wg_full0 || t >= wg_full1; };
+    auto wg_masked = [&](uint32_t t) { return t < wg_full0 || t >= wg_full1 || src.holes(); };
     auto clean_v = [&](uint32_t t, uint32_t slot) {
         uint8_t* const vt = lds + (4u + slot) * TILE;
 #pragma unroll
@@ -332,46 +353,11 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, co
         }
     };
 
-    // prologue: K(0) V(0) K(1) K(2) V(1) K(3) in flight; S(0) and its maximum
-    dma(a.k, kvo, 0, 0);
-    dma(a.v, vvo, 0, 4);
-    dma(a.k, kvo, 1, 1);
-    dma(a.k, kvo, 2, 2);
-    dma(a.v, vvo, 1, 5);
-    dma(a.k, kvo, 3, 3);
-    LLMR_STAGE_BARRIER(5 * DI);  // K(0) has landed
-    if (lane == 0) {
-        atomicMax(&wave_lohi[0], lo_max);
-        atomicMin(&wave_lohi[1], hi_min);
-    }
-    f32x16 h0, h1, h2;
-    {
-        uint32_t ka[CH][2];
-        kaddr(0, ka);
-        static_for<0, NF>([&](auto F) {
-            constexpr int f = F, kb = f / (NF / 2), k = f % (NF / 2);
-            f32x16& s = kb == 0 ? h0 : h1;
-            s = mfma32<T>(kfrag(ka, f), qf[k / 2][k % 2], k == 0 ? f32x16{} : s);
-        });
-        if (masked(0)) mask(h0, h1, 0);
-        float m = h0[0];
-#pragma unroll
-        for (int i = 0; i < 16; i++) m = fmaxf(fmaxf(m, h0[i]), h1[i]);
-        m = xhalf_max(m);
-        seen = __builtin_amdgcn_ballot_w64(m > -INFINITY);
-        m_ref = m > -INFINITY ? m : 0.0f;
-        h0 -= m_ref;
-        h1 -= m_ref;
-    }
-    LLMR_STAGE_BARRIER(2 * DI);  // K(1), K(2), V(0) have landed; every wave is done with K(0)
-    wg_full0 = (__builtin_amdgcn_readfirstlane(wave_lohi[0]) + kKeys - 1u) / kKeys;
-    wg_full1 = (__builtin_amdgcn_readfirstlane(wave_lohi[1]) + 1u) / kKeys;
-
     constexpr int PF = 3;  // fragments in flight ahead of their MFMAs
     uint32_t ka[CH][2];    // K(t+1)'s fragment addresses
     s16x8 kf[PF + 1];      // its fragments in flight: the first PF are read before the tile starts
-    kaddr(1, ka);
-    static_for<0, PF>([&](auto F) { kf[F] = kfrag(ka, F); });
+    f32x16 h0, h1, h2;
+    uint32_t p2 = 0, p3 = 0, p4 = 0;  // pages of the wave's keys of tiles t + 2 .. t + 4
 
     // One tile t: S(t) in (c0, c1), S(t+1) = K(t+1) Q^T to (n0, c0). K(t+1) is in K slot
     // (t+1) % 4, V(t) in V slot vs; K(t+4) is DMAed to K slot t % 4 and V(t+2) to V slot vd.
@@ -380,8 +366,9 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, co
     // half by the time its accumulation starts, the maximum of S(t+1) under the first
     // accumulations, the first fragment reads of K(t+2) under the last ones.
     auto tile = [&](f32x16& c0, f32x16& c1, f32x16& n0, uint32_t t, uint32_t vs, uint32_t vd) {
-        dma(a.k, kvo, t + 4u, t & 3u);
-        dma(a.v, vvo, t + 2u, 4u + vd);
+        dma(a.k, kvo, t + 4u, p4, t & 3u);
+        dma(a.v, vvo, t + 2u, p2, 4u + vd);
+        const uint32_t p5 = src.page(t + 5u);
         if (wg_masked(t)) clean_v(t, vs);
         const bool mask_next = masked(t + 1u);
         uint32_t va[CH], p[16];
@@ -433,6 +420,9 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, co
         rescale(grow, mx, n0, c0);
         seen |= any;
         LLMR_STAGE_BARRIER(2 * DI);
+        p2 = p3;
+        p3 = p4;
+        p4 = (uint32_t)__builtin_amdgcn_readfirstlane(p5);
     };
 
     // V(t) is in V slot t % 3; the score halves rotate with period 3: S(t) in (h0, h1),
@@ -444,46 +434,121 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, co
         t++;
         r0 = r1;
     };
-    while (t + 4u <= n_tiles) {
-        step(h0, h1, h2);
-        step(h2, h0, h1);
-        step(h1, h2, h0);
+    for (bool first = true; t < n_tiles; first = false) {
+        // (the ring's slots go on by t: a source stages a multiple of 12 tiles, or the rest)
+        const uint32_t seg = src.stage(t, n_tiles);
+        if constexpr (Source::kStages) {
+            __syncthreads();
+            src.staged();
+        }
+        if (!src.holes()) sees = sees || (row.jlo != kNoKeys && row.jlo + row.span >= t * kKeys);
+        {   // K(t) V(t) K(t+1) K(t+2) V(t+1) K(t+3) in flight
+            uint32_t pg[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; i++) pg[i] = (uint32_t)__builtin_amdgcn_readfirstlane(src.page(t + i));
+            dma(a.k, kvo, t, pg[0], 0);
+            dma(a.v, vvo, t, pg[0], 4);
+            dma(a.k, kvo, t + 1u, pg[1], 1);
+            dma(a.k, kvo, t + 2u, pg[2], 2);
+            dma(a.v, vvo, t + 1u, pg[1], 5);
+            dma(a.k, kvo, t + 3u, pg[3], 3);
+            p2 = pg[2];
+            p3 = pg[3];
+            p4 = (uint32_t)__builtin_amdgcn_readfirstlane(src.page(t + 4u));
+        }
+        LLMR_STAGE_BARRIER(5 * DI);  // K(t) has landed
+        if (first && lane == 0) {
+            atomicMax(&wave_lohi[0], lo_max);
+            atomicMin((int*)&wave_lohi[1], hi_min);
+        }
+        {   // S(t) and its maximum
+            kaddr(0, ka);
+            static_for<0, NF>([&](auto F) {
+                constexpr int f = F, kb = f / (NF / 2), k = f % (NF / 2);
+                f32x16& s = kb == 0 ? h0 : h1;
+                s = mfma32<T>(kfrag(ka, f), qf[k / 2][k % 2], k == 0 ? f32x16{} - m_ref : s);
+            });
+            if (masked(t)) mask(h0, h1, t);
+            float mx = h0[0];
+#pragma unroll
+            for (int i = 0; i < 16; i++) mx = fmaxf(fmaxf(mx, h0[i]), h1[i]);
+            mx = xhalf_max(mx);
+            const uint64_t any = __builtin_amdgcn_ballot_w64(mx > -INFINITY);
+            rescale(__builtin_amdgcn_ballot_w64(mx > grow_by) | (any & ~seen), mx, h0, h1);
+            seen |= any;
+        }
+        LLMR_STAGE_BARRIER(2 * DI);  // K(t+1), K(t+2), V(t) have landed; every wave is done with K(t)
+        if (first) {
+            wg_full0 = ((uint32_t)__builtin_amdgcn_readfirstlane(wave_lohi[0]) + kKeys - 1u) / kKeys;
+            wg_full1 = ((uint32_t)__builtin_amdgcn_readfirstlane(wave_lohi[1]) + 1u) / kKeys;
+        }
+        kaddr(1, ka);
+        static_for<0, PF>([&](auto F) { kf[F] = kfrag(ka, F); });
+        r0 = 0;
+        while (t + 4u <= seg) {
+            step(h0, h1, h2);
+            step(h2, h0, h1);
+            step(h1, h2, h0);
+        }
+        while (t + 1u < seg) {
+            step(h0, h1, h2);
+            h1 = h0;
+            h0 = h2;
+        }
+        {   // the last staged tile: its scores are in (h0, h1), its V in slot r0
+            uint32_t va[CH], p[16];
+            if (wg_masked(t)) clean_v(t, r0);
+            float rs = 0.0f;
+            static_for<0, 8>([&](auto I) { exp_pair(h0, I, p, rs); });
+            static_for<8, 16>([&](auto I) { exp_pair(h1, I, p, rs); });
+            l_i += rs;
+            vaddr(r0, va);
+            static_for<0, NF>([&](auto F) {
+                constexpr int f = F, kb = f / (NF / 2), cc = (f % (NF / 2)) / CH, dt = f % CH;
+                o[dt] = mfma32<T>(vfrag(va, f), pfrag(p, kb, cc), o[dt]);
+            });
+            t++;
+        }
+        LLMR_WAIT_VMCNT(0);  // no DMA may still be writing LDS when something else goes there
+        __syncthreads();
     }
-    while (t + 1u < n_tiles) {
-        step(h0, h1, h2);
-        h1 = h0;
-        h0 = h2;
-    }
-    {   // last tile: S(n-1) is in (h0, h1), V(n-1) in V slot r0
-        uint32_t va[CH], p[16];
-        if (wg_masked(t)) clean_v(t, r0);
-        float rs = 0.0f;
-        static_for<0, 8>([&](auto I) { exp_pair(h0, I, p, rs); });
-        static_for<8, 16>([&](auto I) { exp_pair(h1, I, p, rs); });
-        l_i += rs;
-        vaddr(r0, va);
-        static_for<0, NF>([&](auto F) {
-            constexpr int f = F, kb = f / (NF / 2), cc = (f % (NF / 2)) / CH, dt = f % CH;
-            o[dt] = mfma32<T>(vfrag(va, f), pfrag(p, kb, cc), o[dt]);
-        });
-    }
-    LLMR_WAIT_VMCNT(0);  // no DMA may still be writing LDS when the rows are staged in it
-    __syncthreads();
-    if (__builtin_amdgcn_readfirstlane(*any_bad) != 0)
+    if (n_tiles != 0 && __builtin_amdgcn_readfirstlane(*any_bad) != 0)
         for (t = 0; t < n_tiles; t++)
             if (wg_masked(t)) add_bad(t);
+
+    const float l_sum = xhalf_sum(l_i);
+    sees = sees || __shfl_xor((int)sees, 32, 64);
+    if (part != nullptr) {
+        float* const po = part + (size_t)(wave * 32u + l32) * D;
+        if (row.live) {
+#pragma unroll
+            for (int dt = 0; dt < CH; dt++)
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+                    *(f32x4*)(po + 32 * dt + 8 * g + 4u * kh) =
+                        f32x4{o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
+            if (kh == 0) {
+                float* const pm = part + 32u * NW * D + wave * 32u + l32;
+                pm[0] = (seen >> lane) & 1u ? m_ref : -INFINITY;
+                pm[32u * NW] = sees ? l_sum : -1.0f;
+            }
+        }
+        return;
+    }
 
     // O = O^T / l through LDS, so that a store writes whole rows: lane l32 holds the dims
     // 32 dt + 8 g + 4 kh .. + 3 of its row; row r's chunk q lies at q ^ (r % CPR)
     uint8_t* const ot = lds + wave * (32u * ROW);
-    const float inv_l = 1.0f / xhalf_sum(l_i);
+    const float inv_l = 1.0f / l_sum;
 #pragma unroll
     for (int dt = 0; dt < CH; dt++)
 #pragma unroll
-        for (int g = 0; g < 4; g++)
-            *(u32x2*)(ot + l32 * ROW + (((4u * dt + g) ^ (l32 % CPR)) << 4) + 8u * kh) =
-                u32x2{pack2<T>(o[dt][4 * g] * inv_l, o[dt][4 * g + 1] * inv_l),
-                      pack2<T>(o[dt][4 * g + 2] * inv_l, o[dt][4 * g + 3] * inv_l)};
+        for (int g = 0; g < 4; g++) {
+            const u32x2 w{pack2<T>(o[dt][4 * g] * inv_l, o[dt][4 * g + 1] * inv_l),
+                          pack2<T>(o[dt][4 * g + 2] * inv_l, o[dt][4 * g + 3] * inv_l)};
+            *(u32x2*)(ot + l32 * ROW + (((4u * dt + g) ^ (l32 % CPR)) << 4) + 8u * kh) = sees ? w : u32x2{0u, 0u};
+        }
+    const uint64_t my_out = out_at();
     // the wave reads back only what it wrote: its LDS operations run in order
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -492,8 +557,8 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, co
     for (uint32_t i = 0; i < 32u / RPI; i++) {
         const uint32_t r = RPI * i + lane / CPR, q = lane % CPR;
         const u32x4 v = *(const u32x4*)(ot + r * ROW + ((q ^ (r % CPR)) << 4));
-        const uint64_t at = ((uint64_t)(uint32_t)__shfl((int)(row.out >> 32), (int)r, 64) << 32) |
-                            (uint32_t)__shfl((int)(uint32_t)row.out, (int)r, 64);
+        const uint64_t at = ((uint64_t)(uint32_t)__shfl((int)(my_out >> 32), (int)r, 64) << 32) |
+                            (uint32_t)__shfl((int)(uint32_t)my_out, (int)r, 64);
         if (__shfl((int)row.live, (int)r, 64)) *(u32x4*)((uint16_t*)a.out + at + 8u * q) = v;
     }
 }
