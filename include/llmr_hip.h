@@ -577,7 +577,7 @@ typedef struct llmr_prompt_attention_params {
     uint32_t n_tokens;       /* rows of q, k, v and out */
     uint32_t n_seqs;
     uint32_t q_stride;       /* elements from one token to the next, and from one */
-    uint32_t q_head_stride;  /* head to the next: multiples of 8, so that rows */
+    uint32_t q_head_stride;  /* head to the next: multiples of 8 (tokens: <= 2^23), so that rows */
     uint32_t kv_stride;      /* [n_tokens, heads, head_dim], columns of a wider */
     uint32_t kv_head_stride; /* row and [heads, n_tokens, head_dim] are all taken */
     uint32_t out_stride;     /* elements from one row of out to the next, a multiple of 8 */

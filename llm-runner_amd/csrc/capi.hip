@@ -1041,11 +1041,18 @@ int check_ints(const void* p, const char* what) {
     return LLMR_OK;
 }
 
-// Rows of 16-bit elements read or written in 16-byte vectors.
+// Rows of 16-bit elements read or written in 16-byte vectors, 64 of them at 32-bit offsets.
 int check_stride8(uint32_t stride, uint64_t width, const char* what) {
-    if (stride % 8 || stride < width)
-        return fail(LLMR_ERR_INVALID_ARG, "%s must be a multiple of 8 and >= %llu (got %u)", what,
+    if (stride % 8 || stride < width || stride > (1u << 23))
+        return fail(LLMR_ERR_INVALID_ARG, "%s must be a multiple of 8, >= %llu and <= 2^23 (got %u)", what,
                     (unsigned long long)width, stride);
+    return LLMR_OK;
+}
+
+// A head's distance: only ever in 64-bit offsets.
+int check_head_stride(uint32_t stride, uint32_t head_dim, const char* what) {
+    if (stride % 8 || stride < head_dim)
+        return fail(LLMR_ERR_INVALID_ARG, "%s must be a multiple of 8 and >= %u (got %u)", what, head_dim, stride);
     return LLMR_OK;
 }
 
@@ -1104,9 +1111,9 @@ int llmr_prompt_attention(llmr_context* ctx, const void* q, const void* k, const
     if (int r = check_16(out, "out")) return r;
     if (int r = check_ints(seq_offsets, "seq_offsets")) return r;
     if (int r = check_stride8(p->q_stride, p->head_dim, "q_stride")) return r;
-    if (int r = check_stride8(p->q_head_stride, p->head_dim, "q_head_stride")) return r;
+    if (int r = check_head_stride(p->q_head_stride, p->head_dim, "q_head_stride")) return r;
     if (int r = check_stride8(p->kv_stride, p->head_dim, "kv_stride")) return r;
-    if (int r = check_stride8(p->kv_head_stride, p->head_dim, "kv_head_stride")) return r;
+    if (int r = check_head_stride(p->kv_head_stride, p->head_dim, "kv_head_stride")) return r;
     if (int r = check_stride8(p->out_stride, (uint64_t)p->n_heads * p->head_dim, "out_stride")) return r;
     if ((uint64_t)p->n_tokens * p->n_heads > 0x7fffffffull)
         return fail(LLMR_ERR_INVALID_ARG, "n_tokens * n_heads must be < 2^31");

@@ -177,50 +177,39 @@ __device__ __forceinline__ uint64_t request_tiles(const SeqAttnArgs& a, const Pa
     for (uint32_t b = 0; b < blocks_of(rq, G); b++) n += block_tiles(a, rq, G, b);
     return n;
 }
-// Tiles before request `upto` (of one key/value head), by one wave.
-__device__ __forceinline__ uint64_t tiles_before(const SeqAttnArgs& a, uint32_t G, uint32_t upto, uint32_t lane) {
-    uint64_t sum = 0;
-    for (uint32_t s = lane; s < upto; s += 64u) sum += request_tiles(a, seqattn::paged_request(a, s), G);
-    return seqattn::uniform64(seqattn::shfl64(seqattn::wave_scan(sum, lane), 63));
-}
-
 template <uint32_t D>
 constexpr size_t tile_part_floats() { return kBlockRows * (D + 2u); }
 
 // Attention over a paged cache for requests of any number of new tokens: the tiles of all
 // (request, key/value head, block of 256 rows) make one line that the workgroups, one a CU,
 // share evenly, as paged_attn_few's waves do; parts of a block that several workgroups take
-// go to scratch, at most two a workgroup, and paged_attn_tiles_join joins them.
+// go to scratch, at most two a workgroup, and paged_attn_join joins them.
 template <uint32_t T, uint32_t D>
-__device__ __forceinline__ void paged_tiles(const SeqAttnArgs& a, uint8_t* lds, float* __restrict__ scratch) {
+__device__ __forceinline__ void paged_tiles(const SeqAttnArgs& a, uint8_t* lds, seqattn::JoinRecord* __restrict__ records,
+                                            float* __restrict__ scratch) {
     constexpr uint32_t NW = 8, ROW = D * 2u;
     const uint32_t tid = threadIdx.x, lane = tid & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t G = a.n_heads / a.n_kv_heads;
     uint32_t* const pages = (uint32_t*)(lds + seqattn::lds_bytes<D>());
 
-    const uint64_t w = tiles_before(a, G, a.n_seqs, lane) * a.n_kv_heads;
+    const auto cost = [&](const PagedRequest& r) { return request_tiles(a, r, G); };
+    seqattn::RequestWindow win;
+    const uint64_t w = seqattn::batch_cost(a, win, lane, cost) * a.n_kv_heads;
     const uint32_t n = (uint32_t)min((uint64_t)gridDim.x, w);  // every workgroup has a tile
-    if (blockIdx.x >= n) return;
+    seqattn::JoinRecord rec{};
+    if (blockIdx.x >= n) {
+        if (tid == 0) records[blockIdx.x].last = 0;
+        return;
+    }
     uint64_t at = seqattn::part_begin(blockIdx.x, w, n);
     const uint64_t end = seqattn::part_begin(blockIdx.x + 1u, w, n);
-    uint32_t s = 0;     // the last request whose tiles begin at or before `at`
-    uint64_t base = 0;  // tiles (all heads) before it
-    for (uint32_t s0 = 0; s0 < a.n_seqs; s0 += 64u) {
-        const uint64_t u = s0 + lane < a.n_seqs ? request_tiles(a, seqattn::paged_request(a, s0 + lane), G) * a.n_kv_heads : 0;
-        const uint64_t inc = seqattn::wave_scan(u, lane);
-        const uint64_t here = __builtin_amdgcn_ballot_w64(base + inc > at);
-        if (here != 0) {
-            const int l = __builtin_ctzll(here);
-            s = s0 + (uint32_t)l;
-            base += seqattn::uniform64(seqattn::shfl64(inc - u, l));
-            break;
-        }
-        base += seqattn::uniform64(seqattn::shfl64(inc, 63));
-    }
+    uint64_t base;  // tiles (all heads) before request s
+    uint32_t s = seqattn::find_request(a, win, lane, cost, a.n_kv_heads, at, base);
 
     while (at < end) {
-        const PagedRequest rq = seqattn::paged_request(a, s);
+        if (s - win.s0 >= 64u) win.load(a, s, lane);
+        const PagedRequest rq = win.get(s);
         const uint64_t per_head = request_tiles(a, rq, G), all = per_head * a.n_kv_heads;
         if (all == 0 || at >= base + all) {
             base += all;
@@ -264,58 +253,18 @@ __device__ __forceinline__ void paged_tiles(const SeqAttnArgs& a, uint8_t* lds, 
                                 : scratch + (2u * blockIdx.x + (t0 == 0 ? 1u : 0u)) * tile_part_floats<D>();
         seqattn::tile_rows<T, D, NW>(a, lds, src, n_keys, row, 0u, hi_min, part, out_at);
         at += t1 - t0;
+        if (t0 == 0 && t1 != tiles)  // (the workgroup's last part: the record is its one)
+            rec = seqattn::JoinRecord{seqattn::part_of(at + (tiles - t1) - 1u, w, n), rq.first, row0,
+                                      min(rows - row0, kBlockRows), kvh, {}};
     }
+    if (tid == 0) records[blockIdx.x] = rec;
 }
 
 template <uint32_t T, uint32_t D>
-__global__ void __launch_bounds__(512, 1) paged_attn_tiles(SeqAttnArgs a, float* __restrict__ scratch) {
+__global__ void __launch_bounds__(512, 1)
+paged_attn_tiles(SeqAttnArgs a, seqattn::JoinRecord* __restrict__ records, float* __restrict__ parts) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[seqattn::lds_bytes<D>() + 4u * (kPageCap + 4u)];
-    paged_tiles<T, D>(a, lds, scratch);
-}
-
-// Joins the parts of a row block that more than one workgroup took, in their order, 32 rows a
-// workgroup. n_wgs: the grid of paged_attn_tiles.
-template <uint32_t T, uint32_t D>
-__global__ void __launch_bounds__(256) paged_attn_tiles_join(SeqAttnArgs a, const float* __restrict__ scratch,
-                                                             uint32_t n_wgs) {
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, kvh = blockIdx.y, row0 = 32u * blockIdx.z;
-    const uint32_t G = a.n_heads / a.n_kv_heads;
-    // the blockIdx.x-th row block of the batch
-    uint32_t s = a.n_seqs, b = 0;
-    uint64_t before = 0;
-    for (uint32_t s0 = 0; s0 < a.n_seqs; s0 += 64u) {
-        const uint64_t u = s0 + lane < a.n_seqs ? blocks_of(seqattn::paged_request(a, s0 + lane), G) : 0;
-        const uint64_t inc = seqattn::wave_scan(u, lane);
-        const uint64_t here = __builtin_amdgcn_ballot_w64(before + inc > blockIdx.x);
-        if (here != 0) {
-            const int l = __builtin_ctzll(here);
-            s = s0 + (uint32_t)l;
-            b = blockIdx.x - (uint32_t)(before + seqattn::uniform64(seqattn::shfl64(inc - u, l)));
-            break;
-        }
-        before += seqattn::uniform64(seqattn::shfl64(inc, 63));
-    }
-    if (s == a.n_seqs) return;
-    const PagedRequest rq = seqattn::paged_request(a, s);
-    const uint32_t tiles = block_tiles(a, rq, G, b), rows = min(rq.rows * G - b * kBlockRows, kBlockRows);
-    if (tiles <= 1u || row0 >= rows) return;
-    const uint64_t w = tiles_before(a, G, a.n_seqs, lane) * a.n_kv_heads;
-    uint64_t begin = tiles_before(a, G, s, lane) * a.n_kv_heads + kvh * request_tiles(a, rq, G);
-    for (uint32_t i = 0; i < b; i++) begin += block_tiles(a, rq, G, i);
-    const uint32_t n = (uint32_t)min((uint64_t)n_wgs, w);
-    const uint32_t g0 = seqattn::part_of(begin, w, n), g1 = seqattn::part_of(begin + tiles - 1u, w, n);
-    if (g0 == g1) return;
-    for (uint32_t e = tid; e < 32u * (D / 4u); e += 256u) {
-        const uint32_t x = row0 + e / (D / 4u), d = 4u * (e % (D / 4u));
-        if (x >= rows) break;
-        f32x4 v;
-        const bool sees = seqattn::join_row(
-            g0, g1, a.scale_log2,
-            [&](uint32_t g) { return scratch + (2u * g + (g == g0 ? 1u : 0u)) * tile_part_floats<D>(); }, kBlockRows, D, x, d, v);
-        const uint32_t r = b * kBlockRows + x;
-        uint16_t* const dst = (uint16_t*)a.out + (size_t)(rq.first + r / G) * a.out_stride + (kvh * G + r % G) * D + d;
-        *(u32x2*)dst = sees ? u32x2{seqattn::pack2<T>(v.x, v.y), seqattn::pack2<T>(v.z, v.w)} : u32x2{0u, 0u};
-    }
+    paged_tiles<T, D>(a, lds, records, parts);
 }
 
 }  // namespace
@@ -331,55 +280,45 @@ static uint32_t few_blocks(uint32_t n_heads, uint32_t n_kv_heads, uint32_t max_n
     const uint64_t rows = (uint64_t)max_new * (n_heads / n_kv_heads);
     return rows <= 16u ? 1u : rows <= 32u ? 2u : rows <= 64u ? 4u : 0u;
 }
-constexpr uint32_t kFewPerCu = 4;  // waves a CU: their rings fill its LDS
-
-template <uint32_t T, uint32_t D>
-static hipError_t launch_paged_tiles(const SeqAttnArgs& a, int num_cus, float* scratch, hipStream_t st) {
-    const uint32_t n = (uint32_t)num_cus, G = a.n_heads / a.n_kv_heads;
-    hipLaunchKernelGGL((paged_attn_tiles<T, D>), dim3(n), dim3(512), 0, st, a, scratch);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    // row blocks there can be: a request of r rows has (r + 255) / 256, and r > 0
-    const uint64_t rows = (uint64_t)a.n_tokens * G, full = rows / kBlockRows;
-    const uint32_t blocks = (uint32_t)(full + (a.n_seqs < rows ? a.n_seqs : rows));
-    hipLaunchKernelGGL((paged_attn_tiles_join<T, D>), dim3(blocks, a.n_kv_heads, kBlockRows / 32u), dim3(256), 0, st, a,
-                       scratch, n);
-    return hipGetLastError();
+// Workers: waves a CU of paged_attn_few, as many as their LDS lets reside, or one workgroup a
+// CU of paged_attn_tiles. Scratch: a record of each, then two parts of each.
+static uint32_t paged_workers(uint32_t nr, int num_cus) {
+    return (uint32_t)num_cus * (nr == 0u ? 1u : nr == 1u ? 4u : nr == 2u ? 3u : 2u);
 }
 
 size_t paged_attention_scratch_bytes(uint32_t dim, uint32_t n_heads, uint32_t n_kv_heads, uint32_t max_new, int num_cus) {
     const uint32_t nr = few_blocks(n_heads, n_kv_heads, max_new);
-    if (nr == 0) return (size_t)2u * num_cus * kBlockRows * (dim + 2u) * sizeof(float);
-    return (size_t)2u * kFewPerCu * num_cus * 16u * nr * (dim + 2u) * sizeof(float);
+    const size_t part = (nr ? 16u * nr : kBlockRows) * (dim + 2u) * sizeof(float);
+    return paged_workers(nr, num_cus) * (sizeof(seqattn::JoinRecord) + 2u * part);
 }
 
-template <uint32_t T, uint32_t D, uint32_t NR>
-static hipError_t launch_few(const SeqAttnArgs& a, int num_cus, float* scratch, hipStream_t st) {
-    const uint32_t n = kFewPerCu * (uint32_t)num_cus;
-    hipLaunchKernelGGL((seqattn::paged_attn_few<T, D, NR>), dim3(n), dim3(64), 0, st, a, scratch);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((seqattn::paged_attn_join<T, D, NR>), dim3(a.n_seqs, a.n_kv_heads), dim3(256), 0, st, a, scratch, n);
-    return hipGetLastError();
+template <uint32_t T, uint32_t D>
+static hipError_t launch_paged(const SeqAttnArgs& a, uint32_t nr, int num_cus, void* scratch, hipStream_t st) {
+    const uint32_t n = paged_workers(nr, num_cus);
+    auto* const records = (seqattn::JoinRecord*)scratch;
+    auto* const parts = (float*)(records + n);
+    auto go = [&](auto work, uint32_t threads, auto join, uint32_t part_rows) {
+        hipLaunchKernelGGL(work, dim3(n), dim3(threads), 0, st, a, records, parts);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL(join, dim3(n, part_rows / 16u), dim3(256), 0, st, a, records, parts);
+        return hipGetLastError();
+    };
+    using namespace seqattn;
+    if (nr == 0u) return go(paged_attn_tiles<T, D>, 512, paged_attn_join<T, D, kBlockRows>, kBlockRows);
+    if (nr == 1u) return go(paged_attn_few<T, D, 1>, 64, paged_attn_join<T, D, 16>, 16);
+    if (nr == 2u) return go(paged_attn_few<T, D, 2>, 64, paged_attn_join<T, D, 32>, 32);
+    return go(paged_attn_few<T, D, 4>, 64, paged_attn_join<T, D, 64>, 64);
 }
 
 hipError_t launch_paged_attention(const SeqAttnArgs& a, uint32_t type, uint32_t dim, int num_cus, void* scratch,
                                   hipStream_t st) {
     const uint32_t nr = few_blocks(a.n_heads, a.n_kv_heads, a.max_new);
-    float* const p = (float*)scratch;
-    auto go = [&](auto t, auto d) {
-        constexpr uint32_t T = decltype(t)::value, D = decltype(d)::value;
-        return nr == 0u ? launch_paged_tiles<T, D>(a, num_cus, p, st)
-               : nr == 1u ? launch_few<T, D, 1>(a, num_cus, p, st)
-               : nr == 2u ? launch_few<T, D, 2>(a, num_cus, p, st)
-                          : launch_few<T, D, 4>(a, num_cus, p, st);
-    };
-    using BF16 = std::integral_constant<uint32_t, kGgmlBF16>;
-    using F16 = std::integral_constant<uint32_t, kGgmlF16>;
-    using D64 = std::integral_constant<uint32_t, 64>;
-    using D128 = std::integral_constant<uint32_t, 128>;
-    if (type == kGgmlBF16) return dim == 128u ? go(BF16{}, D128{}) : go(BF16{}, D64{});
-    return dim == 128u ? go(F16{}, D128{}) : go(F16{}, D64{});
+    if (type == kGgmlBF16)
+        return dim == 128u ? launch_paged<kGgmlBF16, 128>(a, nr, num_cus, scratch, st)
+                           : launch_paged<kGgmlBF16, 64>(a, nr, num_cus, scratch, st);
+    return dim == 128u ? launch_paged<kGgmlF16, 128>(a, nr, num_cus, scratch, st)
+                       : launch_paged<kGgmlF16, 64>(a, nr, num_cus, scratch, st);
 }
 
 }  // namespace llmr

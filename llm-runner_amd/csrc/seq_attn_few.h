@@ -4,15 +4,17 @@
 // kernel is a stream of the cache's pages; what it has to do is to keep enough
 // of them in flight on every CU whatever the requests' lengths are.
 //
-// One wave a workgroup, four or so a CU, each with a ring of two tiles of 32 keys
-// and values in its own LDS, filled by DMA; no wave waits for another. The keys
-// of all (request, key/value head) pairs, cut into units of 32, make one line of
-// W units; wave g of N <= W takes the units [g W / N, (g + 1) W / N) of it. A pair that one
+// One wave a workgroup, four a CU, each with a ring of two units (32 keys, their
+// values, and where a pair begins its queries) in its own LDS, filled by DMA two
+// units ahead, over the ends of pairs; no wave waits for another. The keys of all
+// (request, key/value head) pairs, cut into units of 32, make one line of W units;
+// wave g of N <= W takes the units [g W / N, (g + 1) W / N) of it. A pair that one
 // wave takes whole is written to `out` by it; the parts of the others go to
 // `scratch` (f32 rows, their maximum and sum), at most two a wave (its first part,
-// where the pair began before it, and its last), and a second launch joins them.
-// So any mix of lengths fills the card to within one unit a wave, the scratch
-// depends on no length, and the order of every sum is fixed.
+// where the pair began before it, and its last), and a second launch joins them,
+// by a record that the wave of a pair's first part leaves. So any mix of lengths
+// fills the card to within one unit a wave, the scratch depends on no length, and
+// the order of every sum is fixed.
 //
 // S^T = K Q^T by 16x16x32 MFMAs (16 keys x 16 rows), O^T += V^T P^T with P^T
 // straight from the score registers: a lane's eight weights of a tile are the keys
@@ -87,13 +89,6 @@ __device__ __forceinline__ uint64_t wave_scan(uint64_t v, uint32_t lane) {
     return v;
 }
 
-// Units before request `upto` (of one key/value head), by one wave.
-__device__ __forceinline__ uint64_t units_before(const SeqAttnArgs& a, uint32_t upto, uint32_t lane) {
-    uint64_t sum = 0;
-    for (uint32_t s = lane; s < upto; s += 64u) sum += units_of(paged_request(a, s));
-    return uniform64(shfl64(wave_scan(sum, lane), 63));
-}
-
 // Wave g of n takes the units [part_begin(g), part_begin(g + 1)) of w; the wave that has
 // unit x. (w < 2^38 units x 1024 heads, n < 2^14.)
 __device__ __forceinline__ uint64_t part_begin(uint64_t g, uint64_t w, uint32_t n) { return g * w / n; }
@@ -101,52 +96,122 @@ __device__ __forceinline__ uint32_t part_of(uint64_t x, uint64_t w, uint32_t n) 
     return (uint32_t)(((x + 1u) * n + w - 1u) / w - 1u);
 }
 
+// What a worker leaves about the rows whose first part it has and not the last (last = 0
+// otherwise): parts of the workers it .. last, of rows `row0` .. + n of a request's rows
+// (token, head in group) that starts at token `first`, of key/value head kvh.
+struct JoinRecord {
+    uint32_t last, first, row0, n, kvh, pad[3];
+};
+
+// The requests of a call, 64 at a time in the lanes of a wave, and the units before them.
+struct RequestWindow {
+    PagedRequest mine;  // request s0 + lane
+    uint32_t s0;
+    __device__ __forceinline__ void load(const SeqAttnArgs& a, uint32_t from, uint32_t lane) {
+        s0 = from;
+        mine = from + lane < a.n_seqs ? paged_request(a, from + lane) : PagedRequest{0, 0, 0, 0};
+    }
+    __device__ __forceinline__ PagedRequest get(uint32_t s) const {
+        const int l = (int)(s - s0);
+        return {(uint32_t)__builtin_amdgcn_readlane((int)mine.first, l), (uint32_t)__builtin_amdgcn_readlane((int)mine.rows, l),
+                __builtin_amdgcn_readlane(mine.pos0, l), (uint32_t)__builtin_amdgcn_readlane((int)mine.keys, l)};
+    }
+};
+
+// The sum of cost(request) over the batch, and the window (loaded where one is not enough)
+// moved to the request of unit x (heads * cost units each): it, and the units before it.
+template <typename Cost>
+__device__ __forceinline__ uint64_t batch_cost(const SeqAttnArgs& a, RequestWindow& win, uint32_t lane, const Cost& cost) {
+    uint64_t sum = 0;
+    for (uint32_t s0 = 0; s0 < a.n_seqs; s0 += 64u) {
+        win.load(a, s0, lane);
+        sum += cost(win.mine);
+    }
+    return uniform64(shfl64(wave_scan(sum, lane), 63));
+}
+template <typename Cost>
+__device__ __forceinline__ uint32_t find_request(const SeqAttnArgs& a, RequestWindow& win, uint32_t lane, const Cost& cost,
+                                                 uint32_t heads, uint64_t x, uint64_t& base) {
+    base = 0;
+    for (uint32_t s0 = 0; s0 < a.n_seqs; s0 += 64u) {
+        if (a.n_seqs > 64u) win.load(a, s0, lane);
+        const uint64_t u = cost(win.mine) * heads, inc = wave_scan(u, lane);
+        const uint64_t here = __builtin_amdgcn_ballot_w64(base + inc > x);
+        if (here != 0) {
+            const int l = __builtin_ctzll(here);
+            base += uniform64(shfl64(inc - u, l));
+            return s0 + (uint32_t)l;
+        }
+        base += uniform64(shfl64(inc, 63));
+    }
+    return a.n_seqs;
+}
+
+// Adds a part's O, m, l to (o, m, l); l = -1: no key seen.
+__device__ __forceinline__ void join_part(f32x4& o, float& m, float& l, f32x4 po, float pm, float pl, float c) {
+    if (pl == -1.0f) return;
+    const float mx = fmaxf(m, pm);
+    // (a part whose scores are all -inf has m = -inf and sums of 0 or NaN)
+    const float fo = l == -1.0f || m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mx) * c);
+    const float fp = pm == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((pm - mx) * c);
+    const bool both = l != -1.0f;
+    o = both ? o * fo + po * fp : po * fp;
+    l = both ? l * fo + pl * fp : pl * fp;
+    m = mx;
+}
+
 // A part of a pair in scratch: O[16 NR][D], then m[16 NR], l[16 NR] (l = -1: the row
-// sees no key of this part).
+// sees no key of this part). The records come first.
 template <uint32_t D, uint32_t NR>
 constexpr uint32_t part_floats() { return 16u * NR * (D + 2u); }
 
+// A unit of 32 keys of a pair.
+struct FewUnit {
+    PagedRequest rq;
+    uint32_t s, kvh, u, units;
+    bool first;  // of this wave's part of the pair: its queries come with it
+};
+
 template <uint32_t T, uint32_t D, uint32_t NR>
-__device__ __forceinline__ void few_rows(const SeqAttnArgs& a, uint8_t* lds, float* __restrict__ scratch) {
+__device__ __forceinline__ void few_rows(const SeqAttnArgs& a, uint8_t* lds, JoinRecord* __restrict__ records,
+                                         float* __restrict__ parts) {
     constexpr uint32_t ROW = D * 2u, RPI = 1024u / ROW, CPR = ROW / 16u;
-    constexpr uint32_t IPG = 16u / RPI;        // DMA instructions per 16 keys
-    constexpr uint32_t TILE = kUnit * ROW;     // bytes of a K or V tile; lds: two of K, two of V
+    constexpr uint32_t IPG = 16u / RPI;        // DMA instructions per 16 rows
+    constexpr uint32_t TILE = kUnit * ROW;     // bytes of a K or V tile; lds: two of K, two of V, two of Q
+    constexpr uint32_t QT = 16u * NR * ROW;    // bytes of Q
     constexpr int DMAS = 4 * (int)IPG;         // per unit: K and V, two groups of 16 keys each
+    constexpr int QI = (int)(NR * IPG);        // and Q
     constexpr int CH = D / 32, DT = D / 16;
     constexpr float OFF = T == kGgmlF16 ? 7.0f : 0.0f;
     const uint32_t lane = threadIdx.x, n16 = lane & 15u, g = lane >> 4;
     const uint32_t G = a.n_heads / a.n_kv_heads;
     const float c = a.scale_log2, grow_by = 8.0f / c;
+    const auto cost = [](const PagedRequest& r) { return (uint64_t)units_of(r); };
 
     // this wave's units
-    const uint64_t w1 = units_before(a, a.n_seqs, lane), w = w1 * a.n_kv_heads;
+    RequestWindow win;
+    const uint64_t w = batch_cost(a, win, lane, cost) * a.n_kv_heads;
     const uint32_t n = (uint32_t)min((uint64_t)gridDim.x, w);  // every wave has a unit
-    if (blockIdx.x >= n) return;
-    uint64_t at = part_begin(blockIdx.x, w, n);
-    const uint64_t end = part_begin(blockIdx.x + 1u, w, n);
-    // the request of unit `at`: the last one whose units begin at or before it
-    uint32_t s = 0;
-    uint64_t base = 0;  // units (all heads) before request s
-    for (uint32_t s0 = 0; s0 < a.n_seqs; s0 += 64u) {
-        const uint64_t u = s0 + lane < a.n_seqs ? (uint64_t)units_of(paged_request(a, s0 + lane)) * a.n_kv_heads : 0;
-        const uint64_t inc = wave_scan(u, lane);
-        const uint64_t here = __builtin_amdgcn_ballot_w64(base + inc > at);
-        if (here != 0) {
-            const int l = __builtin_ctzll(here);
-            s = s0 + (uint32_t)l;
-            base += uniform64(shfl64(inc - u, l));
-            break;
-        }
-        base += uniform64(shfl64(inc, 63));
+    JoinRecord rec{};
+    if (blockIdx.x >= n) {
+        if (lane == 0) records[blockIdx.x].last = 0;
+        return;
     }
+    const uint64_t at = part_begin(blockIdx.x, w, n);
+    uint64_t left = part_begin(blockIdx.x + 1u, w, n) - at;  // units to send for
 
-    // DMA lane offsets within 16 keys; fragment addresses within a tile
-    uint32_t kvo[IPG], vvo[IPG];
+    // DMA lane offsets within 16 rows; fragment addresses within a tile
+    uint32_t kvo[IPG], vvo[IPG], qvo[NR * IPG];
 #pragma unroll
     for (uint32_t i = 0; i < IPG; i++) {
         const uint32_t r = RPI * i + lane / CPR, p = lane % CPR;
         kvo[i] = r * ROW + ((p ^ kswz<D>(r)) << 4);
         vvo[i] = r * ROW + ((p ^ fswz<D>(r)) << 4);
+#pragma unroll
+        for (uint32_t b = 0; b < NR; b++) {  // row x = (token x / G, head of the group x % G)
+            const uint32_t x = 16u * b + r;
+            qvo[b * IPG + i] = (x / G * a.q_stride + x % G * a.q_head_stride) * 2u + ((p ^ kswz<D>(r)) << 4);
+        }
     }
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)lds;
     uint32_t kfo[CH], vto[DT];
@@ -158,201 +223,142 @@ __device__ __forceinline__ void few_rows(const SeqAttnArgs& a, uint8_t* lds, flo
         vto[dt] = lds0 + 2u * TILE + r * ROW + (((2u * dt + ((n16 & 3u) >> 1)) ^ fswz<D>(r)) << 4) + 8u * (n16 & 1u);
     }
 
-    while (at < end) {
-        const PagedRequest rq = paged_request(a, s);
-        const uint32_t units = units_of(rq);
-        if (units == 0 || at >= base + (uint64_t)units * a.n_kv_heads) {  // (nothing new: no units)
-            base += (uint64_t)units * a.n_kv_heads;
-            s++;
-            continue;
+    // 16 keys from key k0 on: their page (negative: none)
+    auto page_at = [&](const FewUnit& x, uint32_t k0) -> int32_t {
+        if (k0 >= x.rq.keys) return -1;
+        const int32_t p = a.table[(size_t)x.s * a.max_pages + (k0 >> a.page_log2)];
+        return p >= 0 && (uint32_t)p < a.n_pages ? p : -1;
+    };
+    auto dma = [&](const FewUnit& x, uint32_t slot) {
+        if (x.first) {
+            // the rows there are end before offset rows * q_stride, the first one there is not
+            const uint32_t bytes = ((x.rq.rows - 1u) * a.q_stride + (G - 1u) * a.q_head_stride + D) * 2u;
+            const rsrc_t qr = __builtin_amdgcn_make_buffer_rsrc(
+                (uint8_t*)const_cast<void*>(a.q) +
+                    2u * ((uint64_t)x.rq.first * a.q_stride + (uint64_t)x.kvh * G * a.q_head_stride),
+                (short)0, (int)__builtin_amdgcn_readfirstlane(bytes), 0x00020000);
+            uint8_t* const qd = lds + 4u * TILE + slot * QT;
+#pragma unroll
+            for (int i = 0; i < QI; i++)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(qr, (lds_void*)(qd + 1024u * i), 16, qvo[i], 0, 0, 0);
         }
-        const uint32_t kvh = (uint32_t)((at - base) / units);
-        const uint32_t u0 = (uint32_t)((at - base) % units);
-        const uint32_t u1 = (uint32_t)min((uint64_t)units, u0 + (end - at));
-        const int32_t* const table = a.table + (size_t)s * a.max_pages;
-
-        // rows: 16 r + n16 = (token i, head of the group)
-        const uint32_t rows = rq.rows * G;
-        s16x8 qf[NR][CH];
-        int32_t hi[NR];  // last key the row sees
-        int32_t hi_min = 0x7fffffff;
 #pragma unroll
-        for (int r = 0; r < (int)NR; r++) {
-            const uint32_t x = 16u * r + n16, xc = min(x, rows - 1u), i = xc / G;
-            hi[r] = x < rows ? rq.pos0 + (int32_t)i : -1;
-            if (x < rows) hi_min = min(hi_min, hi[r]);
-            const uint16_t* q = (const uint16_t*)a.q + (size_t)(rq.first + i) * a.q_stride +
-                                (size_t)(kvh * G + xc % G) * a.q_head_stride;
+        for (uint32_t h = 0; h < 2u; h++) {
+            const uint32_t k0 = x.u * kUnit + 16u * h;
+            const int32_t p = page_at(x, k0);
+            const uint64_t off = ((((uint64_t)(uint32_t)max(p, 0) * a.n_kv_heads + x.kvh) << a.page_log2) +
+                                  (k0 & ((1u << a.page_log2) - 1u))) * ROW;
+            const uint32_t keys = p < 0 ? 0u : min(__builtin_elementwise_sub_sat(x.rq.keys, k0), 16u);
+            const int bytes = (int)__builtin_amdgcn_readfirstlane(keys * ROW);
+            const rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((uint8_t*)const_cast<void*>(a.k) + off, (short)0, bytes,
+                                                                0x00020000);
+            const rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((uint8_t*)const_cast<void*>(a.v) + off, (short)0, bytes,
+                                                                0x00020000);
+            uint8_t* const kd = lds + slot * TILE + h * 16u * ROW;
 #pragma unroll
-            for (int ch = 0; ch < CH; ch++) qf[r][ch] = *(const s16x8*)(q + 32 * ch + 8u * g);
-        }
-        hi_min = wave_imin(hi_min);
-
-        f32x4 o[NR][DT];
-        float m_ref[NR], l_i[NR];
-        uint32_t fresh = (1u << NR) - 1u, sees = 0;  // per row block: no maximum yet; a key seen
-        bool bad = false;                            // a masked tile's V has an infinity or NaN
-#pragma unroll
-        for (int r = 0; r < (int)NR; r++) {
-            m_ref[r] = l_i[r] = 0.0f;
-#pragma unroll
-            for (int dt = 0; dt < DT; dt++) o[r][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        }
-
-        // 16 keys from key k0 on: their page (negative: none)
-        auto page_at = [&](uint32_t k0) -> int32_t {
-            if (k0 >= rq.keys) return -1;
-            const int32_t p = table[k0 >> a.page_log2];
-            return p >= 0 && (uint32_t)p < a.n_pages ? p : -1;
-        };
-        auto dma = [&](uint32_t u, uint32_t slot) {
-#pragma unroll
-            for (uint32_t h = 0; h < 2u; h++) {
-                const uint32_t k0 = u * kUnit + 16u * h;
-                const int32_t p = u < u1 ? page_at(k0) : -1;
-                const uint64_t off = ((((uint64_t)(uint32_t)max(p, 0) * a.n_kv_heads + kvh) << a.page_log2) +
-                                      (k0 & ((1u << a.page_log2) - 1u))) * ROW;
-                const uint32_t left = p < 0 ? 0u : min(__builtin_elementwise_sub_sat(rq.keys, k0), 16u);
-                const int bytes = (int)__builtin_amdgcn_readfirstlane(left * ROW);
-                const rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((uint8_t*)const_cast<void*>(a.k) + off, (short)0,
-                                                                    bytes, 0x00020000);
-                const rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((uint8_t*)const_cast<void*>(a.v) + off, (short)0,
-                                                                    bytes, 0x00020000);
-                uint8_t* const kd = lds + slot * TILE + h * 16u * ROW;
-#pragma unroll
-                for (uint32_t i = 0; i < IPG; i++) {
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_void*)(kd + 1024u * i), 16, kvo[i], 0, 0, 0);
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_void*)(kd + 2u * TILE + 1024u * i), 16, vvo[i], 0,
-                                                             0, 0);
-                }
+            for (uint32_t i = 0; i < IPG; i++) {
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_void*)(kd + 1024u * i), 16, kvo[i], 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_void*)(kd + 2u * TILE + 1024u * i), 16, vvo[i], 0, 0, 0);
             }
-        };
-        // a row's weights of a tile are 0 where it does not see the key, and 0 times an
-        // infinity or NaN is NaN: in masked tiles V's are set to 0, and the rows that do see
-        // them, with a weight above 0, get them from memory after the last tile
-        auto clean_v = [&](uint32_t u, uint32_t slot) {
-#pragma unroll
-            for (uint32_t i = 0; i < TILE / 1024u; i++) {
-                u32x4* const p = (u32x4*)(lds + (2u + slot) * TILE + 1024u * i + 16u * lane);
-                const u32x4 x = *p;
-                const bool nf = nonfinite4<T>(x);
-                if (__builtin_amdgcn_ballot_w64(nf) != 0) {
-                    bad = true;
-                    if (nf) *p = finite4<T>(x);
-                }
+        }
+    };
+    // the unit behind x on the line
+    auto next_of = [&](const FewUnit& x) -> FewUnit {
+        FewUnit y = x;
+        y.u++;
+        y.first = false;
+        if (y.u == y.units) {
+            y.u = 0;
+            y.first = true;
+            if (++y.kvh == a.n_kv_heads) {
+                y.kvh = 0;
+                do {  // (units are left, so there is a request that has some)
+                    y.s++;
+                    if (y.s - win.s0 >= 64u) win.load(a, y.s, lane);
+                    y.rq = win.get(y.s);
+                    y.units = units_of(y.rq);
+                } while (y.units == 0 && y.s + 1u < a.n_seqs);
             }
-        };
+        }
+        return y;
+    };
 
-        dma(u0, 0);
-        dma(u0 + 1u, 1);
-        for (uint32_t u = u0; u < u1; u++) {
-            const uint32_t slot = (u - u0) & 1u;
-            // keys past the last one, on no page, or unseen by a row: masked
-            const bool v0 = page_at(u * kUnit) >= 0, v1 = page_at(u * kUnit + 16u) >= 0;
-            const bool masked = !v0 || !v1 || (int32_t)(u * kUnit + kUnit - 1u) > hi_min;
-            asm volatile("" ::: "memory");
-            LLMR_WAIT_VMCNT(DMAS);  // this unit's K and V have landed
-            asm volatile("" ::: "memory");
-            if (masked) clean_v(u, slot);
-            f32x4 sc[NR][2];
+    FewUnit cur, next{};
+    {
+        uint64_t base;
+        cur.s = find_request(a, win, lane, cost, a.n_kv_heads, at, base);
+        cur.rq = win.get(cur.s);
+        cur.units = units_of(cur.rq);
+        cur.kvh = (uint32_t)((at - base) / cur.units);
+        cur.u = (uint32_t)((at - base) % cur.units);
+        cur.first = true;
+        dma(cur, 0);
+        left--;
+        if (left) {
+            next = next_of(cur);
+            dma(next, 1);
+        }
+    }
+    bool begun = cur.u == 0;  // this wave has the first part of the pair it is at
+
+    s16x8 qf[NR][CH];
+    int32_t hi[NR], hi_min = 0;  // last key the row sees
+    f32x4 o[NR][DT];
+    float m_ref[NR], l_i[NR];
+    uint32_t fresh = 0, sees = 0, u0 = 0;  // per row block: no maximum yet; a key seen; the part's first unit
+    bool bad = false;                      // a masked tile's V has an infinity or NaN
+    // a row's weights of a tile are 0 where it does not see the key, and 0 times an
+    // infinity or NaN is NaN: in masked tiles V's are set to 0, and the rows that do see
+    // them, with a weight above 0, get them from memory after the part's last tile
+    auto clean_v = [&](uint32_t slot) {
 #pragma unroll
-            for (int kb = 0; kb < 2; kb++)
+        for (uint32_t i = 0; i < TILE / 1024u; i++) {
+            u32x4* const p = (u32x4*)(lds + (2u + slot) * TILE + 1024u * i + 16u * lane);
+            const u32x4 x = *p;
+            const bool nf = nonfinite4<T>(x);
+            if (__builtin_amdgcn_ballot_w64(nf) != 0) {
+                bad = true;
+                if (nf) *p = finite4<T>(x);
+            }
+        }
+    };
+    auto add_bad = [&]() {
+        for (uint32_t u = u0; u <= cur.u; u++) {
+            const uint32_t j = u * kUnit + (lane & 31u);
+            const int32_t p = page_at(cur, j & ~15u);
+            if ((int32_t)(u * kUnit + kUnit - 1u) <= hi_min && __builtin_amdgcn_ballot_w64(p < 0) == 0) continue;
+            const uint8_t* const vr =
+                (const uint8_t*)a.v + ((((uint64_t)(uint32_t)max(p, 0) * a.n_kv_heads + cur.kvh) << a.page_log2) +
+                                       (j & ((1u << a.page_log2) - 1u))) * ROW;
+            bool nf = false;
+            if (p >= 0 && j < cur.rq.keys)
+                for (uint32_t b = 0; b < CPR; b++) nf = nf || nonfinite4<T>(*(const u32x4*)(vr + 16u * b));
+            for (uint64_t todo = __builtin_amdgcn_ballot_w64(nf) & 0xffffffffull; todo != 0; todo &= todo - 1u) {
+                const int l = __builtin_ctzll(todo);
+                const uint8_t* const row = (const uint8_t*)uniform64(shfl64((uint64_t)(uintptr_t)vr, l));
+                const int32_t key = (int32_t)(u * kUnit) + l;
 #pragma unroll
-                for (int ch = 0; ch < CH; ch++) {
-                    const s16x8 k = *(const lds_s16x8*)(uintptr_t)(kfo[ch] + slot * TILE + (uint32_t)kb * 16u * ROW);
+                for (int dt = 0; dt < DT; dt++) {
+                    const u32x2 v = *(const u32x2*)(row + 32u * dt + 8u * g);
+                    const float x[4] = {lo_f32<T>(v.x), hi_f32<T>(v.x), lo_f32<T>(v.y), hi_f32<T>(v.y)};
 #pragma unroll
                     for (int r = 0; r < (int)NR; r++)
-                        sc[r][kb] = mfma16<T>(k, qf[r][ch], ch == 0 ? f32x4{} - m_ref[r] : sc[r][kb]);
-                }
-            s16x8 pf[NR];
 #pragma unroll
-            for (int r = 0; r < (int)NR; r++) {
-                if (masked) {
-                    const int32_t k0 = (int32_t)(u * kUnit + 4u * g);
-                    bool any = false;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const bool a0 = v0 && k0 + i <= hi[r], a1 = v1 && k0 + 16 + i <= hi[r];
-                        sc[r][0][i] = a0 ? sc[r][0][i] : -INFINITY;
-                        sc[r][1][i] = a1 ? sc[r][1][i] : -INFINITY;
-                        any = any || a0 || a1;
-                    }
-                    if (any) sees |= 1u << r;
-                } else {
-                    sees |= 1u << r;
-                }
-                float mx = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 4; i++) mx = fmaxf(fmaxf(mx, sc[r][0][i]), sc[r][1][i]);
-                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-                const bool fr = (fresh >> r) & 1u;
-                if (__builtin_amdgcn_ballot_w64(mx > grow_by || (fr && mx > -INFINITY)) != 0) {
-                    const float d = fr ? (mx > -INFINITY ? mx : 0.0f) : fmaxf(mx, 0.0f);
-                    const float alpha = fr ? 0.0f : __builtin_amdgcn_exp2f(-d * c);
-                    m_ref[r] += d;
-                    l_i[r] *= alpha;
-#pragma unroll
-                    for (int dt = 0; dt < DT; dt++) o[r][dt] *= alpha;
-                    sc[r][0] -= d;
-                    sc[r][1] -= d;
-                    if (mx > -INFINITY) fresh &= ~(1u << r);
-                }
-                float p[8];
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    p[i] = __builtin_amdgcn_exp2f(fmaf(sc[r][i >> 2][i & 3], c, OFF));
-                    l_i[r] += p[i];
-                }
-                pf[r] = __builtin_bit_cast(s16x8, u32x4{pack2<T>(p[0], p[1]), pack2<T>(p[2], p[3]), pack2<T>(p[4], p[5]),
-                                                       pack2<T>(p[6], p[7])});
-            }
-#pragma unroll
-            for (int dt = 0; dt < DT; dt++) {
-                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(vto[dt] + slot * TILE));
-                const s16x4 up =
-                    __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(vto[dt] + slot * TILE + 16u * ROW));
-                const s16x8 v = s16x8{lo.x, lo.y, lo.z, lo.w, up.x, up.y, up.z, up.w};
-#pragma unroll
-                for (int r = 0; r < (int)NR; r++) o[r][dt] = mfma16<T>(v, pf[r], o[r][dt]);
-            }
-            // every read of this slot has arrived before its next tile is sent for
-            asm volatile("" ::: "memory");
-            __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));
-            asm volatile("" ::: "memory");
-            dma(u + 2u, slot);
-        }
-        if (bad) {
-            for (uint32_t u = u0; u < u1; u++) {
-                const uint32_t j = u * kUnit + (lane & 31u);
-                const int32_t p = j < rq.keys ? page_at(j & ~15u) : -1;
-                if ((int32_t)(u * kUnit + kUnit - 1u) <= hi_min && __builtin_amdgcn_ballot_w64(p < 0) == 0) continue;
-                const uint8_t* const vr =
-                    (const uint8_t*)a.v + ((((uint64_t)(uint32_t)max(p, 0) * a.n_kv_heads + kvh) << a.page_log2) +
-                                           (j & ((1u << a.page_log2) - 1u))) * ROW;
-                bool nf = false;
-                if (p >= 0)
-                    for (uint32_t b = 0; b < CPR; b++) nf = nf || nonfinite4<T>(*(const u32x4*)(vr + 16u * b));
-                for (uint64_t todo = __builtin_amdgcn_ballot_w64(nf) & 0xffffffffull; todo != 0; todo &= todo - 1u) {
-                    const int l = __builtin_ctzll(todo);
-                    const uint8_t* const row = (const uint8_t*)uniform64(shfl64((uint64_t)(uintptr_t)vr, l));
-                    const int32_t key = (int32_t)(u * kUnit) + l;
-#pragma unroll
-                    for (int dt = 0; dt < DT; dt++) {
-                        const u32x2 v = *(const u32x2*)(row + 32u * dt + 8u * g);
-                        const float x[4] = {lo_f32<T>(v.x), hi_f32<T>(v.x), lo_f32<T>(v.y), hi_f32<T>(v.y)};
-#pragma unroll
-                        for (int r = 0; r < (int)NR; r++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++)
-                                o[r][dt][e] += (int)(key <= hi[r]) & (int)!(fabsf(x[e]) < INFINITY) ? x[e] : 0.0f;
-                    }
+                        for (int e = 0; e < 4; e++)
+                            o[r][dt][e] += (int)(key <= hi[r]) & (int)!(fabsf(x[e]) < INFINITY) ? x[e] : 0.0f;
                 }
             }
         }
-
-        const bool whole = u0 == 0 && u1 == units;
-        float* const part = scratch + (size_t)(2u * blockIdx.x + (u0 == 0 ? 1u : 0u)) * part_floats<D, NR>();
+    };
+    // the part that ends with unit cur
+    auto finish = [&]() {
+        const bool last = cur.u + 1u == cur.units, whole = begun && last;
+        const uint32_t rows = cur.rq.rows * G;
+        float* const part = parts + (size_t)(2u * blockIdx.x + (begun ? 1u : 0u)) * part_floats<D, NR>();
+        if (begun && !last) {  // (the wave's last part: the record is its one)
+            const uint64_t end = part_begin(blockIdx.x + 1u, w, n) + (cur.units - 1u - cur.u);  // of the pair
+            rec = JoinRecord{part_of(end - 1u, w, n), cur.rq.first, 0, rows, cur.kvh, {}};
+        }
 #pragma unroll
         for (int r = 0; r < (int)NR; r++) {
             float l = l_i[r];
@@ -365,8 +371,8 @@ __device__ __forceinline__ void few_rows(const SeqAttnArgs& a, uint8_t* lds, flo
             const uint32_t x = 16u * r + n16;
             if (x >= rows) continue;
             if (whole) {
-                const uint32_t i = x / G;
-                uint16_t* const dst = (uint16_t*)a.out + (size_t)(rq.first + i) * a.out_stride + (kvh * G + x % G) * D + 4u * g;
+                uint16_t* const dst = (uint16_t*)a.out + (size_t)(cur.rq.first + x / G) * a.out_stride +
+                                      (cur.kvh * G + x % G) * D + 4u * g;
                 const float inv = 1.0f / l;
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++) {
@@ -382,68 +388,197 @@ __device__ __forceinline__ void few_rows(const SeqAttnArgs& a, uint8_t* lds, flo
                 }
             }
         }
-        at += u1 - u0;
+    };
+
+    for (uint32_t slot = 0;; slot ^= 1u) {
+        // this unit's data have landed; at most the next one's are on their way
         asm volatile("" ::: "memory");
-        LLMR_WAIT_VMCNT(0);  // the last tiles' DMAs (of no keys) are done with the ring
+        if (left == 0) {
+            LLMR_WAIT_VMCNT(0);
+        } else if (next.first) {
+            LLMR_WAIT_VMCNT(DMAS + QI);
+        } else {
+            LLMR_WAIT_VMCNT(DMAS);
+        }
         asm volatile("" ::: "memory");
+        if (cur.first) {
+            const uint32_t rows = cur.rq.rows * G;
+            u0 = cur.u;
+            fresh = (1u << NR) - 1u;
+            sees = 0;
+            bad = false;
+            hi_min = 0x7fffffff;
+#pragma unroll
+            for (int r = 0; r < (int)NR; r++) {
+                const uint32_t x = 16u * r + n16;
+                hi[r] = x < rows ? cur.rq.pos0 + (int32_t)(x / G) : -1;
+                if (x < rows) hi_min = min(hi_min, hi[r]);
+                m_ref[r] = l_i[r] = 0.0f;
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) o[r][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int ch = 0; ch < CH; ch++)
+                    qf[r][ch] = *(const lds_s16x8*)(uintptr_t)(kfo[ch] + 4u * TILE + slot * QT + (uint32_t)r * 16u * ROW);
+            }
+            // (the first token's rows see least)
+            hi_min = __builtin_amdgcn_readfirstlane(hi_min);
+        }
+        // keys past the last one, on no page, or unseen by a row: masked
+        const bool v0 = page_at(cur, cur.u * kUnit) >= 0, v1 = page_at(cur, cur.u * kUnit + 16u) >= 0;
+        const bool masked = !v0 || !v1 || (int32_t)(cur.u * kUnit + kUnit - 1u) > hi_min;
+        if (masked) clean_v(slot);
+        f32x4 sc[NR][2];
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+            for (int ch = 0; ch < CH; ch++) {
+                const s16x8 k = *(const lds_s16x8*)(uintptr_t)(kfo[ch] + slot * TILE + (uint32_t)kb * 16u * ROW);
+#pragma unroll
+                for (int r = 0; r < (int)NR; r++)
+                    sc[r][kb] = mfma16<T>(k, qf[r][ch], ch == 0 ? f32x4{} - m_ref[r] : sc[r][kb]);
+            }
+        s16x8 pf[NR];
+#pragma unroll
+        for (int r = 0; r < (int)NR; r++) {
+            if (masked) {
+                const int32_t k0 = (int32_t)(cur.u * kUnit + 4u * g);
+                bool any = false;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const bool a0 = v0 && k0 + i <= hi[r], a1 = v1 && k0 + 16 + i <= hi[r];
+                    sc[r][0][i] = a0 ? sc[r][0][i] : -INFINITY;
+                    sc[r][1][i] = a1 ? sc[r][1][i] : -INFINITY;
+                    any = any || a0 || a1;
+                }
+                if (any) sees |= 1u << r;
+            } else {
+                sees |= 1u << r;
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; i++) mx = fmaxf(fmaxf(mx, sc[r][0][i]), sc[r][1][i]);
+            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const bool fr = (fresh >> r) & 1u;
+            if (__builtin_amdgcn_ballot_w64(mx > grow_by || (fr && mx > -INFINITY)) != 0) {
+                const float d = fr ? (mx > -INFINITY ? mx : 0.0f) : fmaxf(mx, 0.0f);
+                const float alpha = fr ? 0.0f : __builtin_amdgcn_exp2f(-d * c);
+                m_ref[r] += d;
+                l_i[r] *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) o[r][dt] *= alpha;
+                sc[r][0] -= d;
+                sc[r][1] -= d;
+                if (mx > -INFINITY) fresh &= ~(1u << r);
+            }
+            float p[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                p[i] = __builtin_amdgcn_exp2f(fmaf(sc[r][i >> 2][i & 3], c, OFF));
+                l_i[r] += p[i];
+            }
+            pf[r] = __builtin_bit_cast(s16x8, u32x4{pack2<T>(p[0], p[1]), pack2<T>(p[2], p[3]), pack2<T>(p[4], p[5]),
+                                                   pack2<T>(p[6], p[7])});
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) {
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(vto[dt] + slot * TILE));
+            const s16x4 up =
+                __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(vto[dt] + slot * TILE + 16u * ROW));
+            const s16x8 v = s16x8{lo.x, lo.y, lo.z, lo.w, up.x, up.y, up.z, up.w};
+#pragma unroll
+            for (int r = 0; r < (int)NR; r++) o[r][dt] = mfma16<T>(v, pf[r], o[r][dt]);
+        }
+        // every read of this slot has arrived before its next unit is sent for
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));
+        asm volatile("" ::: "memory");
+        if (left == 0) break;
+        FewUnit after{};
+        const bool more = --left != 0;
+        if (more) {
+            after = next_of(next);
+            dma(after, slot);
+        }
+        if (next.first) {
+            if (bad) add_bad();
+            finish();
+            begun = true;
+        }
+        cur = next;
+        next = after;
     }
+    if (bad) add_bad();
+    finish();
+    if (lane == 0) records[blockIdx.x] = rec;
 }
 
 template <uint32_t T, uint32_t D, uint32_t NR>
-__global__ void __launch_bounds__(64, 1) paged_attn_few(SeqAttnArgs a, float* __restrict__ scratch) {
-    __shared__ __attribute__((aligned(16))) uint8_t lds[4u * kUnit * D * 2u];
-    few_rows<T, D, NR>(a, lds, scratch);
+__global__ void __launch_bounds__(64, 1)
+paged_attn_few(SeqAttnArgs a, JoinRecord* __restrict__ records, float* __restrict__ parts) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[(4u * kUnit + 32u * NR) * D * 2u];
+    few_rows<T, D, NR>(a, lds, records, parts);
 }
 
-// One row's dims d .. d + 3 of the parts g0 .. g1, in their order, divided by the sum; false:
-// the row sees no key. part(g): O[rows][D], m[rows], l[rows] of part g.
-template <typename Part>
-__device__ __forceinline__ bool join_row(uint32_t g0, uint32_t g1, float c, const Part& part, uint32_t rows, uint32_t D,
-                                         uint32_t x, uint32_t d, f32x4& out) {
-    f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
-    float m = -INFINITY, l = 0.0f;
-    bool sees = false;
-    for (uint32_t g = g0; g <= g1; g++) {
-        const float* const p = part(g);
-        const float pm = p[rows * D + x], pl = p[rows * (D + 1u) + x];
-        const f32x4 po = *(const f32x4*)(p + x * D + d);
-        if (pl == -1.0f) continue;  // no key of this part is seen
-        const float mx = fmaxf(m, pm);
-        // (a part whose scores are all -inf has m = -inf and sums of 0 or NaN)
-        const float fo = !sees || m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mx) * c);
-        const float fp = pm == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((pm - mx) * c);
-        o = o * fo + po * fp;
-        l = l * fo + pl * fp;
-        m = mx;
-        sees = true;
-    }
-    out = o * (1.0f / l);
-    return sees;
-}
-
-// Joins the parts of a (request, key/value head) pair that more than one wave took, in
-// their order. waves: the grid of paged_attn_few.
-template <uint32_t T, uint32_t D, uint32_t NR>
-__global__ void __launch_bounds__(256) paged_attn_join(SeqAttnArgs a, const float* __restrict__ scratch, uint32_t waves) {
-    const uint32_t s = blockIdx.x, kvh = blockIdx.y, tid = threadIdx.x;
-    const uint32_t G = a.n_heads / a.n_kv_heads;
-    const PagedRequest rq = paged_request(a, s);
-    const uint32_t units = units_of(rq);
-    if (units <= 1u) return;
-    const uint64_t w = units_before(a, a.n_seqs, tid & 63u) * a.n_kv_heads;
-    const uint64_t begin = units_before(a, s, tid & 63u) * a.n_kv_heads + (uint64_t)kvh * units;
-    const uint32_t n = (uint32_t)min((uint64_t)waves, w);
-    const uint32_t g0 = part_of(begin, w, n), g1 = part_of(begin + units - 1u, w, n);
-    if (g0 == g1) return;
-    for (uint32_t e = tid; e < rq.rows * G * (D / 4u); e += 256u) {
-        const uint32_t x = e / (D / 4u), d = 4u * (e % (D / 4u));
-        f32x4 v;
-        const bool sees = join_row(
-            g0, g1, a.scale_log2,
-            [&](uint32_t g) { return scratch + (size_t)(2u * g + (g == g0 ? 1u : 0u)) * part_floats<D, NR>(); }, 16u * NR, D,
-            x, d, v);
-        uint16_t* const dst = (uint16_t*)a.out + (size_t)(rq.first + x / G) * a.out_stride + (kvh * G + x % G) * D + d;
-        *(u32x2*)dst = sees ? u32x2{pack2<T>(v.x, v.y), pack2<T>(v.z, v.w)} : u32x2{0u, 0u};
+// Joins the parts that worker blockIdx.x's record names, in their order: 16 rows a workgroup
+// (blockIdx.y), eight of them at a time, or fewer with their parts shared by several groups of
+// D / 4 threads, which leaves no row more than a few rounds of loads. PR: rows of a part.
+template <uint32_t T, uint32_t D, uint32_t PR>
+__global__ void __launch_bounds__(256) paged_attn_join(SeqAttnArgs a, const JoinRecord* __restrict__ records,
+                                                       const float* __restrict__ parts) {
+    constexpr uint32_t LPR = D / 4u, GROUPS = 256u / LPR;  // threads of a row, rows or shares at a time
+    __shared__ f32x4 so[GROUPS][LPR];
+    __shared__ float sm[GROUPS], sl[GROUPS];
+    const JoinRecord rec = records[blockIdx.x];
+    const uint32_t x0 = 16u * blockIdx.y;
+    if (rec.last == 0 || x0 >= rec.n) return;
+    const uint32_t rows = min(rec.n - x0, 16u), n_parts = rec.last - blockIdx.x + 1u;
+    // shares of a row's parts: GROUPS / (rows rounded up to a power of two)
+    uint32_t shares = GROUPS;
+    while (shares > 1u && shares * rows > GROUPS) shares /= 2u;
+    const uint32_t at_once = GROUPS / shares;
+    const uint32_t grp = threadIdx.x / LPR, d = 4u * (threadIdx.x % LPR), share = grp % shares;
+    for (uint32_t r0 = 0; r0 < rows; r0 += at_once) {
+        const uint32_t x = x0 + r0 + grp / shares;
+        const bool live = r0 + grp / shares < rows;
+        f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
+        float m = -INFINITY, l = -1.0f;  // l = -1: no key seen
+        if (live) {
+            for (uint32_t i0 = share; i0 < n_parts; i0 += 4u * shares) {
+                float pm[4], pl[4];
+                f32x4 po[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t i = min(i0 + (uint32_t)k * shares, n_parts - 1u);
+                    // a worker's second part where it is the rows' first
+                    const float* const p = parts + (size_t)(2u * (blockIdx.x + i) + (i == 0 ? 1u : 0u)) * (PR * (D + 2u));
+                    pm[k] = p[PR * D + x];
+                    pl[k] = i0 + (uint32_t)k * shares < n_parts ? p[PR * (D + 1u) + x] : -1.0f;
+                    po[k] = *(const f32x4*)(p + x * D + d);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; k++) join_part(o, m, l, po[k], pm[k], pl[k], a.scale_log2);
+            }
+        }
+        if (shares > 1u) {
+            so[grp][threadIdx.x % LPR] = o;
+            if (threadIdx.x % LPR == 0) {
+                sm[grp] = m;
+                sl[grp] = l;
+            }
+            __syncthreads();
+            if (share == 0)
+                for (uint32_t k = 1; k < shares; k++)
+                    join_part(o, m, l, so[grp + k][threadIdx.x % LPR], sm[grp + k], sl[grp + k], a.scale_log2);
+            __syncthreads();
+        }
+        if (live && share == 0) {
+            const uint32_t r = rec.row0 + x, G = a.n_heads / a.n_kv_heads;
+            const f32x4 v = o * (1.0f / l);
+            uint16_t* const dst = (uint16_t*)a.out + (size_t)(rec.first + r / G) * a.out_stride +
+                                  (rec.kvh * G + r % G) * D + d;
+            *(u32x2*)dst = l != -1.0f ? u32x2{pack2<T>(v.x, v.y), pack2<T>(v.z, v.w)} : u32x2{0u, 0u};
+        }
     }
 }
 
