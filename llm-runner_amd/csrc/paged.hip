@@ -19,6 +19,11 @@ __device__ __forceinline__ uint32_t pages_of(uint32_t n, uint32_t log2, uint32_t
 
 constexpr uint32_t kPlanThreads = 256;
 
+template <uint32_t OT>
+__device__ __forceinline__ uint32_t pack16(float x, float y) {
+    return OT == kGgmlF16 ? pack_f16x2(x, y) : pack_bf16x2(x, y);
+}
+
 // Every workgroup scans all the requests' lengths (the sums of new tokens and of
 // pages to take before each request, into LDS), then writes its share of the
 // requests' and tokens' entries: one launch, no workgroup waits for another.
@@ -120,83 +125,73 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedPlanArgs 
     }
 }
 
-template <uint32_t OT>
-__device__ __forceinline__ void put2(void* base, size_t idx, float x, float y) {
-    *(uint32_t*)((uint16_t*)base + idx) = OT == kGgmlF16 ? pack_f16x2(x, y) : pack_bf16x2(x, y);
-}
-
-// One wave per head of a row; lane l holds the pair the rotation takes together
-// (D = 64: two heads a wave).
+// D / 8 lanes a head, 8 elements a lane: four pairs of the rotation, as two vectors of four
+// (pairs (j, j + D / 2): one from each half; pairs (2j, 2j + 1): one behind the other), so
+// that every load is 16 bytes a lane and every store 8. A thread has one head of one row:
+// nothing waits for anything but its own loads. HBM bound: 8192 rows of 32/8 heads, 306 MB.
 template <uint32_t OT, uint32_t D, bool HALVES>
 __global__ void __launch_bounds__(256) qkv_tokens_kernel(QkvTokensArgs a) {
-    constexpr uint32_t P = D / 2u;  // pairs, lanes of a head
-    const uint32_t l = threadIdx.x % P, unit = threadIdx.x / P;
-    const uint32_t r = blockIdx.x, heads = a.n_heads + 2u * a.n_kv_heads;
-    const uint32_t pos = a.positions ? (uint32_t)min(max(a.positions[r], 0), (int32_t)(a.n_positions - 1u)) : r;
-    const uint32_t e0 = HALVES ? l : 2u * l, e1 = HALVES ? l + P : 2u * l + 1u;
-    float c = 1.0f, sn = 0.0f;
-    if (a.rope_cos) {
-        c = a.rope_cos[(size_t)pos * P + l];
-        sn = a.rope_sin[(size_t)pos * P + l];
-    }
-    const int32_t slot = a.slots ? a.slots[r] : 0;
-    for (uint32_t h = blockIdx.y * (256u / P) + unit; h < heads; h += gridDim.y * (256u / P)) {
-        const float* src = a.qkv + (size_t)r * a.qkv_stride + (size_t)h * D;
-        float x0 = src[e0], x1 = src[e1];
-        const bool is_q = h < a.n_heads, is_v = h >= a.n_heads + a.n_kv_heads;
-        const float* w = is_q ? a.q_norm : is_v ? nullptr : a.k_norm;
-        if (w) {
-            float ss = x0 * x0 + x1 * x1;
+    constexpr uint32_t L = D / 8u;  // lanes of a head
+    const uint32_t l = threadIdx.x % L, r = blockIdx.x, h = blockIdx.y * (256u / L) + threadIdx.x / L;
+    if (h >= a.n_heads + 2u * a.n_kv_heads) return;  // (whole heads: the reductions stay within one)
+    const uint32_t e0 = HALVES ? 4u * l : 8u * l, e1 = HALVES ? e0 + D / 2u : e0 + 4u;
+    const float* src = a.qkv + (size_t)r * a.qkv_stride + (size_t)h * D;
+    f32x4 x0 = *(const f32x4*)(src + e0), x1 = *(const f32x4*)(src + e1);
+    const bool is_q = h < a.n_heads, is_v = h >= a.n_heads + a.n_kv_heads;
+    const int32_t slot = a.slots && !is_q ? a.slots[r] : 0;
+    const float* w = is_q ? a.q_norm : is_v ? nullptr : a.k_norm;
+    if (w) {
+        const f32x4 w0 = *(const f32x4*)(w + e0), w1 = *(const f32x4*)(w + e1);
+        const f32x4 q = x0 * x0 + x1 * x1;
+        float ss = (q.x + q.y) + (q.z + q.w);
 #pragma unroll
-            for (uint32_t o = P / 2u; o > 0; o >>= 1) ss += __shfl_xor(ss, (int)o, 64);
-            const float inv = 1.0f / sqrtf(ss / (float)D + a.eps);
-            x0 = x0 * inv * w[e0];
-            x1 = x1 * inv * w[e1];
-        }
-        if (a.rope_cos && !is_v) {
-            const float y0 = x0 * c - x1 * sn, y1 = x0 * sn + x1 * c;
-            x0 = y0;
-            x1 = y1;
-        }
-        void* dst;
-        size_t at;
-        if (is_q) {
-            dst = a.q;
-            at = (size_t)r * a.q_stride + (size_t)h * D;
+        for (uint32_t o = L / 2u; o > 0; o >>= 1) ss += __shfl_xor(ss, (int)o, 64);
+        const float inv = 1.0f / sqrtf(ss / (float)D + a.eps);
+        x0 = x0 * inv * w0;
+        x1 = x1 * inv * w1;
+    }
+    if (a.rope_cos && !is_v) {
+        const uint32_t pos = a.positions ? (uint32_t)min(max(a.positions[r], 0), (int32_t)(a.n_positions - 1u)) : r;
+        const size_t at = (size_t)pos * (D / 2u) + 4u * l;
+        const f32x4 c = *(const f32x4*)(a.rope_cos + at), sn = *(const f32x4*)(a.rope_sin + at);
+        // the first and the second of each pair
+        const f32x4 u = HALVES ? x0 : f32x4{x0.x, x0.z, x1.x, x1.z}, v = HALVES ? x1 : f32x4{x0.y, x0.w, x1.y, x1.w};
+        const f32x4 y0 = u * c - v * sn, y1 = u * sn + v * c;
+        x0 = HALVES ? y0 : f32x4{y0.x, y1.x, y0.y, y1.y};
+        x1 = HALVES ? y1 : f32x4{y0.z, y1.z, y0.w, y1.w};
+    }
+    uint16_t* dst;
+    if (is_q) {
+        dst = (uint16_t*)a.q + (size_t)r * a.q_stride + (size_t)h * D;
+    } else {
+        const uint32_t kh = h - a.n_heads - (is_v ? a.n_kv_heads : 0u);
+        dst = (uint16_t*)(is_v ? a.v : a.k);
+        if (a.slots) {
+            const uint32_t page = (uint32_t)slot >> a.page_log2;
+            if (slot < 0 || page >= a.n_pages) return;
+            dst += ((((size_t)page * a.n_kv_heads + kh) << a.page_log2) + ((uint32_t)slot & ((1u << a.page_log2) - 1u))) * D;
         } else {
-            const uint32_t kh = h - a.n_heads - (is_v ? a.n_kv_heads : 0u);
-            dst = is_v ? a.v : a.k;
-            if (a.slots) {
-                const uint32_t page = (uint32_t)slot >> a.page_log2;
-                if (slot < 0 || page >= a.n_pages) continue;
-                at = ((((size_t)page * a.n_kv_heads + kh) << a.page_log2) +
-                      ((uint32_t)slot & ((1u << a.page_log2) - 1u))) * D;
-            } else {
-                at = (size_t)r * a.kv_stride + (size_t)kh * D;
-            }
-        }
-        if constexpr (HALVES) {
-            ((uint16_t*)dst)[at + e0] = (uint16_t)(OT == kGgmlF16 ? pack_f16x2(x0, 0.0f) : pack_bf16x2(x0, 0.0f));
-            ((uint16_t*)dst)[at + e1] = (uint16_t)(OT == kGgmlF16 ? pack_f16x2(x1, 0.0f) : pack_bf16x2(x1, 0.0f));
-        } else {
-            put2<OT>(dst, at + e0, x0, x1);
+            dst += (size_t)r * a.kv_stride + (size_t)kh * D;
         }
     }
+    *(u32x2*)(dst + e0) = u32x2{pack16<OT>(x0.x, x0.y), pack16<OT>(x0.z, x0.w)};
+    *(u32x2*)(dst + e1) = u32x2{pack16<OT>(x1.x, x1.y), pack16<OT>(x1.z, x1.w)};
 }
 
 }  // namespace
 
 hipError_t launch_paged_plan(const PagedPlanArgs& a, hipStream_t st) {
-    // tokens of a workgroup: 4 a thread; a small step is one workgroup
+    // a token a thread, up to two workgroups a CU; a small step is one workgroup
     const uint32_t items = a.n_tokens > a.n_seqs ? a.n_tokens : a.n_seqs;
-    const uint32_t wgs = (items + 4u * kPlanThreads - 1u) / (4u * kPlanThreads);
-    hipLaunchKernelGGL(paged_plan_kernel, dim3(wgs < 256u ? (wgs ? wgs : 1u) : 256u), dim3(kPlanThreads),
+    const uint32_t wgs = (items + kPlanThreads - 1u) / kPlanThreads;
+    hipLaunchKernelGGL(paged_plan_kernel, dim3(wgs < 512u ? (wgs ? wgs : 1u) : 512u), dim3(kPlanThreads),
                        2u * (a.n_seqs + 1u) * 4u, st, a);
     return hipGetLastError();
 }
 
 hipError_t launch_qkv_tokens(const QkvTokensArgs& a, uint32_t dim, uint32_t otype, bool halves, hipStream_t st) {
-    const dim3 grid(a.n_tokens, 1), block(256);
+    const uint32_t per = 256u / (dim / 8u);  // heads a workgroup
+    const dim3 grid(a.n_tokens, (a.n_heads + 2u * a.n_kv_heads + per - 1u) / per), block(256);
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, a); };
     if (otype == kGgmlBF16) {
         if (dim == 128u) halves ? go(qkv_tokens_kernel<kGgmlBF16, 128, true>) : go(qkv_tokens_kernel<kGgmlBF16, 128, false>);

@@ -17,7 +17,6 @@ are int32 device tensors that nothing here reads back.
 from __future__ import annotations
 
 import dataclasses
-import math
 
 import torch
 
@@ -26,21 +25,29 @@ from .gguf import GGML_BF16, GGML_F16
 from .ops import RenderGraph, default_graph
 
 _TYPES = {torch.float16: GGML_F16, torch.bfloat16: GGML_BF16}
+_I32, _F32 = torch.int32, torch.float32
+# the stream's handle alone, without the Stream object that torch.cuda.current_stream makes
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
 
-def _bind(g: RenderGraph, *tensors) -> RenderGraph:
+# The checks below are written out flat: a call's host time is what single-token steps wait for.
+
+
+def _graph(g: RenderGraph | None, *tensors) -> RenderGraph:
     """The graph, on its device's current stream; every tensor has to be on that device."""
-    g = g or default_graph()
+    if g is None:
+        g = default_graph()
     dev = g.ctx.device
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.get_device() != dev):
+        if t.get_device() != dev:
             raise ValueError(f"all tensors must be on the graph's device (cuda:{dev})")
-    g.ctx.set_stream(torch.cuda.current_stream(dev).cuda_stream)
+    g.ctx.set_stream(_raw_stream(dev))
     return g
 
 
-def _ints(t: torch.Tensor, what: str, n: int):
-    if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < n:
+def _ints(t: torch.Tensor, what: str, n: int) -> int:
+    if t.dtype is not _I32 or t.numel() < n or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous int32 device tensor of >= {n} elements")
     return t.data_ptr()
 
@@ -48,7 +55,7 @@ def _ints(t: torch.Tensor, what: str, n: int):
 def _vec(t, what: str, n: int):
     if t is None:
         return None
-    if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() < n:
+    if t.dtype is not _F32 or t.numel() < n or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous f32 device tensor of >= {n} elements")
     return t.data_ptr()
 
@@ -56,20 +63,19 @@ def _vec(t, what: str, n: int):
 def _heads(t: torch.Tensor, what: str):
     """(tokens, heads, dim) and the strides of tokens and heads of a 3-D view with contiguous heads; a
     dimension of one has no stride of its own and gets one that the library takes."""
-    if t.dim() != 3 or t.stride(2) != 1:
+    if t.dim() != 3:
         raise ValueError(f"{what} must be [tokens, heads, head_dim] with contiguous heads")
     T, H, D = t.shape
-    ts, hs, _ = t.stride()
+    ts, hs, ds = t.stride()
+    if ds != 1:
+        raise ValueError(f"{what} must be [tokens, heads, head_dim] with contiguous heads")
     return T, H, D, ts if T > 1 else H * D, hs if H > 1 else D
 
 
-def _rows_out(out, T: int, width: int, like: torch.Tensor):
-    if out is None:
-        return torch.empty(T, width, dtype=like.dtype, device=like.device), width
-    if out.dtype != like.dtype or out.dim() != 2 or out.shape[0] != T or out.shape[1] != width or (
-            width > 1 and out.stride(1) != 1):
+def _out_stride(out: torch.Tensor, T: int, width: int, like: torch.Tensor) -> int:
+    if out.dtype is not like.dtype or out.shape != (T, width) or out.stride(1) != 1:
         raise ValueError(f"out must be a [{T}, {width}] view of q's dtype with contiguous rows")
-    return out, out.stride(0) if T > 1 else width
+    return out.stride(0) if T > 1 else width
 
 
 def _cache(k: torch.Tensor, v: torch.Tensor):
@@ -78,9 +84,10 @@ def _cache(k: torch.Tensor, v: torch.Tensor):
     return k.shape
 
 
-def _type(what: str, *tensors) -> int:
-    t = _TYPES.get(tensors[0].dtype)
-    if t is None or any(x.dtype != tensors[0].dtype for x in tensors):
+def _type(what: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> int:
+    d = q.dtype
+    t = _TYPES.get(d)
+    if t is None or k.dtype is not d or v.dtype is not d:
         raise ValueError(f"{what} must share one dtype, float16 or bfloat16")
     return t
 
@@ -94,17 +101,19 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_offs
     its rows that belong to no request keep what they hold (a new `out`: undefined)."""
     T, H, D, qs, qh = _heads(q, "q")
     Tk, Hk, Dk, ks, kh = _heads(k, "k")
-    if v.shape != k.shape or v.stride() != k.stride() or Tk != T or Dk != D:
+    if Tk != T or Dk != D or v.shape != k.shape or v.stride() != k.stride():
         raise ValueError("k and v must be [tokens, n_kv_heads, head_dim] alike, with q's tokens and head_dim")
     t = _type("q, k and v", q, k, v)
-    out, os_ = _rows_out(out, T, H * D, q)
+    if out is None:
+        out = torch.empty(T, H * D, dtype=q.dtype, device=q.device)
+    os_ = _out_stride(out, T, H * D, q)
     n = seq_offsets.numel() - 1
     if n < 0:
         raise ValueError("seq_offsets must have n_seqs + 1 elements")
     off = _ints(seq_offsets, "seq_offsets", 1)
-    g = _bind(g, q, k, v, seq_offsets, out)
-    p = capi.PromptAttentionParams(D, H, Hk, T, n, qs, qh, ks, kh, os_, scale if scale is not None else 1.0 / math.sqrt(D))
-    g.ctx.prompt_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), t, out.data_ptr(), off, p)
+    _graph(g, q, k, v, seq_offsets, out).ctx.prompt_attention(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), t, out.data_ptr(), off,
+        capi.PromptAttentionParams(D, H, Hk, T, n, qs, qh, ks, kh, os_, D ** -0.5 if scale is None else scale))
     return out
 
 
@@ -130,19 +139,17 @@ def paged_plan(past_len: torch.Tensor, new_len: torch.Tensor, free_pages: torch.
     [n_seqs]; free_pages [capacity] with free_count [1] of them free, taken from the end; block_table
     [n_seqs, max_pages], whose new entries are filled in; batch receives the rest. The new tokens' sum is
     at most batch.slots' length."""
-    n = past_len.numel()
+    n, T = past_len.numel(), batch.slots.numel()
     if block_table.dim() != 2 or block_table.shape[0] != n or new_len.numel() != n:
         raise ValueError("past_len, new_len and block_table's rows must be one per request")
-    if batch.seq_offsets.numel() != n + 1 or batch.positions.numel() != batch.slots.numel():
+    if batch.seq_offsets.numel() != n + 1 or batch.positions.numel() != T:
         raise ValueError("batch must be PagedBatch.empty(n_seqs, n_tokens)")
-    T = batch.slots.numel()
+    off, kvl, slots, pos, pages = batch.seq_offsets, batch.kv_len, batch.slots, batch.positions, batch.pages
     args = (_ints(past_len, "past_len", n), _ints(new_len, "new_len", n), _ints(free_pages, "free_pages", 0),
-            _ints(free_count, "free_count", 1), _ints(block_table, "block_table", 0),
-            _ints(batch.seq_offsets, "seq_offsets", n + 1), _ints(batch.kv_len, "kv_len", n),
-            _ints(batch.slots, "slots", T), _ints(batch.positions, "positions", T), _ints(batch.pages, "pages", 2))
-    g = _bind(g, past_len, new_len, free_pages, free_count, block_table, batch.seq_offsets, batch.kv_len, batch.slots,
-              batch.positions, batch.pages)
-    g.ctx.paged_plan(*args, capi.PagedPlanParams(n, T, page_size, block_table.shape[1], free_pages.numel()))
+            _ints(free_count, "free_count", 1), _ints(block_table, "block_table", 0), _ints(off, "seq_offsets", 0),
+            _ints(kvl, "kv_len", n), _ints(slots, "slots", 0), _ints(pos, "positions", 0), _ints(pages, "pages", 2))
+    _graph(g, past_len, new_len, free_pages, free_count, block_table, off, kvl, slots, pos, pages).ctx.paged_plan(
+        *args, capi.PagedPlanParams(n, T, page_size, block_table.shape[1], free_pages.numel()))
     return batch
 
 
@@ -155,7 +162,7 @@ def qkv_tokens(qkv: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Ten
     caches [n_pages, n_kv_heads, page_size, D], a row with slot -1 nowhere; without, rows [T, n_kv_heads, D].
     rope: (cos, sin) f32 [n_positions, D / 2], taken at positions (int32 [T]; None: the row), rotating the
     pairs (j, j + D/2), or (2j, 2j + 1) where halves is False."""
-    if qkv.dim() != 2 or qkv.dtype != torch.float32 or (qkv.shape[1] > 1 and qkv.stride(1) != 1):
+    if qkv.dim() != 2 or qkv.dtype is not _F32 or (qkv.shape[1] > 1 and qkv.stride(1) != 1):
         raise ValueError("qkv must be a 2-D f32 view with contiguous rows")
     T, H, D, qs, qh = _heads(q, "q")
     if qkv.shape[0] != T or qh != D:
@@ -181,22 +188,10 @@ def qkv_tokens(qkv: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Ten
         n_pos = cos.shape[0]
     pp = _ints(positions, "positions", T) if positions is not None else None
     args = (_vec(q_norm, "q_norm", D), _vec(k_norm, "k_norm", D), _vec(cos, "rope_cos", 0), _vec(sin, "rope_sin", 0))
-    g = _bind(g, qkv, q, k, v, slots, positions, q_norm, k_norm, cos, sin)
     p = capi.QkvTokensParams(D, H, Hk, T, qkv.stride(0) if T > 1 else qkv.shape[1] + -qkv.shape[1] % 4, qs, t, ks, page,
-                             n_pages, n_pos, int(halves), eps)
-    g.ctx.qkv_tokens(qkv.data_ptr(), *args, pp, sp, q.data_ptr(), k.data_ptr(), v.data_ptr(), p)
-
-
-def _paged_params(q, k_cache, v_cache, seq_offsets, kv_len, block_table, max_new, scale, os_):
-    T, H, D, qs, qh = _heads(q, "q")
-    n_pages, Hk, page, Dk = _cache(k_cache, v_cache)
-    n = kv_len.numel()
-    if Dk != D or qh != D:
-        raise ValueError("q must be [tokens, n_heads, head_dim], heads side by side, with the caches' head_dim")
-    if seq_offsets.numel() != n + 1 or block_table.dim() != 2 or block_table.shape[0] != n:
-        raise ValueError("kv_len, block_table's rows and seq_offsets (one more) must be one per request")
-    return capi.PagedAttentionParams(D, H, Hk, T, n, min(max_new, T), page, n_pages, block_table.shape[1], qs, os_,
-                                     scale if scale is not None else 1.0 / math.sqrt(D))
+                             n_pages, n_pos, halves, eps)
+    on = [x for x in (qkv, q, k, v, slots, positions, q_norm, k_norm, cos, sin) if x is not None]
+    _graph(g, *on).ctx.qkv_tokens(qkv.data_ptr(), *args, pp, sp, q.data_ptr(), k.data_ptr(), v.data_ptr(), p)
 
 
 def paged_attention_scratch(q: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tensor, max_new: int,
@@ -206,7 +201,7 @@ def paged_attention_scratch(q: torch.Tensor, k_cache: torch.Tensor, block_table:
     n_pages, Hk, page, _ = k_cache.shape
     p = capi.PagedAttentionParams(D, H, Hk, T, block_table.shape[0], min(max_new, T), page, n_pages,
                                   block_table.shape[1], H * D, H * D, 1.0)
-    g = _bind(g, q)
+    g = _graph(g, q)
     return torch.empty(g.ctx.paged_attention_scratch_bytes(p), dtype=torch.uint8, device=q.device)
 
 
@@ -219,17 +214,24 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     counted), block_table [n_seqs, max_pages]; max_new: the most new tokens of a request (1 while every request
     decodes). out [T, n_heads * D] of q's dtype (rows of no request keep what they hold; a new `out`:
     undefined). scratch: paged_attention_scratch's, one per call that may overlap another; None: a new one."""
-    out, os_ = _rows_out(out, q.shape[0], q.shape[1] * q.shape[2] if q.dim() == 3 else 0, q)
+    T, H, D, qs, qh = _heads(q, "q")
+    n_pages, Hk, page, Dk = _cache(k_cache, v_cache)
+    n = kv_len.numel()
+    if Dk != D or qh != D:
+        raise ValueError("q must be [tokens, n_heads, head_dim], heads side by side, with the caches' head_dim")
+    if seq_offsets.numel() != n + 1 or block_table.dim() != 2 or block_table.shape[0] != n:
+        raise ValueError("kv_len, block_table's rows and seq_offsets (one more) must be one per request")
     t = _type("q and the caches", q, k_cache, v_cache)
-    p = _paged_params(q, k_cache, v_cache, seq_offsets, kv_len, block_table, max_new, scale, os_)
-    off, kvl = _ints(seq_offsets, "seq_offsets", 1), _ints(kv_len, "kv_len", 0)
-    tab = _ints(block_table, "block_table", 0)
-    g = _bind(g, q, k_cache, v_cache, seq_offsets, kv_len, block_table, out, scratch)
+    if out is None:
+        out = torch.empty(T, H * D, dtype=q.dtype, device=q.device)
+    p = capi.PagedAttentionParams(D, H, Hk, T, n, min(max_new, T), page, n_pages, block_table.shape[1], qs,
+                                  _out_stride(out, T, H * D, q), D ** -0.5 if scale is None else scale)
+    off, kvl, tab = _ints(seq_offsets, "seq_offsets", 0), _ints(kv_len, "kv_len", 0), _ints(block_table, "block_table", 0)
+    g = _graph(g, q, k_cache, v_cache, seq_offsets, kv_len, block_table, out)
     if scratch is None:
-        need = g.ctx.paged_attention_scratch_bytes(p)
-        if need:
-            scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
-    sp, sn = (scratch.data_ptr(), scratch.numel() * scratch.element_size()) if scratch is not None else (None, 0)
-    g.ctx.paged_attention(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), t, out.data_ptr(), off, kvl, tab, sp, sn,
-                          p)
+        scratch = torch.empty(g.ctx.paged_attention_scratch_bytes(p), dtype=torch.uint8, device=q.device)
+    elif scratch.get_device() != q.get_device() or not scratch.is_contiguous():
+        raise ValueError("scratch must be a contiguous tensor on q's device")
+    g.ctx.paged_attention(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), t, out.data_ptr(), off, kvl, tab,
+                          scratch.data_ptr(), scratch.numel() * scratch.element_size(), p)
     return out
