@@ -1123,7 +1123,7 @@ int llmr_prompt_attention(llmr_context* ctx, const void* q, const void* k, const
     a.q_stride = p->q_stride, a.q_head_stride = p->q_head_stride;
     a.kv_stride = p->kv_stride, a.kv_head_stride = p->kv_head_stride, a.out_stride = p->out_stride;
     a.scale_log2 = p->scale * 1.4426950408889634f;
-    return launched(llmr::launch_prompt_attention(a, type, p->head_dim, ctx->cur), "prompt_attention");
+    return launched(llmr::launch_prompt_attention(a, type, p->head_dim, ctx->num_cus, ctx->cur), "prompt_attention");
 }
 
 int llmr_paged_plan(llmr_context* ctx, const int32_t* past_len, const int32_t* new_len, const int32_t* free_pages,

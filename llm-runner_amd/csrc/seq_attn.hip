@@ -172,15 +172,20 @@ __device__ __forceinline__ uint32_t block_keys(const SeqAttnArgs& a, const Paged
 __device__ __forceinline__ uint32_t block_tiles(const SeqAttnArgs& a, const PagedRequest& rq, uint32_t G, uint32_t b) {
     return max((block_keys(a, rq, G, b) + seqattn::kKeys - 1u) / seqattn::kKeys, 1u);
 }
-__device__ __forceinline__ uint64_t request_tiles(const SeqAttnArgs& a, const PagedRequest& rq, uint32_t G) {
+// A block's units on the line: its tiles, the first of them kStart units more, for what
+// beginning a block costs (pages staged, the first tiles waited for: about four tiles' time;
+// without it a workgroup that got ten blocks of one tile was the last by far: 24 requests of
+// 1 to 511 new tokens 72 -> 40 us).
+constexpr uint32_t kStart = 4;
+__device__ __forceinline__ uint64_t request_units(const SeqAttnArgs& a, const PagedRequest& rq, uint32_t G) {
     uint64_t n = 0;
-    for (uint32_t b = 0; b < blocks_of(rq, G); b++) n += block_tiles(a, rq, G, b);
+    for (uint32_t b = 0; b < blocks_of(rq, G); b++) n += block_tiles(a, rq, G, b) + kStart;
     return n;
 }
 template <uint32_t D>
 constexpr size_t tile_part_floats() { return kBlockRows * (D + 2u); }
 
-// Attention over a paged cache for requests of any number of new tokens: the tiles of all
+// Attention over a paged cache for requests of any number of new tokens: the units of all
 // (request, key/value head, block of 256 rows) make one line that the workgroups, one a CU,
 // share evenly, as paged_attn_few's waves do; parts of a block that several workgroups take
 // go to scratch, at most two a workgroup, and paged_attn_join joins them.
@@ -193,10 +198,10 @@ __device__ __forceinline__ void paged_tiles(const SeqAttnArgs& a, uint8_t* lds, 
     const uint32_t G = a.n_heads / a.n_kv_heads;
     uint32_t* const pages = (uint32_t*)(lds + seqattn::lds_bytes<D>());
 
-    const auto cost = [&](const PagedRequest& r) { return request_tiles(a, r, G); };
+    const auto cost = [&](const PagedRequest& r) { return request_units(a, r, G); };
     seqattn::RequestWindow win;
     const uint64_t w = seqattn::batch_cost(a, win, lane, cost) * a.n_kv_heads;
-    const uint32_t n = (uint32_t)min((uint64_t)gridDim.x, w);  // every workgroup has a tile
+    const uint32_t n = (uint32_t)min((uint64_t)gridDim.x, w);  // every workgroup has a unit
     seqattn::JoinRecord rec{};
     if (blockIdx.x >= n) {
         if (tid == 0) records[blockIdx.x].last = 0;
@@ -204,13 +209,13 @@ __device__ __forceinline__ void paged_tiles(const SeqAttnArgs& a, uint8_t* lds, 
     }
     uint64_t at = seqattn::part_begin(blockIdx.x, w, n);
     const uint64_t end = seqattn::part_begin(blockIdx.x + 1u, w, n);
-    uint64_t base;  // tiles (all heads) before request s
+    uint64_t base;  // units (all heads) before request s
     uint32_t s = seqattn::find_request(a, win, lane, cost, a.n_kv_heads, at, base);
 
     while (at < end) {
         if (s - win.s0 >= 64u) win.load(a, s, lane);
         const PagedRequest rq = win.get(s);
-        const uint64_t per_head = request_tiles(a, rq, G), all = per_head * a.n_kv_heads;
+        const uint64_t per_head = request_units(a, rq, G), all = per_head * a.n_kv_heads;
         if (all == 0 || at >= base + all) {
             base += all;
             s++;
@@ -219,11 +224,14 @@ __device__ __forceinline__ void paged_tiles(const SeqAttnArgs& a, uint8_t* lds, 
         const uint32_t kvh = (uint32_t)((at - base) / per_head);
         uint64_t x = (at - base) % per_head;
         uint32_t b = 0, tiles;
-        while (x >= (tiles = block_tiles(a, rq, G, b))) {
-            x -= tiles;
+        while (x >= (tiles = block_tiles(a, rq, G, b)) + kStart) {
+            x -= tiles + kStart;
             b++;
         }
-        const uint32_t t0 = (uint32_t)x, t1 = (uint32_t)min((uint64_t)tiles, x + (end - at));
+        const uint64_t y = min((uint64_t)tiles + kStart, x + (end - at));  // units [x, y) of the block
+        const uint32_t t0 = x > kStart ? (uint32_t)x - kStart : 0u, t1 = y > kStart ? (uint32_t)y - kStart : 0u;
+        at += y - x;
+        if (t0 == t1) continue;  // (of the first tile's units none but the last carries it)
         const uint32_t keys = block_keys(a, rq, G, b), key0 = t0 * seqattn::kKeys;
         const uint32_t n_keys = min(keys, t1 * seqattn::kKeys) - min(keys, key0);
 
@@ -252,7 +260,6 @@ __device__ __forceinline__ void paged_tiles(const SeqAttnArgs& a, uint8_t* lds, 
                                 ? nullptr
                                 : scratch + (2u * blockIdx.x + (t0 == 0 ? 1u : 0u)) * tile_part_floats<D>();
         seqattn::tile_rows<T, D, NW>(a, lds, src, n_keys, row, 0u, hi_min, part, out_at);
-        at += t1 - t0;
         if (t0 == 0 && t1 != tiles)  // (the workgroup's last part: the record is its one)
             rec = seqattn::JoinRecord{seqattn::part_of(at + (tiles - t1) - 1u, w, n), rq.first, row0,
                                       min(rows - row0, kBlockRows), kvh, {}};
@@ -269,10 +276,24 @@ paged_attn_tiles(SeqAttnArgs a, seqattn::JoinRecord* __restrict__ records, float
 
 }  // namespace
 
-hipError_t launch_prompt_attention(const SeqAttnArgs& a, uint32_t type, uint32_t dim, hipStream_t st) {
-    if (type == kGgmlBF16)
-        return dim == 128u ? launch_tiles<kGgmlBF16, 128, 8>(a, st) : launch_tiles<kGgmlBF16, 64, 8>(a, st);
-    return dim == 128u ? launch_tiles<kGgmlF16, 128, 8>(a, st) : launch_tiles<kGgmlF16, 64, 8>(a, st);
+hipError_t launch_prompt_attention(const SeqAttnArgs& a, uint32_t type, uint32_t dim, int num_cus, hipStream_t st) {
+    auto go = [&](auto t, auto d) {
+        constexpr uint32_t T = decltype(t)::value, D = decltype(d)::value;
+        // 128 rows a workgroup where all of them are on the card at once (one a CU, two with
+        // head_dim 64: their LDS): a tile takes a wave alone on its SIMD as long as two, so fewer
+        // rows on more CUs end earlier. 512 tokens of 32/8 heads, 128: 19.5 -> 16.9 us, 1000: 30.7
+        // -> 26.6; 24/8 heads, 64, 1024: 23.2 -> 19.9, 2048: 40.4 -> 34.9. Past that a second round
+        // may cost what it gains: 10 x 200 tokens of 24/8 heads, 128: 20.4 against 25.6.
+        const uint64_t rows = (uint64_t)a.n_tokens * (a.n_heads / a.n_kv_heads);
+        const bool fits = (rows + 127u) / 128u * a.n_kv_heads <= (uint64_t)num_cus * (D == 64u ? 2u : 1u);
+        return fits ? launch_tiles<T, D, 4>(a, st) : launch_tiles<T, D, 8>(a, st);
+    };
+    using BF16 = std::integral_constant<uint32_t, kGgmlBF16>;
+    using F16 = std::integral_constant<uint32_t, kGgmlF16>;
+    using D64 = std::integral_constant<uint32_t, 64>;
+    using D128 = std::integral_constant<uint32_t, 128>;
+    if (type == kGgmlBF16) return dim == 128u ? go(BF16{}, D128{}) : go(BF16{}, D64{});
+    return dim == 128u ? go(F16{}, D128{}) : go(F16{}, D64{});
 }
 
 // Row blocks of 16 of the kernel for few rows that holds max_new tokens of a group; 0: more rows.
@@ -301,7 +322,7 @@ static hipError_t launch_paged(const SeqAttnArgs& a, uint32_t nr, int num_cus, v
         hipLaunchKernelGGL(work, dim3(n), dim3(threads), 0, st, a, records, parts);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
-        hipLaunchKernelGGL(join, dim3(n, part_rows / 16u), dim3(256), 0, st, a, records, parts);
+        hipLaunchKernelGGL(join, dim3(part_rows / 16u, n), dim3(256), 0, st, a, records, parts);
         return hipGetLastError();
     };
     using namespace seqattn;

@@ -520,19 +520,22 @@ paged_attn_few(SeqAttnArgs a, JoinRecord* __restrict__ records, float* __restric
     few_rows<T, D, NR>(a, lds, records, parts);
 }
 
-// Joins the parts that worker blockIdx.x's record names, in their order: 16 rows a workgroup
-// (blockIdx.y), eight of them at a time, or fewer with their parts shared by several groups of
-// D / 4 threads, which leaves no row more than a few rounds of loads. PR: rows of a part.
+// Joins the parts that worker blockIdx.y's record names, in their order: 16 rows a workgroup
+// (blockIdx.x; side by side, so that a record's rows go to all XCDs: 512 new tokens behind
+// 30000, every fourth worker with a record, 21.6 -> 12.0 us), as many of them at a time as the
+// threads hold, or fewer with their parts shared by several groups of D / 4 threads, so that no
+// row takes more than a few rounds of loads (35 parts of four rows: 21.8 -> 6.0). PR: rows of a
+// part.
 template <uint32_t T, uint32_t D, uint32_t PR>
 __global__ void __launch_bounds__(256) paged_attn_join(SeqAttnArgs a, const JoinRecord* __restrict__ records,
                                                        const float* __restrict__ parts) {
     constexpr uint32_t LPR = D / 4u, GROUPS = 256u / LPR;  // threads of a row, rows or shares at a time
     __shared__ f32x4 so[GROUPS][LPR];
     __shared__ float sm[GROUPS], sl[GROUPS];
-    const JoinRecord rec = records[blockIdx.x];
-    const uint32_t x0 = 16u * blockIdx.y;
+    const uint32_t worker = blockIdx.y, x0 = 16u * blockIdx.x;
+    const JoinRecord rec = records[worker];
     if (rec.last == 0 || x0 >= rec.n) return;
-    const uint32_t rows = min(rec.n - x0, 16u), n_parts = rec.last - blockIdx.x + 1u;
+    const uint32_t rows = min(rec.n - x0, 16u), n_parts = rec.last - worker + 1u;
     // shares of a row's parts: GROUPS / (rows rounded up to a power of two)
     uint32_t shares = GROUPS;
     while (shares > 1u && shares * rows > GROUPS) shares /= 2u;
@@ -551,7 +554,7 @@ __global__ void __launch_bounds__(256) paged_attn_join(SeqAttnArgs a, const Join
                 for (int k = 0; k < 4; k++) {
                     const uint32_t i = min(i0 + (uint32_t)k * shares, n_parts - 1u);
                     // a worker's second part where it is the rows' first
-                    const float* const p = parts + (size_t)(2u * (blockIdx.x + i) + (i == 0 ? 1u : 0u)) * (PR * (D + 2u));
+                    const float* const p = parts + (size_t)(2u * (worker + i) + (i == 0 ? 1u : 0u)) * (PR * (D + 2u));
                     pm[k] = p[PR * D + x];
                     pl[k] = i0 + (uint32_t)k * shares < n_parts ? p[PR * (D + 1u) + x] : -1.0f;
                     po[k] = *(const f32x4*)(p + x * D + d);

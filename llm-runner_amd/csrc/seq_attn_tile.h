@@ -434,7 +434,8 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, So
         t++;
         r0 = r1;
     };
-    for (bool first = true; t < n_tiles; first = false) {
+    for (bool first = true; first || (Source::kStages && t < n_tiles); first = false) {
+        if (Source::kStages && n_tiles == 0) break;
         // (the ring's slots go on by t: a source stages a multiple of 12 tiles, or the rest)
         const uint32_t seg = src.stage(t, n_tiles);
         if constexpr (Source::kStages) {
