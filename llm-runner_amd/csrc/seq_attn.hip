@@ -80,13 +80,11 @@ __global__ void __launch_bounds__(64 * NW, 1) prompt_attn_tiles(SeqAttnArgs a) {
     }
     row.live = row.live && start <= (int32_t)tok;
     const uint32_t lo = (uint32_t)max(start, 0);
-    row.jlo = row.live ? (lo > kv0 ? lo - kv0 : 0u) : seqattn::kNoKeys;
-    row.span = row.live ? tok - kv0 - row.jlo : 0u;
+    row.lo = lo > kv0 ? (int)(lo - kv0) : 0;
+    row.hi = row.live ? (int)(tok - kv0) : -1;
     row.q = (const uint8_t*)a.q + 2u * ((uint64_t)tok * a.q_stride + (uint64_t)head * a.q_head_stride);
-    const uint32_t lo_max = (uint32_t)seqattn::wave_imax(row.live ? (int)row.jlo : 0);
-    const int hi_min = seqattn::wave_imin(row.live ? (int)(tok - kv0) : 0x7ffffffe);
     PackedKeys src{(uint64_t)kv0 * a.kv_stride + (uint64_t)kvh * a.kv_head_stride, a.kv_stride * 2u, t1 + 1u - kv0};
-    seqattn::tile_rows<T, D, NW>(a, lds, src, t1 + 1u - kv0, row, lo_max, hi_min, nullptr, [&]() {
+    seqattn::tile_rows<T, D, NW>(a, lds, src, t1 + 1u - kv0, row, nullptr, [&]() {
         const uint32_t x = min(row0 + 32u * wave + (lane & 31u), rows - 1u);
         return (uint64_t)(x / G) * a.out_stride + (kvh * G + x % G) * D;
     });
@@ -99,12 +97,10 @@ hipError_t launch_tiles(const SeqAttnArgs& a, hipStream_t st) {
     return hipGetLastError();
 }
 
-
-
 using seqattn::PagedRequest;
 constexpr uint32_t kBlockRows = 256;  // rows of a workgroup of paged_attn_tiles
-constexpr uint32_t kPageCap = 8192;   // pages staged at a time: 2040 tiles of the smallest pages
-constexpr uint32_t kStageTiles = 2040;
+constexpr uint32_t kPageCap = 4096;   // pages staged at a time: 1020 tiles of the smallest pages
+constexpr uint32_t kStageTiles = 1020;
 
 // Keys in the pages of a cache: fragment tiles of 64 keys from key0 on. The request's pages
 // lie in LDS, kStageTiles tiles of them at a time, checked (~0: none).
@@ -173,10 +169,10 @@ __device__ __forceinline__ uint32_t block_tiles(const SeqAttnArgs& a, const Page
     return max((block_keys(a, rq, G, b) + seqattn::kKeys - 1u) / seqattn::kKeys, 1u);
 }
 // A block's units on the line: its tiles, the first of them kStart units more, for what
-// beginning a block costs (pages staged, the first tiles waited for: about four tiles' time;
-// without it a workgroup that got ten blocks of one tile was the last by far: 24 requests of
-// 1 to 511 new tokens 72 -> 40 us).
-constexpr uint32_t kStart = 4;
+// beginning a block costs (pages staged, the first tiles waited for, the end written). Without
+// it a workgroup that got ten blocks of one tile was the last by far: 24 requests of 1 to 511
+// new tokens 72 us; with 2, 3, 4, 6, 8, 10, 14: 43.4, 41.6, 40.0, 37.3, 37.8, 38.5, 39.6.
+constexpr uint32_t kStart = 6;
 __device__ __forceinline__ uint64_t request_units(const SeqAttnArgs& a, const PagedRequest& rq, uint32_t G) {
     uint64_t n = 0;
     for (uint32_t b = 0; b < blocks_of(rq, G); b++) n += block_tiles(a, rq, G, b) + kStart;
@@ -244,11 +240,9 @@ __device__ __forceinline__ void paged_tiles(const SeqAttnArgs& a, uint8_t* lds, 
         seqattn::RowOfLane row;
         row.live = row0 + 32u * wave + (lane & 31u) < rows;
         const int64_t pos = (int64_t)rq.pos0 + i - key0;  // last key it sees, of this part
-        const bool any = row.live && pos >= 0;
-        row.jlo = any ? 0u : seqattn::kNoKeys;
-        row.span = any ? (uint32_t)min(pos, (int64_t)0x7ffffffe) : 0u;
+        row.lo = 0;
+        row.hi = row.live ? (int)min(max(pos, (int64_t)-1), (int64_t)0x7ffffffe) : -1;
         row.q = (const uint8_t*)a.q + 2u * ((uint64_t)(rq.first + i) * a.q_stride + (uint64_t)(kvh * G + r % G) * a.q_head_stride);
-        const int hi_min = seqattn::wave_imin(row.live ? (any ? (int)row.span : -1) : 0x7ffffffe);
 
         // (the workgroup's last part is done with LDS)
         __syncthreads();
@@ -259,7 +253,7 @@ __device__ __forceinline__ void paged_tiles(const SeqAttnArgs& a, uint8_t* lds, 
         float* const part = t0 == 0 && t1 == tiles
                                 ? nullptr
                                 : scratch + (2u * blockIdx.x + (t0 == 0 ? 1u : 0u)) * tile_part_floats<D>();
-        seqattn::tile_rows<T, D, NW>(a, lds, src, n_keys, row, 0u, hi_min, part, out_at);
+        seqattn::tile_rows<T, D, NW>(a, lds, src, n_keys, row, part, out_at);
         if (t0 == 0 && t1 != tiles)  // (the workgroup's last part: the record is its one)
             rec = seqattn::JoinRecord{seqattn::part_of(at + (tiles - t1) - 1u, w, n), rq.first, row0,
                                       min(rows - row0, kBlockRows), kvh, {}};

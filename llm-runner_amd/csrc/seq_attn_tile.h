@@ -12,12 +12,17 @@
 //
 // S^T = K Q^T (32 keys x 32 rows an MFMA; Q in registers as the B operand), then
 // O^T += V^T P^T with P^T straight from the score registers. K and V tiles of 64
-// keys come by DMA into LDS rings of four and three slots, V row-major, read by
-// transposing reads. The scores start from -m_ref (a row's reference maximum),
-// so that p = exp2(c (s - m_ref)) is one multiplication and one exp2; m_ref is
-// raised lazily, when a maximum exceeds it by more than 2^8 in p. Scores,
-// maxima, sums and O are f32; P is rounded to the input type for its MFMA (bf16
-// or fp16, half a step 2^-8 or 2^-11 of each weight).
+// keys come by DMA into LDS rings of four slots each, K four tiles ahead and V
+// three; V lies row-major and is read by transposing reads. The scores start from
+// -m_ref (a row's reference maximum), so that p = exp2(c (s - m_ref)) is one
+// multiplication and one exp2; m_ref is raised lazily, when a maximum exceeds it by
+// more than 2^8 in p. Scores, maxima, sums and O are f32; P is rounded to the input
+// type for its MFMA (bf16 or fp16, half a step 2^-8 or 2^-11 of each weight).
+//
+// A wave whose 32 rows see nothing of a tile only moves its share of the DMA and
+// waits; masks are applied for the side (a request's beginning, the diagonal) that
+// cuts through a tile. 24 packed prompts of 13 to 414 tokens, fp16, 24/8 heads of 64:
+// 26.8 -> 23.7 us, bf16, 32/8 heads of 128: 43.7 -> 37.6.
 //
 // fp16 weights carry a factor 2^7, which the division takes out again: weights
 // below 2^-14 of the reference would lose bits, now below 2^-21, and the lazy
@@ -92,17 +97,6 @@ __device__ __forceinline__ float xhalf_sum(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-__device__ __forceinline__ int wave_imin(int v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
-    return __builtin_amdgcn_readfirstlane(v);
-}
-__device__ __forceinline__ int wave_imax(int v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
-    return __builtin_amdgcn_readfirstlane(v);
-}
-
 // Where a 16-byte chunk of key r lies within its row in an LDS slot: chunk c at
 // c ^ swizzle(r). K: a fragment read's 16 lanes (16 keys, one chunk) touch 16
 // distinct places of the 256 bytes the banks cover (a row of 256 bytes, or two
@@ -120,24 +114,22 @@ constexpr uint32_t kKeys = 64;  // keys of a tile
 
 template <uint32_t D>
 constexpr uint32_t tile_bytes() { return kKeys * D * 2u; }
-// LDS of a workgroup: four K and three V slots, then three words of its own; the
+// LDS of a workgroup: four K and four V slots, then three words of its own; the
 // epilogue stages 32 rows a wave in the rings.
 template <uint32_t D>
-constexpr uint32_t lds_bytes() { return 7u * tile_bytes<D>() + 16u; }
+constexpr uint32_t lds_bytes() { return 8u * tile_bytes<D>() + 16u; }
 
 // A lane's row. Keys are counted from the first one the workgroup takes; the row sees the
-// keys j with (uint32_t)(j - jlo) <= span (jlo = kNoKeys, span = 0: none).
-constexpr uint32_t kNoKeys = 0x80000000u;
+// keys lo .. hi (hi < lo: none); neither falls from row to row of a wave.
 struct RowOfLane {
-    uint32_t jlo, span;
+    int lo, hi;
     const uint8_t* q;  // the row's first byte (some row's, for a lane that has none)
     bool live;         // the lane has a row
 };
 
 // One workgroup: its rows over n_keys keys, into `out`, or, where part is given, as a part
 // to be joined with others: O[32 NW][D] f32, then m, then l (l = -1: the row sees no key of
-// the part). lo_max, hi_min: over the wave's rows, the last key that comes before one and
-// the first that comes behind one, less 1. Source: where keys come from,
+// the part). Source: where keys come from,
 //   uint32_t stage(t, n): tiles [t, its result) of n are made ready; kStages: a barrier and
 //     staged() come before the first is asked for;
 //   uint32_t page(t): of the wave's keys of tile t (read where lgkmcnt(0) is waited for);
@@ -150,8 +142,7 @@ struct RowOfLane {
 // out_at(): element offset of the lane's row in `out`.
 template <uint32_t T, uint32_t D, uint32_t NW, typename Source, typename OutAt>
 __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, Source& src, uint32_t n_keys,
-                                          const RowOfLane& row, uint32_t lo_max, int hi_min, float* part,
-                                          const OutAt& out_at) {
+                                          const RowOfLane& row, float* part, const OutAt& out_at) {
     constexpr uint32_t ROW = D * 2u, TILE = tile_bytes<D>();
     constexpr int NF = D / 8;                       // K fragments of a tile, and V fragments
     constexpr int CH = D / 32;                      // 32-dim blocks of a row
@@ -163,8 +154,8 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, So
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t l32 = lane & 31u, kh = lane >> 5;
     const float c = a.scale_log2, grow_by = 8.0f / c;
-    uint32_t* const wave_lohi = (uint32_t*)(lds + 7u * TILE);  // lo_max, hi_min over the workgroup
-    uint32_t* const any_bad = wave_lohi + 2;                    // a masked tile's V has an infinity or NaN
+    int* const wave_lohi = (int*)(lds + 8u * TILE);         // the workgroup's largest lo, smallest hi
+    uint32_t* const any_bad = (uint32_t*)(wave_lohi + 2);  // a masked tile's V has an infinity or NaN
 
     // Q fragments (B operand): row l32, dims 32 ch + 16 kh + 8 st ..
     s16x8 qf[CH][2];
@@ -175,7 +166,7 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, So
 
     if (tid == 0) {
         wave_lohi[0] = 0;
-        wave_lohi[1] = 0x7fffffffu;
+        wave_lohi[1] = 0x7ffffffe;
         *any_bad = 0;
     }
 
@@ -248,32 +239,60 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, So
     uint64_t seen = 0;  // lanes whose m_ref is a maximum of theirs
 
     const uint32_t n_tiles = (n_keys + kKeys - 1u) / kKeys;
-    // tiles [full0, full1) are seen whole by every row of the wave
-    const uint32_t full0 = (lo_max + kKeys - 1u) / kKeys, full1 = (uint32_t)(hi_min + 1) / kKeys;
-    auto masked = [&](uint32_t t) { return t < full0 || t >= full1 || src.holes(); };
+    // over the wave's rows that see a key: tiles [see0, see1) are seen by some, tiles [full0,
+    // full1) whole by every. lo and hi do not fall from row to row, so the first and the last of
+    // them say it.
+    uint32_t see0 = ~0u, see1 = 0, full0 = 0, full1 = ~0u;
+    int lo_max = 0, hi_min = 0x7ffffffe;
+    const uint64_t some = __builtin_amdgcn_ballot_w64(row.live && row.hi >= row.lo);
+    if (some != 0) {
+        const uint32_t a0 = (uint32_t)__builtin_ctzll(some), a1 = 63u - (uint32_t)__builtin_clzll(some);
+        see0 = (uint32_t)__builtin_amdgcn_readlane(row.lo, (int)(a0 & 31u)) / kKeys;
+        see1 = (uint32_t)__builtin_amdgcn_readlane(row.hi, (int)a1) / kKeys + 1u;
+        lo_max = __builtin_amdgcn_readlane(row.lo, (int)a1);
+        hi_min = __builtin_amdgcn_readlane(row.hi, (int)(a0 & 31u));
+        full0 = ((uint32_t)lo_max + kKeys - 1u) / kKeys;
+        full1 = ((uint32_t)hi_min + 1u) / kKeys;
+    }
     bool sees = false;  // a key
 
-    // scores of the keys a row does not see to -inf
+    // scores of the keys a row does not see to -inf: a compare with a constant and a select
+    // a score, for each side that the tile needs
     auto mask = [&](f32x16& h0, f32x16& h1, uint32_t t) {
-        const uint32_t rel = t * kKeys + 4u * kh - row.jlo;
+        int k0 = (int)(t * kKeys + 4u * kh);
+        // (without it the 64 compares of the first tile seen, the same all the time, are made ahead
+        // of everything, into scalars that spill)
+        asm volatile("" : "+v"(k0));
+        const bool holes = src.holes();
+        if (t >= full1 || holes) {
+            const int d = row.hi - k0;
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const uint32_t k = rel + 8u * (i >> 2) + (i & 3);
-            h0[i] = k <= row.span ? h0[i] : -INFINITY;
-            h1[i] = k + 32u <= row.span ? h1[i] : -INFINITY;
+            for (int i = 0; i < 16; i++) {
+                h0[i] = 8 * (i >> 2) + (i & 3) <= d ? h0[i] : -INFINITY;
+                h1[i] = 8 * (i >> 2) + (i & 3) + 32 <= d ? h1[i] : -INFINITY;
+            }
         }
-        if (src.holes()) {
+        if (t < full0 || holes) {
+            const int d = row.lo - k0;
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                h0[i] = 8 * (i >> 2) + (i & 3) >= d ? h0[i] : -INFINITY;
+                h1[i] = 8 * (i >> 2) + (i & 3) + 32 >= d ? h1[i] : -INFINITY;
+            }
+        }
+        if (holes) {
             const uint32_t on = src.groups(t);
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                const uint32_t k = rel + 8u * (i >> 2) + (i & 3);
+                const int k = k0 + 8 * (i >> 2) + (i & 3);
                 const bool p0 = (on >> (i >> 3)) & 1u, p1 = (on >> (2 + (i >> 3))) & 1u;
                 h0[i] = p0 ? h0[i] : -INFINITY;
                 h1[i] = p1 ? h1[i] : -INFINITY;
-                sees = sees || (p0 && k <= row.span) || (p1 && k + 32u <= row.span);
+                sees = sees || (p0 && k >= row.lo && k <= row.hi) || (p1 && k + 32 >= row.lo && k + 32 <= row.hi);
             }
         }
     };
+    auto masked = [&](uint32_t t) { return t < full0 || t >= full1 || src.holes(); };
     auto rescale = [&](uint64_t grow, float mx, f32x16& n0, f32x16& n1) {
         if (grow != 0) {
             const bool fresh = ((seen >> lane) & 1u) == 0;
@@ -302,12 +321,12 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, So
 
     // Infinities and NaN in V rows that some row of the workgroup does not see: its
     // weight there is 0, and 0 times them is NaN. Where a tile is masked they are set to 0
-    // in LDS before anyone reads it; the rows that do see them, with a weight above 0, get
-    // them from memory after the last tile.
+    // in LDS a tile before anyone reads it; the rows that do see them, with a weight above 0,
+    // get them from memory after the last tile.
     uint32_t wg_full0 = 0, wg_full1 = 0;
     auto wg_masked = [&](uint32_t t) { return t < wg_full0 || t >= wg_full1 || src.holes(); };
-    auto clean_v = [&](uint32_t t, uint32_t slot) {
-        uint8_t* const vt = lds + (4u + slot) * TILE;
+    auto clean_v = [&](uint32_t t) {
+        uint8_t* const vt = lds + (4u + (t & 3u)) * TILE;
 #pragma unroll
         for (uint32_t b = 0; b < TILE / (NW * 1024u); b++) {
             u32x4* const at = (u32x4*)(vt + (b * NW + wave) * 1024u + lane * 16u);
@@ -321,10 +340,6 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, So
                 }
             }
         }
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));  // lgkmcnt(0), the DMAs go on
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
     };
     auto add_bad = [&](uint32_t t) {
         const uint32_t j = t * kKeys + lane;
@@ -338,7 +353,7 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, So
         }
         for (uint64_t bad = __builtin_amdgcn_ballot_w64(n); bad != 0; bad &= bad - 1u) {
             const uint32_t key = t * kKeys + (uint32_t)__builtin_ctzll(bad);  // < n_keys: a lane found it there
-            const bool sees = key - row.jlo <= row.span;
+            const bool in = (int)key >= row.lo && (int)key <= row.hi;
             const uint8_t* const vr = src.row(a.v, key);
 #pragma unroll
             for (int dt = 0; dt < CH; dt++)
@@ -348,7 +363,7 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, So
                     const float x[4] = {lo_f32<T>(v.x), hi_f32<T>(v.x), lo_f32<T>(v.y), hi_f32<T>(v.y)};
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        o[dt][4 * g + e] += (int)sees & (int)!(fabsf(x[e]) < INFINITY) ? x[e] : 0.0f;
+                        o[dt][4 * g + e] += (int)in & (int)!(fabsf(x[e]) < INFINITY) ? x[e] : 0.0f;
                 }
         }
     };
@@ -357,22 +372,69 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, So
     uint32_t ka[CH][2];    // K(t+1)'s fragment addresses
     s16x8 kf[PF + 1];      // its fragments in flight: the first PF are read before the tile starts
     f32x16 h0, h1, h2;
-    uint32_t p2 = 0, p3 = 0, p4 = 0;  // pages of the wave's keys of tiles t + 2 .. t + 4
+    uint32_t p3 = 0, p4 = 0, p5 = 0;  // pages of the wave's keys of tiles t + 3, t + 4 and t + 5
+    uint32_t seg = 0;                 // tiles below it are ready
 
-    // One tile t: S(t) in (c0, c1), S(t+1) = K(t+1) Q^T to (n0, c0). K(t+1) is in K slot
-    // (t+1) % 4, V(t) in V slot vs; K(t+4) is DMAed to K slot t % 4 and V(t+2) to V slot vd.
-    // The MFMAs are issued in a fixed order with the vector work spread between them: the
-    // exponentials of S(t)'s first half before c0 is written again, those of the second
-    // half by the time its accumulation starts, the maximum of S(t+1) under the first
-    // accumulations, the first fragment reads of K(t+2) under the last ones.
-    auto tile = [&](f32x16& c0, f32x16& c1, f32x16& n0, uint32_t t, uint32_t vs, uint32_t vd) {
+    // S(t) by itself, into (n0, n1), and its maximum
+    auto scores = [&](f32x16& n0, f32x16& n1, uint32_t t) {
+        uint32_t kt[CH][2];
+        kaddr(t & 3u, kt);
+        static_for<0, NF>([&](auto F) {
+            constexpr int f = F, kb = f / (NF / 2), k = f % (NF / 2);
+            f32x16& s = kb == 0 ? n0 : n1;
+            s = mfma32<T>(kfrag(kt, f), qf[k / 2][k % 2], k == 0 ? f32x16{} - m_ref : s);
+        });
+        if (masked(t)) mask(n0, n1, t);
+        float mx = n0[0];
+#pragma unroll
+        for (int i = 0; i < 16; i++) mx = fmaxf(fmaxf(mx, n0[i]), n1[i]);
+        mx = xhalf_max(mx);
+        const uint64_t any = __builtin_amdgcn_ballot_w64(mx > -INFINITY);
+        rescale(__builtin_amdgcn_ballot_w64(mx > grow_by) | (any & ~seen), mx, n0, n1);
+        seen |= any;
+    };
+    // the first fragments of K(t), which the tile before it expects
+    auto first_frags = [&](uint32_t t) {
+        kaddr(t & 3u, ka);
+        static_for<0, PF>([&](auto F) { kf[F] = kfrag(ka, F); });
+    };
+    // O += P(t) V(t) by itself, S(t) in (c0, c1)
+    auto accumulate = [&](const f32x16& c0, const f32x16& c1, uint32_t t) {
+        uint32_t va[CH], p[16];
+        float rs = 0.0f;
+        static_for<0, 8>([&](auto I) { exp_pair(c0, I, p, rs); });
+        static_for<8, 16>([&](auto I) { exp_pair(c1, I, p, rs); });
+        l_i += rs;
+        vaddr(t & 3u, va);
+        static_for<0, NF>([&](auto F) {
+            constexpr int f = F, kb = f / (NF / 2), cc = (f % (NF / 2)) / CH, dt = f % CH;
+            o[dt] = mfma32<T>(vfrag(va, f), pfrag(p, kb, cc), o[dt]);
+        });
+    };
+    // What every wave does in tile t, whatever it sees of it: K(t+4) to K slot t % 4, V(t+3) to
+    // V slot (t+3) % 4 (both last read in tile t - 1), V(t+1) looked through where it is masked.
+    auto send = [&](uint32_t t) {
         dma(a.k, kvo, t + 4u, p4, t & 3u);
-        dma(a.v, vvo, t + 2u, p2, 4u + vd);
-        const uint32_t p5 = src.page(t + 5u);
-        if (wg_masked(t)) clean_v(t, vs);
+        dma(a.v, vvo, t + 3u, p3, 4u + ((t + 3u) & 3u));
+        p5 = src.page(t + 5u);
+        if (t + 1u < seg && wg_masked(t + 1u)) clean_v(t + 1u);
+    };
+    auto sent = [&]() {
+        LLMR_STAGE_BARRIER(2 * DI);
+        p3 = p4;
+        p4 = (uint32_t)__builtin_amdgcn_readfirstlane(p5);
+    };
+
+    // One tile t: S(t) in (c0, c1), S(t+1) = K(t+1) Q^T to (n0, c0). The MFMAs are issued in a
+    // fixed order with the vector work spread between them: the exponentials of S(t)'s first
+    // half before c0 is written again, those of the second half by the time its accumulation
+    // starts, the maximum of S(t+1) under the first accumulations, the first fragment reads of
+    // K(t+2) under the last ones.
+    auto tile = [&](f32x16& c0, f32x16& c1, f32x16& n0, uint32_t t) {
+        send(t);
         const bool mask_next = masked(t + 1u);
         uint32_t va[CH], p[16];
-        vaddr(vs, va);
+        vaddr(t & 3u, va);
         s16x8 vf[PF + 1];
         float rs = 0.0f, mt = -INFINITY, mx = 0.0f;
         uint64_t grow = 0, any = 0;
@@ -419,95 +481,74 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, So
         l_i += rs;
         rescale(grow, mx, n0, c0);
         seen |= any;
-        LLMR_STAGE_BARRIER(2 * DI);
-        p2 = p3;
-        p3 = p4;
-        p4 = (uint32_t)__builtin_amdgcn_readfirstlane(p5);
+        sent();
     };
 
-    // V(t) is in V slot t % 3; the score halves rotate with period 3: S(t) in (h0, h1),
-    // (h2, h0), (h1, h2)
-    uint32_t t = 0, r0 = 0;
-    auto step = [&](f32x16& c0, f32x16& c1, f32x16& n0) {
-        const uint32_t r1 = r0 == 2u ? 0u : r0 + 1u, r2 = r0 == 0u ? 2u : r0 - 1u;
-        tile(c0, c1, n0, t, r0, r2);
-        t++;
-        r0 = r1;
-    };
+    uint32_t t = 0;
     for (bool first = true; first || (Source::kStages && t < n_tiles); first = false) {
         if (Source::kStages && n_tiles == 0) break;
-        // (the ring's slots go on by t: a source stages a multiple of 12 tiles, or the rest)
-        const uint32_t seg = src.stage(t, n_tiles);
+        // (the rings' slots go on by t: a source stages a multiple of four tiles, or the rest)
+        seg = src.stage(t, n_tiles);
         if constexpr (Source::kStages) {
             __syncthreads();
             src.staged();
         }
-        if (!src.holes()) sees = sees || (row.jlo != kNoKeys && row.jlo + row.span >= t * kKeys);
-        {   // K(t) V(t) K(t+1) K(t+2) V(t+1) K(t+3) in flight
+        if (!src.holes()) sees = sees || (row.hi >= row.lo && row.hi >= (int)(t * kKeys));
+        {
             uint32_t pg[4];
 #pragma unroll
             for (uint32_t i = 0; i < 4u; i++) pg[i] = (uint32_t)__builtin_amdgcn_readfirstlane(src.page(t + i));
-            dma(a.k, kvo, t, pg[0], 0);
-            dma(a.v, vvo, t, pg[0], 4);
-            dma(a.k, kvo, t + 1u, pg[1], 1);
-            dma(a.k, kvo, t + 2u, pg[2], 2);
-            dma(a.v, vvo, t + 1u, pg[1], 5);
-            dma(a.k, kvo, t + 3u, pg[3], 3);
-            p2 = pg[2];
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; i++) {  // K(t) V(t) K(t+1) V(t+1) K(t+2) V(t+2) K(t+3) in flight
+                dma(a.k, kvo, t + i, pg[i], i);
+                if (i < 3u) dma(a.v, vvo, t + i, pg[i], 4u + i);
+            }
             p3 = pg[3];
             p4 = (uint32_t)__builtin_amdgcn_readfirstlane(src.page(t + 4u));
         }
-        LLMR_STAGE_BARRIER(5 * DI);  // K(t) has landed
+        // the wave's tiles of this segment: [see0, end)
+        const uint32_t end = min(see1, seg);
+        LLMR_STAGE_BARRIER(6 * DI);  // K(t) has landed
         if (first && lane == 0) {
             atomicMax(&wave_lohi[0], lo_max);
-            atomicMin((int*)&wave_lohi[1], hi_min);
+            atomicMin(&wave_lohi[1], hi_min);
         }
-        {   // S(t) and its maximum
-            kaddr(0, ka);
-            static_for<0, NF>([&](auto F) {
-                constexpr int f = F, kb = f / (NF / 2), k = f % (NF / 2);
-                f32x16& s = kb == 0 ? h0 : h1;
-                s = mfma32<T>(kfrag(ka, f), qf[k / 2][k % 2], k == 0 ? f32x16{} - m_ref : s);
-            });
-            if (masked(t)) mask(h0, h1, t);
-            float mx = h0[0];
-#pragma unroll
-            for (int i = 0; i < 16; i++) mx = fmaxf(fmaxf(mx, h0[i]), h1[i]);
-            mx = xhalf_max(mx);
-            const uint64_t any = __builtin_amdgcn_ballot_w64(mx > -INFINITY);
-            rescale(__builtin_amdgcn_ballot_w64(mx > grow_by) | (any & ~seen), mx, h0, h1);
-            seen |= any;
-        }
-        LLMR_STAGE_BARRIER(2 * DI);  // K(t+1), K(t+2), V(t) have landed; every wave is done with K(t)
+        if (see0 <= t && t < end) scores(h0, h1, t);
+        LLMR_STAGE_BARRIER(2 * DI);  // K(t+1), V(t), K(t+2), V(t+1) have landed
         if (first) {
-            wg_full0 = ((uint32_t)__builtin_amdgcn_readfirstlane(wave_lohi[0]) + kKeys - 1u) / kKeys;
-            wg_full1 = ((uint32_t)__builtin_amdgcn_readfirstlane(wave_lohi[1]) + 1u) / kKeys;
+            wg_full0 = (uint32_t)(__builtin_amdgcn_readfirstlane(wave_lohi[0]) + (int)kKeys - 1) / kKeys;
+            wg_full1 = (uint32_t)(__builtin_amdgcn_readfirstlane(wave_lohi[1]) + 1) / kKeys;
         }
-        kaddr(1, ka);
-        static_for<0, PF>([&](auto F) { kf[F] = kfrag(ka, F); });
-        r0 = 0;
-        while (t + 4u <= seg) {
-            step(h0, h1, h2);
-            step(h2, h0, h1);
-            step(h1, h2, h0);
+        if (wg_masked(t)) {
+            clean_v(t);
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));  // lgkmcnt(0), the DMAs go on
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
         }
-        while (t + 1u < seg) {
-            step(h0, h1, h2);
-            h1 = h0;
-            h0 = h2;
-        }
-        {   // the last staged tile: its scores are in (h0, h1), its V in slot r0
-            uint32_t va[CH], p[16];
-            if (wg_masked(t)) clean_v(t, r0);
-            float rs = 0.0f;
-            static_for<0, 8>([&](auto I) { exp_pair(h0, I, p, rs); });
-            static_for<8, 16>([&](auto I) { exp_pair(h1, I, p, rs); });
-            l_i += rs;
-            vaddr(r0, va);
-            static_for<0, NF>([&](auto F) {
-                constexpr int f = F, kb = f / (NF / 2), cc = (f % (NF / 2)) / CH, dt = f % CH;
-                o[dt] = mfma32<T>(vfrag(va, f), pfrag(p, kb, cc), o[dt]);
-            });
+        // Before the wave's first tile it sees nothing, then come its scores; S(t+1) is computed
+        // beside P(t) V(t), the score halves rotating with period 3 (S(t) in (h0, h1), (h2, h0),
+        // (h1, h2)); then its last P V, and nothing again.
+        while (t < seg) {
+            if (t >= see0 && t + 1u < end) {
+                first_frags(t + 1u);
+                while (t + 4u <= end) {
+                    tile(h0, h1, h2, t);
+                    tile(h2, h0, h1, t + 1u);
+                    tile(h1, h2, h0, t + 2u);
+                    t += 3u;
+                }
+                while (t + 1u < end) {
+                    tile(h0, h1, h2, t);
+                    h1 = h0;
+                    h0 = h2;
+                    t++;
+                }
+            }
+            send(t);
+            if (t >= see0 && t + 1u == end) accumulate(h0, h1, t);
+            if (t + 1u == see0 && see0 < end) scores(h0, h1, see0);
+            sent();
             t++;
         }
         LLMR_WAIT_VMCNT(0);  // no DMA may still be writing LDS when something else goes there
