@@ -564,7 +564,8 @@ LLMR_API int llmr_flash_attention_pc(llmr_context* ctx, const void* q, const voi
  * within [0, n_tokens], a page outside [0, n_pages) or past the table's columns
  * is a page of keys nobody sees, a slot outside the cache stores nothing. Rows
  * that belong to no request (a batch padded to a captured size) are left as they
- * are. None of these calls allocates.
+ * are. None of these calls allocates; the attention's out may not overlap its
+ * keys or values.
  * ------------------------------------------------------------------------- */
 
 /* Most requests of one llmr_paged_plan or llmr_paged_attention call. */
@@ -590,8 +591,8 @@ typedef struct llmr_prompt_attention_params {
  * and out of type F16 or BF16, 16-byte aligned; seq_offsets [n_seqs + 1],
  * nondecreasing (a request may have no rows). Scores, the running maximum and
  * sum and the accumulated rows are f32; the softmax weights are rounded to
- * `type` for the products with v, and the sums that divide are of the rounded
- * weights. A key or value row changes no row of out that does not see it,
+ * `type` for the products with v, the sums that divide are of the weights
+ * before that. A key or value row changes no row of out that does not see it,
  * whatever it holds (infinities and NaN too). Of the reference's
  * attention_prefill (dependencies/llm_text.c3l/shaders/llm.slang), for a whole
  * batch of prompts in one launch. */

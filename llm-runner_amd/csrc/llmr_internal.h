@@ -211,7 +211,6 @@ struct SeqAttnArgs {
     uint32_t page_log2, n_pages, max_pages, max_new;
     float scale_log2;         // softmax scale * log2(e)
 };
-constexpr uint32_t kMaxSeqs = 4096;
 hipError_t launch_prompt_attention(const SeqAttnArgs& a, uint32_t type, uint32_t dim, int num_cus, hipStream_t st);
 size_t paged_attention_scratch_bytes(uint32_t dim, uint32_t n_heads, uint32_t n_kv_heads, uint32_t max_new, int num_cus);
 hipError_t launch_paged_attention(const SeqAttnArgs& a, uint32_t type, uint32_t dim, int num_cus, void* scratch,

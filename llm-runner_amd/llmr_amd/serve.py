@@ -26,6 +26,7 @@ from .ops import RenderGraph, default_graph
 
 _TYPES = {torch.float16: GGML_F16, torch.bfloat16: GGML_BF16}
 _I32, _F32 = torch.int32, torch.float32
+_U32 = 0xffffffff  # the parameters' integers
 # the stream's handle alone, without the Stream object that torch.cuda.current_stream makes
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda dev: torch.cuda.current_stream(dev).cuda_stream)
@@ -69,12 +70,14 @@ def _heads(t: torch.Tensor, what: str):
     ts, hs, ds = t.stride()
     if ds != 1:
         raise ValueError(f"{what} must be [tokens, heads, head_dim] with contiguous heads")
+    if ts > _U32 or hs > _U32:
+        raise ValueError(f"{what}'s strides must be under 2^32 elements")
     return T, H, D, ts if T > 1 else H * D, hs if H > 1 else D
 
 
 def _out_stride(out: torch.Tensor, T: int, width: int, like: torch.Tensor) -> int:
-    if out.dtype is not like.dtype or out.shape != (T, width) or out.stride(1) != 1:
-        raise ValueError(f"out must be a [{T}, {width}] view of q's dtype with contiguous rows")
+    if out.dtype is not like.dtype or out.shape != (T, width) or out.stride(1) != 1 or out.stride(0) > _U32:
+        raise ValueError(f"out must be a [{T}, {width}] view of q's dtype with contiguous rows, under 2^32 apart")
     return out.stride(0) if T > 1 else width
 
 
@@ -162,8 +165,8 @@ def qkv_tokens(qkv: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Ten
     caches [n_pages, n_kv_heads, page_size, D], a row with slot -1 nowhere; without, rows [T, n_kv_heads, D].
     rope: (cos, sin) f32 [n_positions, D / 2], taken at positions (int32 [T]; None: the row), rotating the
     pairs (j, j + D/2), or (2j, 2j + 1) where halves is False."""
-    if qkv.dim() != 2 or qkv.dtype is not _F32 or (qkv.shape[1] > 1 and qkv.stride(1) != 1):
-        raise ValueError("qkv must be a 2-D f32 view with contiguous rows")
+    if qkv.dim() != 2 or qkv.dtype is not _F32 or (qkv.shape[1] > 1 and qkv.stride(1) != 1) or qkv.stride(0) > _U32:
+        raise ValueError("qkv must be a 2-D f32 view with contiguous rows, under 2^32 apart")
     T, H, D, qs, qh = _heads(q, "q")
     if qkv.shape[0] != T or qh != D:
         raise ValueError("q must be [tokens, n_heads, head_dim] with qkv's tokens and heads side by side")
@@ -199,6 +202,8 @@ def paged_attention_scratch(q: torch.Tensor, k_cache: torch.Tensor, block_table:
     """A scratch tensor for paged_attention calls of these shapes (llmr_paged_attention_scratch_bytes)."""
     T, H, D = q.shape
     n_pages, Hk, page, _ = k_cache.shape
+    if max_new < 0:
+        raise ValueError("max_new must be >= 0")
     p = capi.PagedAttentionParams(D, H, Hk, T, block_table.shape[0], min(max_new, T), page, n_pages,
                                   block_table.shape[1], H * D, H * D, 1.0)
     g = _graph(g, q)
@@ -221,6 +226,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise ValueError("q must be [tokens, n_heads, head_dim], heads side by side, with the caches' head_dim")
     if seq_offsets.numel() != n + 1 or block_table.dim() != 2 or block_table.shape[0] != n:
         raise ValueError("kv_len, block_table's rows and seq_offsets (one more) must be one per request")
+    if max_new < 0:
+        raise ValueError("max_new must be >= 0")
     t = _type("q and the caches", q, k_cache, v_cache)
     if out is None:
         out = torch.empty(T, H * D, dtype=q.dtype, device=q.device)

@@ -2,8 +2,9 @@
 64 bits, element by element.
 
 Where a tolerance is compared, it is this bound. With u = eps / 2 of the type (half a step):
-  - a softmax weight is rounded to the type once, and the sum that divides is of the rounded weights: the result
-    is a mean with weights p_j (1 + d_j), |d_j| <= u, off by at most 2 u A / (1 - u), A = sum_j p_j |v_j|;
+  - a softmax weight is rounded to the type once, for its product with v: weights p_j (1 + d_j), |d_j| <= u. The
+    sum that divides is of the weights before that: the result is off by at most u A, A = sum_j p_j |v_j|; by
+    at most 2 u A / (1 - u), which is what is allowed here, were it of the rounded ones;
   - a score is a f32 sum of D products: off by at most (D + 4) 2^-24 sum_d |q_d k_jd| scale (the four: the scale,
     its product with log2(e), the running maximum's subtraction), its exponential relatively as much, and 2^-22
     for exp2 itself and the sums' own f32 additions (their terms are non-negative: a tree over 64 lanes or fewer
@@ -129,6 +130,38 @@ def test_prompt_attention(dev, dtype, D, H, Hk, lens, pad):
     assert serve.prompt_attention(q, k, v, off, out=out) is out
     torch.cuda.synchronize()
     _prompt_check(q, k, v, at, out, 1 / math.sqrt(D), f"{dtype} D={D} H={H}/{Hk}", 7.0)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("D,H,Hk,lens", [(64, 24, 8, [2800, 150]), (64, 18, 6, [13, 40, 200, 1, 370, 90] * 6),
+                                         (128, 20, 5, [5, 130, 64, 300] * 5)], ids=["long", "ragged", "ragged128"])
+def test_prompt_attention_more_rows_than_the_card_holds(dev, dtype, D, H, Hk, lens):
+    """256 rows a workgroup: waves whose rows begin or end tiles away from their neighbours'."""
+    from llmr_amd import serve
+    q, k, v, at, off = _prompt_case(dev, dtype, D, H, Hk, lens, seed=len(lens))
+    out = serve.prompt_attention(q, k, v, off)
+    torch.cuda.synchronize()
+    _prompt_check(q, k, v, at, out, 1 / math.sqrt(D), f"{dtype} D={D} H={H}/{Hk}")
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_prompt_attention_unseen_values_across_requests(dev, bad):
+    """Keys and values of one packed request that are not finite reach no row of its neighbours, whichever tile of a
+    shared workgroup they lie in."""
+    from llmr_amd import serve
+    lens = [30, 100, 200, 7, 64, 64, 90, 1, 150]
+    q, k, v, at, off = _prompt_case(dev, BF16, 128, 8, 2, lens, seed=17)
+    ref = serve.prompt_attention(q, k, v, off)
+    for i in (1, 3, 5, 8):
+        for t in (k, v):
+            t[at[i]:at[i + 1]] = bad
+    out = serve.prompt_attention(q, k, v, off)
+    torch.cuda.synchronize()
+    for i, (a, b) in enumerate(zip(at, at[1:])):
+        if i in (1, 3, 5, 8):
+            assert not bool(out[a:b].isfinite().any()), i
+        else:
+            assert torch.equal(out[a:b], ref[a:b]), i
 
 
 @pytest.mark.parametrize("layout", ["columns", "heads"])
@@ -372,6 +405,44 @@ def test_paged_attention(dev, dtype, D, H, Hk, page, past, new, pad):
     out2 = serve.paged_attention(q, kc, vc, off, kvl, wide, q.shape[0])
     torch.cuda.synchronize()
     _paged_check(q, rows, at, kv, out2, 1 / math.sqrt(D), "wide")
+
+
+# more requests than a wave's lanes, some of them with nothing new, at the ends too
+MANY = [(128, 8, 2, [0, 1, 1, 0, 1] * 40), (64, 8, 2, [0, 5, 1, 8] * 30 + [0] * 70 + [3]), (128, 8, 2, [16, 0, 9, 1] * 20),
+        (64, 4, 1, [0] * 65 + [70, 1, 0, 300, 2] * 14 + [0] * 3)]
+
+
+@pytest.mark.parametrize("D,H,Hk,new", MANY, ids=["1", "8", "16", "300"])
+def test_paged_attention_many_requests(dev, D, H, Hk, new):
+    from llmr_amd import serve
+    past = [(37 * i * i) % 211 for i in range(len(new))]
+    q, kc, vc, rows, at, off, kvl, table, kv = _paged_case(dev, BF16, D, H, Hk, 16, past, new, 2, seed=len(new))
+    out = torch.full((q.shape[0], H * D), 7.0, dtype=BF16, device=dev)
+    serve.paged_attention(q, kc, vc, off, kvl, table, max(new), out=out)
+    torch.cuda.synchronize()
+    _paged_check(q, rows, at, kv, out, 1 / math.sqrt(D), f"{len(new)} requests")
+    assert bool((out[at[-1]:] == 7).all())
+
+
+@pytest.mark.parametrize("hole", [None, 1000, 68000], ids=["whole", "hole-early", "hole-late"])
+def test_paged_attention_table_longer_than_is_staged_at_once(dev, hole):
+    """2048 new tokens behind 70000 keys: a workgroup's share is more tiles than it keeps pages of. Keys on no page
+    are nobody's; the first and last rows of the chunk are looked at."""
+    from llmr_amd import serve
+    D, H, Hk, page, past, new = 64, 32, 8, 16, 70000, 2048
+    q, kc, vc, rows, at, off, kvl, table, kv = _paged_case(dev, F16, D, H, Hk, page, [past], [new], seed=5)
+    k, v = rows[0]
+    if hole is not None:
+        table[0, hole // page] = -1
+        lo = hole // page * page
+        k, v = (torch.cat([t[:lo], t[lo + page:]]) for t in (k, v))
+        past -= page
+    out = serve.paged_attention(q, kc, vc, off, kvl, table, new)
+    torch.cuda.synchronize()
+    vm = float(v.double().abs().max())
+    for a, b in ((0, 20), (new - 20, new)):
+        o, A, e = _definition(q[a:b], k, v, 1 / math.sqrt(D), past + a)
+        _check(out[a:b].unflatten(1, (H, D)), o, A, e, vm, past + b, F16, f"rows {a} .. {b}")
 
 
 @pytest.mark.parametrize("qstd", [30.0, 0.01])

@@ -63,3 +63,25 @@ def test_shapes_are_checked():
         serve.paged_attention(q, cache, cache.float(), i32(3), i32(2), i32(4).view(2, 2), 1)
     with pytest.raises(ValueError, match="qkv"):
         serve.qkv_tokens(torch.zeros(4, 3 * 64), q, q[:, :1], q[:, :1])
+
+
+def test_max_new_is_not_negative():
+    i32 = lambda n: torch.zeros(n, dtype=torch.int32)  # noqa: E731
+    cache, q = torch.zeros(3, 1, 16, 64, dtype=F16), torch.zeros(4, 2, 64, dtype=F16)
+    with pytest.raises(ValueError, match="max_new"):
+        serve.paged_attention(q, cache, cache.clone(), i32(3), i32(2), i32(4).view(2, 2), -1)
+    with pytest.raises(ValueError, match="max_new"):
+        serve.paged_attention_scratch(q, cache, i32(4).view(2, 2), -1)
+
+
+def test_strides_past_32_bits_are_refused():
+    """(They would be cut to the parameters' 32 bits.)"""
+    far = lambda n, h: torch.empty_strided((n, h, 64), (64, 1 << 32, 1), dtype=F16, device="meta")  # noqa: E731
+    off = torch.tensor([0, 4], dtype=torch.int32)
+    q = torch.zeros(4, 2, 64, dtype=F16)
+    with pytest.raises(ValueError, match="2\\^32"):
+        serve.prompt_attention(q, far(4, 2), far(4, 2), off)
+    with pytest.raises(ValueError, match="2\\^32"):
+        serve.prompt_attention(far(4, 2), q, q.clone(), off)
+    with pytest.raises(ValueError, match="2\\^32"):
+        serve.qkv_tokens(torch.empty_strided((4, 256), (1 << 32, 1), device="meta"), q, q[:, :1], q[:, :1])
