@@ -1,7 +1,9 @@
 /*
  * llmr_hip.h - C-ABI of the MI355X (gfx950) backend for llm-runner's DiT
  * transformer-block hot path: GGUF block-quantized dequant-GEMM (Q8_0, Q4_K)
- * and non-causal flash attention.
+ * and non-causal flash attention; and for batches of requests of the text path
+ * beside it: causal attention with grouped heads over packed prompts and over a
+ * paged key/value cache, with what plans and fills that cache.
  *
  * Plain C: POD arguments, device pointers as void*, sizes as uint32_t/size_t,
  * int status (0 = OK). Nothing here names a HIP or torch type, so a C3

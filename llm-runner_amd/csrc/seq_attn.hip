@@ -274,10 +274,11 @@ hipError_t launch_prompt_attention(const SeqAttnArgs& a, uint32_t type, uint32_t
     auto go = [&](auto t, auto d) {
         constexpr uint32_t T = decltype(t)::value, D = decltype(d)::value;
         // 128 rows a workgroup where all of them are on the card at once (one a CU, two with
-        // head_dim 64: their LDS): a tile takes a wave alone on its SIMD as long as two, so fewer
-        // rows on more CUs end earlier. 512 tokens of 32/8 heads, 128: 19.5 -> 16.9 us, 1000: 30.7
-        // -> 26.6; 24/8 heads, 64, 1024: 23.2 -> 19.9, 2048: 40.4 -> 34.9. Past that a second round
-        // may cost what it gains: 10 x 200 tokens of 24/8 heads, 128: 20.4 against 25.6.
+        // head_dim 64: their LDS): a tile takes a wave alone on its SIMD nearly as long as two, so
+        // fewer rows on more CUs end earlier. With 256 and 128 rows, us: 512 tokens of 32/8 heads,
+        // 128: 19.6, 16.9; 1000: 30.7, 27.1; 24/8 heads, 64, 1024: 23.3, 19.5; 2048: 41.9, 35.3.
+        // Past that there is a second round: 10 x 200 tokens of 24/8 heads, 128: 17.7, 25.3; 4096
+        // of 32/8: 139, 178.
         const uint64_t rows = (uint64_t)a.n_tokens * (a.n_heads / a.n_kv_heads);
         const bool fits = (rows + 127u) / 128u * a.n_kv_heads <= (uint64_t)num_cus * (D == 64u ? 2u : 1u);
         return fits ? launch_tiles<T, D, 4>(a, st) : launch_tiles<T, D, 8>(a, st);
