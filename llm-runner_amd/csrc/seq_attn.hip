@@ -308,23 +308,27 @@ size_t paged_attention_scratch_bytes(uint32_t dim, uint32_t n_heads, uint32_t n_
     return paged_workers(nr, num_cus) * (sizeof(seqattn::JoinRecord) + 2u * part);
 }
 
+template <uint32_t R>
+using Rows = std::integral_constant<uint32_t, R>;
+
 template <uint32_t T, uint32_t D>
 static hipError_t launch_paged(const SeqAttnArgs& a, uint32_t nr, int num_cus, void* scratch, hipStream_t st) {
+    using namespace seqattn;
     const uint32_t n = paged_workers(nr, num_cus);
     auto* const records = (seqattn::JoinRecord*)scratch;
     auto* const parts = (float*)(records + n);
-    auto go = [&](auto work, uint32_t threads, auto join, uint32_t part_rows) {
+    auto go = [&](auto work, uint32_t threads, auto join, auto part) {
+        constexpr uint32_t PR = decltype(part)::value;
         hipLaunchKernelGGL(work, dim3(n), dim3(threads), 0, st, a, records, parts);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
-        hipLaunchKernelGGL(join, dim3(part_rows / 16u, n), dim3(256), 0, st, a, records, parts);
+        hipLaunchKernelGGL(join, dim3(PR / 16u, n), dim3(join_threads<D, PR>()), 0, st, a, records, parts);
         return hipGetLastError();
     };
-    using namespace seqattn;
-    if (nr == 0u) return go(paged_attn_tiles<T, D>, 512, paged_attn_join<T, D, kBlockRows>, kBlockRows);
-    if (nr == 1u) return go(paged_attn_few<T, D, 1>, 64, paged_attn_join<T, D, 16>, 16);
-    if (nr == 2u) return go(paged_attn_few<T, D, 2>, 64, paged_attn_join<T, D, 32>, 32);
-    return go(paged_attn_few<T, D, 4>, 64, paged_attn_join<T, D, 64>, 64);
+    if (nr == 0u) return go(paged_attn_tiles<T, D>, 512, paged_attn_join<T, D, kBlockRows>, Rows<kBlockRows>{});
+    if (nr == 1u) return go(paged_attn_few<T, D, 1>, 64, paged_attn_join<T, D, 16>, Rows<16>{});
+    if (nr == 2u) return go(paged_attn_few<T, D, 2>, 64, paged_attn_join<T, D, 32>, Rows<32>{});
+    return go(paged_attn_few<T, D, 4>, 64, paged_attn_join<T, D, 64>, Rows<64>{});
 }
 
 hipError_t launch_paged_attention(const SeqAttnArgs& a, uint32_t type, uint32_t dim, int num_cus, void* scratch,

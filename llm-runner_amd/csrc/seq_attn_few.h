@@ -531,10 +531,18 @@ paged_attn_few(SeqAttnArgs a, JoinRecord* __restrict__ records, float* __restric
 // threads hold, or fewer with their parts shared by several groups of D / 4 threads, so that no
 // row takes more than a few rounds of loads (35 parts of four rows: 21.8 -> 6.0). PR: rows of a
 // part.
+// Parts of 16 rows come from many waves (138 of five rows where one of 20306 keys is the
+// longest of five): 16 rows or shares at a time, eight parts' loads in flight a thread; 56 ->
+// 42 us for that call, 14.0 -> 12.6 for one request of 1100 keys. Larger parts are fewer and
+// have rows enough: with as many threads 24 mixed requests took 43 us for 39.
+template <uint32_t D, uint32_t PR>
+constexpr uint32_t join_threads() { return PR == 16u ? 4u * D : 256u; }
+
 template <uint32_t T, uint32_t D, uint32_t PR>
-__global__ void __launch_bounds__(256) paged_attn_join(SeqAttnArgs a, const JoinRecord* __restrict__ records,
-                                                       const float* __restrict__ parts) {
-    constexpr uint32_t LPR = D / 4u, GROUPS = 256u / LPR;  // threads of a row, rows or shares at a time
+__global__ void __launch_bounds__((join_threads<D, PR>()))
+paged_attn_join(SeqAttnArgs a, const JoinRecord* __restrict__ records, const float* __restrict__ parts) {
+    constexpr uint32_t LPR = D / 4u, GROUPS = join_threads<D, PR>() / LPR;  // threads of a row, rows or shares at a time
+    constexpr uint32_t LOADS = PR == 16u ? 8u : 4u;  // parts of a thread in flight
     __shared__ f32x4 so[GROUPS][LPR];
     __shared__ float sm[GROUPS], sl[GROUPS];
     const uint32_t worker = blockIdx.y, x0 = 16u * blockIdx.x;
@@ -552,11 +560,11 @@ __global__ void __launch_bounds__(256) paged_attn_join(SeqAttnArgs a, const Join
         f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
         float m = -INFINITY, l = -1.0f;  // l = -1: no key seen
         if (live) {
-            for (uint32_t i0 = share; i0 < n_parts; i0 += 4u * shares) {
-                float pm[4], pl[4];
-                f32x4 po[4];
+            for (uint32_t i0 = share; i0 < n_parts; i0 += LOADS * shares) {
+                float pm[LOADS], pl[LOADS];
+                f32x4 po[LOADS];
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
+                for (int k = 0; k < (int)LOADS; k++) {
                     const uint32_t i = min(i0 + (uint32_t)k * shares, n_parts - 1u);
                     // a worker's second part where it is the rows' first
                     const float* const p = parts + (size_t)(2u * (worker + i) + (i == 0 ? 1u : 0u)) * (PR * (D + 2u));
@@ -565,7 +573,7 @@ __global__ void __launch_bounds__(256) paged_attn_join(SeqAttnArgs a, const Join
                     po[k] = *(const f32x4*)(p + x * D + d);
                 }
 #pragma unroll
-                for (int k = 0; k < 4; k++) join_part(o, m, l, po[k], pm[k], pl[k], a.scale_log2);
+                for (int k = 0; k < (int)LOADS; k++) join_part(o, m, l, po[k], pm[k], pl[k], a.scale_log2);
             }
         }
         if (shares > 1u) {
