@@ -241,7 +241,9 @@ __device__ __forceinline__ void paged_tiles(const SeqAttnArgs& a, uint8_t* lds, 
         row.live = row0 + 32u * wave + (lane & 31u) < rows;
         const int64_t pos = (int64_t)rq.pos0 + i - key0;  // last key it sees, of this part
         row.lo = 0;
-        row.hi = row.live ? (int)min(max(pos, (int64_t)-1), (int64_t)0x7ffffffe) : -1;
+        // not past the part's keys: where a length passes the end of the table, which need not be
+        // the end of a tile, what the last tile holds behind them is no key
+        row.hi = row.live ? (int)min(max(pos, (int64_t)-1), (int64_t)n_keys - 1) : -1;
         row.q = (const uint8_t*)a.q + 2u * ((uint64_t)(rq.first + i) * a.q_stride + (uint64_t)(kvh * G + r % G) * a.q_head_stride);
 
         // (the workgroup's last part is done with LDS)

@@ -683,3 +683,26 @@ def test_paged_attention_refuses(dev):
         serve.paged_attention(q, kc, vc, torch.zeros(big + 1, dtype=torch.int32, device=dev),
                               torch.zeros(big, dtype=torch.int32, device=dev),
                               torch.zeros(big, 1, dtype=torch.int32, device=dev), 1)
+
+
+# ---- what the chunk form counts -----------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("D,cols", [(128, 1), (64, 2), (128, 3), (64, 4), (64, 5), (128, 15)])
+@pytest.mark.parametrize("new", [1, 12, 70])
+def test_paged_attention_lengths_past_the_table(dev, dtype, D, cols, new):
+    """Requests that outgrew their table (paged_plan's kv_len goes on): the keys are those of its pages and no other,
+    at every remainder of a tile that the table may end at, in the form for few rows and in the one for chunks."""
+    from llmr_amd import serve
+    cap = 16 * cols
+    q, kc, vc, rows, at, off, _, table, _ = _paged_case(dev, dtype, D, 4, 2, 16, [cap, cap, cap], [new] * 3, seed=cols)
+    lens = [cap + 1000, cap + 20, 2 ** 31 - 1]
+    out = serve.paged_attention(q, kc, vc, off, torch.tensor(lens, dtype=torch.int32, device=dev),
+                                table[:, :cols].contiguous(), new)
+    torch.cuda.synchronize()
+    for i, (a, b) in enumerate(zip(at, at[1:])):
+        k, v = (x[:cap] for x in rows[i])
+        o, A, e = _definition(q[a:b], k, v, 1 / math.sqrt(D), lens[i] - new)
+        _check(out[a:b].unflatten(1, (4, D)), o, A, e, float(v.double().abs().max()), cap, dtype,
+               f"{cols} pages, length {lens[i]}, {new} new")
