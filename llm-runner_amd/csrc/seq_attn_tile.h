@@ -563,7 +563,10 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, So
             if (wg_masked(t)) add_bad(t);
 
     const float l_sum = xhalf_sum(l_i);
-    sees = sees || __shfl_xor((int)sees, 32, 64);
+    // the row's other lane has seen the keys between its own (asked by every lane: behind a `||` the
+    // lanes that have seen some would not take part, and the others would read nothing from them)
+    const int other = __shfl_xor((int)sees, 32, 64);
+    sees = sees || other != 0;
     if (part != nullptr) {
         float* const po = part + (size_t)(wave * 32u + l32) * D;
         if (row.live) {

@@ -706,3 +706,26 @@ def test_paged_attention_lengths_past_the_table(dev, dtype, D, cols, new):
         o, A, e = _definition(q[a:b], k, v, 1 / math.sqrt(D), lens[i] - new)
         _check(out[a:b].unflatten(1, (4, D)), o, A, e, float(v.double().abs().max()), cap, dtype,
                f"{cols} pages, length {lens[i]}, {new} new")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("D,new,hole", [(128, 64, 3), (64, 64, 0), (128, 64, 1), (64, 20, 0), (128, 150, 0), (64, 150, 4),
+                                        (128, 150, 9), (64, 5, 0)])
+def test_paged_attention_rows_of_a_chunk_around_a_missing_page(dev, dtype, D, new, hole):
+    """A chunk over an empty cache with one page lacking (as paged_plan enters it): rows that see only the first few
+    keys of a page are whole, before the hole and behind it."""
+    from llmr_amd import serve
+    q, kc, vc, rows, at, off, kvl, table, kv = _paged_case(dev, dtype, D, 4, 2, 16, [0], [new], seed=hole + new)
+    table[0, hole] = -1
+    out = torch.full((new, 4 * D), 7.0, dtype=dtype, device=dev)
+    serve.paged_attention(q, kc, vc, off, kvl, table, new, out=out)
+    torch.cuda.synchronize()
+    k, v = rows[0]
+    lo, hi = min(16 * hole, new), min(16 * hole + 16, new)
+    seen = [torch.cat([x[:lo], x[hi:]]) for x in (k, v)]
+    for a, b, kk, vv, first in ((0, lo, k[:lo], v[:lo], 0), (lo, hi, k[:lo], v[:lo], lo), (hi, new, *seen, lo)):
+        if b > a and len(kk):
+            o, A, e = _definition(q[a:b], kk, vv, 1 / math.sqrt(D), first)
+            _check(out[a:b].unflatten(1, (4, D)), o, A, e, float(vv.double().abs().max()), new, dtype, f"rows {a} .. {b}")
+        else:  # keys of the missing page alone
+            assert bool((out[a:b] == 0).all()), (a, b)
