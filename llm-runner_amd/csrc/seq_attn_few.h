@@ -466,7 +466,8 @@ __device__ __forceinline__ void few_rows(const SeqAttnArgs& a, uint8_t* lds, Joi
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
             const bool fr = (fresh >> r) & 1u;
             if (__builtin_amdgcn_ballot_w64(mx > grow_by || (fr && mx > -INFINITY)) != 0) {
-                const float d = fr ? (mx > -INFINITY ? mx : 0.0f) : fmaxf(mx, 0.0f);
+                // (only rows whose own maximum calls for it)
+                const float d = fr ? (mx > -INFINITY ? mx : 0.0f) : (mx > grow_by ? mx : 0.0f);
                 const float alpha = fr ? 0.0f : __builtin_amdgcn_exp2f(-d * c);
                 m_ref[r] += d;
                 l_i[r] *= alpha;

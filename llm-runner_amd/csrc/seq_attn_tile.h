@@ -300,7 +300,9 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, So
     auto rescale = [&](uint64_t grow, float mx, f32x16& n0, f32x16& n1) {
         if (grow != 0) {
             const bool fresh = ((seen >> lane) & 1u) == 0;
-            const float d = fresh ? (mx > -INFINITY ? mx : 0.0f) : fmaxf(mx, 0.0f);
+            // only rows whose own maximum calls for it: what another row of the wave sees changes no
+            // bit of this one (0 leaves everything as it is)
+            const float d = fresh ? (mx > -INFINITY ? mx : 0.0f) : (mx > grow_by ? mx : 0.0f);
             const float alpha = fresh ? 0.0f : __builtin_amdgcn_exp2f(-d * c);
             m_ref += d;
             l_i *= alpha;

@@ -729,3 +729,41 @@ def test_paged_attention_rows_of_a_chunk_around_a_missing_page(dev, dtype, D, ne
             _check(out[a:b].unflatten(1, (4, D)), o, A, e, float(vv.double().abs().max()), new, dtype, f"rows {a} .. {b}")
         else:  # keys of the missing page alone
             assert bool((out[a:b] == 0).all()), (a, b)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens", [[200], [90, 60, 150]], ids=["one", "packed"])
+def test_prompt_attention_unseen_keys_change_no_bit(dev, dtype, D, lens):
+    """A key far above the others raises the maximum of the rows that see it: the rows before it and other requests'
+    in the same wave keep their bits."""
+    from llmr_amd import serve
+    q, k, v, at, off = _prompt_case(dev, dtype, D, 4, 2, lens, seed=31)
+    clean = serve.prompt_attention(q, k, v, off)
+    for row in (100, 137, at[-1] - 3):
+        far = k.clone()
+        far[row] *= 60
+        out = serve.prompt_attention(q, far, v, off)
+        torch.cuda.synchronize()
+        end = next(e for e in at if e > row)
+        assert not torch.equal(out[row:end], clean[row:end]), row
+        assert torch.equal(out[:row], clean[:row]) and torch.equal(out[end:], clean[end:]), row
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new", [8, 24, 100])
+def test_paged_attention_unseen_keys_change_no_bit(dev, dtype, D, new):
+    """The same over a cache long enough that every wave takes several tiles."""
+    from llmr_amd import serve
+    past = 30000
+    q, kc, vc, rows, at, off, kvl, table, kv = _paged_case(dev, dtype, D, 16, 8, 16, [past], [new], seed=32)
+    clean = serve.paged_attention(q, kc, vc, off, kvl, table, new)
+    for first in (new // 2, new - 2):
+        page, at_page = int(table[0, (past + first) // 16]), (past + first) % 16
+        far = kc.clone()
+        far[page, :, at_page] *= 60
+        out = serve.paged_attention(q, far, vc, off, kvl, table, new)
+        torch.cuda.synchronize()
+        assert not torch.equal(out[first:], clean[first:]), first
+        assert torch.equal(out[:first], clean[:first]), first
