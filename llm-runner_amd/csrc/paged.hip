@@ -18,6 +18,7 @@ __device__ __forceinline__ uint32_t pages_of(uint32_t n, uint32_t log2, uint32_t
 }
 
 constexpr uint32_t kPlanThreads = 256;
+constexpr uint32_t kMaxGridRows = 1u << 23;
 
 template <uint32_t OT>
 __device__ __forceinline__ uint32_t pack16(float x, float y) {
@@ -135,8 +136,9 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedPlanArgs 
 template <uint32_t OT, uint32_t D, bool HALVES>
 __global__ void __launch_bounds__(256) qkv_tokens_kernel(QkvTokensArgs a) {
     constexpr uint32_t L = D / 8u;  // lanes of a head
-    const uint32_t l = threadIdx.x % L, r = blockIdx.x, h = blockIdx.y * (256u / L) + threadIdx.x / L;
-    if (h >= a.n_heads + 2u * a.n_kv_heads) return;  // (whole heads: the reductions stay within one)
+    const uint32_t l = threadIdx.x % L, h = blockIdx.y * (256u / L) + threadIdx.x / L;
+    const uint32_t r = blockIdx.z * kMaxGridRows + blockIdx.x;
+    if (r >= a.n_tokens || h >= a.n_heads + 2u * a.n_kv_heads) return;  // (whole heads: the reductions stay within one)
     const uint32_t e0 = HALVES ? 4u * l : 8u * l, e1 = HALVES ? e0 + D / 2u : e0 + 4u;
     const float* src = a.qkv + (size_t)r * a.qkv_stride + (size_t)h * D;
     f32x4 x0 = *(const f32x4*)(src + e0), x1 = *(const f32x4*)(src + e1);
@@ -194,7 +196,9 @@ hipError_t launch_paged_plan(const PagedPlanArgs& a, hipStream_t st) {
 
 hipError_t launch_qkv_tokens(const QkvTokensArgs& a, uint32_t dim, uint32_t otype, bool halves, hipStream_t st) {
     const uint32_t per = 256u / (dim / 8u);  // heads a workgroup
-    const dim3 grid(a.n_tokens, (a.n_heads + 2u * a.n_kv_heads + per - 1u) / per), block(256);
+    // rows go on in z where there are more than x takes (its threads, 256 a row, stay under 2^32)
+    const uint32_t x = a.n_tokens < kMaxGridRows ? a.n_tokens : kMaxGridRows;
+    const dim3 grid(x, (a.n_heads + 2u * a.n_kv_heads + per - 1u) / per, (a.n_tokens + x - 1u) / x), block(256);
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, a); };
     if (otype == kGgmlBF16) {
         if (dim == 128u) halves ? go(qkv_tokens_kernel<kGgmlBF16, 128, true>) : go(qkv_tokens_kernel<kGgmlBF16, 128, false>);

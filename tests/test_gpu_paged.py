@@ -409,3 +409,30 @@ def test_a_run_of_steps(dev, captured):
             count += held
             lens[s], seen[s] = 0, [None, None]
             table[s] = -1
+
+
+def test_qkv_tokens_more_rows_than_one_grid_dimension(dev):
+    """2^24 rows and more (workgroups of 256 threads: more than 2^32 threads along one dimension of a grid)."""
+    from llmr_amd import serve
+    D, T = 64, 2 ** 24 + 37
+    g = torch.Generator(device=dev).manual_seed(3)
+    qkv = torch.randn(T, 3 * D, generator=g, device=dev)
+    w = torch.rand(D, generator=g, device=dev) + 0.5
+    pos = torch.randint(0, 900, (T,), generator=g, device=dev, dtype=torch.int32)
+    tabs = _tables(dev, 900, D)
+    q, k, v = (torch.zeros(T, 1, D, dtype=BF16, device=dev) for _ in range(3))
+    serve.qkv_tokens(qkv, q, k, v, positions=pos, q_norm=w, k_norm=w, rope=tabs)
+    torch.cuda.synchronize()
+    assert torch.equal(v[:, 0], qkv[:, 2 * D:].bfloat16())
+    n = 1 << 22
+    for a in range(0, T, n):  # the same rows, fewer at a time
+        b = min(T, a + n)
+        parts = [torch.zeros(b - a, 1, D, dtype=BF16, device=dev) for _ in range(3)]
+        serve.qkv_tokens(qkv[a:b], *parts, positions=pos[a:b], q_norm=w, k_norm=w, rope=tabs)
+        assert torch.equal(parts[0], q[a:b]) and torch.equal(parts[1], k[a:b]), a
+    page = 256
+    caches = [torch.zeros(-(-T // page), 1, page, D, dtype=BF16, device=dev) for _ in range(2)]
+    slots = torch.arange(T - 1, -1, -1, dtype=torch.int32, device=dev)
+    serve.qkv_tokens(qkv, q, *caches, slots=slots, positions=pos, q_norm=w, k_norm=w, rope=tabs)
+    torch.cuda.synchronize()
+    assert torch.equal(caches[0].view(-1, D)[:T].flip(0), k[:, 0]) and torch.equal(caches[1].view(-1, D)[:T].flip(0), v[:, 0])
