@@ -186,8 +186,8 @@ def qkv_tokens(qkv: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Ten
     n_pos = 0
     if rope is not None:
         cos, sin = rope
-        if cos.dim() != 2 or cos.shape[1] != D // 2 or sin.shape != cos.shape:
-            raise ValueError("rope must be (cos, sin) of [n_positions, head_dim / 2]")
+        if cos.dim() != 2 or cos.shape[1] != D // 2 or sin.shape != cos.shape or cos.shape[0] == 0:
+            raise ValueError("rope must be (cos, sin) of [n_positions, head_dim / 2], n_positions >= 1")
         n_pos = cos.shape[0]
     pp = _ints(positions, "positions", T) if positions is not None else None
     args = (_vec(q_norm, "q_norm", D), _vec(k_norm, "k_norm", D), _vec(cos, "rope_cos", 0), _vec(sin, "rope_sin", 0))

@@ -85,3 +85,12 @@ def test_strides_past_32_bits_are_refused():
         serve.prompt_attention(far(4, 2), q, q.clone(), off)
     with pytest.raises(ValueError, match="2\\^32"):
         serve.qkv_tokens(torch.empty_strided((4, 256), (1 << 32, 1), device="meta"), q, q[:, :1], q[:, :1])
+
+
+def test_empty_rotation_tables_are_refused():
+    """(An empty tensor's address is null, which stands for no rotation.)"""
+    q = torch.zeros(4, 2, 64, dtype=F16)
+    tabs = tuple(torch.zeros(0, 32) for _ in range(2))
+    for positions in (None, torch.zeros(4, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="rope"):
+            serve.qkv_tokens(torch.zeros(4, 4 * 64), q, q[:, :1], q[:, :1].clone(), positions=positions, rope=tabs)
