@@ -93,4 +93,4 @@ def test_empty_rotation_tables_are_refused():
     tabs = tuple(torch.zeros(0, 32) for _ in range(2))
     for positions in (None, torch.zeros(4, dtype=torch.int32)):
         with pytest.raises(ValueError, match="rope"):
-            serve.qkv_tokens(torch.zeros(4, 4 * 64), q, q[:, :1], q[:, :1].clone(), positions=positions, rope=tabs)
+            serve.qkv_tokens(torch.zeros(4, 4 * 64), q, q[:, :1], q[:, 1:], positions=positions, rope=tabs)
