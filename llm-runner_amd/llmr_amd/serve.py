@@ -70,9 +70,15 @@ def _heads(t: torch.Tensor, what: str):
     ts, hs, ds = t.stride()
     if ds != 1:
         raise ValueError(f"{what} must be [tokens, heads, head_dim] with contiguous heads")
+    ts, hs = ts if T > 1 else H * D, hs if H > 1 else D
     if ts > _U32 or hs > _U32:
         raise ValueError(f"{what}'s strides must be under 2^32 elements")
-    return T, H, D, ts if T > 1 else H * D, hs if H > 1 else D
+    return T, H, D, ts, hs
+
+
+def _alike(k: torch.Tensor, v: torch.Tensor) -> bool:
+    """Whether v has k's shape and strides, but for those of a dimension of one."""
+    return v.shape == k.shape and (v.stride() == k.stride() or _heads(v, "v")[3:] == _heads(k, "k")[3:])
 
 
 def _out_stride(out: torch.Tensor, T: int, width: int, like: torch.Tensor) -> int:
@@ -104,7 +110,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_offs
     its rows that belong to no request keep what they hold (a new `out`: undefined)."""
     T, H, D, qs, qh = _heads(q, "q")
     Tk, Hk, Dk, ks, kh = _heads(k, "k")
-    if Tk != T or Dk != D or v.shape != k.shape or v.stride() != k.stride():
+    if Tk != T or Dk != D or not _alike(k, v):
         raise ValueError("k and v must be [tokens, n_kv_heads, head_dim] alike, with q's tokens and head_dim")
     t = _type("q, k and v", q, k, v)
     if out is None:
@@ -178,7 +184,7 @@ def qkv_tokens(qkv: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Ten
     else:
         Tk, Hk, Dk, ks, kh = _heads(k, "k")
         sp = None
-        if v.shape != k.shape or v.stride() != k.stride() or Tk != T or kh != D:
+        if not _alike(k, v) or Tk != T or kh != D:
             raise ValueError("k and v must be [tokens, n_kv_heads, head_dim] alike, heads side by side")
     if Dk != D or qkv.shape[1] < (H + 2 * Hk) * D:
         raise ValueError("k and v must have q's head_dim, and qkv (n_heads + 2 n_kv_heads) * head_dim columns")

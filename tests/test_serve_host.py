@@ -94,3 +94,43 @@ def test_empty_rotation_tables_are_refused():
     for positions in (None, torch.zeros(4, dtype=torch.int32)):
         with pytest.raises(ValueError, match="rope"):
             serve.qkv_tokens(torch.zeros(4, 4 * 64), q, q[:, :1], q[:, 1:], positions=positions, rope=tabs)
+
+
+class _Recorder:
+    """A graph on no device whose context keeps what a call would be issued with."""
+    device = -1  # a host tensor's get_device()
+
+    def __init__(self):
+        self.ctx, self.calls = self, []
+
+    def set_stream(self, stream):
+        pass
+
+    def __getattr__(self, name):
+        return lambda *args: self.calls.append((name, args))
+
+
+def test_strides_of_dimensions_of_one_do_not_matter(monkeypatch):
+    """One token, or one key/value head: its stride in that dimension is nothing, also where k's and v's differ."""
+    monkeypatch.setattr(serve, "_raw_stream", lambda dev: 0)
+    off = torch.tensor([0, 1], dtype=torch.int32)
+    wide = torch.zeros(5, 8, 64, dtype=F16)
+    for T, Hk in ((1, 2), (1, 1), (5, 1)):
+        q = torch.zeros(T, 2, 64, dtype=F16)
+        k = torch.zeros(T, Hk, 64, dtype=F16)
+        v = torch.zeros(5, Hk, 64, dtype=F16)[:T].as_strided((T, Hk, 64), (64 * Hk if T > 1 else 512, 64 if Hk > 1 else 640, 1))
+        if Hk == 1:  # past the parameters' 32 bits, were it one that counts
+            k = k.as_strided(k.shape, (64, 1 << 33, 1))
+        g = _Recorder()
+        serve.prompt_attention(q, k, v, off, g=g)
+        serve.qkv_tokens(torch.zeros(T, (2 + 2 * Hk) * 64), q, k, v, g=g)
+        (name, a), (name2, b) = g.calls
+        p, r = a[-1], b[-1]
+        assert (name, p.kv_stride, p.kv_head_stride) == ("prompt_attention", Hk * 64, 64)
+        assert (name2, r.kv_stride) == ("qkv_tokens", Hk * 64)
+    for k, v in ((wide[:, :2], torch.zeros(5, 2, 64, dtype=F16)), (wide[:, :1], torch.zeros(5, 1, 64, dtype=F16))):
+        q = torch.zeros(5, 2, 64, dtype=F16)
+        with pytest.raises(ValueError, match="alike"):  # strides that count do have to be the same
+            serve.prompt_attention(q, k, v, off, g=_Recorder())
+        with pytest.raises(ValueError, match="alike"):
+            serve.qkv_tokens(torch.zeros(5, 8 * 64), q, k, v, g=_Recorder())
