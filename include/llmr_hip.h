@@ -566,8 +566,8 @@ LLMR_API int llmr_flash_attention_pc(llmr_context* ctx, const void* q, const voi
  * within [0, n_tokens], a page outside [0, n_pages) or past the table's columns
  * is a page of keys nobody sees, a slot outside the cache stores nothing. Rows
  * that belong to no request (a batch padded to a captured size) are left as they
- * are. None of these calls allocates; the attention's out may not overlap its
- * keys or values.
+ * are. None of these calls allocates. The attention's out may be q itself (the same
+ * rows at the same stride), and overlaps no other array otherwise.
  * ------------------------------------------------------------------------- */
 
 /* Most requests of one llmr_paged_plan or llmr_paged_attention call. */
@@ -594,8 +594,8 @@ typedef struct llmr_prompt_attention_params {
  * nondecreasing (a request may have no rows). Scores, the running maximum and
  * sum and the accumulated rows are f32; the softmax weights are rounded to
  * `type` for the products with v, the sums that divide are of the weights
- * before that. A key or value row changes no row of out that does not see it,
- * whatever it holds (infinities and NaN too). Of the reference's
+ * before that. A key or value row changes no bit of a row of out that does not see
+ * it, whatever it holds (infinities and NaN too). Of the reference's
  * attention_prefill (dependencies/llm_text.c3l/shaders/llm.slang), for a whole
  * batch of prompts in one launch. */
 LLMR_API int llmr_prompt_attention(llmr_context* ctx, const void* q, const void* k, const void* v, uint32_t type,
@@ -698,8 +698,8 @@ LLMR_API int llmr_paged_attention(llmr_context* ctx, const void* q, const void* 
                                   const llmr_paged_attention_params* params);
 
 /* Bytes of the scratch of an llmr_paged_attention call on this context's device with
- * these params (0 where the call needs none or would refuse them). Lengths do not
- * matter: it holds for every replay of a captured call. */
+ * these params (0 where the call needs none or they are refused; strides are not looked
+ * at). Lengths do not matter: it holds for every replay of a captured call. */
 LLMR_API size_t llmr_paged_attention_scratch_bytes(llmr_context* ctx, const llmr_paged_attention_params* params);
 
 /* ---------------------------------------------------------------------------

@@ -107,7 +107,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_offs
     """Causal attention of packed prompts (llmr_prompt_attention). q [T, n_heads, D], k and v [T, n_kv_heads,
     D] f16 or bf16, any strides of tokens and heads (column slices of one QKV buffer, head-major buffers
     transposed); seq_offsets int32 [n_seqs + 1]; scale 1/sqrt(D) by default. out [T, n_heads * D], q's dtype;
-    its rows that belong to no request keep what they hold (a new `out`: undefined)."""
+    its rows that belong to no request keep what they hold (a new `out`: undefined). out may be q's own rows
+    and overlaps nothing else."""
     T, H, D, qs, qh = _heads(q, "q")
     Tk, Hk, Dk, ks, kh = _heads(k, "k")
     if Tk != T or Dk != D or not _alike(k, v):
@@ -224,7 +225,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     caches [n_pages, n_kv_heads, page_size, D], seq_offsets [n_seqs + 1], kv_len [n_seqs] (the new tokens
     counted), block_table [n_seqs, max_pages]; max_new: the most new tokens of a request (1 while every request
     decodes). out [T, n_heads * D] of q's dtype (rows of no request keep what they hold; a new `out`:
-    undefined). scratch: paged_attention_scratch's, one per call that may overlap another; None: a new one."""
+    undefined), which may be q's own rows and overlaps nothing else. scratch: paged_attention_scratch's, one per
+    call that may overlap another; None: a new one."""
     T, H, D, qs, qh = _heads(q, "q")
     n_pages, Hk, page, Dk = _cache(k_cache, v_cache)
     n = kv_len.numel()

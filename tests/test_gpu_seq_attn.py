@@ -767,3 +767,21 @@ def test_paged_attention_unseen_keys_change_no_bit(dev, dtype, D, new):
         torch.cuda.synchronize()
         assert not torch.equal(out[first:], clean[first:]), first
         assert torch.equal(out[:first], clean[:first]), first
+
+
+@pytest.mark.parametrize("D,H,Hk", [(128, 8, 2), (64, 5, 1)])
+def test_out_may_be_q(dev, D, H, Hk):
+    """The queries' own rows as the output's, in every form: prompts, few rows, chunks, parts of several workgroups."""
+    from llmr_amd import serve
+    for lens in ([70, 0, 200], [900, 1100, 2000]):
+        q, k, v, at, off = _prompt_case(dev, BF16, D, H, Hk, lens, 5, seed=41)
+        ref = serve.prompt_attention(q, k, v, off, out=q.clone().flatten(1))
+        serve.prompt_attention(q, k, v, off, out=q.flatten(1))
+        torch.cuda.synchronize()
+        assert torch.equal(q.flatten(1), ref)
+    for past, new in (([9000, 3, 70], [1, 1, 1]), ([4000, 0], [6, 4]), ([5000, 100, 0], [300, 1, 70])):
+        q, kc, vc, rows, at, off, kvl, table, kv = _paged_case(dev, BF16, D, H, Hk, 16, past, new, seed=42)
+        ref = serve.paged_attention(q, kc, vc, off, kvl, table, max(new))
+        serve.paged_attention(q, kc, vc, off, kvl, table, max(new), out=q.flatten(1))
+        torch.cuda.synchronize()
+        assert torch.equal(q.flatten(1), ref), new
