@@ -294,12 +294,16 @@ hipError_t launch_prompt_attention(const SeqAttnArgs& a, uint32_t type, uint32_t
 }
 
 // Row blocks of 16 of the kernel for few rows that holds max_new tokens of a group; 0: more rows.
+// For the call's max_new, not a request's own new tokens. 64 ragged contexts, single tokens, 30/6
+// heads: 116 us with few rows, 151 in 256-row blocks; four long contexts with 32 and 64 rows a
+// head are faster in those (the figures beside paged_attn_few).
 static uint32_t few_blocks(uint32_t n_heads, uint32_t n_kv_heads, uint32_t max_new) {
     const uint64_t rows = (uint64_t)max_new * (n_heads / n_kv_heads);
     return rows <= 16u ? 1u : rows <= 32u ? 2u : rows <= 64u ? 4u : 0u;
 }
-// Workers: waves a CU of paged_attn_few, as many as their LDS lets reside, or one workgroup a
-// CU of paged_attn_tiles. Scratch: a record of each, then two parts of each.
+// Workers: waves a CU of paged_attn_few, as many as their LDS lets reside at head_dim 128 (at 64
+// too, where it would let twice as many), or one workgroup a CU of paged_attn_tiles. Scratch: a
+// record of each, then two parts of each.
 static uint32_t paged_workers(uint32_t nr, int num_cus) {
     return (uint32_t)num_cus * (nr == 0u ? 1u : nr == 1u ? 4u : nr == 2u ? 3u : 2u);
 }

@@ -4,9 +4,13 @@
 // kernel is a stream of the cache's pages; what it has to do is to keep enough
 // of them in flight on every CU whatever the requests' lengths are.
 //
-// One wave a workgroup, four a CU, each with a ring of two units (32 keys, their
-// values, and where a pair begins its queries) in its own LDS, filled by DMA two
-// units ahead, over the ends of pairs; no wave waits for another. The keys of all
+// One wave a workgroup, four, three or two a CU (up to 16, 32, 64 rows: what the LDS of
+// head_dim 128 lets reside), each with a ring of two units (32 keys, their
+// values, and where a pair begins its queries) in its own LDS, sent for by DMA two
+// units ahead, over the ends of pairs; no wave waits for another. (As built, the
+// block table's entries are vector loads, and waiting for one waits for the DMAs in
+// flight too, four times a unit: it is the other waves' units that keep the memory
+// busy meanwhile.) The keys of all
 // (request, key/value head) pairs, cut into units of 32, make one line of W units;
 // wave g of N <= W takes the units [g W / N, (g + 1) W / N) of it. A pair that one
 // wave takes whole is written to `out` by it; the parts of the others go to
@@ -21,10 +25,15 @@
 // 4g .. 4g+3 and 16+4g .. of its row (g = lane / 16), and the transposing reads of V
 // give the same keys.
 //
-// Memory bounds it: 4 x 85000 keys of 32/8 heads of 128 (1.39 GB) 270 us, 5.1 TB/s, which
-// is what a large copy reaches; 64 ragged contexts of 100 to 12000 keys, 30/6 heads, fp16
-// (0.47 GB) 106 us and 5 for the join. Queries by ordinary loads at a pair's beginning, a wave waiting
-// for its own, and a join that searched for its parts: 320 and 141.
+// Memory bounds it where enough is in flight, single tokens at head_dim 128: 4 x 85000
+// keys of 32/8 heads (1.39 GB) 270 us and 6 for the join, 5.1 TB/s, which is what a large
+// copy reaches; 64 ragged contexts of 100 to 12000 keys, 30/6 heads, fp16 (0.47 GB) 109 and
+// 5, with pages of 16, 64 and 256 alike. Queries by ordinary loads at a pair's beginning, a wave
+// waiting for its own, and a join that searched for its parts: 320 and 141. Head_dim 64
+// has half the bytes in flight: 213 us for the 4 x 85000 keys (3.3 TB/s). More rows take
+// longer than the bytes: 8 and 16 new tokens (32 and 64 rows) 366 and 687 us at 128, 296
+// and 493 at 64, where paged_attn_tiles takes 284 and 285, 145 and 153; the 64 rows of 128
+// do not fit the registers (200 bytes a lane go to scratch memory, within the loop too).
 #pragma once
 
 #include "seq_attn_tile.h"

@@ -12,21 +12,26 @@
 //
 // S^T = K Q^T (32 keys x 32 rows an MFMA; Q in registers as the B operand), then
 // O^T += V^T P^T with P^T straight from the score registers. K and V tiles of 64
-// keys come by DMA into LDS rings of four slots each, K four tiles ahead and V
-// three; V lies row-major and is read by transposing reads. The scores start from
+// keys come by DMA into LDS rings of four slots each, K sent for four tiles ahead and V
+// three; V lies row-major and is read by transposing reads. (As hipcc builds the
+// prompts' kernel, it takes those reads for dependent on every DMA in flight and waits
+// for all of them, vmcnt(0), before a tile's first one: what was sent for in the same
+// tile has the time of its score products to land, and the tile pays the rest. The
+// kernel over pages has no such wait in its loop.) The scores start from
 // -m_ref (a row's reference maximum), so that p = exp2(c (s - m_ref)) is one
-// multiplication and one exp2; m_ref is raised lazily, when a maximum exceeds it by
-// more than 2^8 in p. Scores, maxima, sums and O are f32; P is rounded to the input
+// multiplication and one exp2; m_ref is raised lazily, when the row's maximum exceeds
+// it by more than 2^8 in p. Scores, maxima, sums and O are f32; P is rounded to the input
 // type for its MFMA (bf16 or fp16, half a step 2^-8 or 2^-11 of each weight).
 //
 // A wave whose 32 rows see nothing of a tile only moves its share of the DMA and
 // waits; masks are applied for the side (a request's beginning, the diagonal) that
 // cuts through a tile. What bounds long prompts is the matrix cores at the clock the
-// power limit leaves: 16384 tokens, bf16, 32/8 heads of 128 take 1900-2060 us, 1070 to
+// power limit leaves: 16384 tokens, bf16, 32/8 heads of 128 take 1890-2060 us, 1070 to
 // 1160 TFLOP/s, where a library product of 8192^3 reaches 1236. Short ones are latency:
 // 20 tokens 8 us (launch and the search for the request 3, the first tiles landed 3,
-// one tile's exponentials and products, the rows' end), a further tile 1.3. 24 packed prompts of 13 to 414 tokens, fp16, 24/8 heads of 64:
-// 26.8 -> 23.7 us, bf16, 32/8 heads of 128: 43.7 -> 37.6.
+// one tile's exponentials and products, the rows' end), a further tile 1.3, and a block's
+// tiles are one after another: 1000 tokens 27-29 us, 2048 62. 24 packed prompts of 13 to
+// 414 tokens, fp16, 24/8 heads of 64: 23-24.5 us.
 //
 // fp16 weights carry a factor 2^7, which the division takes out again: weights
 // below 2^-14 of the reference would lose bits, now below 2^-21, and the lazy
