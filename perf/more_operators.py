@@ -1,0 +1,440 @@
+"""Performance cases of the text path in few bits: linears in 8-bit integers, and the paged key/value cache in 4 bits.
+
+A step of a batch of requests is: rows to integers (`int8.quantize_rows`, with the block's norm on the way), the QKV
+product (`int8.matmul`), its rows into query rows and a cache of 4-bit blocks (`serve.qkv_tokens_mx4`), attention of
+the new tokens over that cache (`serve.paged_attention_mx4`), rows to integers, the output product.
+
+The cases are of three kinds:
+  linear  rows -> integers with a scale a row -> product with integer weights with a scale an output channel
+  store   a projection's rows -> norm, rotation -> query rows, keys and values as blocks of 32 4-bit numbers with a
+          shared power of two in their slots; read back as the values they stand for (`serve.mx4_rows`)
+  attend  causal attention of the requests' new tokens over the pages of such a cache
+
+A case is a dict of plain values; `prepare` makes its inputs on the GPU from the seed alone, `run` is one pass,
+`exact` the same result in 64 bits.
+"""
+import math
+import os
+import random
+import sys
+
+import torch
+
+own = False
+
+DEV = "cuda"
+DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+SIZES = {"f32": 4, "f16": 2, "bf16": 2}
+BLOCK = 32  # elements that share a power of two
+
+
+def _framework():
+    """The framework's operators; imported only for its own passes."""
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "llm-runner_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    from llmr_amd import int8, serve
+    return int8, serve
+
+
+def _ints(text):
+    return [int(x) for x in text.split(",")]
+
+
+def _text(values):
+    return ",".join(str(v) for v in values)
+
+
+def _ragged(n, lo, hi, key):
+    """n lengths spread over [lo, hi] by their logarithm."""
+    r = random.Random(key)
+    return [max(lo, min(hi, int(round(math.exp(r.uniform(math.log(lo), math.log(hi))))))) for _ in range(n)]
+
+
+def listed():
+    return [
+        # the QKV projection of one token: latency
+        {"name": "linear_1", "kind": "linear", "tokens": 1, "in": 4096, "out": 6144, "x": "f32", "y": "f32",
+         "norm": True},
+        # the output projection of a decode batch: the weights' bytes
+        {"name": "linear_64", "kind": "linear", "tokens": 64, "in": 4096, "out": 4096, "x": "bf16", "y": "f32",
+         "norm": False},
+        # single tokens and chunks of several requests in one step, into an MLP of odd width
+        {"name": "linear_777", "kind": "linear", "tokens": 777, "in": 3840, "out": 10213, "x": "f32", "y": "bf16",
+         "norm": True},
+        # the MLP of a long prompt, its widest product
+        {"name": "linear_8192", "kind": "linear", "tokens": 8192, "in": 3840, "out": 20480, "x": "bf16", "y": "bf16",
+         "norm": False},
+        # the projection's rows of a decode step, into the cache
+        {"name": "store_64", "kind": "store", "type": "bf16", "heads": 32, "kv_heads": 8, "dim": 128, "page": 16,
+         "tokens": 64, "slack": 0, "norm": True, "rope": "halves"},
+        # the projection's rows of a long prompt, into the cache
+        {"name": "store_8192", "kind": "store", "type": "bf16", "heads": 32, "kv_heads": 8, "dim": 128, "page": 16,
+         "tokens": 8192, "slack": 100, "norm": True, "rope": "halves"},
+        # one request being answered: latency of one token
+        {"name": "attend_1", "kind": "attend", "type": "bf16", "heads": 32, "kv_heads": 8, "dim": 128, "page": 16,
+         "past": "1100", "new": "1", "pad": 0},
+        # a serving batch in its decode phase, ragged contexts, 30 heads in groups of five
+        {"name": "attend_64", "kind": "attend", "type": "f16", "heads": 30, "kv_heads": 6, "dim": 128, "page": 16,
+         "past": _text(_ragged(64, 100, 12000, 6)), "new": _text([1] * 64), "pad": 0},
+        # a few requests with long documents in the cache: HBM bound
+        {"name": "attend_long_4", "kind": "attend", "type": "bf16", "heads": 32, "kv_heads": 8, "dim": 128, "page": 64,
+         "past": "131000,98304,70001,40000", "new": "1,1,1,1", "pad": 0},
+        # four speculated tokens a request, heads of 64 in groups of seven
+        {"name": "attend_4x16", "kind": "attend", "type": "f16", "heads": 28, "kv_heads": 4, "dim": 64, "page": 32,
+         "past": _text(_ragged(16, 2000, 30000, 8)), "new": _text([4] * 16), "pad": 0},
+        # a prompt taken in chunks: 512 new tokens behind 30000 cached ones
+        {"name": "attend_512_of_30k", "kind": "attend", "type": "bf16", "heads": 32, "kv_heads": 8, "dim": 128,
+         "page": 32, "past": "30001", "new": "512", "pad": 0},
+        # chunks and single tokens of many requests in one step, padded to the captured batch's rows
+        {"name": "attend_mixed_24", "kind": "attend", "type": "f16", "heads": 16, "kv_heads": 4, "dim": 64, "page": 16,
+         "past": _text(_ragged(24, 1, 9000, 7)), "new": _text([1] * 16 + [5, 5, 33, 64, 100, 257, 300, 511]), "pad": 17},
+    ]
+
+
+def _log(rng, lo, hi):
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    kind = rng.choice(["linear", "linear", "linear", "store", "attend", "attend", "attend"])
+    if kind == "linear":
+        tokens = _log(rng, 1, 8192)
+        k, n = 16 * _log(rng, 4, 900), _log(rng, 60, 20480)  # rows of whole 16 bytes, channels of any number
+        while tokens * k * n > 8192 * 3840 * 20480:
+            n //= 2
+        return {"kind": "linear", "tokens": tokens, "in": k, "out": n, "x": rng.choice(["f32", "bf16", "f16"]),
+                "y": rng.choice(["f32", "bf16", "f16"]), "norm": rng.random() < 0.5}
+    kv_heads, group = rng.choice([(8, 4), (8, 3), (6, 5), (4, 4), (4, 7), (2, 8), (1, 16), (8, 1), (12, 2)])
+    heads = {"type": rng.choice(["bf16", "f16"]), "heads": kv_heads * group, "kv_heads": kv_heads,
+             "dim": rng.choice([64, 128, 128]), "page": rng.choice([16, 16, 32, 64, 128])}
+    if kind == "store":
+        return {"kind": "store", **heads, "tokens": _log(rng, 1, 8192), "slack": rng.randint(0, 100),
+                "norm": rng.random() < 0.5, "rope": rng.choice(["halves", "pairs", "none"])}
+    form = rng.choice(["decode", "chunk", "mixed"])
+    n = _log(rng, 1, 128) if form == "decode" else _log(rng, 1, 16)
+    if form == "decode":
+        new = [rng.choice([1, 1, 1, 2, 4]) if rng.random() < 0.2 else 1 for _ in range(n)]
+        past = [_log(rng, 1, min(131072, 300000 // n)) for _ in range(n)]
+    else:
+        new = [_log(rng, 1, max(1, 2000 // n)) if form == "chunk" or rng.random() < 0.4 else 1 for _ in range(n)]
+        past = [rng.choice([0, _log(rng, 1, 32768 // n)]) for _ in range(n)]
+    return {"kind": "attend", **heads, "past": _text(past), "new": _text(new),
+            "pad": rng.choice([0, 0, rng.randint(1, 40)])}
+
+
+# ---- inputs -------------------------------------------------------------------
+
+
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _randn(g, *shape, std=1.0, mean=0.0, dtype=torch.float32):
+    return torch.randn(*shape, generator=g, device=DEV).mul_(std).add_(mean).to(dtype)
+
+
+def _i32(values):
+    return torch.tensor(values, dtype=torch.int32, device=DEV)
+
+
+def _pages(lens, page):
+    return [-(-n // page) for n in lens]
+
+
+def _offsets(lens):
+    at = [0]
+    for n in lens:
+        at.append(at[-1] + n)
+    return at
+
+
+def prepare(case, seed):
+    g = _gen(seed)
+    s = {"case": case, "kind": case["kind"]}
+    return {"linear": _prepare_linear, "store": _prepare_store, "attend": _prepare_attend}[case["kind"]](case, g, s)
+
+
+def _prepare_linear(case, g, s):
+    T, K, N = case["tokens"], case["in"], case["out"]
+    # a residual stream: rows of different size, a few channels far above the others
+    x = _randn(g, T, K) * torch.exp(_randn(g, T, 1, std=0.5))
+    x *= torch.where(torch.rand(K, generator=g, device=DEV) < 0.003, 12.0, 1.0)
+    s["x"] = x.to(DTYPES[case["x"]])
+    s["norm"] = _randn(g, K, std=0.1, mean=1.0) if case["norm"] else None
+    s["eps"] = 1e-6
+    w = _randn(g, N, K, std=0.02) * torch.exp(_randn(g, N, 1, std=0.3))
+    s["w_scales"] = w.abs().amax(dim=1) / 127.0
+    s["w"] = torch.round(w / s["w_scales"][:, None]).clamp_(-127, 127).to(torch.int8)
+    s["q"] = torch.empty(T, K, dtype=torch.int8, device=DEV)
+    s["scales"] = torch.empty(T, dtype=torch.float32, device=DEV)
+    s["out"] = torch.empty(T, N, dtype=DTYPES[case["y"]], device=DEV)
+    return s
+
+
+def _prepare_store(case, g, s):
+    H, Hk, D, T, page = case["heads"], case["kv_heads"], case["dim"], case["tokens"], case["page"]
+    dt = DTYPES[case["type"]]
+    n_pages = -(-(T + case["slack"]) // page)
+    s["qkv"] = _randn(g, T, (H + 2 * Hk) * D, std=1.7)
+    slots = torch.randperm(n_pages * page, generator=g, device=DEV, dtype=torch.int32)[:T]
+    if T > 100:  # prompts take whole runs of slots
+        slots = torch.sort(slots).values
+    s["slots"] = slots.contiguous()
+    s["positions"] = torch.randint(0, 16384, (T,), generator=g, device=DEV, dtype=torch.int32)
+    s["norms"] = tuple(_randn(g, D, std=0.1, mean=1.0) for _ in range(2)) if case["norm"] else (None, None)
+    s["rope"] = None
+    if case["rope"] != "none":
+        freq = 10000.0 ** (-torch.arange(0, D // 2, dtype=torch.float64, device=DEV) * 2 / D)
+        angle = torch.arange(16384, dtype=torch.float64, device=DEV)[:, None] * freq
+        s["rope"] = (angle.cos().float(), angle.sin().float())
+    s["halves"], s["eps"] = case["rope"] == "halves", 1e-6
+    s["q"] = torch.zeros(T, H, D, dtype=dt, device=DEV)
+    s["rows"] = tuple(torch.zeros(T, Hk, D, dtype=dt, device=DEV) for _ in range(2))
+    for x in "kv":
+        s[x] = torch.zeros(n_pages, Hk, page, D // 2, dtype=torch.uint8, device=DEV)
+        s[x + "_scales"] = torch.full((n_pages, Hk, page, D // BLOCK), 127, dtype=torch.uint8, device=DEV)
+    return s
+
+
+def _prepare_attend(case, g, s):
+    dt = DTYPES[case["type"]]
+    H, Hk, D, page = case["heads"], case["kv_heads"], case["dim"], case["page"]
+    s["scale"] = 1.0 / math.sqrt(D)
+    new = _ints(case["new"])
+    at = _offsets(new)
+    T = at[-1] + case["pad"]
+    s["at"], s["offsets"] = at, _i32(at)
+    s["q"] = _randn(g, T, H, D, std=1.5, dtype=dt)
+    s["out"] = torch.zeros(T, H * D, dtype=dt, device=DEV)
+    kv = [p + n for p, n in zip(_ints(case["past"]), new)]
+    need = _pages(kv, page)
+    total, most = sum(need), max(need)
+    order = torch.randperm(total + 8, generator=g, device=DEV, dtype=torch.int32)  # pages as a used pool hands them out
+    table = torch.full((len(kv), most), -1, dtype=torch.int32, device=DEV)
+    used = 0
+    for i, n in enumerate(need):
+        table[i, :n] = order[used:used + n]
+        used += n
+    s["kv"], s["kv_len"], s["table"], s["page"], s["max_new"] = kv, _i32(kv), table, page, max(new)
+    for x in "kv":
+        s[x] = torch.empty(total + 8, Hk, page, D // 2, dtype=torch.uint8, device=DEV)
+        s[x + "_scales"] = torch.empty(total + 8, Hk, page, D // BLOCK, dtype=torch.uint8, device=DEV)
+        for i in range(0, total + 8, 4096):
+            rows = _randn(g, *s[x][i:i + 4096].shape[:3], D)
+            s[x][i:i + 4096], s[x + "_scales"][i:i + 4096] = _blocks(rows)
+    # the same rows by request, for the plain form's one batch: row of each (request, place), -1 where there is none
+    place = torch.arange(max(new), device=DEV)[None] + s["offsets"][:-1, None]
+    s["rows_of"] = torch.where(place < s["offsets"][1:, None], place, -1).long()
+    return s
+
+
+# ---- one pass -------------------------------------------------------------------
+
+
+def run(s):
+    kind = s["kind"]
+    if own:
+        int8, serve = _framework()
+        if kind == "linear":
+            q, scales = int8.quantize_rows(s["x"], norm=s["norm"], eps=s["eps"], q=s["q"], scales=s["scales"])
+            return int8.matmul(q, scales, s["w"], s["w_scales"], out=s["out"])
+        k, v = serve.Mx4Cache(s["k"], s["k_scales"]), serve.Mx4Cache(s["v"], s["v_scales"])
+        if kind == "store":
+            serve.qkv_tokens_mx4(s["qkv"], s["q"], k, v, s["slots"], positions=s["positions"], q_norm=s["norms"][0],
+                                 k_norm=s["norms"][1], eps=s["eps"], rope=s["rope"], halves=s["halves"])
+            serve.mx4_rows(k, v, s["slots"], *s["rows"])
+            return [s["q"], *s["rows"]]
+        return serve.paged_attention_mx4(s["q"], k, v, s["offsets"], s["kv_len"], s["table"], s["max_new"], s["scale"],
+                                         out=s["out"])
+    return {"linear": _plain_linear, "store": _plain_store, "attend": _plain_attend}[kind](s)
+
+
+# What is rounded to few bits is computed in 64: next to a border between two of them 32 would say nothing.
+
+
+def _plain_linear(s):
+    x = s["x"].double()
+    y = x if s["norm"] is None else x * s["norm"].double()
+    top = y.abs().amax(dim=1, keepdim=True)
+    q = torch.round(y * 127.0 / torch.where(top > 0, top, 1.0))
+    if s["norm"] is not None:  # the rows' size only enters their scales
+        top = top / torch.sqrt(x.square().mean(dim=1, keepdim=True) + s["eps"])
+    s["out"].copy_(torch.matmul(q.float(), s["w"].float().t()) * (top / 127.0).float() * s["w_scales"])
+    return s["out"]
+
+
+def _blocks(x):
+    """[..., D] -> bytes of two 4-bit numbers (the even dim low) [..., D / 2] and of the powers of two, + 127,
+    [..., D / 32]. The power: of the largest magnitude, rounded to two significant bits, two less."""
+    b = x.double().unflatten(-1, (-1, BLOCK))
+    f, e = torch.frexp(b.abs().amax(dim=-1))  # f in [0.5, 1), or 0
+    e = torch.where(f > 0, e + (f >= 0.875).int() - 3, -23).clamp_(-23, 13)
+    a = torch.ldexp(b.abs(), -e[..., None])
+    # 0, 0.5, 1, 1.5, 2, 3, 4, 6; halfway to the even number
+    code = ((a > 0.25).to(torch.uint8) + (a >= 0.75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) + (a >= 3.5) + (a > 5.0))
+    code = (code | (b < 0).to(torch.uint8) << 3).flatten(-2)
+    return code[..., 0::2] | code[..., 1::2] << 4, (e + 127).to(torch.uint8)
+
+
+def _values(data, scales):
+    """The f32 values that blocks stand for."""
+    table = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], device=DEV)
+    table = torch.cat([table, -table])
+    code = torch.stack([data & 15, data >> 4], dim=-1).flatten(-2)
+    x = table[code.int()].unflatten(-1, (-1, BLOCK))
+    return torch.ldexp(x, scales.int()[..., None] - 127).flatten(-2)
+
+
+def _plain_norm_rope(x, w, s):
+    x = x.double()
+    if w is not None:
+        x = x / torch.sqrt(x.square().mean(dim=-1, keepdim=True) + s["eps"]) * w.double()
+    if s["rope"] is None:
+        return x
+    c, sn = (t[s["positions"].long()][:, None].double() for t in s["rope"])
+    D = x.shape[-1]
+    a, b = (x[..., :D // 2], x[..., D // 2:]) if s["halves"] else (x[..., 0::2], x[..., 1::2])
+    a, b = a * c - b * sn, a * sn + b * c
+    return torch.cat([a, b], dim=-1) if s["halves"] else torch.stack([a, b], dim=-1).flatten(-2)
+
+
+def _plain_store(s):
+    T, H, D = s["q"].shape
+    Hk, page = s["k"].shape[1], s["k"].shape[2]
+    x = s["qkv"].view(T, H + 2 * Hk, D)
+    s["q"].copy_(_plain_norm_rope(x[:, :H], s["norms"][0], s))
+    at, off = s["slots"].long().div(page, rounding_mode="floor"), s["slots"].long() % page
+    s["k"][at, :, off], s["k_scales"][at, :, off] = _blocks(_plain_norm_rope(x[:, H:H + Hk], s["norms"][1], s))
+    s["v"][at, :, off], s["v_scales"][at, :, off] = _blocks(x[:, H + Hk:])
+    s["rows"][0].copy_(_values(s["k"][at, :, off], s["k_scales"][at, :, off]))
+    s["rows"][1].copy_(_values(s["v"][at, :, off], s["v_scales"][at, :, off]))
+    return [s["q"], *s["rows"]]
+
+
+def _plain_attend(s):
+    """All requests as one batch, padded to the most new tokens and the longest context."""
+    T, H, D = s["q"].shape
+    Hk = s["k"].shape[1]
+    pages = s["table"].clamp(min=0).long()
+    k, v = (_values(s[x][pages], s[x + "_scales"][pages]).transpose(1, 2).reshape(len(pages), Hk, -1, D)
+            for x in "kv")
+    rows = s["rows_of"]
+    n, m = rows.shape
+    q = s["q"].float()[rows.clamp(min=0)]                                        # [n, m, H, D]
+    q = q.view(n, m, Hk, H // Hk, D).permute(0, 2, 3, 1, 4).reshape(n, Hk, -1, D)
+    p = torch.matmul(q, k.transpose(2, 3).contiguous()).mul_(s["scale"])         # [n, Hk, G m, keys]
+    new = (s["offsets"][1:] - s["offsets"][:-1])[:, None]
+    last = s["kv_len"][:, None] - new + torch.arange(m, device=DEV)              # the last key that a row sees
+    hidden = torch.arange(k.shape[2], device=DEV) > last[..., None]              # [n, m, keys]
+    p.view(n, Hk, -1, m, k.shape[2]).masked_fill_(hidden[:, None, None], -math.inf)
+    p.sub_(p.amax(dim=-1, keepdim=True)).exp_()
+    p.div_(p.sum(dim=-1, keepdim=True))
+    o = torch.matmul(p, v).view(n, Hk, H // Hk, m, D).permute(0, 3, 1, 2, 4).reshape(n, m, H * D)
+    real = rows >= 0
+    s["out"][rows[real]] = o[real].to(s["out"].dtype)
+    return s["out"]
+
+
+# ---- what a pass cannot do without -------------------------------------------------
+
+
+def work(case):
+    if case["kind"] == "linear":
+        T, K, N = case["tokens"], case["in"], case["out"]
+        return {"bytes": T * K * SIZES[case["x"]] + 4 * K * case["norm"] + N * K + 4 * N + T * N * SIZES[case["y"]],
+                "flops": 2 * T * N * K}
+    H, Hk, D = case["heads"], case["kv_heads"], case["dim"]
+    row = D // 2 + D // BLOCK  # bytes of a cached row
+    if case["kind"] == "store":
+        T = case["tokens"]
+        tables = T * D * 4 if case["rope"] != "none" else 0
+        # the projection's rows in; queries, blocks and the values of the blocks out
+        return {"bytes": T * ((H + 2 * Hk) * D * 4 + H * D * 2 + 2 * Hk * (row + 2 * D)) + tables + 8 * T,
+                "flops": T * (H + Hk) * D * 6}
+    new, past = _ints(case["new"]), _ints(case["past"])
+    pairs = sum(n * p + n * (n + 1) // 2 for p, n in zip(past, new))
+    return {"bytes": 4 * D * H * sum(new) + 2 * Hk * row * sum(p + n for p, n in zip(past, new) if n),
+            "flops": 4 * D * H * pairs}
+
+
+# ---- the result in 64 bits ---------------------------------------------------------
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    return {"linear": _exact_linear, "store": _exact_store, "attend": _exact_attend}[case["kind"]](case, s)
+
+
+def _exact_linear(case, s):
+    x = s["x"].double()
+    if s["norm"] is not None:
+        x = s["norm"].double() * x / torch.sqrt((x ** 2).sum(1, keepdim=True) / case["in"] + s["eps"])
+    step = x.abs().max(dim=1, keepdim=True).values / 127
+    q = torch.clamp(torch.round(x / torch.where(step > 0, step, torch.ones_like(step))), -127, 127)
+    out = torch.empty(case["tokens"], case["out"], dtype=torch.float64, device=DEV)
+    for a in range(0, case["out"], 4096):  # the weights a part at a time
+        w = s["w"][a:a + 4096].double() * s["w_scales"][a:a + 4096].double()[:, None]
+        out[:, a:a + 4096] = (q * step) @ w.t().contiguous()
+    return out
+
+
+def _exact_round4(x):
+    """To the nearest of a block's numbers: the power of two from the largest of the block, then half steps of a
+    number's own power of two, ties to the even multiple."""
+    b = x.unflatten(-1, (-1, BLOCK))
+    top = b.abs().max(dim=-1, keepdim=True).values
+    f, e = torch.frexp(top)  # top = f 2^e, f in [0.5, 1); at 0.875 and above it rounds up to the next power
+    e = torch.where(top > 0, e - 1 + (f >= 0.875).int(), torch.full_like(e, -1000)) - 2
+    unit = torch.ldexp(torch.ones_like(top), e.clamp(-23, 13))
+    a = (b / unit).clamp(-6, 6)
+    step = torch.where(a.abs() >= 4, 2.0, torch.where(a.abs() >= 2, 1.0, 0.5)).to(a.dtype)
+    return (torch.round(a / step) * step * unit).flatten(-2)
+
+
+def _exact_store(case, s):
+    T, H, D = s["q"].shape
+    Hk = case["kv_heads"]
+    x = s["qkv"].double().reshape(T, H + 2 * Hk, D)
+    parts = []
+    for y, w in ((x[:, :H], s["norms"][0]), (x[:, H:H + Hk], s["norms"][1])):
+        if w is not None:
+            y = y / torch.sqrt((y ** 2).sum(-1, keepdim=True) / D + s["eps"]) * w.double()
+        if s["rope"] is not None:
+            z = torch.complex(*(t.double()[s["positions"].long()] for t in s["rope"]))[:, None, :]
+            if s["halves"]:
+                y = torch.complex(y[..., :D // 2].contiguous(), y[..., D // 2:].contiguous()) * z
+                y = torch.cat([y.real, y.imag], dim=-1)
+            else:
+                y = torch.view_as_real(torch.view_as_complex(y.reshape(T, -1, D // 2, 2).contiguous()) * z).flatten(-2)
+        parts.append(y)
+    return [parts[0], _exact_round4(parts[1]), _exact_round4(x[:, H + Hk:].contiguous())]
+
+
+def _exact_values(data, scales):
+    """The 64-bit values of blocks, from the numbers' bits: sign, two of exponent, one of mantissa."""
+    code = torch.stack([data % 16, torch.div(data, 16, rounding_mode="floor")], dim=-1).flatten(-2).long()
+    e, m = (code // 2) % 4, (code % 2).double()
+    mag = torch.where(e == 0, m / 2, (1 + m / 2) * 2.0 ** (e - 1).double())
+    return (torch.where(code >= 8, -mag, mag).unflatten(-1, (-1, BLOCK)) * 2.0 ** (scales.double()[..., None] - 127)).flatten(-2)
+
+
+def _exact_attend(case, s):
+    H, Hk, D, page = case["heads"], case["kv_heads"], case["dim"], case["page"]
+    G = H // Hk
+    out = s["out"].double()
+    for i in range(len(s["at"]) - 1):
+        a, b = s["at"][i], s["at"][i + 1]
+        n = s["kv"][i]
+        place = torch.arange(n, device=DEV)
+        at, off = s["table"][i].long()[place // page], place % page
+        for h in range(Hk):
+            k, v = (_exact_values(s[x][at, h, off], s[x + "_scales"][at, h, off]) for x in "kv")
+            for r in range(a, b, 64):
+                e = min(b, r + 64)
+                w = torch.tensordot(s["q"][r:e, h * G:(h + 1) * G].double(), k, dims=([2], [1])) * s["scale"]
+                seen = torch.arange(n - b + r, n - b + e, device=DEV)
+                w = torch.where((place[None, :] > seen[:, None])[:, None, :], torch.full_like(w, -math.inf), w)
+                w = torch.exp(w - torch.logsumexp(w, dim=-1, keepdim=True))
+                out[r:e, h * G * D:(h + 1) * G * D] = torch.tensordot(w, v, dims=([2], [0])).reshape(e - r, G * D)
+    return out
