@@ -264,13 +264,18 @@ def _plain_linear(s):
     return s["out"]
 
 
+def _pow2(e):
+    """2^e in 64 bits for whole e, exactly (torch's own powers are rounded)."""
+    return ((e.long() + 1023) << 52).view(torch.float64)
+
+
 def _blocks(x):
     """[..., D] -> bytes of two 4-bit numbers (the even dim low) [..., D / 2] and of the powers of two, + 127,
     [..., D / 32]. The power: of the largest magnitude, rounded to two significant bits, two less."""
     b = x.double().unflatten(-1, (-1, BLOCK))
     f, e = torch.frexp(b.abs().amax(dim=-1))  # f in [0.5, 1), or 0
     e = torch.where(f > 0, e + (f >= 0.875).int() - 3, -23).clamp_(-23, 13)
-    a = torch.ldexp(b.abs(), -e[..., None])
+    a = b.abs() * _pow2(-e)[..., None]
     # 0, 0.5, 1, 1.5, 2, 3, 4, 6; halfway to the even number
     code = ((a > 0.25).to(torch.uint8) + (a >= 0.75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) + (a >= 3.5) + (a > 5.0))
     code = (code | (b < 0).to(torch.uint8) << 3).flatten(-2)
@@ -283,7 +288,7 @@ def _values(data, scales):
     table = torch.cat([table, -table])
     code = torch.stack([data & 15, data >> 4], dim=-1).flatten(-2)
     x = table[code.int()].unflatten(-1, (-1, BLOCK))
-    return torch.ldexp(x, scales.int()[..., None] - 127).flatten(-2)
+    return (x * _pow2(scales.int() - 127).float()[..., None]).flatten(-2)
 
 
 def _plain_norm_rope(x, w, s):
@@ -386,7 +391,7 @@ def _exact_round4(x):
     top = b.abs().max(dim=-1, keepdim=True).values
     f, e = torch.frexp(top)  # top = f 2^e, f in [0.5, 1); at 0.875 and above it rounds up to the next power
     e = torch.where(top > 0, e - 1 + (f >= 0.875).int(), torch.full_like(e, -1000)) - 2
-    unit = torch.ldexp(torch.ones_like(top), e.clamp(-23, 13))
+    unit = torch.tensor([2.0 ** i for i in range(-23, 14)], dtype=torch.float64, device=DEV)[e.clamp(-23, 13).long() + 23]
     a = (b / unit).clamp(-6, 6)
     step = torch.where(a.abs() >= 4, 2.0, torch.where(a.abs() >= 2, 1.0, 0.5)).to(a.dtype)
     return (torch.round(a / step) * step * unit).flatten(-2)
@@ -415,8 +420,9 @@ def _exact_values(data, scales):
     """The 64-bit values of blocks, from the numbers' bits: sign, two of exponent, one of mantissa."""
     code = torch.stack([data % 16, torch.div(data, 16, rounding_mode="floor")], dim=-1).flatten(-2).long()
     e, m = (code // 2) % 4, (code % 2).double()
-    mag = torch.where(e == 0, m / 2, (1 + m / 2) * 2.0 ** (e - 1).double())
-    return (torch.where(code >= 8, -mag, mag).unflatten(-1, (-1, BLOCK)) * 2.0 ** (scales.double()[..., None] - 127)).flatten(-2)
+    mag = torch.where(e == 0, m / 2, (1 + m / 2) * (1 << (e - 1).clamp(min=0)).double())
+    unit = torch.tensor([2.0 ** (i - 127) for i in range(256)], dtype=torch.float64, device=DEV)[scales.long()]
+    return (torch.where(code >= 8, -mag, mag).unflatten(-1, (-1, BLOCK)) * unit[..., None]).flatten(-2)
 
 
 def _exact_attend(case, s):
