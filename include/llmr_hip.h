@@ -703,6 +703,109 @@ LLMR_API int llmr_paged_attention(llmr_context* ctx, const void* q, const void* 
 LLMR_API size_t llmr_paged_attention_scratch_bytes(llmr_context* ctx, const llmr_paged_attention_params* params);
 
 /* ---------------------------------------------------------------------------
+ * The same batches in few bits: a key/value cache of 4-bit numbers, and linears
+ * in 8-bit integers. A step is llmr_paged_plan, llmr_quantize_rows_i8 and
+ * llmr_matmul_i8 (the QKV projection), llmr_qkv_tokens_mx4,
+ * llmr_paged_attention_mx4, then integers again for the output projection. What
+ * is said above of lengths, offsets, tables and slots holds here too. None of
+ * these calls allocates.
+ * ------------------------------------------------------------------------- */
+
+/* A cache of rows in 4 bits, in the OCP microscaling layout: 32 elements of a row
+ * are E2M1 numbers (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives; code = sign
+ * bit 3, then that index) with one power of two. data [n_pages, n_kv_heads,
+ * page_size, head_dim / 2]: byte i of a row holds element 2i in its low half and
+ * 2i + 1 in its high one; scales [n_pages, n_kv_heads, page_size, head_dim / 32]:
+ * exponent + 127, 255 for a block that is NaN. Both 16-byte aligned. A key takes
+ * head_dim * 17 / 32 bytes where F16 takes 2 * head_dim. */
+typedef struct llmr_mx4_cache {
+    void* data;
+    void* scales;
+} llmr_mx4_cache;
+
+/* llmr_qkv_tokens whose key and value rows go to such caches, at slots (required;
+ * params->kv_stride is not looked at; params->out_type is q's). A block's power of
+ * two is that of its largest magnitude, rounded to two significant bits, less two,
+ * kept in [-23, 13] (so that every value is an F16 and a BF16 number); its elements
+ * are rounded to nearest even and end at 6 times it. Norm and rotation of keys are
+ * taken in 64 bits, so that a value next to the border of two numbers does not
+ * depend on an order of sums; queries as llmr_qkv_tokens' are. A block with an
+ * infinity or NaN is NaN. k and v may not overlap each other, q or an input. */
+LLMR_API int llmr_qkv_tokens_mx4(llmr_context* ctx, const float* qkv, const float* q_norm, const float* k_norm,
+                                 const float* rope_cos, const float* rope_sin, const int32_t* positions,
+                                 const int32_t* slots, void* q, const llmr_mx4_cache* k, const llmr_mx4_cache* v,
+                                 const llmr_qkv_tokens_params* params);
+
+/* llmr_paged_attention over such caches: the same requests, pages, rows and
+ * scratch rules. q and out of type F16 or BF16; a key or value is what its block
+ * stands for, in that type (as llmr_qkv_tokens_mx4 writes them: exactly). The
+ * scratch is llmr_paged_attention_mx4_scratch_bytes'. */
+LLMR_API int llmr_paged_attention_mx4(llmr_context* ctx, const void* q, const llmr_mx4_cache* k,
+                                      const llmr_mx4_cache* v, uint32_t type, void* out, const int32_t* seq_offsets,
+                                      const int32_t* kv_len, const int32_t* block_table, void* scratch,
+                                      size_t scratch_bytes, const llmr_paged_attention_params* params);
+LLMR_API size_t llmr_paged_attention_mx4_scratch_bytes(llmr_context* ctx, const llmr_paged_attention_params* params);
+
+typedef struct llmr_mx4_rows_params {
+    uint32_t head_dim;   /* 64 or 128 */
+    uint32_t n_kv_heads; /* at most 1024 */
+    uint32_t n_rows;
+    uint32_t out_type;   /* F16 or BF16 */
+    uint32_t out_stride; /* elements from one row to the next, a multiple of 8 */
+    uint32_t page_size;  /* 16, 32, 64, 128 or 256 */
+    uint32_t n_pages;
+} llmr_mx4_rows_params;
+
+/* Rows of such caches as the values they stand for: row r of k_out and v_out
+ * [n_rows, n_kv_heads, head_dim] is what slot slots[r] holds, as
+ * llmr_prompt_attention reads keys and values. A row whose slot is outside the
+ * cache is left as it is. k_out and v_out overlap no other array. */
+LLMR_API int llmr_mx4_rows(llmr_context* ctx, const llmr_mx4_cache* k, const llmr_mx4_cache* v, const int32_t* slots,
+                           void* k_out, void* v_out, const llmr_mx4_rows_params* params);
+
+/* Longest row of the 8-bit linears: 128 * 128 * in_dim stays within an int32. */
+#define LLMR_MAX_I8_DIM 131056u
+
+typedef struct llmr_quantize_rows_params {
+    uint32_t n_rows;
+    uint32_t dim;      /* a multiple of 16, at most LLMR_MAX_I8_DIM */
+    uint32_t x_type;   /* F32, F16 or BF16 */
+    uint32_t x_stride; /* elements from one row to the next, rows 16-byte aligned */
+    uint32_t q_stride; /* bytes from one row to the next, a multiple of 16 */
+    float eps;         /* with norm */
+} llmr_quantize_rows_params;
+
+/* Rows to 8-bit integers with a scale each. With y = x * norm (norm f32 [dim] or
+ * NULL: y = x) and a the row's largest |y|,
+ *   q[r, k] = 127 y / a rounded to nearest even (0 where a is 0)
+ *   scales[r] = a / 127, with norm times 1 / sqrt(sum x^2 / dim + eps)
+ * so that scales[r] * q[r, k] stands for x, or for its RMS norm
+ * (llmr_batch_rmsnorm's; the norm's size only enters the scale). 64-bit
+ * arithmetic, scales rounded once. A row with an infinity or NaN has q = 0 and
+ * scale NaN. Weights [out_dim, in_dim] get their scales a channel by the same call
+ * without norm. q and scales overlap no other array. */
+LLMR_API int llmr_quantize_rows_i8(llmr_context* ctx, const void* x, const float* norm, int8_t* q, float* scales,
+                                   const llmr_quantize_rows_params* params);
+
+typedef struct llmr_matmul_i8_params {
+    uint32_t n_rows;     /* tokens */
+    uint32_t out_dim;    /* output channels: rows of w */
+    uint32_t in_dim;     /* a multiple of 16, at most LLMR_MAX_I8_DIM */
+    uint32_t x_stride;   /* bytes from one row to the next, multiples of 16, at most */
+    uint32_t w_stride;   /* 2^23 */
+    uint32_t out_type;   /* F32, F16 or BF16 */
+    uint32_t out_stride; /* elements from one row to the next, at most 2^28 */
+} llmr_matmul_i8_params;
+
+/* out[t, n] = x_scales[t] * w_scales[n] * sum_k x[t, k] * w[n, k]: x int8 [n_rows,
+ * in_dim], w int8 [out_dim, in_dim], 16-byte aligned; scales f32. The sum is exact
+ * (int32); it is rounded to f32, multiplied by x_scales[t], then by w_scales[n], and
+ * rounded to out_type. out needs its type's alignment only, any out_dim is taken.
+ * out overlaps no other array. */
+LLMR_API int llmr_matmul_i8(llmr_context* ctx, const int8_t* x, const float* x_scales, const int8_t* w,
+                            const float* w_scales, void* out, const llmr_matmul_i8_params* params);
+
+/* ---------------------------------------------------------------------------
  * Block glue: the row reductions and elementwise ops the DiT blocks run
  * between the GEMMs and attention. Each replaces a chain of the reference's
  * dispatches over one tensor with one pass, and writes its result directly in

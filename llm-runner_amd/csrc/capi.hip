@@ -1092,6 +1092,78 @@ int check_paged_attention(const llmr_paged_attention_params* p) {
     return LLMR_OK;
 }
 
+// What llmr_qkv_tokens and its form for 4-bit caches check alike (all but where k and v go).
+int check_qkv_tokens(const float* qkv, const float* q_norm, const float* k_norm, const float* rope_cos,
+                     const float* rope_sin, const int32_t* positions, const int32_t* slots, const void* q,
+                     const llmr_qkv_tokens_params* p) {
+    if (!p) return fail(LLMR_ERR_INVALID_ARG, "null params");
+    if (!is_16bit(p->out_type))
+        return fail(LLMR_ERR_UNSUPPORTED, "output type %u not supported (F16=1, BF16=30)", p->out_type);
+    if (int r = check_heads(p->head_dim, p->n_heads, p->n_kv_heads)) return r;
+    if (!(p->eps >= 0.0f) || !std::isfinite(p->eps)) return fail(LLMR_ERR_INVALID_ARG, "eps must be finite and >= 0");
+    if (p->n_tokens > 0x7fffffffu) return fail(LLMR_ERR_INVALID_ARG, "n_tokens too large (%u)", p->n_tokens);
+    if (p->rope_halves > 1) return fail(LLMR_ERR_INVALID_ARG, "rope_halves must be 0 or 1");
+    if ((rope_cos == nullptr) != (rope_sin == nullptr))
+        return fail(LLMR_ERR_INVALID_ARG, "rope_cos and rope_sin must both be given or both be null");
+    if (p->n_tokens == 0) return ok();
+    const uint64_t D = p->head_dim, width = (p->n_heads + 2ull * p->n_kv_heads) * D;
+    if (int r = check_16(qkv, "qkv")) return r;
+    if (p->qkv_stride % 4 || p->qkv_stride < width)
+        return fail(LLMR_ERR_INVALID_ARG, "qkv_stride must be a multiple of 4 and >= %llu (got %u)",
+                    (unsigned long long)width, p->qkv_stride);
+    if (int r = check_vec(q_norm, "q_norm", false)) return r;
+    if (int r = check_vec(k_norm, "k_norm", false)) return r;
+    if (int r = check_vec(rope_cos, "rope_cos", false)) return r;
+    if (int r = check_vec(rope_sin, "rope_sin", false)) return r;
+    if (int r = check_16(q, "q")) return r;
+    if (int r = check_stride8(p->q_stride, p->n_heads * D, "q_stride")) return r;
+    if (rope_cos) {
+        if (p->n_positions == 0 || p->n_positions > 0x7fffffffu)
+            return fail(LLMR_ERR_INVALID_ARG, "n_positions must be in [1, 2^31)");
+        if (!positions && p->n_tokens > p->n_positions)
+            return fail(LLMR_ERR_INVALID_ARG, "n_tokens %u > n_positions %u without positions", p->n_tokens,
+                        p->n_positions);
+        if (positions)
+            if (int r = check_ints(positions, "positions")) return r;
+    }
+    if (slots) {
+        if (int r = check_ints(slots, "slots")) return r;
+        if (!page_log2(p->page_size)) return LLMR_ERR_INVALID_ARG;
+        if ((uint64_t)p->n_pages * p->page_size > 0x7fffffffull)
+            return fail(LLMR_ERR_INVALID_ARG, "n_pages * page_size must be < 2^31");
+    }
+    return LLMR_OK;
+}
+
+// The checks and the arguments that attention over a paged cache shares whatever the cache holds (a is
+// filled but for k and v).
+int paged_args(const void* q, void* out, const int32_t* seq_offsets, const int32_t* kv_len, const int32_t* block_table,
+               const void* scratch, size_t scratch_bytes, size_t need, const llmr_paged_attention_params* p,
+               llmr::SeqAttnArgs& a) {
+    if (int r = check_16(q, "q")) return r;
+    if (int r = check_16(out, "out")) return r;
+    if (int r = check_ints(seq_offsets, "seq_offsets")) return r;
+    if (int r = check_ints(kv_len, "kv_len")) return r;
+    if (p->max_pages)
+        if (int r = check_ints(block_table, "block_table")) return r;
+    if (int r = check_stride8(p->q_stride, (uint64_t)p->n_heads * p->head_dim, "q_stride")) return r;
+    if (int r = check_stride8(p->out_stride, (uint64_t)p->n_heads * p->head_dim, "out_stride")) return r;
+    if ((uint64_t)p->n_tokens * p->n_heads > 0x7fffffffull)
+        return fail(LLMR_ERR_INVALID_ARG, "n_tokens * n_heads must be < 2^31");
+    if (need) {
+        if (int r = check_16(scratch, "scratch")) return r;
+        if (scratch_bytes < need)
+            return fail(LLMR_ERR_INVALID_ARG, "scratch holds %zu bytes, needs %zu", scratch_bytes, need);
+    }
+    a.q = q, a.out = out, a.offsets = seq_offsets, a.kv_len = kv_len;
+    a.table = block_table;
+    a.n_heads = p->n_heads, a.n_kv_heads = p->n_kv_heads, a.n_tokens = p->n_tokens, a.n_seqs = p->n_seqs;
+    a.q_stride = p->q_stride, a.q_head_stride = p->head_dim, a.out_stride = p->out_stride;
+    a.page_log2 = page_log2(p->page_size), a.n_pages = p->n_pages, a.max_pages = p->max_pages, a.max_new = p->max_new;
+    a.scale_log2 = p->scale * 1.4426950408889634f;
+    return LLMR_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1163,50 +1235,15 @@ int llmr_qkv_tokens(llmr_context* ctx, const float* qkv, const float* q_norm, co
                     const float* rope_cos, const float* rope_sin, const int32_t* positions, const int32_t* slots,
                     void* q, void* k, void* v, const llmr_qkv_tokens_params* p) {
     if (int r = check_ctx(ctx)) return r;
-    if (!p) return fail(LLMR_ERR_INVALID_ARG, "null params");
-    if (!is_16bit(p->out_type))
-        return fail(LLMR_ERR_UNSUPPORTED, "output type %u not supported (F16=1, BF16=30)", p->out_type);
-    if (int r = check_heads(p->head_dim, p->n_heads, p->n_kv_heads)) return r;
-    if (!(p->eps >= 0.0f) || !std::isfinite(p->eps)) return fail(LLMR_ERR_INVALID_ARG, "eps must be finite and >= 0");
-    if (p->n_tokens > 0x7fffffffu) return fail(LLMR_ERR_INVALID_ARG, "n_tokens too large (%u)", p->n_tokens);
-    if (p->rope_halves > 1) return fail(LLMR_ERR_INVALID_ARG, "rope_halves must be 0 or 1");
-    if ((rope_cos == nullptr) != (rope_sin == nullptr))
-        return fail(LLMR_ERR_INVALID_ARG, "rope_cos and rope_sin must both be given or both be null");
+    if (int r = check_qkv_tokens(qkv, q_norm, k_norm, rope_cos, rope_sin, positions, slots, q, p)) return r;
     if (p->n_tokens == 0) return ok();
-    const uint64_t D = p->head_dim, width = (p->n_heads + 2ull * p->n_kv_heads) * D;
-    if (int r = check_16(qkv, "qkv")) return r;
-    if (p->qkv_stride % 4 || p->qkv_stride < width)
-        return fail(LLMR_ERR_INVALID_ARG, "qkv_stride must be a multiple of 4 and >= %llu (got %u)",
-                    (unsigned long long)width, p->qkv_stride);
-    if (int r = check_vec(q_norm, "q_norm", false)) return r;
-    if (int r = check_vec(k_norm, "k_norm", false)) return r;
-    if (int r = check_vec(rope_cos, "rope_cos", false)) return r;
-    if (int r = check_vec(rope_sin, "rope_sin", false)) return r;
-    if (int r = check_16(q, "q")) return r;
     if (int r = check_16(k, "k")) return r;
     if (int r = check_16(v, "v")) return r;
-    if (int r = check_stride8(p->q_stride, p->n_heads * D, "q_stride")) return r;
-    if (rope_cos) {
-        if (p->n_positions == 0 || p->n_positions > 0x7fffffffu)
-            return fail(LLMR_ERR_INVALID_ARG, "n_positions must be in [1, 2^31)");
-        if (!positions && p->n_tokens > p->n_positions)
-            return fail(LLMR_ERR_INVALID_ARG, "n_tokens %u > n_positions %u without positions", p->n_tokens,
-                        p->n_positions);
-        if (positions)
-            if (int r = check_ints(positions, "positions")) return r;
-    }
-    uint32_t log2 = 0;
-    if (slots) {
-        if (int r = check_ints(slots, "slots")) return r;
-        if (!(log2 = page_log2(p->page_size))) return LLMR_ERR_INVALID_ARG;
-        if ((uint64_t)p->n_pages * p->page_size > 0x7fffffffull)
-            return fail(LLMR_ERR_INVALID_ARG, "n_pages * page_size must be < 2^31");
-    } else if (int r = check_stride8(p->kv_stride, p->n_kv_heads * D, "kv_stride")) {
-        return r;
-    }
+    if (!slots)
+        if (int r = check_stride8(p->kv_stride, (uint64_t)p->n_kv_heads * p->head_dim, "kv_stride")) return r;
     llmr::QkvTokensArgs a{qkv, q_norm, k_norm, rope_cos, rope_sin, rope_cos ? positions : nullptr, slots, q, k, v,
-                          p->n_heads, p->n_kv_heads, p->n_tokens, p->qkv_stride, p->q_stride, p->kv_stride, log2,
-                          p->n_pages, p->n_positions, p->eps};
+                          p->n_heads, p->n_kv_heads, p->n_tokens, p->qkv_stride, p->q_stride, p->kv_stride,
+                          slots ? page_log2(p->page_size) : 0u, p->n_pages, p->n_positions, p->eps};
     return launched(llmr::launch_qkv_tokens(a, p->head_dim, p->out_type, p->rope_halves != 0, ctx->cur), "qkv_tokens");
 }
 
@@ -1223,36 +1260,201 @@ int llmr_paged_attention(llmr_context* ctx, const void* q, const void* k_cache, 
     if (int r = check_paged_attention(p)) return r;
     if (!is_16bit(type)) return fail(LLMR_ERR_UNSUPPORTED, "type %u not supported (F16=1, BF16=30)", type);
     if (p->n_tokens == 0 || p->n_seqs == 0 || p->max_new == 0) return ok();
-    if (int r = check_16(q, "q")) return r;
-    if (int r = check_16(out, "out")) return r;
     if (p->n_pages) {
         if (int r = check_16(k_cache, "k_cache")) return r;
         if (int r = check_16(v_cache, "v_cache")) return r;
     }
-    if (int r = check_ints(seq_offsets, "seq_offsets")) return r;
-    if (int r = check_ints(kv_len, "kv_len")) return r;
-    if (p->max_pages)
-        if (int r = check_ints(block_table, "block_table")) return r;
-    if (int r = check_stride8(p->q_stride, (uint64_t)p->n_heads * p->head_dim, "q_stride")) return r;
-    if (int r = check_stride8(p->out_stride, (uint64_t)p->n_heads * p->head_dim, "out_stride")) return r;
-    if ((uint64_t)p->n_tokens * p->n_heads > 0x7fffffffull)
-        return fail(LLMR_ERR_INVALID_ARG, "n_tokens * n_heads must be < 2^31");
     const size_t need =
         llmr::paged_attention_scratch_bytes(p->head_dim, p->n_heads, p->n_kv_heads, p->max_new, ctx->num_cus);
-    if (need) {
-        if (int r = check_16(scratch, "scratch")) return r;
-        if (scratch_bytes < need)
-            return fail(LLMR_ERR_INVALID_ARG, "scratch holds %zu bytes, needs %zu", scratch_bytes, need);
-    }
     llmr::SeqAttnArgs a{};
-    a.q = q, a.k = k_cache, a.v = v_cache, a.out = out, a.offsets = seq_offsets, a.kv_len = kv_len;
-    a.table = block_table;
-    a.n_heads = p->n_heads, a.n_kv_heads = p->n_kv_heads, a.n_tokens = p->n_tokens, a.n_seqs = p->n_seqs;
-    a.q_stride = p->q_stride, a.q_head_stride = p->head_dim, a.out_stride = p->out_stride;
-    a.page_log2 = page_log2(p->page_size), a.n_pages = p->n_pages, a.max_pages = p->max_pages, a.max_new = p->max_new;
-    a.scale_log2 = p->scale * 1.4426950408889634f;
+    if (int r = paged_args(q, out, seq_offsets, kv_len, block_table, scratch, scratch_bytes, need, p, a)) return r;
+    a.k = k_cache, a.v = v_cache;
     return launched(llmr::launch_paged_attention(a, type, p->head_dim, ctx->num_cus, scratch, ctx->cur),
                     "paged_attention");
+}
+
+}  // extern "C"
+
+// --- the same batches in few bits -------------------------------------------------
+
+namespace {
+
+int check_mx4(const llmr_mx4_cache* c, const char* what) {
+    if (!c || !c->data || !c->scales) return fail(LLMR_ERR_INVALID_ARG, "null %s cache", what);
+    if (!aligned(c->data, 16) || !aligned(c->scales, 16))
+        return fail(LLMR_ERR_INVALID_ARG, "%s cache's data and scales must be 16-byte aligned", what);
+    return LLMR_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int llmr_qkv_tokens_mx4(llmr_context* ctx, const float* qkv, const float* q_norm, const float* k_norm,
+                        const float* rope_cos, const float* rope_sin, const int32_t* positions, const int32_t* slots,
+                        void* q, const llmr_mx4_cache* k, const llmr_mx4_cache* v, const llmr_qkv_tokens_params* p) {
+    if (int r = check_ctx(ctx)) return r;
+    if (int r = check_qkv_tokens(qkv, q_norm, k_norm, rope_cos, rope_sin, positions, slots, q, p)) return r;
+    if (p->n_tokens == 0) return ok();
+    if (!slots) return fail(LLMR_ERR_INVALID_ARG, "null slots pointer");
+    if (int r = check_mx4(k, "k")) return r;
+    if (int r = check_mx4(v, "v")) return r;
+    const uint64_t rows = (uint64_t)p->n_pages * p->page_size * p->n_kv_heads, D = p->head_dim;
+    const struct {
+        const void* p;
+        uint64_t n;
+    } out[] = {{k->data, rows * D / 2}, {k->scales, rows * D / 32}, {v->data, rows * D / 2}, {v->scales, rows * D / 32},
+               {q, ((uint64_t)(p->n_tokens - 1) * p->q_stride + p->n_heads * D) * 2}},
+      in = {qkv, ((uint64_t)(p->n_tokens - 1) * p->qkv_stride + (p->n_heads + 2ull * p->n_kv_heads) * D) * 4};
+    for (int i = 0; i < 5; i++) {
+        for (int j = 0; j < i; j++)
+            if (overlap(out[i].p, out[i].n, out[j].p, out[j].n))
+                return fail(LLMR_ERR_INVALID_ARG, "the caches and q must not overlap");
+        if (overlap(out[i].p, out[i].n, in.p, in.n))
+            return fail(LLMR_ERR_INVALID_ARG, "the caches and q must not overlap qkv");
+    }
+    llmr::QkvTokensArgs a{qkv, q_norm, k_norm, rope_cos, rope_sin, rope_cos ? positions : nullptr, slots, q, k->data,
+                          v->data, p->n_heads, p->n_kv_heads, p->n_tokens, p->qkv_stride, p->q_stride, 0,
+                          page_log2(p->page_size), p->n_pages, p->n_positions, p->eps};
+    return launched(llmr::launch_qkv_tokens_mx4(a, (uint8_t*)k->scales, (uint8_t*)v->scales, p->head_dim, p->out_type,
+                                                p->rope_halves != 0, ctx->cur), "qkv_tokens_mx4");
+}
+
+size_t llmr_paged_attention_mx4_scratch_bytes(llmr_context* ctx, const llmr_paged_attention_params* p) {
+    if (check_ctx(ctx) || check_paged_attention(p)) return 0;
+    if (p->n_tokens == 0 || p->n_seqs == 0 || p->max_new == 0) return 0;
+    return llmr::paged_attention_mx4_scratch_bytes(p->head_dim, p->n_heads, p->n_kv_heads, p->max_new, ctx->num_cus);
+}
+
+int llmr_paged_attention_mx4(llmr_context* ctx, const void* q, const llmr_mx4_cache* k, const llmr_mx4_cache* v,
+                             uint32_t type, void* out, const int32_t* seq_offsets, const int32_t* kv_len,
+                             const int32_t* block_table, void* scratch, size_t scratch_bytes,
+                             const llmr_paged_attention_params* p) {
+    if (int r = check_ctx(ctx)) return r;
+    if (int r = check_paged_attention(p)) return r;
+    if (!is_16bit(type)) return fail(LLMR_ERR_UNSUPPORTED, "type %u not supported (F16=1, BF16=30)", type);
+    if (p->n_tokens == 0 || p->n_seqs == 0 || p->max_new == 0) return ok();
+    if (p->n_pages) {
+        if (int r = check_mx4(k, "k")) return r;
+        if (int r = check_mx4(v, "v")) return r;
+    }
+    const size_t need =
+        llmr::paged_attention_mx4_scratch_bytes(p->head_dim, p->n_heads, p->n_kv_heads, p->max_new, ctx->num_cus);
+    llmr::SeqAttnArgs a{};
+    if (int r = paged_args(q, out, seq_offsets, kv_len, block_table, scratch, scratch_bytes, need, p, a)) return r;
+    a.k = p->n_pages ? k->data : nullptr, a.v = p->n_pages ? v->data : nullptr;
+    return launched(llmr::launch_paged_attention_mx4(a, p->n_pages ? (const uint8_t*)k->scales : nullptr,
+                                                     p->n_pages ? (const uint8_t*)v->scales : nullptr, type,
+                                                     p->head_dim, ctx->num_cus, scratch, ctx->cur),
+                    "paged_attention_mx4");
+}
+
+int llmr_mx4_rows(llmr_context* ctx, const llmr_mx4_cache* k, const llmr_mx4_cache* v, const int32_t* slots,
+                  void* k_out, void* v_out, const llmr_mx4_rows_params* p) {
+    if (int r = check_ctx(ctx)) return r;
+    if (!p) return fail(LLMR_ERR_INVALID_ARG, "null params");
+    if (!is_16bit(p->out_type))
+        return fail(LLMR_ERR_UNSUPPORTED, "output type %u not supported (F16=1, BF16=30)", p->out_type);
+    if (int r = check_heads(p->head_dim, p->n_kv_heads, p->n_kv_heads)) return r;
+    if (p->n_rows > 0x7fffffffu) return fail(LLMR_ERR_INVALID_ARG, "n_rows too large (%u)", p->n_rows);
+    const uint32_t log2 = page_log2(p->page_size);
+    if (!log2) return LLMR_ERR_INVALID_ARG;
+    if ((uint64_t)p->n_pages * p->page_size > 0x7fffffffull)
+        return fail(LLMR_ERR_INVALID_ARG, "n_pages * page_size must be < 2^31");
+    if (p->n_rows == 0 || p->n_pages == 0) return ok();
+    if (int r = check_mx4(k, "k")) return r;
+    if (int r = check_mx4(v, "v")) return r;
+    if (int r = check_ints(slots, "slots")) return r;
+    if (int r = check_16(k_out, "k_out")) return r;
+    if (int r = check_16(v_out, "v_out")) return r;
+    const uint64_t width = (uint64_t)p->n_kv_heads * p->head_dim;
+    if (int r = check_stride8(p->out_stride, width, "out_stride")) return r;
+    const uint64_t bytes = ((uint64_t)(p->n_rows - 1) * p->out_stride + width) * 2;
+    const uint64_t rows = (uint64_t)p->n_pages * p->page_size * p->n_kv_heads, D = p->head_dim;
+    const struct {
+        const void* p;
+        uint64_t n;
+    } in[] = {{k->data, rows * D / 2}, {k->scales, rows * D / 32}, {v->data, rows * D / 2}, {v->scales, rows * D / 32},
+              {slots, 4ull * p->n_rows}};
+    for (auto& x : in)
+        if (overlap(k_out, bytes, x.p, x.n) || overlap(v_out, bytes, x.p, x.n))
+            return fail(LLMR_ERR_INVALID_ARG, "k_out and v_out must not overlap the caches or slots");
+    if (overlap(k_out, bytes, v_out, bytes)) return fail(LLMR_ERR_INVALID_ARG, "k_out overlaps v_out");
+    llmr::Mx4RowsArgs a{{(uint8_t*)k->data, (uint8_t*)k->scales}, {(uint8_t*)v->data, (uint8_t*)v->scales}, slots, k_out,
+                        v_out, p->n_kv_heads, p->n_rows, p->out_stride, log2, p->n_pages};
+    return launched(llmr::launch_mx4_rows(a, p->head_dim, p->out_type, ctx->cur), "mx4_rows");
+}
+
+static int check_i8_dim(uint32_t dim, const char* what) {
+    if (dim == 0 || dim % 16 || dim > LLMR_MAX_I8_DIM)
+        return fail(LLMR_ERR_INVALID_ARG, "%s must be a multiple of 16 in [16, %u] (got %u)", what, LLMR_MAX_I8_DIM, dim);
+    return LLMR_OK;
+}
+
+static int check_i8_stride(uint32_t stride, uint32_t dim, const char* what) {
+    if (stride % 16 || stride < dim || stride > (1u << 23))
+        return fail(LLMR_ERR_INVALID_ARG, "%s must be a multiple of 16, >= %u and <= 2^23 (got %u)", what, dim, stride);
+    return LLMR_OK;
+}
+
+int llmr_quantize_rows_i8(llmr_context* ctx, const void* x, const float* norm, int8_t* q, float* scales,
+                          const llmr_quantize_rows_params* p) {
+    if (int r = check_ctx(ctx)) return r;
+    if (!p) return fail(LLMR_ERR_INVALID_ARG, "null params");
+    if (!is_act_type(p->x_type))
+        return fail(LLMR_ERR_UNSUPPORTED, "input type %u not supported (F32=0, F16=1, BF16=30)", p->x_type);
+    if (int r = check_i8_dim(p->dim, "dim")) return r;
+    if (p->n_rows > 0x7fffffffu) return fail(LLMR_ERR_INVALID_ARG, "n_rows too large (%u)", p->n_rows);
+    if (norm && (!(p->eps >= 0.0f) || !std::isfinite(p->eps)))
+        return fail(LLMR_ERR_INVALID_ARG, "eps must be finite and >= 0");
+    if (p->n_rows == 0) return ok();
+    const uint32_t size = p->x_type == LLMR_GGML_F32 ? 4u : 2u;
+    if (int r = check_16(x, "x")) return r;
+    if (int r = check_vec(norm, "norm", false)) return r;
+    if (int r = check_16(q, "q")) return r;
+    if (int r = check_ints(scales, "scales")) return r;
+    if ((uint64_t)p->x_stride * size % 16 || p->x_stride < p->dim)
+        return fail(LLMR_ERR_INVALID_ARG, "x_stride must be a multiple of %u and >= %u (got %u)", 16u / size, p->dim,
+                    p->x_stride);
+    if (p->q_stride % 16 || p->q_stride < p->dim)
+        return fail(LLMR_ERR_INVALID_ARG, "q_stride must be a multiple of 16 and >= %u (got %u)", p->dim, p->q_stride);
+    const uint64_t n = p->n_rows - 1ull, xb = (n * p->x_stride + p->dim) * size, qb = n * p->q_stride + p->dim;
+    if (overlap(q, qb, x, xb) || overlap(scales, 4 * n + 4, x, xb) || overlap(q, qb, scales, 4 * n + 4) ||
+        overlap(q, qb, norm, norm ? 4ull * p->dim : 0) || overlap(scales, 4 * n + 4, norm, norm ? 4ull * p->dim : 0))
+        return fail(LLMR_ERR_INVALID_ARG, "q and scales must overlap no other array");
+    llmr::QuantizeRowsArgs a{x, norm, q, scales, p->n_rows, p->dim, p->x_stride, p->q_stride, p->eps};
+    return launched(llmr::launch_quantize_rows_i8(a, p->x_type, ctx->num_cus, ctx->cur), "quantize_rows_i8");
+}
+
+int llmr_matmul_i8(llmr_context* ctx, const int8_t* x, const float* x_scales, const int8_t* w, const float* w_scales,
+                   void* out, const llmr_matmul_i8_params* p) {
+    if (int r = check_ctx(ctx)) return r;
+    if (!p) return fail(LLMR_ERR_INVALID_ARG, "null params");
+    if (!is_act_type(p->out_type))
+        return fail(LLMR_ERR_UNSUPPORTED, "output type %u not supported (F32=0, F16=1, BF16=30)", p->out_type);
+    if (int r = check_i8_dim(p->in_dim, "in_dim")) return r;
+    if (p->n_rows > 0x7fffffffu || p->out_dim > 0x7fffffffu)
+        return fail(LLMR_ERR_INVALID_ARG, "n_rows and out_dim must be < 2^31");
+    if (p->n_rows == 0 || p->out_dim == 0) return ok();
+    if (int r = check_16(x, "x")) return r;
+    if (int r = check_16(w, "w")) return r;
+    if (int r = check_ints(x_scales, "x_scales")) return r;
+    if (int r = check_ints(w_scales, "w_scales")) return r;
+    const uint32_t size = p->out_type == LLMR_GGML_F32 ? 4u : 2u;
+    if (!out || !aligned(out, size)) return fail(LLMR_ERR_INVALID_ARG, "out must be non-null and aligned to its type");
+    if (int r = check_i8_stride(p->x_stride, p->in_dim, "x_stride")) return r;
+    if (int r = check_i8_stride(p->w_stride, p->in_dim, "w_stride")) return r;
+    if (p->out_stride < p->out_dim || p->out_stride > (1u << 28))
+        return fail(LLMR_ERR_INVALID_ARG, "out_stride must be >= out_dim (%u) and <= 2^28 (got %u)", p->out_dim,
+                    p->out_stride);
+    const uint64_t ob = ((uint64_t)(p->n_rows - 1) * p->out_stride + p->out_dim) * size;
+    if (overlap(out, ob, x, (uint64_t)(p->n_rows - 1) * p->x_stride + p->in_dim) ||
+        overlap(out, ob, w, (uint64_t)(p->out_dim - 1) * p->w_stride + p->in_dim) ||
+        overlap(out, ob, x_scales, 4ull * p->n_rows) || overlap(out, ob, w_scales, 4ull * p->out_dim))
+        return fail(LLMR_ERR_INVALID_ARG, "out must overlap no other array");
+    llmr::MatmulI8Args a{x, x_scales, w, w_scales, out, p->n_rows, p->out_dim, p->in_dim, p->x_stride, p->w_stride,
+                         p->out_stride};
+    return launched(llmr::launch_matmul_i8(a, p->out_type, ctx->num_cus, ctx->cur), "matmul_i8");
 }
 
 }  // extern "C"

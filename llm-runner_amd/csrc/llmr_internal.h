@@ -247,6 +247,48 @@ struct QkvTokensArgs {
 };
 hipError_t launch_qkv_tokens(const QkvTokensArgs& a, uint32_t dim, uint32_t otype, bool halves, hipStream_t st);
 
+// The same batches in few bits (mx4.hip, mx4_attn.hip, int8.hip). Caches: rows of dim / 2 bytes and
+// dim / 32 scales, pages as above.
+struct Mx4Pages {
+    uint8_t* data;
+    uint8_t* scales;
+};
+// a's k and v are the caches' data, a.slots non-null.
+hipError_t launch_qkv_tokens_mx4(const QkvTokensArgs& a, uint8_t* k_scales, uint8_t* v_scales, uint32_t dim,
+                                 uint32_t qtype, bool halves, hipStream_t st);
+struct Mx4RowsArgs {
+    Mx4Pages k, v;
+    const int32_t* slots;
+    void* k_out;
+    void* v_out;
+    uint32_t n_kv_heads, n_rows, out_stride, page_log2, n_pages;
+};
+hipError_t launch_mx4_rows(const Mx4RowsArgs& a, uint32_t dim, uint32_t otype, hipStream_t st);
+size_t paged_attention_mx4_scratch_bytes(uint32_t dim, uint32_t n_heads, uint32_t n_kv_heads, uint32_t max_new,
+                                         int num_cus);
+// a.k and a.v are the caches' data.
+hipError_t launch_paged_attention_mx4(const SeqAttnArgs& a, const uint8_t* k_scales, const uint8_t* v_scales,
+                                      uint32_t type, uint32_t dim, int num_cus, void* scratch, hipStream_t st);
+
+struct QuantizeRowsArgs {
+    const void* x;
+    const float* norm;  // [dim] or null
+    int8_t* q;
+    float* scales;
+    uint32_t rows, dim, x_stride, q_stride;
+    float eps;
+};
+hipError_t launch_quantize_rows_i8(const QuantizeRowsArgs& a, uint32_t xtype, int num_cus, hipStream_t st);
+struct MatmulI8Args {
+    const int8_t* x;
+    const float* x_scales;
+    const int8_t* w;
+    const float* w_scales;
+    void* out;
+    uint32_t M, N, K, x_stride, w_stride, out_stride;  // tokens, channels, depth
+};
+hipError_t launch_matmul_i8(const MatmulI8Args& a, uint32_t otype, int num_cus, hipStream_t st);
+
 // --- block glue (glue.hip). Strides are in elements; the C-ABI layer checks
 // that every vector access is aligned (dims, strides and column offsets % 4,
 // pointers 16-byte aligned) and that dims fit the kernels' register rows.

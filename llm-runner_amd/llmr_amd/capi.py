@@ -127,6 +127,29 @@ class PagedAttentionParams(ctypes.Structure):
         "q_stride", "out_stride")] + [("scale", ctypes.c_float)]
 
 
+class Mx4Cache(ctypes.Structure):
+    """llmr_mx4_cache."""
+    _fields_ = [("data", ctypes.c_void_p), ("scales", ctypes.c_void_p)]
+
+
+class Mx4RowsParams(ctypes.Structure):
+    """llmr_mx4_rows_params."""
+    _fields_ = [(n, ctypes.c_uint32) for n in (
+        "head_dim", "n_kv_heads", "n_rows", "out_type", "out_stride", "page_size", "n_pages")]
+
+
+class QuantizeRowsParams(ctypes.Structure):
+    """llmr_quantize_rows_params."""
+    _fields_ = [(n, ctypes.c_uint32) for n in (
+        "n_rows", "dim", "x_type", "x_stride", "q_stride")] + [("eps", ctypes.c_float)]
+
+
+class MatmulI8Params(ctypes.Structure):
+    """llmr_matmul_i8_params."""
+    _fields_ = [(n, ctypes.c_uint32) for n in (
+        "n_rows", "out_dim", "in_dim", "x_stride", "w_stride", "out_type", "out_stride")]
+
+
 # Most requests of one paged_plan or paged_attention call (LLMR_MAX_SEQS).
 MAX_SEQS = 4096
 
@@ -199,6 +222,16 @@ _SIGS = {
     "llmr_paged_attention": (ctypes.c_int, [_vp, _vp, _vp, _vp, _u32, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t,
                                             ctypes.POINTER(PagedAttentionParams)]),
     "llmr_paged_attention_scratch_bytes": (ctypes.c_size_t, [_vp, ctypes.POINTER(PagedAttentionParams)]),
+    "llmr_qkv_tokens_mx4": (ctypes.c_int, [_vp] * 9 + [ctypes.POINTER(Mx4Cache)] * 2 +
+                            [ctypes.POINTER(QkvTokensParams)]),
+    "llmr_paged_attention_mx4": (ctypes.c_int, [_vp, _vp, ctypes.POINTER(Mx4Cache), ctypes.POINTER(Mx4Cache), _u32, _vp,
+                                                _vp, _vp, _vp, _vp, ctypes.c_size_t,
+                                                ctypes.POINTER(PagedAttentionParams)]),
+    "llmr_paged_attention_mx4_scratch_bytes": (ctypes.c_size_t, [_vp, ctypes.POINTER(PagedAttentionParams)]),
+    "llmr_mx4_rows": (ctypes.c_int, [_vp, ctypes.POINTER(Mx4Cache), ctypes.POINTER(Mx4Cache), _vp, _vp, _vp,
+                                     ctypes.POINTER(Mx4RowsParams)]),
+    "llmr_quantize_rows_i8": (ctypes.c_int, [_vp] * 5 + [ctypes.POINTER(QuantizeRowsParams)]),
+    "llmr_matmul_i8": (ctypes.c_int, [_vp] * 6 + [ctypes.POINTER(MatmulI8Params)]),
     "llmr_gguf_open": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(_vp)]),
     "llmr_gguf_close": (ctypes.c_int, [_vp]),
     "llmr_gguf_info": (ctypes.c_int, [_vp, ctypes.POINTER(_u32), ctypes.POINTER(ctypes.c_uint64),
@@ -439,3 +472,27 @@ class Context:
 
     def paged_attention_scratch_bytes(self, params: PagedAttentionParams) -> int:
         return lib().llmr_paged_attention_scratch_bytes(self._h, params)
+
+    # --- the same batches in few bits ---
+
+    def qkv_tokens_mx4(self, qkv, q_norm, k_norm, rope_cos, rope_sin, positions, slots, q, k: Mx4Cache, v: Mx4Cache,
+                       params: QkvTokensParams) -> None:
+        check(lib().llmr_qkv_tokens_mx4(self._h, qkv, q_norm, k_norm, rope_cos, rope_sin, positions, slots, q, k, v,
+                                        params))
+
+    def paged_attention_mx4(self, q, k: Mx4Cache, v: Mx4Cache, type_, out, seq_offsets, kv_len, block_table, scratch,
+                            scratch_bytes, params: PagedAttentionParams) -> None:
+        check(lib().llmr_paged_attention_mx4(self._h, q, k, v, type_, out, seq_offsets, kv_len, block_table, scratch,
+                                             scratch_bytes, params))
+
+    def paged_attention_mx4_scratch_bytes(self, params: PagedAttentionParams) -> int:
+        return lib().llmr_paged_attention_mx4_scratch_bytes(self._h, params)
+
+    def mx4_rows(self, k: Mx4Cache, v: Mx4Cache, slots, k_out, v_out, params: Mx4RowsParams) -> None:
+        check(lib().llmr_mx4_rows(self._h, k, v, slots, k_out, v_out, params))
+
+    def quantize_rows_i8(self, x, norm, q, scales, params: QuantizeRowsParams) -> None:
+        check(lib().llmr_quantize_rows_i8(self._h, x, norm, q, scales, params))
+
+    def matmul_i8(self, x, x_scales, w, w_scales, out, params: MatmulI8Params) -> None:
+        check(lib().llmr_matmul_i8(self._h, x, x_scales, w, w_scales, out, params))

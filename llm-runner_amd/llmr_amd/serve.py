@@ -10,7 +10,9 @@ rows seq_offsets[s] .. seq_offsets[s + 1]. A step of a batch:
     serve.paged_attention(q, k_cache, v_cache, batch.seq_offsets, batch.kv_len, block_table, max_new)
 
 A prompt that needs no cache (the text encoder's) goes through qkv_tokens
-without slots and prompt_attention. Each function issues one C-ABI call on the
+without slots and prompt_attention. A cache in 4 bits (Mx4Cache) is filled by
+qkv_tokens_mx4, read by paged_attention_mx4, and read back by mx4_rows; the
+projections in 8-bit integers are in int8. Each function issues one C-ABI call on the
 current torch stream of the graph's device; lengths, offsets, tables and slots
 are int32 device tensors that nothing here reads back.
 """
@@ -163,6 +165,26 @@ def paged_plan(past_len: torch.Tensor, new_len: torch.Tensor, free_pages: torch.
     return batch
 
 
+def _rope(rope, D: int):
+    """(cos, sin, rows of the tables) of a rotation, or None, None, 0."""
+    if rope is None:
+        return None, None, 0
+    cos, sin = rope
+    if cos.dim() != 2 or cos.shape[1] != D // 2 or sin.shape != cos.shape or cos.shape[0] == 0:
+        raise ValueError("rope must be (cos, sin) of [n_positions, head_dim / 2], n_positions >= 1")
+    return cos, sin, cos.shape[0]
+
+
+def _qkv_rows(qkv: torch.Tensor, q: torch.Tensor):
+    """q's tokens, heads, head_dim and token stride, and qkv's row stride."""
+    if qkv.dim() != 2 or qkv.dtype is not _F32 or (qkv.shape[1] > 1 and qkv.stride(1) != 1) or qkv.stride(0) > _U32:
+        raise ValueError("qkv must be a 2-D f32 view with contiguous rows, under 2^32 apart")
+    T, H, D, qs, qh = _heads(q, "q")
+    if qkv.shape[0] != T or qh != D:
+        raise ValueError("q must be [tokens, n_heads, head_dim] with qkv's tokens and heads side by side")
+    return T, H, D, qs, qkv.stride(0) if T > 1 else qkv.shape[1] + -qkv.shape[1] % 4
+
+
 def qkv_tokens(qkv: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                slots: torch.Tensor | None = None, positions: torch.Tensor | None = None,
                q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, eps: float = 1e-6,
@@ -172,11 +194,7 @@ def qkv_tokens(qkv: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Ten
     caches [n_pages, n_kv_heads, page_size, D], a row with slot -1 nowhere; without, rows [T, n_kv_heads, D].
     rope: (cos, sin) f32 [n_positions, D / 2], taken at positions (int32 [T]; None: the row), rotating the
     pairs (j, j + D/2), or (2j, 2j + 1) where halves is False."""
-    if qkv.dim() != 2 or qkv.dtype is not _F32 or (qkv.shape[1] > 1 and qkv.stride(1) != 1) or qkv.stride(0) > _U32:
-        raise ValueError("qkv must be a 2-D f32 view with contiguous rows, under 2^32 apart")
-    T, H, D, qs, qh = _heads(q, "q")
-    if qkv.shape[0] != T or qh != D:
-        raise ValueError("q must be [tokens, n_heads, head_dim] with qkv's tokens and heads side by side")
+    T, H, D, qs, row = _qkv_rows(qkv, q)
     t = _type("q, k and v", q, k, v)
     ks = n_pages = page = 0
     if slots is not None:
@@ -189,17 +207,10 @@ def qkv_tokens(qkv: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Ten
             raise ValueError("k and v must be [tokens, n_kv_heads, head_dim] alike, heads side by side")
     if Dk != D or qkv.shape[1] < (H + 2 * Hk) * D:
         raise ValueError("k and v must have q's head_dim, and qkv (n_heads + 2 n_kv_heads) * head_dim columns")
-    cos = sin = None
-    n_pos = 0
-    if rope is not None:
-        cos, sin = rope
-        if cos.dim() != 2 or cos.shape[1] != D // 2 or sin.shape != cos.shape or cos.shape[0] == 0:
-            raise ValueError("rope must be (cos, sin) of [n_positions, head_dim / 2], n_positions >= 1")
-        n_pos = cos.shape[0]
+    cos, sin, n_pos = _rope(rope, D)
     pp = _ints(positions, "positions", T) if positions is not None else None
     args = (_vec(q_norm, "q_norm", D), _vec(k_norm, "k_norm", D), _vec(cos, "rope_cos", 0), _vec(sin, "rope_sin", 0))
-    p = capi.QkvTokensParams(D, H, Hk, T, qkv.stride(0) if T > 1 else qkv.shape[1] + -qkv.shape[1] % 4, qs, t, ks, page,
-                             n_pages, n_pos, halves, eps)
+    p = capi.QkvTokensParams(D, H, Hk, T, row, qs, t, ks, page, n_pages, n_pos, halves, eps)
     on = [x for x in (qkv, q, k, v, slots, positions, q_norm, k_norm, cos, sin) if x is not None]
     _graph(g, *on).ctx.qkv_tokens(qkv.data_ptr(), *args, pp, sp, q.data_ptr(), k.data_ptr(), v.data_ptr(), p)
 
@@ -249,4 +260,117 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise ValueError("scratch must be a contiguous tensor on q's device")
     g.ctx.paged_attention(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), t, out.data_ptr(), off, kvl, tab,
                           scratch.data_ptr(), scratch.numel() * scratch.element_size(), p)
+    return out
+
+
+@dataclasses.dataclass
+class Mx4Cache:
+    """A key or value cache in 4 bits (llmr_mx4_cache): data uint8 [n_pages, n_kv_heads, page_size, head_dim / 2], two
+    E2M1 numbers a byte, and scales uint8 [n_pages, n_kv_heads, page_size, head_dim / 32], a power of two + 127 for
+    each 32 of them."""
+    data: torch.Tensor
+    scales: torch.Tensor
+
+    @staticmethod
+    def empty(n_pages: int, n_kv_heads: int, page_size: int, head_dim: int, device="cuda") -> "Mx4Cache":
+        """A cache whose rows are 0."""
+        return Mx4Cache(*(torch.zeros(n_pages, n_kv_heads, page_size, n, dtype=torch.uint8, device=device)
+                          for n in (head_dim // 2, head_dim // 32)))
+
+
+def _mx4(k: Mx4Cache, v: Mx4Cache):
+    """(pages, heads, page size, head_dim) of a pair of caches, and the structures of the call."""
+    kd, ks, vd, vs = k.data, k.scales, v.data, v.scales
+    if kd.dim() != 4 or not (kd.dtype is ks.dtype is vd.dtype is vs.dtype is torch.uint8) or not (
+            kd.is_contiguous() and ks.is_contiguous() and vd.is_contiguous() and vs.is_contiguous()):
+        raise ValueError("the caches' data and scales must be contiguous uint8 tensors of four dimensions")
+    n, h, page, half = kd.shape
+    if vd.shape != kd.shape or half % 16 or ks.shape != (n, h, page, half // 16) or vs.shape != ks.shape:
+        raise ValueError("the caches must be [n_pages, n_kv_heads, page_size, head_dim / 2] with scales [.., head_dim "
+                         "/ 32], alike")
+    return n, h, page, 2 * half, capi.Mx4Cache(kd.data_ptr(), ks.data_ptr()), capi.Mx4Cache(vd.data_ptr(), vs.data_ptr())
+
+
+def qkv_tokens_mx4(qkv: torch.Tensor, q: torch.Tensor, k: Mx4Cache, v: Mx4Cache, slots: torch.Tensor,
+                   positions: torch.Tensor | None = None, q_norm: torch.Tensor | None = None,
+                   k_norm: torch.Tensor | None = None, eps: float = 1e-6, rope: tuple | None = None,
+                   halves: bool = True, g: RenderGraph | None = None) -> None:
+    """qkv_tokens into 4-bit caches (llmr_qkv_tokens_mx4): qkv, q, norms, rotation and positions as there; slots int32
+    [T], a row with slot -1 goes nowhere, the others' slots are distinct. q f16 or bf16."""
+    T, H, D, qs, row = _qkv_rows(qkv, q)
+    t = _TYPES.get(q.dtype)
+    if t is None:
+        raise ValueError("q must be float16 or bfloat16")
+    n_pages, Hk, page, Dk, ck, cv = _mx4(k, v)
+    if Dk != D or qkv.shape[1] < (H + 2 * Hk) * D:
+        raise ValueError("k and v must have q's head_dim, and qkv (n_heads + 2 n_kv_heads) * head_dim columns")
+    cos, sin, n_pos = _rope(rope, D)
+    pp = _ints(positions, "positions", T) if positions is not None else None
+    args = (_vec(q_norm, "q_norm", D), _vec(k_norm, "k_norm", D), _vec(cos, "rope_cos", 0), _vec(sin, "rope_sin", 0), pp,
+            _ints(slots, "slots", T))
+    p = capi.QkvTokensParams(D, H, Hk, T, row, qs, t, 0, page, n_pages, n_pos, halves, eps)
+    on = [x for x in (qkv, q, k.data, k.scales, v.data, v.scales, slots, positions, q_norm, k_norm, cos, sin)
+          if x is not None]
+    _graph(g, *on).ctx.qkv_tokens_mx4(qkv.data_ptr(), *args, q.data_ptr(), ck, cv, p)
+
+
+def mx4_rows(k: Mx4Cache, v: Mx4Cache, slots: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor,
+             g: RenderGraph | None = None) -> None:
+    """Cached rows as the values they stand for (llmr_mx4_rows): row r of k_out and v_out [n, n_kv_heads, head_dim], f16
+    or bf16, is what slot slots[r] holds (left as it is where that is outside the cache)."""
+    n_pages, Hk, page, D, ck, cv = _mx4(k, v)
+    n, h, d, os_, oh = _heads(k_out, "k_out")
+    t = _TYPES.get(k_out.dtype)
+    if t is None or v_out.dtype is not k_out.dtype or not _alike(k_out, v_out):
+        raise ValueError("k_out and v_out must be f16 or bf16 rows alike")
+    if (h, d) != (Hk, D) or oh != D:
+        raise ValueError("k_out and v_out must be [n, n_kv_heads, head_dim] of the caches, heads side by side")
+    sp = _ints(slots, "slots", n)
+    _graph(g, k.data, k.scales, v.data, v.scales, slots, k_out, v_out).ctx.mx4_rows(
+        ck, cv, sp, k_out.data_ptr(), v_out.data_ptr(), capi.Mx4RowsParams(D, Hk, n, t, os_, page, n_pages))
+
+
+def paged_attention_mx4_scratch(q: torch.Tensor, k: Mx4Cache, block_table: torch.Tensor, max_new: int,
+                                g: RenderGraph | None = None) -> torch.Tensor:
+    """A scratch tensor for paged_attention_mx4 calls of these shapes (llmr_paged_attention_mx4_scratch_bytes)."""
+    T, H, D = q.shape
+    n_pages, Hk, page, _ = k.data.shape
+    if max_new < 0:
+        raise ValueError("max_new must be >= 0")
+    p = capi.PagedAttentionParams(D, H, Hk, T, block_table.shape[0], min(max_new, T), page, n_pages,
+                                  block_table.shape[1], H * D, H * D, 1.0)
+    g = _graph(g, q)
+    return torch.empty(g.ctx.paged_attention_mx4_scratch_bytes(p), dtype=torch.uint8, device=q.device)
+
+
+def paged_attention_mx4(q: torch.Tensor, k: Mx4Cache, v: Mx4Cache, seq_offsets: torch.Tensor, kv_len: torch.Tensor,
+                        block_table: torch.Tensor, max_new: int, scale: float | None = None,
+                        out: torch.Tensor | None = None, scratch: torch.Tensor | None = None,
+                        g: RenderGraph | None = None) -> torch.Tensor:
+    """paged_attention over 4-bit caches (llmr_paged_attention_mx4): the arguments as there, q f16 or bf16; scratch:
+    paged_attention_mx4_scratch's, one per call that may overlap another; None: a new one."""
+    T, H, D, qs, qh = _heads(q, "q")
+    n_pages, Hk, page, Dk, ck, cv = _mx4(k, v)
+    n = kv_len.numel()
+    if Dk != D or qh != D:
+        raise ValueError("q must be [tokens, n_heads, head_dim], heads side by side, with the caches' head_dim")
+    if seq_offsets.numel() != n + 1 or block_table.dim() != 2 or block_table.shape[0] != n:
+        raise ValueError("kv_len, block_table's rows and seq_offsets (one more) must be one per request")
+    if max_new < 0:
+        raise ValueError("max_new must be >= 0")
+    t = _TYPES.get(q.dtype)
+    if t is None:
+        raise ValueError("q must be float16 or bfloat16")
+    if out is None:
+        out = torch.empty(T, H * D, dtype=q.dtype, device=q.device)
+    p = capi.PagedAttentionParams(D, H, Hk, T, n, min(max_new, T), page, n_pages, block_table.shape[1], qs,
+                                  _out_stride(out, T, H * D, q), D ** -0.5 if scale is None else scale)
+    off, kvl, tab = _ints(seq_offsets, "seq_offsets", 0), _ints(kv_len, "kv_len", 0), _ints(block_table, "block_table", 0)
+    g = _graph(g, q, k.data, k.scales, v.data, v.scales, seq_offsets, kv_len, block_table, out)
+    if scratch is None:
+        scratch = torch.empty(g.ctx.paged_attention_mx4_scratch_bytes(p), dtype=torch.uint8, device=q.device)
+    elif scratch.get_device() != q.get_device() or not scratch.is_contiguous():
+        raise ValueError("scratch must be a contiguous tensor on q's device")
+    g.ctx.paged_attention_mx4(q.data_ptr(), ck, cv, t, out.data_ptr(), off, kvl, tab, scratch.data_ptr(),
+                              scratch.numel() * scratch.element_size(), p)
     return out

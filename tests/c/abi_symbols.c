@@ -58,6 +58,12 @@ static const struct {
     {"llmr_qkv_tokens", (void (*)(void))(uintptr_t)llmr_qkv_tokens},
     {"llmr_paged_attention", (void (*)(void))(uintptr_t)llmr_paged_attention},
     {"llmr_paged_attention_scratch_bytes", (void (*)(void))(uintptr_t)llmr_paged_attention_scratch_bytes},
+    {"llmr_qkv_tokens_mx4", (void (*)(void))(uintptr_t)llmr_qkv_tokens_mx4},
+    {"llmr_paged_attention_mx4", (void (*)(void))(uintptr_t)llmr_paged_attention_mx4},
+    {"llmr_paged_attention_mx4_scratch_bytes", (void (*)(void))(uintptr_t)llmr_paged_attention_mx4_scratch_bytes},
+    {"llmr_mx4_rows", (void (*)(void))(uintptr_t)llmr_mx4_rows},
+    {"llmr_quantize_rows_i8", (void (*)(void))(uintptr_t)llmr_quantize_rows_i8},
+    {"llmr_matmul_i8", (void (*)(void))(uintptr_t)llmr_matmul_i8},
     {"llmr_q8_lora_merge", (void (*)(void))(uintptr_t)llmr_q8_lora_merge},
     {"llmr_flash_attention", (void (*)(void))(uintptr_t)llmr_flash_attention},
     {"llmr_flash_attention_pc", (void (*)(void))(uintptr_t)llmr_flash_attention_pc},
