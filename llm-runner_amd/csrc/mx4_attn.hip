@@ -1,6 +1,6 @@
 // mx4_attn.hip - attention of a batch of requests over a paged cache in 4 bits
 // (llmr_paged_attention_mx4).
-#include "seq_attn_few.h"
+#include "mx4_attn_few.h"
 
 namespace llmr {
 namespace {
@@ -52,16 +52,59 @@ __global__ void __launch_bounds__(64) mx4_attn_rows(SeqAttnArgs a, const uint8_t
 
 }  // namespace
 
-size_t paged_attention_mx4_scratch_bytes(uint32_t, uint32_t, uint32_t, uint32_t, int) { return 0; }
+// Row blocks of 16 of the kernel for few rows that holds max_new tokens of a group; 0: more rows.
+static uint32_t mx4_blocks(uint32_t n_heads, uint32_t n_kv_heads, uint32_t max_new) {
+    const uint64_t rows = (uint64_t)max_new * (n_heads / n_kv_heads);
+    return rows <= 16u ? 1u : rows <= 32u ? 2u : rows <= 64u ? 4u : 0u;
+}
+static uint32_t mx4_workers(uint32_t nr, int num_cus) {
+    return (uint32_t)num_cus * (nr == 1u ? mx4attn::few_waves<1>() : nr == 2u ? mx4attn::few_waves<2>() : mx4attn::few_waves<4>());
+}
+
+size_t paged_attention_mx4_scratch_bytes(uint32_t dim, uint32_t n_heads, uint32_t n_kv_heads, uint32_t max_new,
+                                         int num_cus) {
+    const uint32_t nr = mx4_blocks(n_heads, n_kv_heads, max_new);
+    if (nr == 0) return 0;
+    const size_t part = 16u * nr * (dim + 2u) * sizeof(float);
+    return mx4_workers(nr, num_cus) * (sizeof(seqattn::JoinRecord) + 2u * part);
+}
+
+template <uint32_t R>
+using Rows = std::integral_constant<uint32_t, R>;
+
+template <uint32_t T, uint32_t D>
+static hipError_t launch_mx4(const mx4attn::Mx4Args& m4, uint32_t nr, int num_cus, void* scratch, hipStream_t st) {
+    using namespace mx4attn;
+    const SeqAttnArgs& a = m4.a;
+    if (nr == 0) {
+        hipLaunchKernelGGL((mx4_attn_rows<T, D>), dim3(a.n_tokens * a.n_heads), dim3(64), 0, st, a, m4.k_scales, m4.v_scales);
+        return hipGetLastError();
+    }
+    const uint32_t n = mx4_workers(nr, num_cus);
+    auto* const records = (JoinRecord*)scratch;
+    auto* const parts = (float*)(records + n);
+    auto go = [&](auto work, uint32_t threads, auto join, auto part) {
+        constexpr uint32_t PR = decltype(part)::value;
+        hipLaunchKernelGGL(work, dim3(n), dim3(threads), 0, st, m4, records, parts);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL(join, dim3(PR / 16u, n), dim3(join_threads<D, PR>()), 0, st, a, records, parts);
+        return hipGetLastError();
+    };
+    if (nr == 1u) return go(mx4_attn_few<T, D, 1>, 64 * kWaves, paged_attn_join<T, D, 16>, Rows<16>{});
+    if (nr == 2u) return go(mx4_attn_few<T, D, 2>, 64 * kWaves, paged_attn_join<T, D, 32>, Rows<32>{});
+    return go(mx4_attn_few<T, D, 4>, 64 * kWaves, paged_attn_join<T, D, 64>, Rows<64>{});
+}
 
 hipError_t launch_paged_attention_mx4(const SeqAttnArgs& a, const uint8_t* k_scales, const uint8_t* v_scales,
-                                      uint32_t type, uint32_t dim, int, void*, hipStream_t st) {
-    auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(a.n_tokens * a.n_heads), dim3(64), 0, st, a, k_scales, v_scales);
-    };
-    if (type == kGgmlBF16) dim == 128u ? go(mx4_attn_rows<kGgmlBF16, 128>) : go(mx4_attn_rows<kGgmlBF16, 64>);
-    else dim == 128u ? go(mx4_attn_rows<kGgmlF16, 128>) : go(mx4_attn_rows<kGgmlF16, 64>);
-    return hipGetLastError();
+                                      uint32_t type, uint32_t dim, int num_cus, void* scratch, hipStream_t st) {
+    const uint32_t nr = mx4_blocks(a.n_heads, a.n_kv_heads, a.max_new);
+    const mx4attn::Mx4Args m4{a, k_scales, v_scales};
+    if (type == kGgmlBF16)
+        return dim == 128u ? launch_mx4<kGgmlBF16, 128>(m4, nr, num_cus, scratch, st)
+                           : launch_mx4<kGgmlBF16, 64>(m4, nr, num_cus, scratch, st);
+    return dim == 128u ? launch_mx4<kGgmlF16, 128>(m4, nr, num_cus, scratch, st)
+                       : launch_mx4<kGgmlF16, 64>(m4, nr, num_cus, scratch, st);
 }
 
 }  // namespace llmr

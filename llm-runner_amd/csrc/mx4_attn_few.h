@@ -1,0 +1,384 @@
+// mx4_attn_few.h - attention over a paged cache in 4 bits for requests of few new tokens
+// (mx4_attn.hip): at most 16 NR rows (new tokens x query heads of a group) a key/value head.
+//
+// As paged_attn_few, a stream of the cache: the keys of all (request, key/value head) pairs, cut
+// into units of 32, make one line that the workers share evenly; a worker has at most two parts of
+// pairs, which paged_attn_join joins. What differs follows from the rows being short (64 bytes of
+// numbers and 4 of powers of two at head_dim 128):
+//  - a worker is a workgroup of four waves that take its units in turn and add up their rows in
+//    LDS at a pair's end. With a wave a worker, as many waves as the short rows need would leave
+//    four times the parts to join;
+//  - keys and values come into registers, a unit ahead: a lane has a quarter of a key's row (a
+//    block of 32, at head_dim 128), which is what its products with the queries take if the dims
+//    are dealt out so (lane group g: dims D/4 g ..; the queries alike), so that keys need no LDS;
+//  - v_cvt_scalef32_pk_{bf16,f16}_fp4 turns two numbers and their power of two into 16-bit values,
+//    exactly, at the rate of an f32 fma: a unit's 8192 elements are 128 instructions. The values
+//    are written to LDS as 16-bit rows and read transposed.
+// S^T = K Q^T and O^T += V^T P^T by 16x16x32 MFMAs, the softmax and the treatment of masked keys
+// as in paged_attn_few.
+#pragma once
+
+#include "seq_attn_few.h"
+
+namespace llmr {
+namespace mx4attn {
+namespace {
+
+using namespace seqattn;
+
+constexpr uint32_t kWaves = 4;  // of a worker
+
+struct Mx4Args {
+    SeqAttnArgs a;
+    const uint8_t* k_scales;
+    const uint8_t* v_scales;
+};
+
+// Eight numbers (a dword) times a power of two, as 16-bit values.
+template <uint32_t T>
+__device__ __forceinline__ s16x8 values8(uint32_t w, float s) {
+    u32x4 o;
+    if constexpr (T == kGgmlBF16) {
+        o.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0));
+        o.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1));
+        o.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2));
+        o.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3));
+    } else {
+        o.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 0));
+        o.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 1));
+        o.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 2));
+        o.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 3));
+    }
+    return __builtin_bit_cast(s16x8, o);
+}
+__device__ __forceinline__ float power(uint32_t byte) { return __uint_as_float(byte << 23); }  // (255: NaN comes out)
+
+// A unit's share of a lane: of keys n16 and 16 + n16, dims D/4 g .. + D/4 - 1.
+template <uint32_t D>
+struct Mx4Unit {
+    uint32_t k[2][D / 32], v[2][D / 32];
+    uint32_t ks[2], vs[2];
+    bool on0, on1;  // (uniform) the halves have a page
+};
+
+template <uint32_t D, uint32_t NR>
+constexpr uint32_t few_lds_bytes() { return kWaves * (32u * D * 2u) + kWaves * 16u * 2u * 4u; }
+
+template <uint32_t T, uint32_t D, uint32_t NR>
+__device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRecord* __restrict__ records,
+                                         float* __restrict__ parts) {
+    const SeqAttnArgs& a = m4.a;
+    constexpr uint32_t ROW4 = D / 2u, CB = D / 8u, SROW = D / 32u;  // bytes: a row's numbers, a lane's, a row's powers
+    constexpr uint32_t ROW = D * 2u, TILE = 32u * ROW;              // of 16-bit values: a row, a wave's tile of V
+    constexpr int ND = D / 32, DT = D / 16;
+    constexpr float OFF = T == kGgmlF16 ? 7.0f : 0.0f;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, n16 = lane & 15u, g = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t G = a.n_heads / a.n_kv_heads;
+    const float c = a.scale_log2, grow_by = 8.0f / c;
+    const auto cost = [](const PagedRequest& r) { return (uint64_t)units_of(r); };
+
+    RequestWindow win;
+    const uint64_t w = batch_cost(a, win, lane, cost) * a.n_kv_heads;
+    // a unit a wave at least, while there are few
+    const uint32_t n = (uint32_t)min((uint64_t)gridDim.x, (w + kWaves - 1u) / kWaves);
+    JoinRecord rec{};
+    if (blockIdx.x >= n) {
+        if (tid == 0) records[blockIdx.x].last = 0;
+        return;
+    }
+    uint64_t at = part_begin(blockIdx.x, w, n);
+    const uint64_t end = part_begin(blockIdx.x + 1u, w, n);
+
+    // rows x = 16 r + n16: token x / G, head of the group x % G
+    uint32_t tok[NR], qoff[NR];
+#pragma unroll
+    for (int r = 0; r < (int)NR; r++) {
+        const uint32_t x = 16u * r + n16;
+        tok[r] = x / G;
+        qoff[r] = tok[r] * a.q_stride + (x % G) * a.q_head_stride + D / 4u * g;
+    }
+    const uint32_t kvo = n16 * ROW4 + g * CB, so = n16 * SROW + (D == 128u ? g : g >> 1);
+    uint8_t* const vt = lds + wave * TILE;
+    const uint32_t vt0 = (uint32_t)(uintptr_t)(lds_void*)vt;
+    uint32_t vto[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++) {
+        const uint32_t r = 4u * g + (n16 >> 2);
+        vto[dt] = vt0 + r * ROW + (((2u * dt + ((n16 & 3u) >> 1)) ^ fswz<D>(r)) << 4) + 8u * (n16 & 1u);
+    }
+
+    uint64_t base;
+    uint32_t s = find_request(a, win, lane, cost, a.n_kv_heads, at, base);
+    PagedRequest rq = win.get(s);
+    uint32_t units = units_of(rq), kvh = (uint32_t)((at - base) / units), u0 = (uint32_t)((at - base) % units);
+
+    while (true) {
+        const uint32_t u1 = (uint32_t)min((uint64_t)units, u0 + (end - at));  // units [u0, u1) of the pair are this part
+        const uint32_t rows = rq.rows * G;
+        const uint32_t count = u1 - u0 > wave ? (u1 - u0 - wave + kWaves - 1u) / kWaves : 0u;  // of them this wave's
+        const int32_t hi_min = rq.pos0;  // (the first token's rows see least)
+        s16x8 qf[NR][ND];
+        int32_t hi[NR];  // last key the row sees
+        f32x4 o[NR][DT];
+        float m_ref[NR], l_i[NR];
+        uint32_t fresh = (1u << NR) - 1u, sees = 0;  // per row block: no maximum yet; a key seen
+        const uint8_t* const q0 = (const uint8_t*)a.q + 2u * ((uint64_t)rq.first * a.q_stride + (uint64_t)kvh * G * a.q_head_stride);
+#pragma unroll
+        for (int r = 0; r < (int)NR; r++) {
+            const bool live = 16u * r + n16 < rows;
+            hi[r] = live ? rq.pos0 + (int32_t)tok[r] : -1;
+            const uint8_t* const qr = q0 + 2u * (live ? qoff[r] : D / 4u * g);
+#pragma unroll
+            for (int ch = 0; ch < ND; ch++) qf[r][ch] = *(const s16x8*)(qr + 16 * ch);
+            m_ref[r] = l_i[r] = 0.0f;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) o[r][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+
+        // pages of this wave's units i0 .. i0 + 31, a half a lane (negative: none)
+        int32_t pages = -1;
+        auto window = [&](uint32_t i0) {
+            const uint32_t k0 = (u0 + wave + kWaves * (i0 + (lane >> 1))) * kUnit + 16u * (lane & 1u);
+            pages = -1;
+            if (i0 + (lane >> 1) < count && k0 < rq.keys) {
+                const int32_t p = a.table[(size_t)s * a.max_pages + (k0 >> a.page_log2)];
+                pages = p >= 0 && (uint32_t)p < a.n_pages ? p : -1;
+            }
+        };
+        auto load = [&](Mx4Unit<D>& x, uint32_t i) {
+            if ((i & 31u) == 0) window(i);
+            const uint32_t k0 = (u0 + wave + kWaves * i) * kUnit;
+#pragma unroll
+            for (uint32_t h = 0; h < 2u; h++) {
+                const uint32_t k = k0 + 16u * h;
+                const int32_t p = __builtin_amdgcn_readlane(pages, (int)(2u * (i & 31u) + h));
+                const uint64_t row = (((uint64_t)(uint32_t)max(p, 0) * a.n_kv_heads + kvh) << a.page_log2) +
+                                     (k & ((1u << a.page_log2) - 1u));
+                // keys past the last one, and those of no page, read as zero
+                const uint32_t keys = p < 0 ? 0u : min(__builtin_elementwise_sub_sat(rq.keys, k), 16u);
+                const auto rsrc = [&](const void* b, uint32_t size) {
+                    return __builtin_amdgcn_make_buffer_rsrc((uint8_t*)const_cast<void*>(b) + row * size, (short)0,
+                                                             (int)__builtin_amdgcn_readfirstlane(keys * size), 0x00020000);
+                };
+                const rsrc_t kr = rsrc(a.k, ROW4), vr = rsrc(a.v, ROW4), ksr = rsrc(m4.k_scales, SROW),
+                             vsr = rsrc(m4.v_scales, SROW);
+                if constexpr (D == 128u) {
+                    const u32x4 kk = __builtin_amdgcn_raw_buffer_load_b128(kr, kvo, 0, 0);
+                    const u32x4 vv = __builtin_amdgcn_raw_buffer_load_b128(vr, kvo, 0, 0);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        x.k[h][e] = kk[e];
+                        x.v[h][e] = vv[e];
+                    }
+                } else {
+                    const u32x2 kk = __builtin_amdgcn_raw_buffer_load_b64(kr, kvo, 0, 0);
+                    const u32x2 vv = __builtin_amdgcn_raw_buffer_load_b64(vr, kvo, 0, 0);
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        x.k[h][e] = kk[e];
+                        x.v[h][e] = vv[e];
+                    }
+                }
+                x.ks[h] = __builtin_amdgcn_raw_buffer_load_b8(ksr, so, 0, 0);
+                x.vs[h] = __builtin_amdgcn_raw_buffer_load_b8(vsr, so, 0, 0);
+                (h == 0 ? x.on0 : x.on1) = p >= 0;
+            }
+        };
+        auto step = [&](Mx4Unit<D>& x, uint32_t i) {
+            const uint32_t u = u0 + wave + kWaves * i;
+            // keys past the last one, on no page, or unseen by a row: masked
+            const bool masked = !x.on0 || !x.on1 || (int32_t)(u * kUnit + kUnit - 1u) > hi_min;
+            if (masked) {
+                // a row's weight of a key it does not see is 0, and 0 times NaN is NaN: such blocks of V are
+                // set to 0 here, and the rows that do see them become NaN at once
+                const uint64_t b0 = __builtin_amdgcn_ballot_w64(x.vs[0] == 255u), b1 = __builtin_amdgcn_ballot_w64(x.vs[1] == 255u);
+                if ((b0 | b1) != 0) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        for (uint64_t b = h == 0 ? b0 : b1; b != 0; b &= b - 1u) {
+                            const uint32_t l = (uint32_t)__builtin_ctzll(b);
+                            const int32_t key = (int32_t)(u * kUnit + 16u * h + (l & 15u));
+                            const uint32_t block = D == 128u ? l >> 4 : l >> 5;
+#pragma unroll
+                            for (int r = 0; r < (int)NR; r++)
+#pragma unroll
+                                for (int dt = 0; dt < DT; dt++)
+                                    if (key <= hi[r] && (uint32_t)dt >> 1 == block) o[r][dt] += __uint_as_float(0x7fc00000u);
+                        }
+                        if (x.vs[h] == 255u) {
+                            x.vs[h] = 0;
+#pragma unroll
+                            for (int e = 0; e < ND; e++) x.v[h][e] = 0;
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (uint32_t h = 0; h < 2u; h++) {
+                const uint32_t r = 16u * h + n16;
+                const float sv = power(x.vs[h]);
+#pragma unroll
+                for (uint32_t e = 0; e < (uint32_t)ND; e++)
+                    *(s16x8*)(vt + r * ROW + (((ND * g + e) ^ fswz<D>(r)) << 4)) = values8<T>(x.v[h][e], sv);
+            }
+            f32x4 sc[NR][2];
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++) {
+                const float sk = power(x.ks[kb]);
+#pragma unroll
+                for (int ch = 0; ch < ND; ch++) {
+                    const s16x8 k = values8<T>(x.k[kb][ch], sk);
+#pragma unroll
+                    for (int r = 0; r < (int)NR; r++)
+                        sc[r][kb] = mfma16<T>(k, qf[r][ch], ch == 0 ? f32x4{} - m_ref[r] : sc[r][kb]);
+                }
+            }
+            s16x8 pf[NR];
+#pragma unroll
+            for (int r = 0; r < (int)NR; r++) {
+                if (masked) {
+                    const int32_t k0 = (int32_t)(u * kUnit + 4u * g);
+                    bool any = false;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const bool a0 = x.on0 && k0 + e <= hi[r], a1 = x.on1 && k0 + 16 + e <= hi[r];
+                        sc[r][0][e] = a0 ? sc[r][0][e] : -INFINITY;
+                        sc[r][1][e] = a1 ? sc[r][1][e] : -INFINITY;
+                        any = any || a0 || a1;
+                    }
+                    if (any) sees |= 1u << r;
+                } else {
+                    sees |= 1u << r;
+                }
+                float mx = -INFINITY;
+#pragma unroll
+                for (int e = 0; e < 4; e++) mx = fmaxf(fmaxf(mx, sc[r][0][e]), sc[r][1][e]);
+                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                const bool fr = (fresh >> r) & 1u;
+                if (__builtin_amdgcn_ballot_w64(mx > grow_by || (fr && mx > -INFINITY)) != 0) {
+                    // (only rows whose own maximum calls for it)
+                    const float d = fr ? (mx > -INFINITY ? mx : 0.0f) : (mx > grow_by ? mx : 0.0f);
+                    const float alpha = fr ? 0.0f : __builtin_amdgcn_exp2f(-d * c);
+                    m_ref[r] += d;
+                    l_i[r] *= alpha;
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++) o[r][dt] *= alpha;
+                    sc[r][0] -= d;
+                    sc[r][1] -= d;
+                    if (mx > -INFINITY) fresh &= ~(1u << r);
+                }
+                float p[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    p[e] = __builtin_amdgcn_exp2f(fmaf(sc[r][e >> 2][e & 3], c, OFF));
+                    l_i[r] += p[e];
+                }
+                pf[r] = __builtin_bit_cast(s16x8, u32x4{pack2<T>(p[0], p[1]), pack2<T>(p[2], p[3]), pack2<T>(p[4], p[5]),
+                                                       pack2<T>(p[6], p[7])});
+            }
+            asm volatile("" ::: "memory");  // (a wave's LDS accesses run in order: the reads follow its own writes)
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) {
+                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(vto[dt]));
+                const s16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(vto[dt] + 16u * ROW));
+                const s16x8 v = s16x8{lo.x, lo.y, lo.z, lo.w, up.x, up.y, up.z, up.w};
+#pragma unroll
+                for (int r = 0; r < (int)NR; r++) o[r][dt] = mfma16<T>(v, pf[r], o[r][dt]);
+            }
+            asm volatile("" ::: "memory");
+        };
+        if (count != 0) {
+            Mx4Unit<D> x, y;
+            load(x, 0);
+            for (uint32_t i = 0;; i += 2u) {
+                if (i + 1u < count) load(y, i + 1u);
+                step(x, i);
+                if (i + 1u >= count) break;
+                if (i + 2u < count) load(x, i + 2u);
+                step(y, i + 1u);
+                if (i + 2u >= count) break;
+            }
+        }
+
+        // the four waves' rows: through LDS, 16 of them at a time
+        const bool begun = u0 == 0, last = u1 == units;
+        float* const part = parts + (size_t)(2u * blockIdx.x + (begun ? 1u : 0u)) * part_floats<D, NR>();
+        float* const ml = (float*)(lds + kWaves * TILE);  // [kWaves][2][16]: m, l
+        at += u1 - u0;
+        if (begun && !last)  // (the worker's last part: the record is its one)
+            rec = JoinRecord{part_of(at + (units - u1) - 1u, w, n), rq.first, 0, rows, kvh, {}};
+#pragma unroll
+        for (int r = 0; r < (int)NR; r++) {
+            if (16u * r >= rows) break;
+            float l = l_i[r];
+            l += __shfl_xor(l, 16, 64);
+            l += __shfl_xor(l, 32, 64);
+            // a row's four lanes have seen different keys of a masked unit
+            uint32_t sn = (sees >> r) & 1u;
+            sn |= (uint32_t)__shfl_xor((int)sn, 16, 64);
+            sn |= (uint32_t)__shfl_xor((int)sn, 32, 64);
+            f32x4* const ow = (f32x4*)vt;  // [16][D / 4], chunk q of row x at q ^ x
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) ow[n16 * (D / 4u) + ((4u * dt + g) ^ n16)] = o[r][dt];
+            if (g == 0) {
+                ml[wave * 32u + n16] = (fresh >> r) & 1u ? -INFINITY : m_ref[r];
+                ml[wave * 32u + 16u + n16] = sn ? l : -1.0f;
+            }
+            __syncthreads();
+            const uint32_t here = min(rows - 16u * r, 16u);
+            for (uint32_t it = tid; it < here * (D / 4u); it += 64u * kWaves) {
+                const uint32_t x = it / (D / 4u), q = it % (D / 4u);
+                f32x4 oj{0.0f, 0.0f, 0.0f, 0.0f};
+                float mj = -INFINITY, lj = -1.0f;
+#pragma unroll
+                for (uint32_t v = 0; v < kWaves; v++)
+                    join_part(oj, mj, lj, ((const f32x4*)(lds + v * TILE))[x * (D / 4u) + (q ^ x)], ml[v * 32u + x],
+                              ml[v * 32u + 16u + x], c);
+                const uint32_t row = 16u * r + x;
+                if (begun && last) {
+                    uint16_t* const dst = (uint16_t*)a.out + (size_t)(rq.first + row / G) * a.out_stride +
+                                          (kvh * G + row % G) * D + 4u * q;
+                    const f32x4 v = oj * (1.0f / lj);
+                    *(u32x2*)dst = lj != -1.0f ? u32x2{pack2<T>(v.x, v.y), pack2<T>(v.z, v.w)} : u32x2{0u, 0u};
+                } else {
+                    *(f32x4*)(part + row * D + 4u * q) = oj;
+                    if (q == 0) {
+                        part[16u * NR * D + row] = mj;
+                        part[16u * NR * (D + 1u) + row] = lj;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        if (at >= end) break;
+        // the next pair (units are left, so there is a request that has some)
+        u0 = 0;
+        if (++kvh == a.n_kv_heads) {
+            kvh = 0;
+            do {
+                s++;
+                if (s - win.s0 >= 64u) win.load(a, s, lane);
+                rq = win.get(s);
+                units = units_of(rq);
+            } while (units == 0 && s + 1u < a.n_seqs);
+        }
+    }
+    if (tid == 0) records[blockIdx.x] = rec;
+}
+
+// Waves a SIMD: what the registers let reside.
+template <uint32_t NR>
+constexpr uint32_t few_waves() { return NR == 1u ? 3u : NR == 2u ? 2u : 1u; }
+
+template <uint32_t T, uint32_t D, uint32_t NR>
+__global__ void __launch_bounds__(64 * kWaves, few_waves<NR>())
+mx4_attn_few(Mx4Args m4, JoinRecord* __restrict__ records, float* __restrict__ parts) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[few_lds_bytes<D, NR>()];
+    few_rows<T, D, NR>(m4, lds, records, parts);
+}
+
+}  // namespace
+}  // namespace mx4attn
+}  // namespace llmr
