@@ -34,25 +34,6 @@ struct Mx4Args {
     const uint8_t* v_scales;
 };
 
-// Eight numbers (a dword) times a power of two, as 16-bit values.
-template <uint32_t T>
-__device__ __forceinline__ s16x8 values8(uint32_t w, float s) {
-    u32x4 o;
-    if constexpr (T == kGgmlBF16) {
-        o.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0));
-        o.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1));
-        o.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2));
-        o.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3));
-    } else {
-        o.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 0));
-        o.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 1));
-        o.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 2));
-        o.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 3));
-    }
-    return __builtin_bit_cast(s16x8, o);
-}
-__device__ __forceinline__ float power(uint32_t byte) { return __uint_as_float(byte << 23); }  // (255: NaN comes out)
-
 // A unit's share of a lane: of keys n16 and 16 + n16, dims D/4 g .. + D/4 - 1.
 template <uint32_t D>
 struct Mx4Unit {
@@ -217,18 +198,18 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
 #pragma unroll
             for (uint32_t h = 0; h < 2u; h++) {
                 const uint32_t r = 16u * h + n16;
-                const float sv = power(x.vs[h]);
+                const float sv = power4(x.vs[h]);
 #pragma unroll
                 for (uint32_t e = 0; e < (uint32_t)ND; e++)
-                    *(s16x8*)(vt + r * ROW + (((ND * g + e) ^ fswz<D>(r)) << 4)) = values8<T>(x.v[h][e], sv);
+                    *(u32x4*)(vt + r * ROW + (((ND * g + e) ^ fswz<D>(r)) << 4)) = values8<T>(x.v[h][e], sv);
             }
             f32x4 sc[NR][2];
 #pragma unroll
             for (int kb = 0; kb < 2; kb++) {
-                const float sk = power(x.ks[kb]);
+                const float sk = power4(x.ks[kb]);
 #pragma unroll
                 for (int ch = 0; ch < ND; ch++) {
-                    const s16x8 k = values8<T>(x.k[kb][ch], sk);
+                    const s16x8 k = __builtin_bit_cast(s16x8, values8<T>(x.k[kb][ch], sk));
 #pragma unroll
                     for (int r = 0; r < (int)NR; r++)
                         sc[r][kb] = mfma16<T>(k, qf[r][ch], ch == 0 ? f32x4{} - m_ref[r] : sc[r][kb]);

@@ -148,7 +148,36 @@ struct RowOfLane {
 //   bool holes(): some staged page is none; uint32_t groups(t): bit i: the keys 16 i .. of
 //     tile t have a page;
 //   const uint8_t* row(base, j): key j < n_keys's row (null: on no page).
+// kBlocks4: keys and values are blocks of 4-bit numbers; instead of tile, voffset and row
+//   Blocks4<D> fetch(base, scales, t, page, lane): the lane's piece of the wave's keys of tile t,
+//   k_scales, v_scales, and uint32_t nan_blocks(j): bit i: block i of key j < n_keys's value is NaN.
 // out_at(): element offset of the lane's row in `out`.
+//
+// A lane's piece of a tile of blocks: key 8 wave + lane / 8, dims D / 8 * (lane % 8) ..
+template <uint32_t D>
+struct Blocks4 {
+    uint32_t n[D / 64];  // eight numbers each
+    uint32_t power;      // + 127
+};
+// Eight numbers (a dword) times a power of two, as 16-bit values: exact.
+template <uint32_t T>
+__device__ __forceinline__ u32x4 values8(uint32_t w, float s) {
+    u32x4 o;
+    if constexpr (T == kGgmlBF16) {
+        o.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0));
+        o.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1));
+        o.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2));
+        o.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3));
+    } else {
+        o.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 0));
+        o.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 1));
+        o.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 2));
+        o.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 3));
+    }
+    return o;
+}
+__device__ __forceinline__ float power4(uint32_t byte) { return __uint_as_float(byte << 23); }  // (255: NaN comes out)
+
 template <uint32_t T, uint32_t D, uint32_t NW, typename Source, typename OutAt>
 __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, Source& src, uint32_t n_keys,
                                           const RowOfLane& row, float* part, const OutAt& out_at) {
@@ -159,6 +188,8 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, So
     constexpr uint32_t DI = kKeys / RPI / NW;       // DMA instructions per tile and wave
     constexpr uint32_t CPR = ROW / 16u;             // 16-byte chunks of a key row
     constexpr float OFF = T == kGgmlF16 ? 7.0f : 0.0f;
+    constexpr bool B4 = Source::kBlocks4;
+    static_assert(!B4 || NW == 8, "a wave has eight keys of a tile of blocks");
     const uint32_t tid = threadIdx.x, lane = tid & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t l32 = lane & 31u, kh = lane >> 5;
@@ -182,11 +213,13 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, So
     // instruction i of wave w fills the keys RPI (DI w + i) + lane / CPR of a slot,
     // the lane's chunk landing at lane % CPR of its key's row
     uint32_t kvo[DI], vvo[DI];
+    if constexpr (!B4) {
 #pragma unroll
-    for (int i = 0; i < (int)DI; i++) {
-        const uint32_t r = RPI * (DI * wave + i) + lane / CPR, p = lane % CPR;
-        kvo[i] = src.voffset(r, p ^ kswz<D>(r));
-        vvo[i] = src.voffset(r, p ^ vswz<D>(r));
+        for (int i = 0; i < (int)DI; i++) {
+            const uint32_t r = RPI * (DI * wave + i) + lane / CPR, p = lane % CPR;
+            kvo[i] = src.voffset(r, p ^ kswz<D>(r));
+            vvo[i] = src.voffset(r, p ^ vswz<D>(r));
+        }
     }
     auto dma = [&](const void* base, const uint32_t (&vo)[DI], uint32_t t, uint32_t page, uint32_t slot) {
         const rsrc_t r = src.tile(base, t, page);
@@ -194,6 +227,23 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, So
 #pragma unroll
         for (int i = 0; i < (int)DI; i++)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(dst + 1024u * i), 16, vo[i], 0, 0, 0);
+    };
+    // kBlocks4: the pieces of K(t + 3) and V(t + 2) on their way while tile t is worked on, and a piece
+    // into the 16-bit tile of a slot
+    Blocks4<D> bk, bv;
+    auto fetch_k = [&](uint32_t t, uint32_t page) {
+        if constexpr (B4) bk = src.fetch(a.k, src.k_scales, t, page, lane);
+    };
+    auto fetch_v = [&](uint32_t t, uint32_t page) {
+        if constexpr (B4) bv = src.fetch(a.v, src.v_scales, t, page, lane);
+    };
+    auto put = [&](const Blocks4<D>& x, uint32_t slot, bool is_v) {
+        const uint32_t r = 8u * wave + (lane >> 3), sub = lane & 7u;
+        const float s = power4(x.power);
+#pragma unroll
+        for (uint32_t i = 0; i < D / 64u; i++)
+            *(u32x4*)(lds + slot * TILE + r * ROW + (((D / 64u * sub + i) ^ (is_v ? vswz<D>(r) : kswz<D>(r))) << 4)) =
+                values8<T>(x.n[i], s);
     };
 
     // K fragment: keys 32 kb + l32, chunk 4 ch + 2 kh + st. V^T fragment (transposing
@@ -354,6 +404,18 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, So
     };
     auto add_bad = [&](uint32_t t) {
         const uint32_t j = t * kKeys + lane;
+        if constexpr (B4) {
+            const uint32_t blocks = j < n_keys ? src.nan_blocks(j) : 0u;
+            for (uint64_t bad = __builtin_amdgcn_ballot_w64(blocks != 0); bad != 0; bad &= bad - 1u) {
+                const int l = __builtin_ctzll(bad), key = (int)(t * kKeys) + l;
+                const uint32_t of = (uint32_t)__builtin_amdgcn_readlane((int)blocks, l);
+                const bool in = key >= row.lo && key <= row.hi;
+#pragma unroll
+                for (int dt = 0; dt < CH; dt++)
+                    if (in && ((of >> dt) & 1u)) o[dt] += __uint_as_float(0x7fc00000u);
+            }
+            return;
+        } else {
         bool n = false;
         if (j < n_keys) {
             const uint8_t* const vr = src.row(a.v, j);
@@ -376,6 +438,7 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, So
                     for (int e = 0; e < 4; e++)
                         o[dt][4 * g + e] += (int)in & (int)!(fabsf(x[e]) < INFINITY) ? x[e] : 0.0f;
                 }
+        }
         }
     };
 
@@ -424,14 +487,24 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, So
     };
     // What every wave does in tile t, whatever it sees of it: K(t+4) to K slot t % 4, V(t+3) to
     // V slot (t+3) % 4 (both last read in tile t - 1), V(t+1) looked through where it is masked.
+    // Blocks: K(t+3) and V(t+2), fetched in tile t - 1, to their slots (last read in tiles t - 2: their
+    // first fragments in t - 2, and t - 2), and the next ones fetched.
     auto send = [&](uint32_t t) {
-        dma(a.k, kvo, t + 4u, p4, t & 3u);
-        dma(a.v, vvo, t + 3u, p3, 4u + ((t + 3u) & 3u));
+        if constexpr (B4) {
+            put(bk, (t + 3u) & 3u, false);
+            put(bv, 4u + ((t + 2u) & 3u), true);
+            fetch_k(t + 4u, p4);
+            fetch_v(t + 3u, p3);
+        } else {
+            dma(a.k, kvo, t + 4u, p4, t & 3u);
+            dma(a.v, vvo, t + 3u, p3, 4u + ((t + 3u) & 3u));
+        }
         p5 = src.page(t + 5u);
         if (t + 1u < seg && wg_masked(t + 1u)) clean_v(t + 1u);
     };
     auto sent = [&]() {
-        LLMR_STAGE_BARRIER(2 * DI);
+        if constexpr (B4) LLMR_STAGE_BARRIER(63);
+        else LLMR_STAGE_BARRIER(2 * DI);
         p3 = p4;
         p4 = (uint32_t)__builtin_amdgcn_readfirstlane(p5);
     };
@@ -509,23 +582,41 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, So
             uint32_t pg[4];
 #pragma unroll
             for (uint32_t i = 0; i < 4u; i++) pg[i] = (uint32_t)__builtin_amdgcn_readfirstlane(src.page(t + i));
+            if constexpr (B4) {
+                Blocks4<D> k[3], v[2];
 #pragma unroll
-            for (uint32_t i = 0; i < 4u; i++) {  // K(t) V(t) K(t+1) V(t+1) K(t+2) V(t+2) K(t+3) in flight
-                dma(a.k, kvo, t + i, pg[i], i);
-                if (i < 3u) dma(a.v, vvo, t + i, pg[i], 4u + i);
+                for (uint32_t i = 0; i < 3u; i++) {
+                    k[i] = src.fetch(a.k, src.k_scales, t + i, pg[i], lane);
+                    if (i < 2u) v[i] = src.fetch(a.v, src.v_scales, t + i, pg[i], lane);
+                }
+                fetch_k(t + 3u, pg[3]);
+                fetch_v(t + 2u, pg[2]);
+#pragma unroll
+                for (uint32_t i = 0; i < 3u; i++) {
+                    put(k[i], i, false);
+                    if (i < 2u) put(v[i], 4u + i, true);
+                }
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < 4u; i++) {  // K(t) V(t) K(t+1) V(t+1) K(t+2) V(t+2) K(t+3) in flight
+                    dma(a.k, kvo, t + i, pg[i], i);
+                    if (i < 3u) dma(a.v, vvo, t + i, pg[i], 4u + i);
+                }
             }
             p3 = pg[3];
             p4 = (uint32_t)__builtin_amdgcn_readfirstlane(src.page(t + 4u));
         }
         // the wave's tiles of this segment: [see0, end)
         const uint32_t end = min(see1, seg);
-        LLMR_STAGE_BARRIER(6 * DI);  // K(t) has landed
+        if constexpr (B4) LLMR_STAGE_BARRIER(63);  // K(t) .. K(t+2), V(t), V(t+1) are there
+        else LLMR_STAGE_BARRIER(6 * DI);           // K(t) has landed
         if (first && lane == 0) {
             atomicMax(&wave_lohi[0], lo_max);
             atomicMin(&wave_lohi[1], hi_min);
         }
         if (see0 <= t && t < end) scores(h0, h1, t);
-        LLMR_STAGE_BARRIER(2 * DI);  // K(t+1), V(t), K(t+2), V(t+1) have landed
+        if constexpr (B4) LLMR_STAGE_BARRIER(63);
+        else LLMR_STAGE_BARRIER(2 * DI);  // K(t+1), V(t), K(t+2), V(t+1) have landed
         if (first) {
             wg_full0 = (uint32_t)(__builtin_amdgcn_readfirstlane(wave_lohi[0]) + (int)kKeys - 1) / kKeys;
             wg_full1 = (uint32_t)(__builtin_amdgcn_readfirstlane(wave_lohi[1]) + 1) / kKeys;
