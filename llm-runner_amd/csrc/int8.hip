@@ -1,5 +1,4 @@
-// int8.hip - linears in 8-bit integers: rows to integers with a scale each
-// (llmr_quantize_rows_i8) and the product with integer weights (llmr_matmul_i8).
+// int8.hip - rows to 8-bit integers with a scale each (llmr_quantize_rows_i8).
 #include "llmr_device.h"
 #include "llmr_internal.h"
 
@@ -8,8 +7,6 @@
 
 namespace llmr {
 namespace {
-
-typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // Eight elements from x on, as f32.
 template <uint32_t XT>
@@ -117,47 +114,6 @@ __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(QuantizeRows
     }
 }
 
-// (The empty asm keeps the product y apart: hipcc makes one v_fma_mixlo_f16 of a product and its
-// conversion to f16, contraction or not, which rounds once where the definition rounds twice.)
-template <uint32_t OT>
-__device__ __forceinline__ void store1(void* out, uint64_t at, float y) {
-    if constexpr (OT == kGgmlF16) asm("" : "+v"(y));
-    if constexpr (OT == kGgmlF32) ((float*)out)[at] = y;
-    else if constexpr (OT == kGgmlF16) ((_Float16*)out)[at] = (_Float16)y;
-    else ((__bf16*)out)[at] = (__bf16)y;
-}
-
-// 16 channels x 16 tokens a wave, 16x16x64 MFMAs (a lane: 16 bytes of row lane % 16, from 16 (lane /
-// 16) on; results: channels 4 (lane / 16) .. + 3 of token lane % 16).
-template <uint32_t OT>
-__global__ void __launch_bounds__(64) matmul_i8_kernel(MatmulI8Args a) {
-    const uint32_t lane = threadIdx.x, l16 = lane & 15u, g = lane >> 4;
-    const uint32_t tiles_n = (a.N + 15u) / 16u;
-    const uint64_t tiles = (uint64_t)tiles_n * ((a.M + 15u) / 16u);
-    for (uint64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        const uint32_t n0 = (uint32_t)(tile % tiles_n) * 16u, m0 = (uint32_t)(tile / tiles_n) * 16u;
-        const uint32_t m = m0 + l16, n = n0 + l16;
-        const int8_t* const xr = a.x + (uint64_t)min(m, a.M - 1u) * a.x_stride;
-        const int8_t* const wr = a.w + (uint64_t)min(n, a.N - 1u) * a.w_stride;
-        i32x4 acc{0, 0, 0, 0};
-        for (uint32_t k0 = 0; k0 < a.K; k0 += 64u) {
-            const uint32_t k = k0 + 16u * g;
-            const i32x4 zero{0, 0, 0, 0};
-            const i32x4 x = k < a.K ? *(const i32x4*)(xr + k) : zero;
-            const i32x4 w = k < a.K ? *(const i32x4*)(wr + k) : zero;
-            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, x, acc, 0, 0, 0);
-        }
-        if (m < a.M) {
-            const float xs = a.x_scales[m];
-#pragma unroll
-            for (uint32_t i = 0; i < 4u; i++) {
-                const uint32_t c = n0 + 4u * g + i;
-                if (c < a.N) store1<OT>(a.out, (uint64_t)m * a.out_stride + c, (float)acc[i] * xs * a.w_scales[c]);
-            }
-        }
-    }
-}
-
 }  // namespace
 
 hipError_t launch_quantize_rows_i8(const QuantizeRowsArgs& a, uint32_t xtype, int num_cus, hipStream_t st) {
@@ -166,16 +122,6 @@ hipError_t launch_quantize_rows_i8(const QuantizeRowsArgs& a, uint32_t xtype, in
     if (xtype == kGgmlF32) a.norm ? go(quantize_rows_kernel<kGgmlF32, true>) : go(quantize_rows_kernel<kGgmlF32, false>);
     else if (xtype == kGgmlF16) a.norm ? go(quantize_rows_kernel<kGgmlF16, true>) : go(quantize_rows_kernel<kGgmlF16, false>);
     else a.norm ? go(quantize_rows_kernel<kGgmlBF16, true>) : go(quantize_rows_kernel<kGgmlBF16, false>);
-    return hipGetLastError();
-}
-
-hipError_t launch_matmul_i8(const MatmulI8Args& a, uint32_t otype, int num_cus, hipStream_t st) {
-    const uint64_t tiles = (uint64_t)((a.N + 15u) / 16u) * ((a.M + 15u) / 16u);
-    const uint32_t grid = (uint32_t)(tiles < (1u << 24) ? tiles : (1u << 24));
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(64), 0, st, a); };
-    if (otype == kGgmlF32) go(matmul_i8_kernel<kGgmlF32>);
-    else if (otype == kGgmlF16) go(matmul_i8_kernel<kGgmlF16>);
-    else go(matmul_i8_kernel<kGgmlBF16>);
     return hipGetLastError();
 }
 
