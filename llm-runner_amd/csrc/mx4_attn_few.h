@@ -27,6 +27,9 @@ namespace {
 using namespace seqattn;
 
 constexpr uint32_t kWaves = 4;  // of a worker
+// A pair's units on the line: those of its keys, the first of them kPairStart units more, for what a
+// pair costs a worker (its pages, queries and first rows waited for, its rows added up).
+constexpr uint32_t kPairStart = 12;
 
 struct Mx4Args {
     SeqAttnArgs a;
@@ -57,7 +60,7 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t G = a.n_heads / a.n_kv_heads;
     const float c = a.scale_log2, grow_by = 8.0f / c;
-    const auto cost = [](const PagedRequest& r) { return (uint64_t)units_of(r); };
+    const auto cost = [](const PagedRequest& r) { return r.rows ? (uint64_t)units_of(r) + kPairStart : 0ull; };
 
     RequestWindow win;
     const uint64_t w = batch_cost(a, win, lane, cost) * a.n_kv_heads;
@@ -92,10 +95,15 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
     uint64_t base;
     uint32_t s = find_request(a, win, lane, cost, a.n_kv_heads, at, base);
     PagedRequest rq = win.get(s);
-    uint32_t units = units_of(rq), kvh = (uint32_t)((at - base) / units), u0 = (uint32_t)((at - base) % units);
+    uint32_t units = units_of(rq), kvh = (uint32_t)((at - base) / (units + kPairStart));
+    uint32_t x0 = (uint32_t)((at - base) % (units + kPairStart));
 
     while (true) {
-        const uint32_t u1 = (uint32_t)min((uint64_t)units, u0 + (end - at));  // units [u0, u1) of the pair are this part
+        // [x0, x1) of the pair on the line: its units [u0, u1)
+        const uint32_t x1 = (uint32_t)min((uint64_t)units + kPairStart, x0 + (end - at));
+        const uint32_t u0 = x0 > kPairStart ? x0 - kPairStart : 0u, u1 = x1 > kPairStart ? x1 - kPairStart : 0u;
+        at += x1 - x0;
+        if (u0 != u1) {
         const uint32_t rows = rq.rows * G;
         const uint32_t count = u1 - u0 > wave ? (u1 - u0 - wave + kWaves - 1u) / kWaves : 0u;  // of them this wave's
         const int32_t hi_min = rq.pos0;  // (the first token's rows see least)
@@ -287,7 +295,6 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
         const bool begun = u0 == 0, last = u1 == units;
         float* const part = parts + (size_t)(2u * blockIdx.x + (begun ? 1u : 0u)) * part_floats<D, NR>();
         float* const ml = (float*)(lds + kWaves * TILE);  // [kWaves][2][16]: m, l
-        at += u1 - u0;
         if (begun && !last)  // (the worker's last part: the record is its one)
             rec = JoinRecord{part_of(at + (units - u1) - 1u, w, n), rq.first, 0, rows, kvh, {}};
 #pragma unroll
@@ -333,9 +340,10 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
             }
             __syncthreads();
         }
+        }
         if (at >= end) break;
         // the next pair (units are left, so there is a request that has some)
-        u0 = 0;
+        x0 = 0;
         if (++kvh == a.n_kv_heads) {
             kvh = 0;
             do {
