@@ -1297,8 +1297,13 @@ int llmr_qkv_tokens_mx4(llmr_context* ctx, const float* qkv, const float* q_norm
     if (int r = check_qkv_tokens(qkv, q_norm, k_norm, rope_cos, rope_sin, positions, slots, q, p)) return r;
     if (p->n_tokens == 0) return ok();
     if (!slots) return fail(LLMR_ERR_INVALID_ARG, "null slots pointer");
-    if (int r = check_mx4(k, "k")) return r;
-    if (int r = check_mx4(v, "v")) return r;
+    const llmr_mx4_cache none{nullptr, nullptr};
+    if (p->n_pages == 0) {
+        k = v = &none;  // every slot is outside the cache
+    } else {
+        if (int r = check_mx4(k, "k")) return r;
+        if (int r = check_mx4(v, "v")) return r;
+    }
     const uint64_t rows = (uint64_t)p->n_pages * p->page_size * p->n_kv_heads, D = p->head_dim;
     const struct {
         const void* p;

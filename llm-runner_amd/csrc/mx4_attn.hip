@@ -34,7 +34,7 @@ struct Mx4Keys : seqattn::PagedKeys<D / 2u> {
             const uint8_t* const s = v_scales + ((((uint64_t)p * this->n_kv_heads + this->kvh) << this->log2) +
                                                  (at & ((1u << this->log2) - 1u))) * (D / 32u);
 #pragma unroll
-            for (uint32_t i = 0; i < D / 32u; i++) bits |= s[i] == 255u ? 1u << i : 0u;
+            for (uint32_t i = 0; i < D / 32u; i++) bits |= s[i] > mx4attn::kTopPower ? 1u << i : 0u;
         }
         return bits;
     }
@@ -97,7 +97,11 @@ static hipError_t launch_mx4(const mx4attn::Mx4Args& m4, uint32_t nr, int num_cu
 hipError_t launch_paged_attention_mx4(const SeqAttnArgs& a, const uint8_t* k_scales, const uint8_t* v_scales,
                                       uint32_t type, uint32_t dim, int num_cus, void* scratch, hipStream_t st) {
     const uint32_t nr = mx4_blocks(a.n_heads, a.n_kv_heads, a.max_new);
-    const mx4attn::Mx4Args m4{a, k_scales, v_scales};
+    mx4attn::Mx4Args m4{a, k_scales, v_scales};
+    if (a.n_pages == 0) {  // mx4_attn_few reads a cache's first rows for a page that there is not, and drops them
+        m4.a.k = m4.a.v = scratch;
+        m4.k_scales = m4.v_scales = (const uint8_t*)scratch;
+    }
     if (type == kGgmlBF16)
         return dim == 128u ? launch_mx4<kGgmlBF16, 128>(m4, nr, num_cus, scratch, st)
                            : launch_mx4<kGgmlBF16, 64>(m4, nr, num_cus, scratch, st);

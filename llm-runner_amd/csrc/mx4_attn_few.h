@@ -26,7 +26,10 @@ namespace {
 
 using namespace seqattn;
 
-constexpr uint32_t kWaves = 4;  // of a worker
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+
+constexpr uint32_t kWaves = 4;         // of a worker
+constexpr uint32_t kTopPower = 127 + 13;  // of what llmr_qkv_tokens_mx4 writes; above it values may be infinite
 // A pair's units on the line: those of its keys, the first of them kPairStart units more, for what a
 // pair costs a worker (its pages, queries and first rows waited for, its rows added up).
 constexpr uint32_t kPairStart = 12;
@@ -42,7 +45,7 @@ template <uint32_t D>
 struct Mx4Unit {
     uint32_t k[2][D / 32], v[2][D / 32];
     uint32_t ks[2], vs[2];
-    bool on0, on1;  // (uniform) the halves have a page
+    bool on[2];  // (uniform) the halves have a page
 };
 
 template <uint32_t D, uint32_t NR>
@@ -74,23 +77,14 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
     uint64_t at = part_begin(blockIdx.x, w, n);
     const uint64_t end = part_begin(blockIdx.x + 1u, w, n);
 
-    // rows x = 16 r + n16: token x / G, head of the group x % G
-    uint32_t tok[NR], qoff[NR];
-#pragma unroll
-    for (int r = 0; r < (int)NR; r++) {
-        const uint32_t x = 16u * r + n16;
-        tok[r] = x / G;
-        qoff[r] = tok[r] * a.q_stride + (x % G) * a.q_head_stride + D / 4u * g;
-    }
     const uint32_t kvo = n16 * ROW4 + g * CB, so = n16 * SROW + (D == 128u ? g : g >> 1);
     uint8_t* const vt = lds + wave * TILE;
     const uint32_t vt0 = (uint32_t)(uintptr_t)(lds_void*)vt;
-    uint32_t vto[DT];
-#pragma unroll
-    for (int dt = 0; dt < DT; dt++) {
-        const uint32_t r = 4u * g + (n16 >> 2);
-        vto[dt] = vt0 + r * ROW + (((2u * dt + ((n16 & 3u) >> 1)) ^ fswz<D>(r)) << 4) + 8u * (n16 & 1u);
-    }
+    // V's tile: chunk q of key r at q ^ fswz(r), fswz even: chunk 2 dt + x of a row is at A ^ 32 dt, and chunk ND g + e
+    // at B ^ 16 e
+    const uint32_t vr0 = 4u * g + (n16 >> 2);
+    uint32_t va = vr0 * ROW + ((((n16 & 3u) >> 1) ^ fswz<D>(vr0)) << 4) + 8u * (n16 & 1u);
+    uint32_t vb = n16 * ROW + (((ND * g) ^ fswz<D>(n16)) << 4);
 
     uint64_t base;
     uint32_t s = find_request(a, win, lane, cost, a.n_kv_heads, at, base);
@@ -109,107 +103,106 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
         const int32_t hi_min = rq.pos0;  // (the first token's rows see least)
         s16x8 qf[NR][ND];
         int32_t hi[NR];  // last key the row sees
-        f32x4 o[NR][DT];
-        float m_ref[NR], l_i[NR];
+        f32x4 o[NR][DT], nm[NR];  // O^T; minus the row's reference maximum, four times: the scores start from it
+        float l_i[NR];
         uint32_t fresh = (1u << NR) - 1u, sees = 0;  // per row block: no maximum yet; a key seen
         const uint8_t* const q0 = (const uint8_t*)a.q + 2u * ((uint64_t)rq.first * a.q_stride + (uint64_t)kvh * G * a.q_head_stride);
 #pragma unroll
         for (int r = 0; r < (int)NR; r++) {
-            const bool live = 16u * r + n16 < rows;
-            hi[r] = live ? rq.pos0 + (int32_t)tok[r] : -1;
-            const uint8_t* const qr = q0 + 2u * (live ? qoff[r] : D / 4u * g);
+            // row x: token x / G, head of the group x % G
+            const uint32_t x = 16u * r + n16 < rows ? 16u * r + n16 : 0u;
+            hi[r] = 16u * r + n16 < rows ? rq.pos0 + (int32_t)(x / G) : -1;
+            const uint8_t* const qr = q0 + 2u * (x / G * a.q_stride + x % G * a.q_head_stride + D / 4u * g);
 #pragma unroll
             for (int ch = 0; ch < ND; ch++) qf[r][ch] = *(const s16x8*)(qr + 16 * ch);
-            m_ref[r] = l_i[r] = 0.0f;
+            nm[r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            l_i[r] = 0.0f;
 #pragma unroll
             for (int dt = 0; dt < DT; dt++) o[r][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
 
-        // pages of this wave's units i0 .. i0 + 31, a half a lane (negative: none)
-        int32_t pages = -1;
+        // the cache's rows where the halves of this wave's units i0 .. i0 + 31 begin, a half a lane (-1: no
+        // page): the vector ALU makes them for 32 units at once, and a unit takes its two into scalars
+        int64_t rows0 = -1;
         auto window = [&](uint32_t i0) {
             const uint32_t k0 = (u0 + wave + kWaves * (i0 + (lane >> 1))) * kUnit + 16u * (lane & 1u);
-            pages = -1;
+            rows0 = -1;
             if (i0 + (lane >> 1) < count && k0 < rq.keys) {
-                const int32_t p = a.table[(size_t)s * a.max_pages + (k0 >> a.page_log2)];
-                pages = p >= 0 && (uint32_t)p < a.n_pages ? p : -1;
+                const uint32_t p = (uint32_t)a.table[(size_t)s * a.max_pages + (k0 >> a.page_log2)];
+                if (p < a.n_pages)
+                    rows0 = (int64_t)((((uint64_t)p * a.n_kv_heads + kvh) << a.page_log2) + (k0 & ((1u << a.page_log2) - 1u)));
             }
         };
+        // A half's 16 rows are one page's, so all of them are the cache's to read, those of keys past the last
+        // one too; for a half of no page, the cache's first rows are read. step() sets such values to 0.
         auto load = [&](Mx4Unit<D>& x, uint32_t i) {
             if ((i & 31u) == 0) window(i);
-            const uint32_t k0 = (u0 + wave + kWaves * i) * kUnit;
 #pragma unroll
             for (uint32_t h = 0; h < 2u; h++) {
-                const uint32_t k = k0 + 16u * h;
-                const int32_t p = __builtin_amdgcn_readlane(pages, (int)(2u * (i & 31u) + h));
-                const uint64_t row = (((uint64_t)(uint32_t)max(p, 0) * a.n_kv_heads + kvh) << a.page_log2) +
-                                     (k & ((1u << a.page_log2) - 1u));
-                // keys past the last one, and those of no page, read as zero
-                const uint32_t keys = p < 0 ? 0u : min(__builtin_elementwise_sub_sat(rq.keys, k), 16u);
-                const auto rsrc = [&](const void* b, uint32_t size) {
-                    return __builtin_amdgcn_make_buffer_rsrc((uint8_t*)const_cast<void*>(b) + row * size, (short)0,
-                                                             (int)__builtin_amdgcn_readfirstlane(keys * size), 0x00020000);
-                };
-                const rsrc_t kr = rsrc(a.k, ROW4), vr = rsrc(a.v, ROW4), ksr = rsrc(m4.k_scales, SROW),
-                             vsr = rsrc(m4.v_scales, SROW);
+                const int l = (int)(2u * (i & 31u) + h);
+                const int32_t hi32 = __builtin_amdgcn_readlane((int32_t)(rows0 >> 32), l);
+                const uint32_t lo32 = (uint32_t)__builtin_amdgcn_readlane((int32_t)rows0, l);
+                x.on[h] = hi32 >= 0;
+                const uint64_t row = hi32 >= 0 ? (uint64_t)(uint32_t)hi32 << 32 | lo32 : 0ull;
+                const uint8_t* const kp = (const uint8_t*)a.k + row * ROW4;
+                const uint8_t* const vp = (const uint8_t*)a.v + row * ROW4;
                 if constexpr (D == 128u) {
-                    const u32x4 kk = __builtin_amdgcn_raw_buffer_load_b128(kr, kvo, 0, 0);
-                    const u32x4 vv = __builtin_amdgcn_raw_buffer_load_b128(vr, kvo, 0, 0);
+                    const u32x4 kk = *(const u32x4*)(kp + kvo), vv = *(const u32x4*)(vp + kvo);
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         x.k[h][e] = kk[e];
                         x.v[h][e] = vv[e];
                     }
                 } else {
-                    const u32x2 kk = __builtin_amdgcn_raw_buffer_load_b64(kr, kvo, 0, 0);
-                    const u32x2 vv = __builtin_amdgcn_raw_buffer_load_b64(vr, kvo, 0, 0);
+                    const u32x2 kk = *(const u32x2*)(kp + kvo), vv = *(const u32x2*)(vp + kvo);
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         x.k[h][e] = kk[e];
                         x.v[h][e] = vv[e];
                     }
                 }
-                x.ks[h] = __builtin_amdgcn_raw_buffer_load_b8(ksr, so, 0, 0);
-                x.vs[h] = __builtin_amdgcn_raw_buffer_load_b8(vsr, so, 0, 0);
-                (h == 0 ? x.on0 : x.on1) = p >= 0;
+                x.ks[h] = *(m4.k_scales + row * SROW + so);
+                x.vs[h] = *(m4.v_scales + row * SROW + so);
             }
         };
         auto step = [&](Mx4Unit<D>& x, uint32_t i) {
             const uint32_t u = u0 + wave + kWaves * i;
             // keys past the last one, on no page, or unseen by a row: masked
-            const bool masked = !x.on0 || !x.on1 || (int32_t)(u * kUnit + kUnit - 1u) > hi_min;
+            const bool masked = !x.on[0] || !x.on[1] || (int32_t)(u * kUnit + kUnit - 1u) > hi_min;
             if (masked) {
-                // a row's weight of a key it does not see is 0, and 0 times NaN is NaN: such blocks of V are
-                // set to 0 here, and the rows that do see them become NaN at once
-                const uint64_t b0 = __builtin_amdgcn_ballot_w64(x.vs[0] == 255u), b1 = __builtin_amdgcn_ballot_w64(x.vs[1] == 255u);
-                if ((b0 | b1) != 0) {
+                // a row's weight of a key it does not see is 0, and 0 times an infinity or NaN is NaN: V's rows
+                // of keys that there are not are set to 0, and so are blocks that are not all finite, whose
+                // rows that do see them become NaN at once
+                const uint32_t last = rq.keys - u * kUnit;  // (of keys; this unit has some, or the part has none at all)
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        for (uint64_t b = h == 0 ? b0 : b1; b != 0; b &= b - 1u) {
-                            const uint32_t l = (uint32_t)__builtin_ctzll(b);
-                            const int32_t key = (int32_t)(u * kUnit + 16u * h + (l & 15u));
-                            const uint32_t block = D == 128u ? l >> 4 : l >> 5;
+                for (uint32_t h = 0; h < 2u; h++) {
+                    const bool is = x.on[h] && 16u * h + n16 < last;
+                    const bool bad = is && x.vs[h] > kTopPower;
+                    for (uint64_t b = __builtin_amdgcn_ballot_w64(bad); b != 0; b &= b - 1u) {
+                        const uint32_t l = (uint32_t)__builtin_ctzll(b);
+                        const int32_t key = (int32_t)(u * kUnit + 16u * h + (l & 15u));
+                        const uint32_t block = D == 128u ? l >> 4 : l >> 5;
 #pragma unroll
-                            for (int r = 0; r < (int)NR; r++)
+                        for (int r = 0; r < (int)NR; r++)
 #pragma unroll
-                                for (int dt = 0; dt < DT; dt++)
-                                    if (key <= hi[r] && (uint32_t)dt >> 1 == block) o[r][dt] += __uint_as_float(0x7fc00000u);
-                        }
-                        if (x.vs[h] == 255u) {
-                            x.vs[h] = 0;
+                            for (int dt = 0; dt < DT; dt++)
+                                if (key <= hi[r] && (uint32_t)dt >> 1 == block) o[r][dt] += __uint_as_float(0x7fc00000u);
+                    }
+                    if (bad || !is) {
+                        x.vs[h] = 0;
 #pragma unroll
-                            for (int e = 0; e < ND; e++) x.v[h][e] = 0;
-                        }
+                        for (int e = 0; e < ND; e++) x.v[h][e] = 0;
                     }
                 }
             }
+            // (the addresses are made anew in each unit: hipcc would keep all of them in registers)
+            asm volatile("" : "+v"(va), "+v"(vb));
 #pragma unroll
-            for (uint32_t h = 0; h < 2u; h++) {
-                const uint32_t r = 16u * h + n16;
-                const float sv = power4(x.vs[h]);
+            for (uint32_t e = 0; e < (uint32_t)ND; e++) {
+                const uint32_t at = vt0 + (vb ^ (e << 4));
 #pragma unroll
-                for (uint32_t e = 0; e < (uint32_t)ND; e++)
-                    *(u32x4*)(vt + r * ROW + (((ND * g + e) ^ fswz<D>(r)) << 4)) = values8<T>(x.v[h][e], sv);
+                for (uint32_t h = 0; h < 2u; h++)
+                    *(lds_u32x4*)(uintptr_t)(at + h * 16u * ROW) = values8<T>(x.v[h][e], power4(x.vs[h]));
             }
             f32x4 sc[NR][2];
 #pragma unroll
@@ -220,7 +213,7 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
                     const s16x8 k = __builtin_bit_cast(s16x8, values8<T>(x.k[kb][ch], sk));
 #pragma unroll
                     for (int r = 0; r < (int)NR; r++)
-                        sc[r][kb] = mfma16<T>(k, qf[r][ch], ch == 0 ? f32x4{} - m_ref[r] : sc[r][kb]);
+                        sc[r][kb] = mfma16<T>(k, qf[r][ch], ch == 0 ? nm[r] : sc[r][kb]);
                 }
             }
             s16x8 pf[NR];
@@ -231,7 +224,7 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
                     bool any = false;
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const bool a0 = x.on0 && k0 + e <= hi[r], a1 = x.on1 && k0 + 16 + e <= hi[r];
+                        const bool a0 = x.on[0] && k0 + e <= hi[r], a1 = x.on[1] && k0 + 16 + e <= hi[r];
                         sc[r][0][e] = a0 ? sc[r][0][e] : -INFINITY;
                         sc[r][1][e] = a1 ? sc[r][1][e] : -INFINITY;
                         any = any || a0 || a1;
@@ -243,14 +236,16 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
                 float mx = -INFINITY;
 #pragma unroll
                 for (int e = 0; e < 4; e++) mx = fmaxf(fmaxf(mx, sc[r][0][e]), sc[r][1][e]);
-                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                // (the lanes' own maxima say whether some row's reference has to rise; its four lanes are asked
+                // only then)
                 const bool fr = (fresh >> r) & 1u;
                 if (__builtin_amdgcn_ballot_w64(mx > grow_by || (fr && mx > -INFINITY)) != 0) {
+                    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+                    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
                     // (only rows whose own maximum calls for it)
                     const float d = fr ? (mx > -INFINITY ? mx : 0.0f) : (mx > grow_by ? mx : 0.0f);
                     const float alpha = fr ? 0.0f : __builtin_amdgcn_exp2f(-d * c);
-                    m_ref[r] += d;
+                    nm[r] -= d;
                     l_i[r] *= alpha;
 #pragma unroll
                     for (int dt = 0; dt < DT; dt++) o[r][dt] *= alpha;
@@ -270,8 +265,9 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
             asm volatile("" ::: "memory");  // (a wave's LDS accesses run in order: the reads follow its own writes)
 #pragma unroll
             for (int dt = 0; dt < DT; dt++) {
-                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(vto[dt]));
-                const s16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(vto[dt] + 16u * ROW));
+                const uint32_t at = vt0 + (va ^ (32u * dt));
+                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)at);
+                const s16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(at + 16u * ROW));
                 const s16x8 v = s16x8{lo.x, lo.y, lo.z, lo.w, up.x, up.y, up.z, up.w};
 #pragma unroll
                 for (int r = 0; r < (int)NR; r++) o[r][dt] = mfma16<T>(v, pf[r], o[r][dt]);
@@ -311,7 +307,7 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
 #pragma unroll
             for (int dt = 0; dt < DT; dt++) ow[n16 * (D / 4u) + ((4u * dt + g) ^ n16)] = o[r][dt];
             if (g == 0) {
-                ml[wave * 32u + n16] = (fresh >> r) & 1u ? -INFINITY : m_ref[r];
+                ml[wave * 32u + n16] = (fresh >> r) & 1u ? -INFINITY : -nm[r].x;
                 ml[wave * 32u + 16u + n16] = sn ? l : -1.0f;
             }
             __syncthreads();

@@ -421,6 +421,45 @@ def test_unseen_values_do_not_matter(dev, dtype, new, row):
         assert torch.equal(o[:new].double().isnan(), ref.isnan()), where
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new", [1, 5, 20, 90])
+def test_what_unused_slots_hold_does_not_matter(dev, dtype, D, new):
+    """Slots behind a request's last key, and pages that nobody holds, with any bytes: no bit of the result changes."""
+    from llmr_amd import serve
+    q, kc, vc, rows, at, off, kvl, table, kv = _paged_case(dev, dtype, D, 8, 2, 64, [70, 3, 500], [new, 1, 1], seed=9, poison=False)
+    ref = serve.paged_attention_mx4(q, kc, vc, off, kvl, table, new)
+    used = torch.zeros(kc.data.shape[0], 64, dtype=torch.bool, device=dev)
+    for i, n in enumerate(kv):
+        j = torch.arange(n, device=dev)
+        used[table[i].long()[j // 64], j % 64] = True
+    free = ~used[:, None, :, None]
+    for power, code in ((255, 0xff), (254, 0x77), (200, 0xf7), (0, 0x11)):
+        c = [serve.Mx4Cache(torch.where(free, code, x.data).to(torch.uint8), torch.where(free, power, x.scales).to(torch.uint8))
+             for x in (kc, vc)]
+        out = serve.paged_attention_mx4(q, *c, off, kvl, table, new)
+        torch.cuda.synchronize()
+        assert torch.equal(out, ref), power
+
+
+def test_a_cache_of_no_pages(dev):
+    """Every key is on a page that there is not: rows are 0."""
+    from llmr_amd import serve
+    for D, new in ((128, 1), (64, 3), (128, 40)):
+        kc, vc = _caches(0, 2, 16, D, dev)
+        q = torch.randn(new, 8, D, device=dev).half()
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+        for table in (torch.zeros(1, 9, dtype=torch.int32, device=dev), torch.zeros(1, 0, dtype=torch.int32, device=dev)):
+            out = serve.paged_attention_mx4(q, kc, vc, i32([0, new]), i32([100]), table, new)
+            torch.cuda.synchronize()
+            assert bool((out == 0).all())
+    serve.qkv_tokens_mx4(torch.randn(3, 6 * 64, device=dev), torch.empty(3, 2, 64, dtype=F16, device=dev),
+                         *(serve.Mx4Cache(torch.empty(1, 2, 16, 32, dtype=torch.uint8, device=dev)[:0],
+                                          torch.empty(1, 2, 16, 2, dtype=torch.uint8, device=dev)[:0]) for _ in range(2)),
+                         torch.tensor([0, -1, 5], dtype=torch.int32, device=dev))
+    torch.cuda.synchronize()
+
+
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("new", [1, 8, 24, 100])
 def test_nan_values_that_rows_see(dev, D, new):
