@@ -52,15 +52,19 @@ mx4_attn_tiles(mx4attn::Mx4Args m4, seqattn::JoinRecord* __restrict__ records, f
 
 }  // namespace
 
-// Row blocks of 16 of the kernel for few rows that holds max_new tokens of a group; 0: more rows.
+// Row blocks of 16 of the kernel for few rows that holds max_new tokens of a group; 0: more rows, for
+// which the tiles are faster at any length. In 32-row blocks and in tiles, us: four contexts of 40000 to
+// 131000 keys of 32/8 heads of 128 with 8 new tokens (32 rows) 102, 212; 16 x 4 tokens at 28/4 heads of
+// 64 (28 rows) 32, 48. With a kernel of 64 rows, and in tiles: the four contexts with 9 to 16 tokens 500,
+// 215 (64: 154, 155), 32 contexts of 100 to 8000 keys 134 to 142, 85 to 91 (64: 52 to 58, 48), one of 500
+// 24 to 29, 22 to 24 (64: 14.5 to 15.8, 13.9 to 15.0).
 static uint32_t mx4_blocks(uint32_t n_heads, uint32_t n_kv_heads, uint32_t max_new) {
     const uint64_t rows = (uint64_t)max_new * (n_heads / n_kv_heads);
-    return rows <= 16u ? 1u : rows <= 32u ? 2u : rows <= 64u ? 4u : 0u;
+    return rows <= 16u ? 1u : rows <= 32u ? 2u : 0u;
 }
 // Workers: workgroups a CU, as many as the registers let reside, or one of mx4_attn_tiles.
 static uint32_t mx4_workers(uint32_t nr, int num_cus) {
-    using namespace mx4attn;
-    return (uint32_t)num_cus * (nr == 0u ? 1u : nr == 1u ? few_waves<1>() : nr == 2u ? few_waves<2>() : few_waves<4>());
+    return (uint32_t)num_cus * (nr == 0u ? 1u : nr == 1u ? mx4attn::few_waves<1>() : mx4attn::few_waves<2>());
 }
 
 size_t paged_attention_mx4_scratch_bytes(uint32_t dim, uint32_t n_heads, uint32_t n_kv_heads, uint32_t max_new,
@@ -90,8 +94,7 @@ static hipError_t launch_mx4(const mx4attn::Mx4Args& m4, uint32_t nr, int num_cu
     };
     if (nr == 0u) return go(mx4_attn_tiles<T, D>, 512, paged_attn_join<T, D, kBlockRows>, Rows<kBlockRows>{});
     if (nr == 1u) return go(mx4_attn_few<T, D, 1>, 64 * kWaves, paged_attn_join<T, D, 16>, Rows<16>{});
-    if (nr == 2u) return go(mx4_attn_few<T, D, 2>, 64 * kWaves, paged_attn_join<T, D, 32>, Rows<32>{});
-    return go(mx4_attn_few<T, D, 4>, 64 * kWaves, paged_attn_join<T, D, 64>, Rows<64>{});
+    return go(mx4_attn_few<T, D, 2>, 64 * kWaves, paged_attn_join<T, D, 32>, Rows<32>{});
 }
 
 hipError_t launch_paged_attention_mx4(const SeqAttnArgs& a, const uint8_t* k_scales, const uint8_t* v_scales,

@@ -40,12 +40,16 @@ struct Mx4Args {
     const uint8_t* v_scales;
 };
 
-// A unit's share of a lane: of keys n16 and 16 + n16, dims D/4 g .. + D/4 - 1.
+// A lane's share of a unit's keys or values: of keys n16 and 16 + n16, dims D/4 g .. + D/4 - 1.
+template <uint32_t D>
+struct Half4 {
+    uint32_t n[2][D / 32], power[2];
+};
 template <uint32_t D>
 struct Mx4Unit {
-    uint32_t k[2][D / 32], v[2][D / 32];
-    uint32_t ks[2], vs[2];
-    bool on[2];  // (uniform) the halves have a page
+    Half4<D> k, v;
+    uint64_t row[2];  // (uniform) the cache's rows where its halves begin
+    bool on[2];       // (uniform) the halves have a page
 };
 
 template <uint32_t D, uint32_t NR>
@@ -135,7 +139,7 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
         };
         // A half's 16 rows are one page's, so all of them are the cache's to read, those of keys past the last
         // one too; for a half of no page, the cache's first rows are read. step() sets such values to 0.
-        auto load = [&](Mx4Unit<D>& x, uint32_t i) {
+        auto place = [&](Mx4Unit<D>& x, uint32_t i) {
             if ((i & 31u) == 0) window(i);
 #pragma unroll
             for (uint32_t h = 0; h < 2u; h++) {
@@ -143,32 +147,31 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
                 const int32_t hi32 = __builtin_amdgcn_readlane((int32_t)(rows0 >> 32), l);
                 const uint32_t lo32 = (uint32_t)__builtin_amdgcn_readlane((int32_t)rows0, l);
                 x.on[h] = hi32 >= 0;
-                const uint64_t row = hi32 >= 0 ? (uint64_t)(uint32_t)hi32 << 32 | lo32 : 0ull;
-                const uint8_t* const kp = (const uint8_t*)a.k + row * ROW4;
-                const uint8_t* const vp = (const uint8_t*)a.v + row * ROW4;
-                if constexpr (D == 128u) {
-                    const u32x4 kk = *(const u32x4*)(kp + kvo), vv = *(const u32x4*)(vp + kvo);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        x.k[h][e] = kk[e];
-                        x.v[h][e] = vv[e];
-                    }
-                } else {
-                    const u32x2 kk = *(const u32x2*)(kp + kvo), vv = *(const u32x2*)(vp + kvo);
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        x.k[h][e] = kk[e];
-                        x.v[h][e] = vv[e];
-                    }
-                }
-                x.ks[h] = *(m4.k_scales + row * SROW + so);
-                x.vs[h] = *(m4.v_scales + row * SROW + so);
+                x.row[h] = hi32 >= 0 ? (uint64_t)(uint32_t)hi32 << 32 | lo32 : 0ull;
             }
         };
+        auto load = [&](Half4<D>& x, const Mx4Unit<D>& at, const void* base, const uint8_t* scales) {
+#pragma unroll
+            for (uint32_t h = 0; h < 2u; h++) {
+                const uint8_t* const p = (const uint8_t*)base + at.row[h] * ROW4;
+                if constexpr (D == 128u) {
+                    const u32x4 n = __builtin_nontemporal_load((const u32x4*)(p + kvo));
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x.n[h][e] = n[e];
+                } else {
+                    const u32x2 n = __builtin_nontemporal_load((const u32x2*)(p + kvo));
+#pragma unroll
+                    for (int e = 0; e < 2; e++) x.n[h][e] = n[e];
+                }
+                x.power[h] = *(scales + at.row[h] * SROW + so);
+            }
+        };
+        // unit i, in x; each of its registers is asked for again, for unit i + 2, as soon as it is free
         auto step = [&](Mx4Unit<D>& x, uint32_t i) {
             const uint32_t u = u0 + wave + kWaves * i;
             // keys past the last one, on no page, or unseen by a row: masked
-            const bool masked = !x.on[0] || !x.on[1] || (int32_t)(u * kUnit + kUnit - 1u) > hi_min;
+            const bool on[2] = {x.on[0], x.on[1]};
+            const bool masked = !on[0] || !on[1] || (int32_t)(u * kUnit + kUnit - 1u) > hi_min;
             if (masked) {
                 // a row's weight of a key it does not see is 0, and 0 times an infinity or NaN is NaN: V's rows
                 // of keys that there are not are set to 0, and so are blocks that are not all finite, whose
@@ -176,8 +179,8 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
                 const uint32_t last = rq.keys - u * kUnit;  // (of keys; this unit has some, or the part has none at all)
 #pragma unroll
                 for (uint32_t h = 0; h < 2u; h++) {
-                    const bool is = x.on[h] && 16u * h + n16 < last;
-                    const bool bad = is && x.vs[h] > kTopPower;
+                    const bool is = on[h] && 16u * h + n16 < last;
+                    const bool bad = is && x.v.power[h] > kTopPower;
                     for (uint64_t b = __builtin_amdgcn_ballot_w64(bad); b != 0; b &= b - 1u) {
                         const uint32_t l = (uint32_t)__builtin_ctzll(b);
                         const int32_t key = (int32_t)(u * kUnit + 16u * h + (l & 15u));
@@ -189,9 +192,9 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
                                 if (key <= hi[r] && (uint32_t)dt >> 1 == block) o[r][dt] += __uint_as_float(0x7fc00000u);
                     }
                     if (bad || !is) {
-                        x.vs[h] = 0;
+                        x.v.power[h] = 0;
 #pragma unroll
-                        for (int e = 0; e < ND; e++) x.v[h][e] = 0;
+                        for (int e = 0; e < ND; e++) x.v.n[h][e] = 0;
                     }
                 }
             }
@@ -202,20 +205,26 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
                 const uint32_t at = vt0 + (vb ^ (e << 4));
 #pragma unroll
                 for (uint32_t h = 0; h < 2u; h++)
-                    *(lds_u32x4*)(uintptr_t)(at + h * 16u * ROW) = values8<T>(x.v[h][e], power4(x.vs[h]));
+                    *(lds_u32x4*)(uintptr_t)(at + h * 16u * ROW) = values8<T>(x.v.n[h][e], power4(x.v.power[h]));
+            }
+            const bool more = i + 2u < count;
+            if (more) {
+                place(x, i + 2u);
+                load(x.v, x, a.v, m4.v_scales);
             }
             f32x4 sc[NR][2];
 #pragma unroll
             for (int kb = 0; kb < 2; kb++) {
-                const float sk = power4(x.ks[kb]);
+                const float sk = power4(x.k.power[kb]);
 #pragma unroll
                 for (int ch = 0; ch < ND; ch++) {
-                    const s16x8 k = __builtin_bit_cast(s16x8, values8<T>(x.k[kb][ch], sk));
+                    const s16x8 k = __builtin_bit_cast(s16x8, values8<T>(x.k.n[kb][ch], sk));
 #pragma unroll
                     for (int r = 0; r < (int)NR; r++)
                         sc[r][kb] = mfma16<T>(k, qf[r][ch], ch == 0 ? nm[r] : sc[r][kb]);
                 }
             }
+            if (more) load(x.k, x, a.k, m4.k_scales);
             s16x8 pf[NR];
 #pragma unroll
             for (int r = 0; r < (int)NR; r++) {
@@ -224,7 +233,7 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
                     bool any = false;
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const bool a0 = x.on[0] && k0 + e <= hi[r], a1 = x.on[1] && k0 + 16 + e <= hi[r];
+                        const bool a0 = on[0] && k0 + e <= hi[r], a1 = on[1] && k0 + 16 + e <= hi[r];
                         sc[r][0][e] = a0 ? sc[r][0][e] : -INFINITY;
                         sc[r][1][e] = a1 ? sc[r][1][e] : -INFINITY;
                         any = any || a0 || a1;
@@ -276,14 +285,16 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
         };
         if (count != 0) {
             Mx4Unit<D> x, y;
-            load(x, 0);
-            for (uint32_t i = 0;; i += 2u) {
-                if (i + 1u < count) load(y, i + 1u);
+            auto first = [&](Mx4Unit<D>& z, uint32_t i) {
+                place(z, i);
+                load(z.v, z, a.v, m4.v_scales);
+                load(z.k, z, a.k, m4.k_scales);
+            };
+            first(x, 0);
+            if (count > 1u) first(y, 1u);
+            for (uint32_t i = 0; i < count; i += 2u) {
                 step(x, i);
-                if (i + 1u >= count) break;
-                if (i + 2u < count) load(x, i + 2u);
-                step(y, i + 1u);
-                if (i + 2u >= count) break;
+                if (i + 1u < count) step(y, i + 1u);
             }
         }
 
@@ -355,7 +366,7 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
 
 // Waves a SIMD: what the registers let reside.
 template <uint32_t NR>
-constexpr uint32_t few_waves() { return NR == 1u ? 3u : NR == 2u ? 2u : 1u; }
+constexpr uint32_t few_waves() { return 4u - NR; }
 
 template <uint32_t T, uint32_t D, uint32_t NR>
 __global__ void __launch_bounds__(64 * kWaves, few_waves<NR>())
