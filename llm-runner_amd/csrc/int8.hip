@@ -51,78 +51,177 @@ __device__ __forceinline__ int round127(double y, double r, double a) {
     return n;
 }
 
-// One row a workgroup at a time, eight elements a thread.
-template <uint32_t XT, bool NORM>
+// A row's sums over the TPR threads that have it (a wave, or the four of a workgroup).
+struct RowSums {
+    double top, ss;  // largest |y|, sum of x^2
+    uint32_t bad;    // an infinity or NaN
+};
+template <uint32_t TPR>
+__device__ __forceinline__ RowSums row_sums(RowSums s) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        s.top = fmax(s.top, __shfl_xor(s.top, o, 64));
+        s.ss += __shfl_xor(s.ss, o, 64);
+    }
+    s.bad = __builtin_amdgcn_ballot_w64(s.bad != 0) != 0 ? 1u : 0u;
+    if constexpr (TPR == kRowThreads) {
+        __shared__ RowSums part[kRowThreads / 64];
+        if ((threadIdx.x & 63u) == 0) part[threadIdx.x >> 6] = s;
+        __syncthreads();
+        s = part[0];
+#pragma unroll
+        for (uint32_t i = 1; i < kRowThreads / 64u; i++) {
+            s.top = fmax(s.top, part[i].top);
+            s.ss += part[i].ss;
+            s.bad |= part[i].bad;
+        }
+        __syncthreads();
+    }
+    return s;
+}
+
+// Eight elements of a row into its sums.
+template <bool NORM>
+__device__ __forceinline__ void add8(RowSums& s, const float (&v)[8], const float (&w)[8]) {
+    if constexpr (NORM) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const double y = (double)v[i] * (double)w[i];  // exact
+            s.top = fmax(s.top, fabs(y));
+            if (!(fabs(y) < (double)INFINITY)) s.bad = 1u;
+            s.ss += (double)v[i] * (double)v[i];
+        }
+    } else {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);  // (NaN above everything)
+        if (m >= 0x7f800000u) s.bad = 1u;
+        else s.top = fmax(s.top, (double)__uint_as_float(m));
+    }
+}
+
+// What rounding a row's elements needs.
+struct RowScale {
+    double r, top;
+    float r32;
+    bool zero, exact;  // no rounding at all; f32 has not the range for it
+};
+template <bool NORM>
+__device__ __forceinline__ RowScale row_scale(const QuantizeRowsArgs& a, const RowSums& s, uint32_t row, bool writes) {
+    RowScale k;
+    k.zero = s.bad != 0 || s.top == 0.0;
+    k.top = s.top;
+    k.r = k.zero ? 0.0 : 127.0 / s.top;
+    k.r32 = (float)k.r;
+    k.exact = s.top < 1e-30 || s.top > 1e30;
+    if (writes) {
+        double f = s.top / 127.0;
+        if (NORM) f /= sqrt(s.ss / (double)a.dim + (double)a.eps);
+        a.scales[row] = s.bad ? __uint_as_float(0x7fc00000u) : s.top == 0.0 ? 0.0f : (float)f;
+    }
+    return k;
+}
+
+// Eight elements to integers. In f32, y, r and their product are each off by 2^-24 of them: 2.3e-5 of a step
+// at 127 steps, so that the nearest whole number is the one of 64 bits unless a half is within 5e-5.
+template <bool NORM>
+__device__ __forceinline__ u32x2 round8(const RowScale& k, const float (&v)[8], const float (&w)[8]) {
+    u32x2 o{0u, 0u};
+    if (k.zero) return o;
+    int n[8];
+    bool near = k.exact;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float t = (NORM ? v[i] * w[i] : v[i]) * k.r32, q = rintf(t);
+        near = near || fabsf(fabsf(t - q) - 0.5f) < 5e-5f;
+        n[i] = (int)q;
+    }
+    if (near) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) n[i] = round127(NORM ? (double)v[i] * (double)w[i] : (double)v[i], k.r, k.top);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) o[i / 4] |= ((uint32_t)n[i] & 0xffu) << (8 * (i % 4));
+    return o;
+}
+
+// TPR threads a row, eight elements a thread and piece, NV pieces held from the sums to the rounding.
+template <uint32_t XT, bool NORM, uint32_t TPR, uint32_t NV>
 __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(QuantizeRowsArgs a) {
-    constexpr uint32_t XS = XT == kGgmlF32 ? 4u : 2u;
-    __shared__ double red[2][kRowThreads / 64];
-    __shared__ uint32_t red_bad[kRowThreads / 64];
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
-    for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const uint8_t* const x = (const uint8_t*)a.x + (uint64_t)row * a.x_stride * XS;
-        double top = 0.0, ss = 0.0;
-        uint32_t bad = 0;
-        for (uint32_t k = 8u * tid; k < a.dim; k += 8u * kRowThreads) {
-            float v[8], w[8];
-            load8<XT>(x + (uint64_t)k * XS, v);
-            if (NORM) load8<kGgmlF32>((const uint8_t*)(a.norm + k), w);
+    constexpr uint32_t XS = XT == kGgmlF32 ? 4u : 2u, PER = kRowThreads / TPR;
+    const uint32_t t = threadIdx.x % TPR;
+    for (uint64_t row = (uint64_t)blockIdx.x * PER + threadIdx.x / TPR; row < a.rows; row += (uint64_t)gridDim.x * PER) {
+        const uint8_t* const x = (const uint8_t*)a.x + row * a.x_stride * XS;
+        float v[NV][8], w[NV][8];
+        RowSums s{0.0, 0.0, 0u};
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const double y = NORM ? (double)v[i] * (double)w[i] : (double)v[i];
-                top = fmax(top, fabs(y));
-                if (!(fabs(y) < (double)INFINITY)) bad = 1u;
-                if (NORM) ss += (double)v[i] * (double)v[i];
+        for (uint32_t c = 0; c < NV; c++) {
+            const uint32_t k = 8u * (t + TPR * c);
+            if (k < a.dim) {
+                load8<XT>(x + (uint64_t)k * XS, v[c]);
+                if (NORM) load8<kGgmlF32>((const uint8_t*)(a.norm + k), w[c]);
             }
         }
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            top = fmax(top, __shfl_xor(top, o, 64));
-            if (NORM) ss += __shfl_xor(ss, o, 64);
-        }
-        bad = __builtin_amdgcn_ballot_w64(bad != 0) != 0 ? 1u : 0u;
-        if (lane == 0) {
-            red[0][wave] = top;
-            red[1][wave] = ss;
-            red_bad[wave] = bad;
-        }
-        __syncthreads();
-        top = fmax(fmax(red[0][0], red[0][1]), fmax(red[0][2], red[0][3]));
-        ss = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
-        bad = red_bad[0] | red_bad[1] | red_bad[2] | red_bad[3];
-        __syncthreads();
-        const bool zero = bad != 0 || top == 0.0;
-        const double r = zero ? 0.0 : 127.0 / top;
-        if (tid == 0) {
-            double s = top / 127.0;
-            if (NORM) s /= sqrt(ss / (double)a.dim + (double)a.eps);
-            a.scales[row] = bad ? __uint_as_float(0x7fc00000u) : top == 0.0 ? 0.0f : (float)s;
-        }
-        int8_t* const q = a.q + (uint64_t)row * a.q_stride;
-        for (uint32_t k = 8u * tid; k < a.dim; k += 8u * kRowThreads) {
-            float v[8], w[8];
-            load8<XT>(x + (uint64_t)k * XS, v);
-            if (NORM) load8<kGgmlF32>((const uint8_t*)(a.norm + k), w);
-            u32x2 o{0u, 0u};
+        for (uint32_t c = 0; c < NV; c++)
+            if (8u * (t + TPR * c) < a.dim) add8<NORM>(s, v[c], w[c]);
+        s = row_sums<TPR>(s);
+        const RowScale sc = row_scale<NORM>(a, s, (uint32_t)row, t == 0);
+        int8_t* const q = a.q + row * a.q_stride;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const double y = NORM ? (double)v[i] * (double)w[i] : (double)v[i];
-                const int n = zero ? 0 : round127(y, r, top);
-                o[i / 4] |= ((uint32_t)n & 0xffu) << (8 * (i % 4));
-            }
-            *(u32x2*)(q + k) = o;
+        for (uint32_t c = 0; c < NV; c++) {
+            const uint32_t k = 8u * (t + TPR * c);
+            if (k < a.dim) *(u32x2*)(q + k) = round8<NORM>(sc, v[c], w[c]);
         }
     }
+}
+
+// Rows too long for the registers: read twice, a workgroup a row.
+template <uint32_t XT, bool NORM>
+__global__ void __launch_bounds__(kRowThreads) quantize_long_rows_kernel(QuantizeRowsArgs a) {
+    constexpr uint32_t XS = XT == kGgmlF32 ? 4u : 2u;
+    for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const uint8_t* const x = (const uint8_t*)a.x + (uint64_t)row * a.x_stride * XS;
+        RowSums s{0.0, 0.0, 0u};
+        float v[8], w[8];
+        for (uint32_t k = 8u * threadIdx.x; k < a.dim; k += 8u * kRowThreads) {
+            load8<XT>(x + (uint64_t)k * XS, v);
+            if (NORM) load8<kGgmlF32>((const uint8_t*)(a.norm + k), w);
+            add8<NORM>(s, v, w);
+        }
+        s = row_sums<kRowThreads>(s);
+        const RowScale sc = row_scale<NORM>(a, s, row, threadIdx.x == 0);
+        int8_t* const q = a.q + (uint64_t)row * a.q_stride;
+        for (uint32_t k = 8u * threadIdx.x; k < a.dim; k += 8u * kRowThreads) {
+            load8<XT>(x + (uint64_t)k * XS, v);
+            if (NORM) load8<kGgmlF32>((const uint8_t*)(a.norm + k), w);
+            *(u32x2*)(q + k) = round8<NORM>(sc, v, w);
+        }
+    }
+}
+
+template <uint32_t XT, bool NORM>
+hipError_t launch_rows(const QuantizeRowsArgs& a, int num_cus, hipStream_t st) {
+    const uint32_t most = (uint32_t)num_cus * 8u;
+    auto go = [&](auto kernel, uint32_t per) {
+        const uint32_t wgs = (a.rows + per - 1u) / per;
+        hipLaunchKernelGGL(kernel, dim3(wgs < most ? wgs : most), dim3(kRowThreads), 0, st, a);
+        return hipGetLastError();
+    };
+    if (a.dim <= 512u) return go(quantize_rows_kernel<XT, NORM, 64, 1>, 4);
+    if (a.dim <= 1024u) return go(quantize_rows_kernel<XT, NORM, 64, 2>, 4);
+    if (a.dim <= 2048u) return go(quantize_rows_kernel<XT, NORM, 256, 1>, 1);
+    if (a.dim <= 4096u) return go(quantize_rows_kernel<XT, NORM, 256, 2>, 1);
+    if (a.dim <= 8192u) return go(quantize_rows_kernel<XT, NORM, 256, 4>, 1);
+    return go(quantize_long_rows_kernel<XT, NORM>, 1);
 }
 
 }  // namespace
 
 hipError_t launch_quantize_rows_i8(const QuantizeRowsArgs& a, uint32_t xtype, int num_cus, hipStream_t st) {
-    const uint32_t grid = a.rows < (uint32_t)num_cus * 8u ? a.rows : (uint32_t)num_cus * 8u;
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(kRowThreads), 0, st, a); };
-    if (xtype == kGgmlF32) a.norm ? go(quantize_rows_kernel<kGgmlF32, true>) : go(quantize_rows_kernel<kGgmlF32, false>);
-    else if (xtype == kGgmlF16) a.norm ? go(quantize_rows_kernel<kGgmlF16, true>) : go(quantize_rows_kernel<kGgmlF16, false>);
-    else a.norm ? go(quantize_rows_kernel<kGgmlBF16, true>) : go(quantize_rows_kernel<kGgmlBF16, false>);
-    return hipGetLastError();
+    if (xtype == kGgmlF32) return a.norm ? launch_rows<kGgmlF32, true>(a, num_cus, st) : launch_rows<kGgmlF32, false>(a, num_cus, st);
+    if (xtype == kGgmlF16) return a.norm ? launch_rows<kGgmlF16, true>(a, num_cus, st) : launch_rows<kGgmlF16, false>(a, num_cus, st);
+    return a.norm ? launch_rows<kGgmlBF16, true>(a, num_cus, st) : launch_rows<kGgmlBF16, false>(a, num_cus, st);
 }
 
 }  // namespace llmr

@@ -71,12 +71,12 @@ __device__ __forceinline__ void store4(const MatmulI8Args& a, uint32_t m, uint32
 // A wave's step is 128 bytes of K: lane (row l16, group g) has bytes 32 g .. 32 g + 31 of a row, as two
 // 16-byte pieces for two 16x16x64 MFMAs (which k a piece is does not matter as long as both operands
 // agree), so that a row is read as whole 128-byte lines. Step s of a workgroup goes to wave s % 8.
-// U steps' loads are sent for at once.
+// U steps' rows are on their way while one is worked on.
 constexpr uint32_t kFewWaves = 8;
 
 template <uint32_t OT, uint32_t MT, uint32_t CT>
 __global__ void __launch_bounds__(64 * kFewWaves) matmul_i8_few(MatmulI8Args a) {
-    constexpr uint32_t U = MT == 1u ? 4u : MT == 2u ? 3u : 2u;
+    constexpr uint32_t U = MT == 1u ? 6u / CT : MT == 2u ? 4u : 3u;
     __shared__ i32x4 red[kFewWaves][CT * MT][64];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, l16 = lane & 15u, g = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -96,30 +96,36 @@ __global__ void __launch_bounds__(64 * kFewWaves) matmul_i8_few(MatmulI8Args a) 
     for (uint32_t c = 0; c < CT; c++)
 #pragma unroll
         for (uint32_t t = 0; t < MT; t++) acc[c][t] = i32x4{0, 0, 0, 0};
-    for (uint32_t s0 = wave; s0 < steps; s0 += U * kFewWaves) {
-        u32x4 wf[U][CT][2], xf[U][MT][2];
+    u32x4 wf[U][CT][2], xf[U][MT][2];
+    auto send = [&](auto B, uint32_t s) {  // step s into buffer B
+        constexpr int u = decltype(B)::value;
+        const uint32_t k = s * 128u;  // (past K for every lane: nothing is read)
 #pragma unroll
-        for (uint32_t u = 0; u < U; u++) {
-            const uint32_t k = (s0 + u * kFewWaves) * 128u;  // (past K for every lane: nothing is read)
+        for (uint32_t h = 0; h < 2u; h++) {
+            const bool in = k + 32u * g + 16u * h < a.K;
 #pragma unroll
-            for (uint32_t h = 0; h < 2u; h++) {
-                const bool in = k + 32u * g + 16u * h < a.K;
+            for (uint32_t c = 0; c < CT; c++) wf[u][c][h] = bload16(wr, in && wo[c] != ~0u ? wo[c] + k + 16u * h : ~0u, 0u);
 #pragma unroll
-                for (uint32_t c = 0; c < CT; c++) wf[u][c][h] = bload16(wr, in && wo[c] != ~0u ? wo[c] + k + 16u * h : ~0u, 0u);
-#pragma unroll
-                for (uint32_t t = 0; t < MT; t++) xf[u][t][h] = bload16(xr, in && xo[t] != ~0u ? xo[t] + k + 16u * h : ~0u, 0u);
-            }
+            for (uint32_t t = 0; t < MT; t++) xf[u][t][h] = bload16(xr, in && xo[t] != ~0u ? xo[t] + k + 16u * h : ~0u, 0u);
         }
+    };
+    static_for<0, (int)U>([&](auto B) { send(B, wave + (uint32_t)decltype(B)::value * kFewWaves); });
+    for (uint32_t s0 = wave; s0 < steps; s0 += U * kFewWaves) {
+        static_for<0, (int)U>([&](auto B) {
+            constexpr int u = decltype(B)::value;
+            const uint32_t s = s0 + (uint32_t)u * kFewWaves;
+            if (s < steps) {
 #pragma unroll
-        for (uint32_t u = 0; u < U; u++)
+                for (uint32_t h = 0; h < 2u; h++)
 #pragma unroll
-            for (uint32_t h = 0; h < 2u; h++)
+                    for (uint32_t c = 0; c < CT; c++)
 #pragma unroll
-                for (uint32_t c = 0; c < CT; c++)
-#pragma unroll
-                    for (uint32_t t = 0; t < MT; t++)
-                        acc[c][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, wf[u][c][h]),
-                                                                         __builtin_bit_cast(i32x4, xf[u][t][h]), acc[c][t], 0, 0, 0);
+                        for (uint32_t t = 0; t < MT; t++)
+                            acc[c][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, wf[u][c][h]),
+                                                                             __builtin_bit_cast(i32x4, xf[u][t][h]), acc[c][t], 0, 0, 0);
+                if (s + U * kFewWaves < steps) send(B, s + U * kFewWaves);
+            }
+        });
     }
 #pragma unroll
     for (uint32_t c = 0; c < CT; c++)
@@ -421,6 +427,114 @@ __global__ void __launch_bounds__(256, 1) matmul_i8_tiles(MatmulI8Args a, uint32
     LLMR_WAIT_VMCNT(0);  // no DMA may still be writing this workgroup's LDS when it exits
 }
 
+// ---- small tiles -----------------------------------------------------------------------
+//
+// Tiles of 64 MB tokens x 128 channels, one a workgroup, for launches that large tiles leave most CUs without: four
+// waves in 2 x 2 of 32 MB x 64, stages of 128 bytes of K in four LDS slots, sent for three stages ahead (a stage
+// takes less than its loads' way from L2 and memory).
+constexpr int kSmallSlots = 4;
+
+template <uint32_t OT, uint32_t MB>
+__global__ void __launch_bounds__(256, 1) matmul_i8_small(MatmulI8Args a, uint32_t tiles_m) {
+    constexpr uint32_t BM = 64u * MB, BN = 128u, SLOT = (BM + BN) * kRow;
+    constexpr int XD = 2 * MB, WD = 4;
+    __shared__ __attribute__((aligned(16))) uint8_t L0[SLOT];
+    __shared__ __attribute__((aligned(16))) uint8_t L1[SLOT];
+    __shared__ __attribute__((aligned(16))) uint8_t L2[SLOT];
+    __shared__ __attribute__((aligned(16))) uint8_t L3[SLOT];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t l32 = lane & 31u, kh = lane >> 5, wm = wave & 1u, wn = wave >> 1;
+    // an XCD has a run of channel tiles with all their token tiles
+    const uint32_t L = xcd_linear(blockIdx.x, gridDim.x), m0 = (L % tiles_m) * BM, n0 = (L / tiles_m) * BN;
+    const uint32_t S = (a.K + kRow - 1u) / kRow;
+    const int8_t* const xb = a.x + (uint64_t)m0 * a.x_stride;
+    const int8_t* const wb = a.w + (uint64_t)n0 * a.w_stride;
+    const uint32_t xsize = (a.M - m0 < BM ? a.M - m0 : BM) * a.x_stride, wsize = (a.N - n0 < BN ? a.N - n0 : BN) * a.w_stride;
+    uint32_t xvoff[XD], wvoff[WD];
+    const uint32_t c0 = (lane & 7u) ^ (lane >> 3);  // of even i; odd i: ^ 1
+#pragma unroll
+    for (int i = 0; i < XD; i++) xvoff[i] = (16u * MB * wave + 8u * i + (lane >> 3)) * a.x_stride + ((c0 ^ (i & 1)) << 4);
+#pragma unroll
+    for (int i = 0; i < WD; i++) wvoff[i] = (32u * wave + 8u * i + (lane >> 3)) * a.w_stride + ((c0 ^ (i & 1)) << 4);
+    uint32_t xoff[4], woff[4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+        const uint32_t ch = 4u * (t >> 1) + 2u * kh + (t & 1);
+        xoff[t] = lds_off(wm * 32u * MB + l32, ch);
+        woff[t] = BM * kRow + lds_off(wn * 64u + l32, ch);
+    }
+    auto send = [&](uint32_t s, uint8_t* slot) {  // (a stage past the last: nothing is read, zeros arrive)
+        const auto xr = make_rsrc(xb + (uint64_t)s * kRow, s < S ? xsize : 0u), wr = make_rsrc(wb + (uint64_t)s * kRow, s < S ? wsize : 0u);
+        const uint32_t past[2] = {s * kRow + (c0 << 4) < a.K ? 0u : 0x80000000u, s * kRow + ((c0 ^ 1u) << 4) < a.K ? 0u : 0x80000000u};
+#pragma unroll
+        for (int i = 0; i < WD; i++) dma16(wr, slot + BM * kRow + wave * (32u * kRow) + 1024u * i, wvoff[i] + past[i & 1]);
+#pragma unroll
+        for (int i = 0; i < XD; i++) dma16(xr, slot + wave * (16u * MB * kRow) + 1024u * i, xvoff[i] + past[i & 1]);
+    };
+    i32x16 acc[2][MB];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (uint32_t b = 0; b < MB; b++) acc[i][b] = i32x16{};
+    auto work = [&](const uint8_t* slot) {
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            i32x4 xf[MB], wf[2];
+#pragma unroll
+            for (uint32_t b = 0; b < MB; b++) xf[b] = *(const i32x4*)(slot + b * 32u * kRow + xoff[t]);
+#pragma unroll
+            for (int i = 0; i < 2; i++) wf[i] = *(const i32x4*)(slot + i * 32 * (int)kRow + woff[t]);
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (uint32_t b = 0; b < MB; b++) acc[i][b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[i], xf[b], acc[i][b], 0, 0, 0);
+        }
+    };
+    send(0, L0);
+    send(1, L1);
+    send(2, L2);
+    LLMR_STAGE_BARRIER(2 * (XD + WD));
+    // Stage s reads slot s % 4 and sends for stage s + 3 into the slot that stage s - 1 read; its end waits until at
+    // most the stages s + 2 and s + 3 are on their way.
+    for (uint32_t s = 0;;) {
+#define LLMR8_SMALL(CUR, DST)            \
+    send(s + 3u, DST);                   \
+    work(CUR);                           \
+    LLMR_STAGE_BARRIER(2 * (XD + WD));   \
+    if (++s == S) break
+        LLMR8_SMALL(L0, L3);
+        LLMR8_SMALL(L1, L0);
+        LLMR8_SMALL(L2, L1);
+        LLMR8_SMALL(L3, L2);
+#undef LLMR8_SMALL
+    }
+    LLMR_WAIT_VMCNT(0);  // no DMA may still be writing this workgroup's LDS when it exits
+#pragma unroll
+    for (uint32_t b = 0; b < MB; b++) {
+        const uint32_t m = m0 + wm * 32u * MB + 32u * b + l32;
+        const float xs = a.x_scales[m < a.M ? m : a.M - 1u];
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (uint32_t g = 0; g < 4u; g++) {
+                const uint32_t c = n0 + wn * 64u + 32u * i + 8u * g + 4u * kh;
+                float ws[4];
+#pragma unroll
+                for (uint32_t e = 0; e < 4u; e++) ws[e] = a.w_scales[c + e < a.N ? c + e : a.N - 1u];
+                if (m < a.M && c < a.N)
+                    store4<OT>(a, m, c, i32x4{acc[i][b][4 * g], acc[i][b][4 * g + 1], acc[i][b][4 * g + 2], acc[i][b][4 * g + 3]}, xs, ws);
+            }
+    }
+}
+
+template <uint32_t OT, uint32_t MB>
+hipError_t launch_small(const MatmulI8Args& a, hipStream_t st) {
+    const uint32_t tm = (a.M + 64u * MB - 1u) / (64u * MB), tn = (a.N + 127u) / 128u;
+    hipLaunchKernelGGL((matmul_i8_small<OT, MB>), dim3(tm * tn), dim3(256), 0, st, a, tm);
+    return hipGetLastError();
+}
+
 template <uint32_t OT, uint32_t MB>
 hipError_t launch_tiles(const MatmulI8Args& a, int num_cus, hipStream_t st) {
     hipLaunchKernelGGL((matmul_i8_tiles<OT, MB>), dim3(num_cus), dim3(256), 0, st, a, (a.M + 64u * MB - 1u) / (64u * MB),
@@ -440,24 +554,39 @@ hipError_t launch_few(const MatmulI8Args& a, int num_cus, hipStream_t st) {
 
 template <uint32_t OT>
 hipError_t launch_matmul(const MatmulI8Args& a, int num_cus, hipStream_t st) {
-    if (a.M <= 16u) return launch_few<OT, 1>(a, num_cus, st);
-    if (a.M <= 32u) return launch_few<OT, 2>(a, num_cus, st);
-    if (a.M <= 64u) return launch_few<OT, 4>(a, num_cus, st);
-    // the tile height whose rounds of tiles take least: a tile's time goes with its products, and a part that all have
-    uint32_t best = 4;
+    // The weight stream where a workgroup of 16 channels a CU covers them, at any M up to 64 (N 4096, M 64, K 1024,
+    // 4096, 14336: 6.4, 12.4, 34 us; small tiles 7.3, 13.3, 42), and past that up to 16 tokens with long rows (N 10240 and
+    // 20480, M 8, K 4096: 13.1, 19.0; small tiles 15.4, 19.1; M 32: 19.2, 27.7 and 15.8, 19.7; M 16, K 1024: 9.0, 9.1 and 6.6, 6.8).
+    if (a.M <= 64u && (a.N <= 16u * (uint32_t)num_cus || (a.M <= 16u && a.K >= 2048u))) {
+        if (a.M <= 16u) return launch_few<OT, 1>(a, num_cus, st);
+        if (a.M <= 32u) return launch_few<OT, 2>(a, num_cus, st);
+        return launch_few<OT, 4>(a, num_cus, st);
+    }
+    // The tiles whose rounds take least, in ns: a stage of 128 bytes of K, and what a round has besides. Fitted to one
+    // round each (S stages of 256 x N, 512 x 4096, 128 x 1024 and so on: within 15%), the largest to full rounds.
+    struct Kind {
+        uint32_t m, n, stage, round;
+    };
+    static const Kind kinds[] = {{64, 128, 410, 1800}, {128, 128, 580, 3000}, {64, 256, 600, 3100},
+                                 {128, 256, 820, 5000}, {192, 256, 1150, 6000}, {256, 256, 1450, 7000}};
+    const uint64_t S = (a.K + kRow - 1u) / kRow;
+    uint32_t best = 0;
     uint64_t least = ~0ull;
-    for (uint32_t mb = 4; mb >= 1u; mb--) {
-        const uint64_t tiles = (uint64_t)((a.M + 64u * mb - 1u) / (64u * mb)) * ((a.N + 255u) / 256u);
-        const uint64_t cost = (tiles + (uint64_t)num_cus - 1u) / (uint64_t)num_cus * (mb + 1u);
-        if (cost < least) {
+    for (uint32_t i = 0; i < 6u; i++) {
+        const Kind& k = kinds[i];
+        const uint64_t tiles = (uint64_t)((a.M + k.m - 1u) / k.m) * ((a.N + k.n - 1u) / k.n);
+        const uint64_t cost = (tiles + (uint64_t)num_cus - 1u) / (uint64_t)num_cus * (S * k.stage + k.round);
+        if (cost < least && (i > 1u || tiles < (1u << 24))) {  // (256 threads each: under 2^32 of them)
             least = cost;
-            best = mb;
+            best = i;
         }
     }
     switch (best) {
-        case 1: return launch_tiles<OT, 1>(a, num_cus, st);
-        case 2: return launch_tiles<OT, 2>(a, num_cus, st);
-        case 3: return launch_tiles<OT, 3>(a, num_cus, st);
+        case 0: return launch_small<OT, 1>(a, st);
+        case 1: return launch_small<OT, 2>(a, st);
+        case 2: return launch_tiles<OT, 1>(a, num_cus, st);
+        case 3: return launch_tiles<OT, 2>(a, num_cus, st);
+        case 4: return launch_tiles<OT, 3>(a, num_cus, st);
         default: return launch_tiles<OT, 4>(a, num_cus, st);
     }
 }
