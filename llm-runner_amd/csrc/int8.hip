@@ -8,22 +8,21 @@
 namespace llmr {
 namespace {
 
-// Eight elements from x on, as f32.
+// Eight elements as they lie, and as f32.
 template <uint32_t XT>
-__device__ __forceinline__ void load8(const uint8_t* x, float (&v)[8]) {
-    if constexpr (XT == kGgmlF32) {
-        const f32x4 a = *(const f32x4*)x, b = *(const f32x4*)(x + 16);
+struct Eight {
+    u32x4 w[XT == kGgmlF32 ? 2 : 1];
+    __device__ __forceinline__ void load(const void* x) {
+        w[0] = *(const u32x4*)x;
+        if constexpr (XT == kGgmlF32) w[1] = *((const u32x4*)x + 1);
+    }
+    __device__ __forceinline__ void values(float (&v)[8]) const {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            v[i] = a[i];
-            v[4 + i] = b[i];
-        }
-    } else {
-        const u32x4 w = *(const u32x4*)x;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t u = w[i];
-            if constexpr (XT == kGgmlBF16) {
+        for (int i = 0; i < (XT == kGgmlF32 ? 8 : 4); i++) {
+            const uint32_t u = w[i / 4][i % 4];
+            if constexpr (XT == kGgmlF32) {
+                v[i] = __uint_as_float(u);
+            } else if constexpr (XT == kGgmlBF16) {
                 v[2 * i] = __uint_as_float(u << 16);
                 v[2 * i + 1] = __uint_as_float(u & 0xffff0000u);
             } else {
@@ -33,7 +32,7 @@ __device__ __forceinline__ void load8(const uint8_t* x, float (&v)[8]) {
             }
         }
     }
-}
+};
 
 constexpr uint32_t kRowThreads = 256;
 
@@ -51,7 +50,7 @@ __device__ __forceinline__ int round127(double y, double r, double a) {
     return n;
 }
 
-// A row's sums over the TPR threads that have it (a wave, or the four of a workgroup).
+// A row's sums over the TPR threads that have it (a wave, or a workgroup).
 struct RowSums {
     double top, ss;  // largest |y|, sum of x^2
     uint32_t bad;    // an infinity or NaN
@@ -64,13 +63,13 @@ __device__ __forceinline__ RowSums row_sums(RowSums s) {
         s.ss += __shfl_xor(s.ss, o, 64);
     }
     s.bad = __builtin_amdgcn_ballot_w64(s.bad != 0) != 0 ? 1u : 0u;
-    if constexpr (TPR == kRowThreads) {
-        __shared__ RowSums part[kRowThreads / 64];
+    if constexpr (TPR > 64u) {
+        __shared__ RowSums part[TPR / 64u];
         if ((threadIdx.x & 63u) == 0) part[threadIdx.x >> 6] = s;
         __syncthreads();
         s = part[0];
 #pragma unroll
-        for (uint32_t i = 1; i < kRowThreads / 64u; i++) {
+        for (uint32_t i = 1; i < TPR / 64u; i++) {
             s.top = fmax(s.top, part[i].top);
             s.ss += part[i].ss;
             s.bad |= part[i].bad;
@@ -146,32 +145,52 @@ __device__ __forceinline__ u32x2 round8(const RowScale& k, const float (&v)[8], 
 }
 
 // TPR threads a row, eight elements a thread and piece, NV pieces held from the sums to the rounding.
+template <uint32_t TPR>
+constexpr uint32_t row_threads() { return TPR > kRowThreads ? TPR : kRowThreads; }
 template <uint32_t XT, bool NORM, uint32_t TPR, uint32_t NV>
-__global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(QuantizeRowsArgs a) {
-    constexpr uint32_t XS = XT == kGgmlF32 ? 4u : 2u, PER = kRowThreads / TPR;
+__global__ void __launch_bounds__(row_threads<TPR>()) quantize_rows_kernel(QuantizeRowsArgs a) {
+    constexpr uint32_t XS = XT == kGgmlF32 ? 4u : 2u, PER = row_threads<TPR>() / TPR;
     const uint32_t t = threadIdx.x % TPR;
     for (uint64_t row = (uint64_t)blockIdx.x * PER + threadIdx.x / TPR; row < a.rows; row += (uint64_t)gridDim.x * PER) {
         const uint8_t* const x = (const uint8_t*)a.x + row * a.x_stride * XS;
-        float v[NV][8], w[NV][8];
+        Eight<XT> e[NV];
+        float v[8], w[8];
         RowSums s{0.0, 0.0, 0u};
+        // (the norm's weights are read twice, from L2: held, they would halve the rows a CU has on their way)
+        auto weights = [&](uint32_t k) {
+            if constexpr (NORM) {
+                Eight<kGgmlF32> n;
+                n.load(a.norm + k);
+                n.values(w);
+            }
+        };
+#pragma unroll
+        for (uint32_t c = 0; c < NV; c++) {
+            const uint32_t k = 8u * (t + TPR * c);
+            if (k < a.dim) e[c].load(x + (uint64_t)k * XS);
+        }
 #pragma unroll
         for (uint32_t c = 0; c < NV; c++) {
             const uint32_t k = 8u * (t + TPR * c);
             if (k < a.dim) {
-                load8<XT>(x + (uint64_t)k * XS, v[c]);
-                if (NORM) load8<kGgmlF32>((const uint8_t*)(a.norm + k), w[c]);
+                weights(k);
+                e[c].values(v);
+                add8<NORM>(s, v, w);
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
-#pragma unroll
-        for (uint32_t c = 0; c < NV; c++)
-            if (8u * (t + TPR * c) < a.dim) add8<NORM>(s, v[c], w[c]);
         s = row_sums<TPR>(s);
         const RowScale sc = row_scale<NORM>(a, s, (uint32_t)row, t == 0);
         int8_t* const q = a.q + row * a.q_stride;
 #pragma unroll
         for (uint32_t c = 0; c < NV; c++) {
             const uint32_t k = 8u * (t + TPR * c);
-            if (k < a.dim) *(u32x2*)(q + k) = round8<NORM>(sc, v[c], w[c]);
+            if (k < a.dim) {
+                weights(k);
+                e[c].values(v);
+                *(u32x2*)(q + k) = round8<NORM>(sc, v, w);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 }
@@ -184,17 +203,25 @@ __global__ void __launch_bounds__(kRowThreads) quantize_long_rows_kernel(Quantiz
         const uint8_t* const x = (const uint8_t*)a.x + (uint64_t)row * a.x_stride * XS;
         RowSums s{0.0, 0.0, 0u};
         float v[8], w[8];
+        auto at = [&](uint32_t k) {
+            Eight<XT> e;
+            e.load(x + (uint64_t)k * XS);
+            e.values(v);
+            if constexpr (NORM) {
+                Eight<kGgmlF32> n;
+                n.load(a.norm + k);
+                n.values(w);
+            }
+        };
         for (uint32_t k = 8u * threadIdx.x; k < a.dim; k += 8u * kRowThreads) {
-            load8<XT>(x + (uint64_t)k * XS, v);
-            if (NORM) load8<kGgmlF32>((const uint8_t*)(a.norm + k), w);
+            at(k);
             add8<NORM>(s, v, w);
         }
         s = row_sums<kRowThreads>(s);
         const RowScale sc = row_scale<NORM>(a, s, row, threadIdx.x == 0);
         int8_t* const q = a.q + (uint64_t)row * a.q_stride;
         for (uint32_t k = 8u * threadIdx.x; k < a.dim; k += 8u * kRowThreads) {
-            load8<XT>(x + (uint64_t)k * XS, v);
-            if (NORM) load8<kGgmlF32>((const uint8_t*)(a.norm + k), w);
+            at(k);
             *(u32x2*)(q + k) = round8<NORM>(sc, v, w);
         }
     }
@@ -203,9 +230,9 @@ __global__ void __launch_bounds__(kRowThreads) quantize_long_rows_kernel(Quantiz
 template <uint32_t XT, bool NORM>
 hipError_t launch_rows(const QuantizeRowsArgs& a, int num_cus, hipStream_t st) {
     const uint32_t most = (uint32_t)num_cus * 8u;
-    auto go = [&](auto kernel, uint32_t per) {
+    auto go = [&](auto kernel, uint32_t per, uint32_t threads = kRowThreads) {
         const uint32_t wgs = (a.rows + per - 1u) / per;
-        hipLaunchKernelGGL(kernel, dim3(wgs < most ? wgs : most), dim3(kRowThreads), 0, st, a);
+        hipLaunchKernelGGL(kernel, dim3(wgs < most ? wgs : most), dim3(threads), 0, st, a);
         return hipGetLastError();
     };
     if (a.dim <= 512u) return go(quantize_rows_kernel<XT, NORM, 64, 1>, 4);
@@ -213,6 +240,7 @@ hipError_t launch_rows(const QuantizeRowsArgs& a, int num_cus, hipStream_t st) {
     if (a.dim <= 2048u) return go(quantize_rows_kernel<XT, NORM, 256, 1>, 1);
     if (a.dim <= 4096u) return go(quantize_rows_kernel<XT, NORM, 256, 2>, 1);
     if (a.dim <= 8192u) return go(quantize_rows_kernel<XT, NORM, 256, 4>, 1);
+    if (a.dim <= 16384u) return go(quantize_rows_kernel<XT, NORM, 512, 4>, 1, 512);
     return go(quantize_long_rows_kernel<XT, NORM>, 1);
 }
 

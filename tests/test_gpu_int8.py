@@ -40,7 +40,7 @@ def _check_rows(x, norm=None, eps=1e-6, **kw):
 
 # one piece of 16; rows shorter than the workgroup, around its 2048 elements, several times it, the longest
 ROWS = [(1, 16), (3, 48), (5, 4096), (2, 2064), (7, 2048), (4, 2032), (300, 272), (64, 3840), (9, 10240), (2, 131056),
-        (2500, 64)]
+        (2500, 64), (5, 512), (6, 528), (7, 1024), (3, 1040), (5, 8192), (2, 8208), (3, 16384), (3, 16400), (11, 5008)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
