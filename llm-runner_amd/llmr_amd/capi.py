@@ -289,6 +289,7 @@ class Context:
     def __init__(self, device: int = 0):
         self.device = device
         self._h = _vp()
+        self._stream = -1  # the last one set; -1: the context's own, from before any was
         check(lib().llmr_create_context(device, ctypes.byref(self._h)))
 
     @property
@@ -307,7 +308,10 @@ class Context:
             pass
 
     def set_stream(self, stream_ptr: int | None) -> None:
-        check(lib().llmr_set_stream(self._h, stream_ptr or None))  # 0/None: HIP null stream
+        stream = stream_ptr or 0  # 0/None: HIP null stream
+        if stream != self._stream:
+            check(lib().llmr_set_stream(self._h, stream or None))
+            self._stream = stream
 
     def stream(self) -> int:
         return lib().llmr_get_stream(self._h) or 0

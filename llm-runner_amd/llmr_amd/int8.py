@@ -9,6 +9,8 @@ device; nothing is read back.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import capi
@@ -20,13 +22,21 @@ _TYPES = {torch.float32: GGML_F32, torch.float16: GGML_F16, torch.bfloat16: GGML
 _I8 = torch.int8
 
 
+# a call's parameters, made once for each set of sizes (a structure costs as much host time as the call)
+_rows_params = functools.lru_cache(maxsize=256)(capi.QuantizeRowsParams)
+_matmul_params = functools.lru_cache(maxsize=256)(capi.MatmulI8Params)
+
+
 def _rows(t: torch.Tensor, what: str):
     """(rows, columns, row stride) of a 2-D view with contiguous rows; one row's stride is nothing and counts as a
     whole row of 16-byte pieces."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and not 0 <= t.stride(0) <= _U32):
-        raise ValueError(f"{what} must be a 2-D view with contiguous rows, under 2^32 apart")
-    n, m = t.shape
-    return n, m, t.stride(0) if n > 1 else m + -m % 16
+    strides = t.stride()
+    if len(strides) == 2:
+        n, m = t.shape
+        row = strides[0] if n > 1 else m + -m % 16
+        if (strides[1] == 1 or m <= 1) and 0 <= row <= _U32:
+            return n, m, row
+    raise ValueError(f"{what} must be a 2-D view with contiguous rows, under 2^32 apart")
 
 
 def _scales(t: torch.Tensor, what: str, n: int) -> int:
@@ -48,14 +58,14 @@ def quantize_rows(x: torch.Tensor, norm: torch.Tensor | None = None, eps: float 
     if scales is None:
         scales = torch.empty(T, dtype=torch.float32, device=x.device)
     qn, qk, qs = _rows(q, "q")
-    if q.dtype is not _I8 or (qn, qk) != (T, K):
+    if q.dtype is not _I8 or qn != T or qk != K:
         raise ValueError("q must be int8 with x's shape")
     if norm is not None and norm.numel() != K:
         raise ValueError("norm must have x's columns")
     sp, np_ = _scales(scales, "scales", T), _vec(norm, "norm", K)
     on = (x, q, scales) if norm is None else (x, q, scales, norm)
     _graph(g, *on).ctx.quantize_rows_i8(x.data_ptr(), np_, q.data_ptr(), sp,
-                                        capi.QuantizeRowsParams(T, K, t, xs, qs, eps))
+                                        _rows_params(T, K, t, xs, qs, eps))
     return q, scales
 
 
@@ -72,10 +82,10 @@ def matmul(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: t
     if out is None:
         out = torch.empty(M, N, dtype=dtype, device=x.device)
     t = _TYPES.get(out.dtype)
-    if t is None or out.shape != (M, N):
+    Mo, No, os_ = _rows(out, "out")
+    if t is None or Mo != M or No != N:
         raise ValueError(f"out must be [{M}, {N}] of float32, float16 or bfloat16")
-    os_ = _rows(out, "out")[2]
     xp, wp = _scales(x_scales, "x_scales", M), _scales(w_scales, "w_scales", N)
     _graph(g, x, x_scales, w, w_scales, out).ctx.matmul_i8(x.data_ptr(), xp, w.data_ptr(), wp, out.data_ptr(),
-                                                           capi.MatmulI8Params(M, N, K, xs, ws, t, os_))
+                                                           _matmul_params(M, N, K, xs, ws, t, os_))
     return out

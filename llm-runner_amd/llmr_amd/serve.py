@@ -278,14 +278,18 @@ class Mx4Cache:
                           for n in (head_dim // 2, head_dim // 32)))
 
 
+_U8 = torch.uint8
+
+
 def _mx4(k: Mx4Cache, v: Mx4Cache):
     """(pages, heads, page size, head_dim) of a pair of caches, and the structures of the call."""
     kd, ks, vd, vs = k.data, k.scales, v.data, v.scales
-    if kd.dim() != 4 or not (kd.dtype is ks.dtype is vd.dtype is vs.dtype is torch.uint8) or not (
+    shape = kd.shape
+    if len(shape) != 4 or not (kd.dtype is ks.dtype is vd.dtype is vs.dtype is _U8) or not (
             kd.is_contiguous() and ks.is_contiguous() and vd.is_contiguous() and vs.is_contiguous()):
         raise ValueError("the caches' data and scales must be contiguous uint8 tensors of four dimensions")
-    n, h, page, half = kd.shape
-    if vd.shape != kd.shape or half % 16 or ks.shape != (n, h, page, half // 16) or vs.shape != ks.shape:
+    n, h, page, half = shape
+    if vd.shape != shape or half % 16 or ks.shape != (n, h, page, half // 16) or vs.shape != ks.shape:
         raise ValueError("the caches must be [n_pages, n_kv_heads, page_size, head_dim / 2] with scales [.., head_dim "
                          "/ 32], alike")
     return n, h, page, 2 * half, capi.Mx4Cache(kd.data_ptr(), ks.data_ptr()), capi.Mx4Cache(vd.data_ptr(), vs.data_ptr())
