@@ -289,7 +289,6 @@ class Context:
     def __init__(self, device: int = 0):
         self.device = device
         self._h = _vp()
-        self._stream = -1  # the last one set; -1: the context's own, from before any was
         check(lib().llmr_create_context(device, ctypes.byref(self._h)))
 
     @property
@@ -308,10 +307,7 @@ class Context:
             pass
 
     def set_stream(self, stream_ptr: int | None) -> None:
-        stream = stream_ptr or 0  # 0/None: HIP null stream
-        if stream != self._stream:
-            check(lib().llmr_set_stream(self._h, stream or None))
-            self._stream = stream
+        check(lib().llmr_set_stream(self._h, stream_ptr or None))  # 0/None: HIP null stream
 
     def stream(self) -> int:
         return lib().llmr_get_stream(self._h) or 0

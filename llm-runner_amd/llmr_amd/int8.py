@@ -9,8 +9,6 @@ device; nothing is read back.
 """
 from __future__ import annotations
 
-import functools
-
 import torch
 
 from . import capi
@@ -20,11 +18,6 @@ from .serve import _U32, _graph, _vec
 
 _TYPES = {torch.float32: GGML_F32, torch.float16: GGML_F16, torch.bfloat16: GGML_BF16}
 _I8 = torch.int8
-
-
-# a call's parameters, made once for each set of sizes (a structure costs as much host time as the call)
-_rows_params = functools.lru_cache(maxsize=256)(capi.QuantizeRowsParams)
-_matmul_params = functools.lru_cache(maxsize=256)(capi.MatmulI8Params)
 
 
 def _rows(t: torch.Tensor, what: str):
@@ -65,7 +58,7 @@ def quantize_rows(x: torch.Tensor, norm: torch.Tensor | None = None, eps: float 
     sp, np_ = _scales(scales, "scales", T), _vec(norm, "norm", K)
     on = (x, q, scales) if norm is None else (x, q, scales, norm)
     _graph(g, *on).ctx.quantize_rows_i8(x.data_ptr(), np_, q.data_ptr(), sp,
-                                        _rows_params(T, K, t, xs, qs, eps))
+                                        capi.QuantizeRowsParams(T, K, t, xs, qs, eps))
     return q, scales
 
 
@@ -87,5 +80,5 @@ def matmul(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: t
         raise ValueError(f"out must be [{M}, {N}] of float32, float16 or bfloat16")
     xp, wp = _scales(x_scales, "x_scales", M), _scales(w_scales, "w_scales", N)
     _graph(g, x, x_scales, w, w_scales, out).ctx.matmul_i8(x.data_ptr(), xp, w.data_ptr(), wp, out.data_ptr(),
-                                                           _matmul_params(M, N, K, xs, ws, t, os_))
+                                                           capi.MatmulI8Params(M, N, K, xs, ws, t, os_))
     return out
