@@ -2,13 +2,15 @@
 //
 //   out[m, n] = x_scales[m] w_scales[n] sum_k x[m, k] w[n, k]
 //
-// The sum is exact in int32, in any order and any split of K, so both kernels give
+// The sum is exact in int32, in any order and any split of K, so every kernel gives
 // the same bits.
 //
-//  - matmul_i8_few, up to 64 tokens: a stream of the weights. A workgroup has 16 or 32
-//    channels and all tokens; its eight waves share K and add up in LDS.
-//  - matmul_i8_tiles: persistent 64..256 x 256 tiles, 128 bytes of K a stage, both
-//    operands by DMA into LDS rings.
+//  - matmul_i8_few, few tokens, or few outputs with long rows: a stream of the weights.
+//    A workgroup has 16 or 32 channels and up to 64 tokens; its eight waves share K and
+//    add up in LDS.
+//  - matmul_i8_small: tiles of 64 or 128 tokens x 128 channels, one a workgroup.
+//  - matmul_i8_tiles: persistent tiles of 64 to 256 tokens x 256 channels, 128 bytes of
+//    K a stage, both operands by DMA into LDS rings.
 // The MFMAs take the weights as A and the tokens as B, so that a lane's results are
 // consecutive channels of one token.
 #include "gemm_q_common.h"
@@ -68,47 +70,56 @@ __device__ __forceinline__ void store4(const MatmulI8Args& a, uint32_t m, uint32
 
 // ---- few tokens ----------------------------------------------------------------------
 //
-// A wave's step is 128 bytes of K: lane (row l16, group g) has bytes 32 g .. 32 g + 31 of a row, as two
-// 16-byte pieces for two 16x16x64 MFMAs (which k a piece is does not matter as long as both operands
-// agree), so that a row is read as whole 128-byte lines. Step s of a workgroup goes to wave s % 8.
-// U steps' rows are on their way while one is worked on.
+// A workgroup has 16 CT channels of 16 MT tokens; its waves share K. A wave's step is 128 bytes of K, step s of a
+// workgroup its wave s % 8's, as two halves of 64 bytes for a 16x16x64 MFMA each; U steps' rows are on their way while
+// one is worked on. A load has lanes 4 r .. 4 r + 3 at four pieces of 16 bytes of row r: four lanes side by side that
+// are on four rows, as the MFMA has them, take about four times as long (64 x 4096 x 4096 12.4 us, 1 x 4096 x 6144 8.7;
+// this way 9.4 and 7.4, of which the pieces' way to the MFMA's lanes, over LDS, is 1.4 and 0.4). Which k a piece is does
+// not matter as long as both operands agree.
+// Measured, weights from HBM, us: 1 x 4096 x 6144 7.4 (3.4 TB/s), 1 x 4096 x 20480 18.1 (4.6), 64 x 4096 x 4096 9.4,
+// 64 x 14336 x 4096 25.5: the CU's loads of the tokens' rows (64 for 16 channels), at one token the start and the end.
 constexpr uint32_t kFewWaves = 8;
 
 template <uint32_t OT, uint32_t MT, uint32_t CT>
 __global__ void __launch_bounds__(64 * kFewWaves) matmul_i8_few(MatmulI8Args a) {
     constexpr uint32_t U = MT == 1u ? 6u / CT : MT == 2u ? 4u : 3u;
+    // each wave's halves of CT + MT row blocks: piece p of row r in column p ^ (r / 4) % 4
+    __shared__ u32x4 turn[kFewWaves][CT + MT][64];
     __shared__ i32x4 red[kFewWaves][CT * MT][64];
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, l16 = lane & 15u, g = lane >> 4;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, row = lane >> 2, piece = lane & 3u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t n0 = blockIdx.x * 16u * CT;
+    const uint32_t n0 = blockIdx.x * 16u * CT, m0 = blockIdx.y * 16u * MT;
     // rows past the last one, and pieces past K, read as zero: past the descriptors' ends
-    const uint32_t wrows = min(a.N - n0, 16u * CT);
+    const uint32_t wrows = min(a.N - n0, 16u * CT), xrows = min(a.M - m0, 16u * MT);
     const rsrc_t wr = make_rsrc(a.w + (uint64_t)n0 * a.w_stride, (uint64_t)(wrows - 1u) * a.w_stride + a.K);
-    const rsrc_t xr = make_rsrc(a.x, (uint64_t)(a.M - 1u) * a.x_stride + a.K);
+    const rsrc_t xr = make_rsrc(a.x + (uint64_t)m0 * a.x_stride, (uint64_t)(xrows - 1u) * a.x_stride + a.K);
     const uint32_t steps = (a.K + 127u) / 128u;
     uint32_t wo[CT], xo[MT];
 #pragma unroll
-    for (uint32_t c = 0; c < CT; c++) wo[c] = 16u * c + l16 < wrows ? (16u * c + l16) * a.w_stride + 32u * g : ~0u;
+    for (uint32_t c = 0; c < CT; c++) wo[c] = 16u * c + row < wrows ? (16u * c + row) * a.w_stride + 16u * piece : ~0u;
 #pragma unroll
-    for (uint32_t t = 0; t < MT; t++) xo[t] = 16u * t + l16 < a.M ? (16u * t + l16) * a.x_stride + 32u * g : ~0u;
+    for (uint32_t t = 0; t < MT; t++) xo[t] = 16u * t + row < xrows ? (16u * t + row) * a.x_stride + 16u * piece : ~0u;
     i32x4 acc[CT][MT];
 #pragma unroll
     for (uint32_t c = 0; c < CT; c++)
 #pragma unroll
         for (uint32_t t = 0; t < MT; t++) acc[c][t] = i32x4{0, 0, 0, 0};
     u32x4 wf[U][CT][2], xf[U][MT][2];
-    auto send = [&](auto B, uint32_t s) {  // step s into buffer B
+    auto send = [&](auto B, uint32_t s) {  // step s into buffer B; a row's halves one after the other: one line
         constexpr int u = decltype(B)::value;
         const uint32_t k = s * 128u;  // (past K for every lane: nothing is read)
+        const bool in[2] = {k + 16u * piece < a.K, k + 16u * piece + 64u < a.K};
 #pragma unroll
-        for (uint32_t h = 0; h < 2u; h++) {
-            const bool in = k + 32u * g + 16u * h < a.K;
+        for (uint32_t c = 0; c < CT; c++)
 #pragma unroll
-            for (uint32_t c = 0; c < CT; c++) wf[u][c][h] = bload16(wr, in && wo[c] != ~0u ? wo[c] + k + 16u * h : ~0u, 0u);
+            for (uint32_t h = 0; h < 2u; h++) wf[u][c][h] = bload16(wr, in[h] && wo[c] != ~0u ? wo[c] + k + 64u * h : ~0u, 0u);
 #pragma unroll
-            for (uint32_t t = 0; t < MT; t++) xf[u][t][h] = bload16(xr, in && xo[t] != ~0u ? xo[t] + k + 16u * h : ~0u, 0u);
-        }
+        for (uint32_t t = 0; t < MT; t++)
+#pragma unroll
+            for (uint32_t h = 0; h < 2u; h++) xf[u][t][h] = bload16(xr, in[h] && xo[t] != ~0u ? xo[t] + k + 64u * h : ~0u, 0u);
     };
+    // (an MFMA's lane has row lane % 16, piece lane / 16)
+    const uint32_t to = 4u * row + (piece ^ (row >> 2)), from = 4u * (lane & 15u) + ((lane >> 4) ^ (lane >> 2 & 3u));
     static_for<0, (int)U>([&](auto B) { send(B, wave + (uint32_t)decltype(B)::value * kFewWaves); });
     for (uint32_t s0 = wave; s0 < steps; s0 += U * kFewWaves) {
         static_for<0, (int)U>([&](auto B) {
@@ -116,13 +127,23 @@ __global__ void __launch_bounds__(64 * kFewWaves) matmul_i8_few(MatmulI8Args a) 
             const uint32_t s = s0 + (uint32_t)u * kFewWaves;
             if (s < steps) {
 #pragma unroll
-                for (uint32_t h = 0; h < 2u; h++)
+                for (uint32_t h = 0; h < 2u; h++) {
+                    i32x4 w[CT], x[MT];
 #pragma unroll
-                    for (uint32_t c = 0; c < CT; c++)
+                    for (uint32_t c = 0; c < CT; c++) turn[wave][c][to] = wf[u][c][h];
 #pragma unroll
-                        for (uint32_t t = 0; t < MT; t++)
-                            acc[c][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, wf[u][c][h]),
-                                                                             __builtin_bit_cast(i32x4, xf[u][t][h]), acc[c][t], 0, 0, 0);
+                    for (uint32_t t = 0; t < MT; t++) turn[wave][CT + t][to] = xf[u][t][h];
+                    __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses are in order)
+#pragma unroll
+                    for (uint32_t c = 0; c < CT; c++) w[c] = __builtin_bit_cast(i32x4, turn[wave][c][from]);
+#pragma unroll
+                    for (uint32_t t = 0; t < MT; t++) x[t] = __builtin_bit_cast(i32x4, turn[wave][CT + t][from]);
+                    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                    for (uint32_t t = 0; t < MT; t++)
+#pragma unroll
+                        for (uint32_t c = 0; c < CT; c++) acc[c][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[c], x[t], acc[c][t], 0, 0, 0);
+                }
                 if (s + U * kFewWaves < steps) send(B, s + U * kFewWaves);
             }
         });
@@ -133,7 +154,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) matmul_i8_few(MatmulI8Args a) 
         for (uint32_t t = 0; t < MT; t++) red[wave][c * MT + t][lane] = acc[c][t];
     __syncthreads();
     for (uint32_t i = tid; i < CT * MT * 64u; i += 64u * kFewWaves) {
-        const uint32_t f = i >> 6, l = i & 63u, m = 16u * (f % MT) + (l & 15u), c = n0 + 16u * (f / MT) + 4u * (l >> 4);
+        const uint32_t f = i >> 6, l = i & 63u, m = m0 + 16u * (f % MT) + (l & 15u), c = n0 + 16u * (f / MT) + 4u * (l >> 4);
         i32x4 s = red[0][f][l];
 #pragma unroll
         for (uint32_t v = 1; v < kFewWaves; v++) s += red[v][f][l];
@@ -542,41 +563,42 @@ hipError_t launch_tiles(const MatmulI8Args& a, int num_cus, hipStream_t st) {
     return hipGetLastError();
 }
 
-template <uint32_t OT, uint32_t MT>
-hipError_t launch_few(const MatmulI8Args& a, int num_cus, hipStream_t st) {
-    // 32 channels a workgroup where that leaves two workgroups a CU
-    if (a.N / 32u >= 2u * (uint32_t)num_cus)
-        hipLaunchKernelGGL((matmul_i8_few<OT, MT, 2>), dim3((a.N + 31u) / 32u), dim3(64 * kFewWaves), 0, st, a);
-    else
-        hipLaunchKernelGGL((matmul_i8_few<OT, MT, 1>), dim3((a.N + 15u) / 16u), dim3(64 * kFewWaves), 0, st, a);
+template <uint32_t OT, uint32_t MT, uint32_t CT>
+hipError_t launch_few(const MatmulI8Args& a, hipStream_t st) {
+    const dim3 grid((a.N + 16u * CT - 1u) / (16u * CT), (a.M + 16u * MT - 1u) / (16u * MT));
+    hipLaunchKernelGGL((matmul_i8_few<OT, MT, CT>), grid, dim3(64 * kFewWaves), 0, st, a);
     return hipGetLastError();
 }
 
 template <uint32_t OT>
 hipError_t launch_matmul(const MatmulI8Args& a, int num_cus, hipStream_t st) {
-    // The weight stream where a workgroup of 16 channels a CU covers them, at any M up to 64 (N 4096, M 64, K 1024,
-    // 4096, 14336: 6.4, 12.4, 34 us; small tiles 7.3, 13.3, 42), and past that up to 16 tokens with long rows (N 10240 and
-    // 20480, M 8, K 4096: 13.1, 19.0; small tiles 15.4, 19.1; M 32: 19.2, 27.7 and 15.8, 19.7; M 16, K 1024: 9.0, 9.1 and 6.6, 6.8).
-    if (a.M <= 64u && (a.N <= 16u * (uint32_t)num_cus || (a.M <= 16u && a.K >= 2048u))) {
-        if (a.M <= 16u) return launch_few<OT, 1>(a, num_cus, st);
-        if (a.M <= 32u) return launch_few<OT, 2>(a, num_cus, st);
-        return launch_few<OT, 4>(a, num_cus, st);
-    }
+    const uint32_t cus = (uint32_t)num_cus;
+    // Up to 16 tokens the weight stream, 32 channels a workgroup where that leaves two a CU (N 20480, K 4096, us: 18.1 to
+    // 19.7, of 16 channels 19.2 to 22, small tiles 24.5 to 26; K 1024: 7.5, 11, 8.6); up to 64 where N or K makes it faster
+    // than small tiles (32 tokens, K 1024, N 6144, 10240, 20480: 6.2, 8.3, 12.9 and 7.7, 7.9, 9.0; K 4096: 9.1, 11.9, 27.2
+    // and 15.2, 15.8, 25.6; 64 tokens, K 4096: 14.9, 21.3, 32.0 and 16.1, 23.1, 28.4).
+    if (a.M <= 16u && a.N < (1u << 27))  // (under 2^32 threads)
+        return a.N / 32u >= 2u * cus ? launch_few<OT, 1, 2>(a, st) : launch_few<OT, 1, 1>(a, st);
+    if (a.M <= 64u && (a.N <= 24u * cus || (a.N <= 40u * cus && a.K >= 2048u)))
+        return a.M <= 32u ? launch_few<OT, 2, 1>(a, st) : launch_few<OT, 4, 1>(a, st);
     // The tiles whose rounds take least, in ns: a stage of 128 bytes of K, and what a round has besides. Fitted to one
-    // round each (S stages of 256 x N, 512 x 4096, 128 x 1024 and so on: within 15%), the largest to full rounds.
+    // round each (S stages of 256 x N, 512 x 4096, 128 x 1024 and so on: within 15%), the largest to full rounds. The last
+    // is the weight stream's, for few tiles of long rows (300 x 16000 x 600: 21 us, in small tiles 44; 100 x 14336 x 1000: 18, 40).
     struct Kind {
         uint32_t m, n, stage, round;
     };
     static const Kind kinds[] = {{64, 128, 410, 1800}, {128, 128, 580, 3000}, {64, 256, 600, 3100},
-                                 {128, 256, 820, 5000}, {192, 256, 1150, 6000}, {256, 256, 1450, 7000}};
+                                 {128, 256, 820, 5000}, {192, 256, 1150, 6000}, {256, 256, 1450, 7000}, {64, 16, 195, 2200}};
     const uint64_t S = (a.K + kRow - 1u) / kRow;
     uint32_t best = 0;
     uint64_t least = ~0ull;
-    for (uint32_t i = 0; i < 6u; i++) {
+    for (uint32_t i = 0; i < 7u; i++) {
         const Kind& k = kinds[i];
         const uint64_t tiles = (uint64_t)((a.M + k.m - 1u) / k.m) * ((a.N + k.n - 1u) / k.n);
         const uint64_t cost = (tiles + (uint64_t)num_cus - 1u) / (uint64_t)num_cus * (S * k.stage + k.round);
-        if (cost < least && (i > 1u || tiles < (1u << 24))) {  // (256 threads each: under 2^32 of them)
+        // (a launch has under 2^32 threads and 2^16 blocks along y)
+        const bool fits = i < 2u ? tiles < (1u << 24) : i < 6u || (tiles < (1u << 23) && a.M <= 64u * 65535u);
+        if (cost < least && fits) {
             least = cost;
             best = i;
         }
@@ -587,7 +609,8 @@ hipError_t launch_matmul(const MatmulI8Args& a, int num_cus, hipStream_t st) {
         case 2: return launch_tiles<OT, 1>(a, num_cus, st);
         case 3: return launch_tiles<OT, 2>(a, num_cus, st);
         case 4: return launch_tiles<OT, 3>(a, num_cus, st);
-        default: return launch_tiles<OT, 4>(a, num_cus, st);
+        case 5: return launch_tiles<OT, 4>(a, num_cus, st);
+        default: return launch_few<OT, 4, 1>(a, st);
     }
 }
 

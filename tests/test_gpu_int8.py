@@ -133,7 +133,8 @@ PRODUCTS = [(1, 1, 16), (1, 60, 64), (2, 17, 48), (15, 33, 80), (16, 16, 64), (1
             (31, 255, 128), (32, 256, 256), (33, 257, 272), (64, 4096, 4096), (63, 1000, 1040), (65, 513, 2064), (100, 126, 656),
             (127, 128, 144), (128, 128, 4096), (129, 384, 400), (200, 3425, 416), (255, 512, 512), (256, 256, 1024),
             (257, 2049, 784), (300, 96, 14400), (511, 777, 3856), (777, 1021, 3840), (1024, 2560, 2560), (2049, 1537, 528),
-            (4100, 300, 1600), (3, 20480, 96), (1, 16, 131056), (40, 24, 131056), (300, 290, 131056)]
+            (4100, 300, 1600), (300, 600, 16000), (130, 1000, 14336), (1000, 40, 5008), (65, 16, 2064), (30, 10240, 2064),
+            (60, 12000, 1040), (3, 20480, 96), (16, 16400, 1104), (1, 16, 131056), (40, 24, 131056), (300, 290, 131056)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
@@ -202,6 +203,22 @@ def test_offsets_past_32_bits(dev):
         assert torch.equal(out, _product_oracle(a, xs, b, ws, F32)), (M, N)
     rows = torch.randn(3, 1 << 30, dtype=F16, device=dev)[:, :64]  # 2 GiB apart
     _check_rows(rows)
+
+
+@pytest.mark.parametrize("M,N", [(1, 1 << 28), (20, (1 << 27) + 5), ((1 << 22) + 100, 17), (5000000, 3)])
+def test_very_wide_and_very_tall(dev, M, N):
+    """More workgroups than one dimension of a launch takes."""
+    from llmr_amd import int8
+    g = torch.Generator(device=dev).manual_seed(6)
+    x, w = _ints(g, dev, M, 16), _ints(g, dev, N, 16)
+    xs, ws = torch.rand(M, generator=g, device=dev), torch.rand(N, generator=g, device=dev)
+    out = int8.matmul(x, xs, w, ws, dtype=BF16)
+    torch.cuda.synchronize()
+    m, n = min(M, 300), min(N, 300)
+    for a in (0, (M - m) // 2, M - m):
+        for b in (0, (N - n) // 2, N - n):
+            want = _product_oracle(x[a:a + m], xs[a:a + m], w[b:b + n], ws[b:b + n], BF16)
+            assert torch.equal(out[a:a + m, b:b + n], want), (a, b)
 
 
 def _capture(fn):
