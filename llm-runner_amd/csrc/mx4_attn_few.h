@@ -8,14 +8,24 @@
 //  - a worker is a workgroup of four waves that take its units in turn and add up their rows in
 //    LDS at a pair's end. With a wave a worker, as many waves as the short rows need would leave
 //    four times the parts to join;
-//  - keys and values come into registers, a unit ahead: a lane has a quarter of a key's row (a
-//    block of 32, at head_dim 128), which is what its products with the queries take if the dims
-//    are dealt out so (lane group g: dims D/4 g ..; the queries alike), so that keys need no LDS;
+//  - keys and values come into registers, two units on their way, each register asked for again as
+//    soon as it is free (4 x 131000..40000 keys 88 -> 80 us), past the caches: a step reads a cache
+//    once. The rows' addresses are made for 32 units at once, a half of a unit a lane;
+//  - a lane has a quarter of a key's row (a block of 32, at head_dim 128), which is what its
+//    products with the queries take if the dims are dealt out so (lane group g: dims D/4 g ..; the
+//    queries alike), so that keys need no LDS. Values pass through LDS in any case: four lanes side
+//    by side have one row, a quarter of the addresses to look up (4 x 131000..40000 keys at head_dim
+//    64 54 -> 48 us; the keys alike, by a way through LDS of their own: 49);
 //  - v_cvt_scalef32_pk_{bf16,f16}_fp4 turns two numbers and their power of two into 16-bit values,
-//    exactly, at the rate of an f32 fma: a unit's 8192 elements are 128 instructions. The values
-//    are written to LDS as 16-bit rows and read transposed.
+//    exactly, at the rate of an f32 fma: a unit's 8192 elements are 64 instructions a wave. The
+//    values are written to LDS as 16-bit rows and read transposed.
 // S^T = K Q^T and O^T += V^T P^T by 16x16x32 MFMAs, the softmax and the treatment of masked keys
-// as in paged_attn_few.
+// as in paged_attn_few: scores, maxima, sums and O are f32; P is rounded to the values' type for
+// its product, as the MFMA takes it.
+// Measured in a graph, us, floors by bytes: 4 x 131000..40000 keys of 8 heads of 128, one token
+// each 79 (71.6 at a large copy's rate: 4.7 TB/s), eight 100; 64 x 100..12000 keys of 6 heads 37
+// (24.3); one of 1100 keys 10.7 (two launches and a pair's start). Bound by HBM at long contexts,
+// at short ones by the workers' starts, the last of them, and the join.
 #pragma once
 
 #include "seq_attn_few.h"
@@ -64,6 +74,7 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
     constexpr int ND = D / 32, DT = D / 16;
     constexpr float OFF = T == kGgmlF16 ? 7.0f : 0.0f;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, n16 = lane & 15u, g = lane >> 4;
+    const uint32_t vrow = lane >> 2, vg = lane & 3u;  // of V's loads
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t G = a.n_heads / a.n_kv_heads;
     const float c = a.scale_log2, grow_by = 8.0f / c;
@@ -81,14 +92,15 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
     uint64_t at = part_begin(blockIdx.x, w, n);
     const uint64_t end = part_begin(blockIdx.x + 1u, w, n);
 
-    const uint32_t kvo = n16 * ROW4 + g * CB, so = n16 * SROW + (D == 128u ? g : g >> 1);
+    const uint32_t ko = n16 * ROW4 + g * CB, kso = n16 * SROW + (D == 128u ? g : g >> 1);
+    const uint32_t vo = vrow * ROW4 + vg * CB, vso = vrow * SROW + (D == 128u ? vg : vg >> 1);
     uint8_t* const vt = lds + wave * TILE;
     const uint32_t vt0 = (uint32_t)(uintptr_t)(lds_void*)vt;
     // V's tile: chunk q of key r at q ^ fswz(r), fswz even: chunk 2 dt + x of a row is at A ^ 32 dt, and chunk ND g + e
     // at B ^ 16 e
     const uint32_t vr0 = 4u * g + (n16 >> 2);
     uint32_t va = vr0 * ROW + ((((n16 & 3u) >> 1) ^ fswz<D>(vr0)) << 4) + 8u * (n16 & 1u);
-    uint32_t vb = n16 * ROW + (((ND * g) ^ fswz<D>(n16)) << 4);
+    uint32_t vb = vrow * ROW + (((ND * vg) ^ fswz<D>(vrow)) << 4);
 
     uint64_t base;
     uint32_t s = find_request(a, win, lane, cost, a.n_kv_heads, at, base);
@@ -150,7 +162,7 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
                 x.row[h] = hi32 >= 0 ? (uint64_t)(uint32_t)hi32 << 32 | lo32 : 0ull;
             }
         };
-        auto load = [&](Half4<D>& x, const Mx4Unit<D>& at, const void* base, const uint8_t* scales) {
+        auto load = [&](Half4<D>& x, const Mx4Unit<D>& at, const void* base, const uint8_t* scales, uint32_t kvo, uint32_t so) {
 #pragma unroll
             for (uint32_t h = 0; h < 2u; h++) {
                 const uint8_t* const p = (const uint8_t*)base + at.row[h] * ROW4;
@@ -179,12 +191,12 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
                 const uint32_t last = rq.keys - u * kUnit;  // (of keys; this unit has some, or the part has none at all)
 #pragma unroll
                 for (uint32_t h = 0; h < 2u; h++) {
-                    const bool is = on[h] && 16u * h + n16 < last;
+                    const bool is = on[h] && 16u * h + vrow < last;
                     const bool bad = is && x.v.power[h] > kTopPower;
                     for (uint64_t b = __builtin_amdgcn_ballot_w64(bad); b != 0; b &= b - 1u) {
                         const uint32_t l = (uint32_t)__builtin_ctzll(b);
-                        const int32_t key = (int32_t)(u * kUnit + 16u * h + (l & 15u));
-                        const uint32_t block = D == 128u ? l >> 4 : l >> 5;
+                        const int32_t key = (int32_t)(u * kUnit + 16u * h + (l >> 2));
+                        const uint32_t block = D == 128u ? l & 3u : (l & 3u) >> 1;
 #pragma unroll
                         for (int r = 0; r < (int)NR; r++)
 #pragma unroll
@@ -210,7 +222,7 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
             const bool more = i + 2u < count;
             if (more) {
                 place(x, i + 2u);
-                load(x.v, x, a.v, m4.v_scales);
+                load(x.v, x, a.v, m4.v_scales, vo, vso);
             }
             f32x4 sc[NR][2];
 #pragma unroll
@@ -224,7 +236,7 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
                         sc[r][kb] = mfma16<T>(k, qf[r][ch], ch == 0 ? nm[r] : sc[r][kb]);
                 }
             }
-            if (more) load(x.k, x, a.k, m4.k_scales);
+            if (more) load(x.k, x, a.k, m4.k_scales, ko, kso);
             s16x8 pf[NR];
 #pragma unroll
             for (int r = 0; r < (int)NR; r++) {
@@ -287,8 +299,8 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
             Mx4Unit<D> x, y;
             auto first = [&](Mx4Unit<D>& z, uint32_t i) {
                 place(z, i);
-                load(z.v, z, a.v, m4.v_scales);
-                load(z.k, z, a.k, m4.k_scales);
+                load(z.v, z, a.v, m4.v_scales, vo, vso);
+                load(z.k, z, a.k, m4.k_scales, ko, kso);
             };
             first(x, 0);
             if (count > 1u) first(y, 1u);
