@@ -544,7 +544,9 @@ paged_attn_few(SeqAttnArgs a, JoinRecord* __restrict__ records, float* __restric
 // Parts of 16 rows come from many waves (138 of five rows where one of 20306 keys is the
 // longest of five): 16 rows or shares at a time, eight parts' loads in flight a thread; 56 ->
 // 42 us for that call, 14.0 -> 12.6 for one request of 1100 keys. Larger parts are fewer and
-// have rows enough: with as many threads 24 mixed requests took 43 us for 39.
+// have rows enough: with as many threads 24 mixed requests took 43 us for 39. Eight loads in
+// flight are worth it for parts of 32 rows too (16 x 4 tokens of 28 heads over a 4-bit cache
+// 32.3 -> 31.5).
 template <uint32_t D, uint32_t PR>
 constexpr uint32_t join_threads() { return PR == 16u ? 4u * D : 256u; }
 
@@ -552,7 +554,7 @@ template <uint32_t T, uint32_t D, uint32_t PR>
 __global__ void __launch_bounds__((join_threads<D, PR>()))
 paged_attn_join(SeqAttnArgs a, const JoinRecord* __restrict__ records, const float* __restrict__ parts) {
     constexpr uint32_t LPR = D / 4u, GROUPS = join_threads<D, PR>() / LPR;  // threads of a row, rows or shares at a time
-    constexpr uint32_t LOADS = PR == 16u ? 8u : 4u;  // parts of a thread in flight
+    constexpr uint32_t LOADS = PR <= 32u ? 8u : 4u;  // parts of a thread in flight
     __shared__ f32x4 so[GROUPS][LPR];
     __shared__ float sm[GROUPS], sl[GROUPS];
     const uint32_t worker = blockIdx.y, x0 = 16u * blockIdx.x;
