@@ -717,7 +717,9 @@ LLMR_API size_t llmr_paged_attention_scratch_bytes(llmr_context* ctx, const llmr
  * page_size, head_dim / 2]: byte i of a row holds element 2i in its low half and
  * 2i + 1 in its high one; scales [n_pages, n_kv_heads, page_size, head_dim / 32]:
  * exponent + 127, 255 for a block that is NaN. Both 16-byte aligned. A key takes
- * head_dim * 17 / 32 bytes where F16 takes 2 * head_dim. */
+ * head_dim * 17 / 32 bytes where F16 takes 2 * head_dim. llmr_qkv_tokens_mx4 writes
+ * exponents in [-23, 13]; a larger one put there by other means may read as
+ * infinite or NaN, a smaller one as rounded to the reader's type. */
 typedef struct llmr_mx4_cache {
     void* data;
     void* scales;
@@ -781,7 +783,7 @@ typedef struct llmr_quantize_rows_params {
  *   scales[r] = a / 127, with norm times 1 / sqrt(sum x^2 / dim + eps)
  * so that scales[r] * q[r, k] stands for x, or for its RMS norm
  * (llmr_batch_rmsnorm's; the norm's size only enters the scale). 64-bit
- * arithmetic, scales rounded once. A row with an infinity or NaN has q = 0 and
+ * arithmetic, scales rounded once (below 2^-149 to 0). A row with an infinity or NaN has q = 0 and
  * scale NaN. Weights [out_dim, in_dim] get their scales a channel by the same call
  * without norm. q and scales overlap no other array. */
 LLMR_API int llmr_quantize_rows_i8(llmr_context* ctx, const void* x, const float* norm, int8_t* q, float* scales,

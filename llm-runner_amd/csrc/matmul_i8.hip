@@ -453,7 +453,6 @@ __global__ void __launch_bounds__(256, 1) matmul_i8_tiles(MatmulI8Args a, uint32
 // Tiles of 64 MB tokens x 128 channels, one a workgroup, for launches that large tiles leave most CUs without: four
 // waves in 2 x 2 of 32 MB x 64, stages of 128 bytes of K in four LDS slots, sent for three stages ahead (a stage
 // takes less than its loads' way from L2 and memory).
-constexpr int kSmallSlots = 4;
 
 template <uint32_t OT, uint32_t MB>
 __global__ void __launch_bounds__(256, 1) matmul_i8_small(MatmulI8Args a, uint32_t tiles_m) {

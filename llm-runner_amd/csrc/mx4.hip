@@ -6,6 +6,9 @@
 // e + 2 the exponent of the largest |x| rounded to two significant bits: the largest is
 // then 3.5 to 7 times 2^e, as far from 6 as rounding to a neighbour would put it. With
 // e + 2 its plain exponent it would be up to 8 and lose a quarter.
+//
+// Bound by memory: 8192 tokens of 32/8 heads of 128 with norms and rotation 55 us (272 MB:
+// 4.9 TB/s), as many rows read back 10.5; 64 tokens 3.6 and 2.5, a launch each.
 #include "llmr_device.h"
 #include "llmr_internal.h"
 
