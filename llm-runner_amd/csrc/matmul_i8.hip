@@ -133,12 +133,12 @@ __global__ void __launch_bounds__(64 * kFewWaves) matmul_i8_few(MatmulI8Args a) 
                     for (uint32_t c = 0; c < CT; c++) turn[wave][c][to] = wf[u][c][h];
 #pragma unroll
                     for (uint32_t t = 0; t < MT; t++) turn[wave][CT + t][to] = xf[u][t][h];
-                    __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses are in order)
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (a wave's LDS accesses run in order)
 #pragma unroll
                     for (uint32_t c = 0; c < CT; c++) w[c] = __builtin_bit_cast(i32x4, turn[wave][c][from]);
 #pragma unroll
                     for (uint32_t t = 0; t < MT; t++) x[t] = __builtin_bit_cast(i32x4, turn[wave][CT + t][from]);
-                    __builtin_amdgcn_wave_barrier();
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
                     for (uint32_t t = 0; t < MT; t++)
 #pragma unroll
