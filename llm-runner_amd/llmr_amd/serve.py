@@ -170,19 +170,24 @@ def _rope(rope, D: int):
     if rope is None:
         return None, None, 0
     cos, sin = rope
-    if cos.dim() != 2 or cos.shape[1] != D // 2 or sin.shape != cos.shape or cos.shape[0] == 0:
+    shape = cos.shape
+    if len(shape) != 2 or shape[1] != D // 2 or sin.shape != shape or shape[0] == 0:
         raise ValueError("rope must be (cos, sin) of [n_positions, head_dim / 2], n_positions >= 1")
-    return cos, sin, cos.shape[0]
+    return cos, sin, shape[0]
 
 
 def _qkv_rows(qkv: torch.Tensor, q: torch.Tensor):
     """q's tokens, heads, head_dim and token stride, and qkv's row stride."""
-    if qkv.dim() != 2 or qkv.dtype is not _F32 or (qkv.shape[1] > 1 and qkv.stride(1) != 1) or qkv.stride(0) > _U32:
+    strides = qkv.stride()
+    if len(strides) != 2 or qkv.dtype is not _F32:
+        raise ValueError("qkv must be a 2-D f32 view with contiguous rows, under 2^32 apart")
+    Tq, width = qkv.shape
+    if (width > 1 and strides[1] != 1) or strides[0] > _U32:
         raise ValueError("qkv must be a 2-D f32 view with contiguous rows, under 2^32 apart")
     T, H, D, qs, qh = _heads(q, "q")
-    if qkv.shape[0] != T or qh != D:
+    if Tq != T or qh != D:
         raise ValueError("q must be [tokens, n_heads, head_dim] with qkv's tokens and heads side by side")
-    return T, H, D, qs, qkv.stride(0) if T > 1 else qkv.shape[1] + -qkv.shape[1] % 4
+    return T, H, D, qs, strides[0] if T > 1 else width + -width % 4
 
 
 def qkv_tokens(qkv: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -289,7 +294,8 @@ def _mx4(k: Mx4Cache, v: Mx4Cache):
             kd.is_contiguous() and ks.is_contiguous() and vd.is_contiguous() and vs.is_contiguous()):
         raise ValueError("the caches' data and scales must be contiguous uint8 tensors of four dimensions")
     n, h, page, half = shape
-    if vd.shape != shape or half % 16 or ks.shape != (n, h, page, half // 16) or vs.shape != ks.shape:
+    of_scales = (n, h, page, half // 16)
+    if half % 16 or vd.shape != shape or ks.shape != of_scales or vs.shape != of_scales:
         raise ValueError("the caches must be [n_pages, n_kv_heads, page_size, head_dim / 2] with scales [.., head_dim "
                          "/ 32], alike")
     return n, h, page, 2 * half, capi.Mx4Cache(kd.data_ptr(), ks.data_ptr()), capi.Mx4Cache(vd.data_ptr(), vs.data_ptr())
