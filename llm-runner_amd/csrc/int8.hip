@@ -6,7 +6,7 @@
 // rows past 16384 elements are read twice. The definition is in 64 bits, so that q does
 // not depend on an order or a contraction; f32 rounds where it provably gives the same
 // (round8). Bound by memory: 8192 x 3840 bf16 19.6 us (4.8 TB/s), 8192 x 4096 f32 with
-// the norm 31 (5.4), 8192 x 10240 f32 with the norm 104 (4.0: 16 waves a CU,
+// the norm 31 (5.4), 8192 x 10240 f32 with the norm 103 (4.1: 16 waves a CU,
 // whose sums and roundings do not hide all of their loads); one row of 4096
 // 3.4 to 4.1, a launch and two dependent loads.
 #include "llmr_device.h"
@@ -166,9 +166,14 @@ __global__ void __launch_bounds__(row_threads<TPR>()) quantize_rows_kernel(Quant
         Eight<XT> e[NV];
         float v[8], w[8];
         RowSums s{0.0, 0.0, 0u};
-        // (the norm's weights are read twice, from L2: held, they would halve the rows a CU has on their way)
-        auto weights = [&](uint32_t k) {
-            if constexpr (NORM) {
+        // the norm's weights are held where that leaves rows enough on their way, and read twice, from L2, where
+        // the pieces are more (8192 x 4096 f32: held 31.4 us, read twice 33.4; one row 4.0, 4.15)
+        constexpr bool HELD = NORM && NV <= 2u;
+        Eight<kGgmlF32> held[HELD ? NV : 1u];
+        auto weights = [&](uint32_t c, uint32_t k) {
+            if constexpr (HELD) {
+                held[c].values(w);
+            } else if constexpr (NORM) {
                 Eight<kGgmlF32> n;
                 n.load(a.norm + k);
                 n.values(w);
@@ -177,13 +182,16 @@ __global__ void __launch_bounds__(row_threads<TPR>()) quantize_rows_kernel(Quant
 #pragma unroll
         for (uint32_t c = 0; c < NV; c++) {
             const uint32_t k = 8u * (t + TPR * c);
-            if (k < a.dim) e[c].load(x + (uint64_t)k * XS);
+            if (k < a.dim) {
+                e[c].load(x + (uint64_t)k * XS);
+                if constexpr (HELD) held[c].load(a.norm + k);
+            }
         }
 #pragma unroll
         for (uint32_t c = 0; c < NV; c++) {
             const uint32_t k = 8u * (t + TPR * c);
             if (k < a.dim) {
-                weights(k);
+                weights(c, k);
                 e[c].values(v);
                 add8<NORM>(s, v, w);
             }
@@ -196,7 +204,7 @@ __global__ void __launch_bounds__(row_threads<TPR>()) quantize_rows_kernel(Quant
         for (uint32_t c = 0; c < NV; c++) {
             const uint32_t k = 8u * (t + TPR * c);
             if (k < a.dim) {
-                weights(k);
+                weights(c, k);
                 e[c].values(v);
                 *(u32x2*)(q + k) = round8<NORM>(sc, v, w);
             }
