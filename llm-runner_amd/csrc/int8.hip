@@ -47,12 +47,15 @@ struct Eight {
 constexpr uint32_t kRowThreads = 256;
 
 // 127 y / a to the nearest whole number, ties to even; r = 127 / a. Where y r is next to a half, the
-// half is compared with exactly (f16 and bf16 rows do have elements there).
+// half is compared with exactly: d is the sign of 254 |y| - (2 k + 1) a. a is a product of up to 48 bits
+// and (2 k + 1) a has up to 56, so its low part is kept; the differences are small and whole multiples
+// of y's last bit, so both are exact. (Rows have such elements: half of the largest one is 63.5.)
 __device__ __forceinline__ int round127(double y, double r, double a) {
     const double v = y * r, q = rint(v);
     int n = (int)q;
     if (fabs(fabs(v - q) - 0.5) < 1e-9) {
-        const double k = floor(fabs(v)), d = fma(254.0, fabs(y), -(2.0 * k + 1.0) * a);
+        const double k = floor(fabs(v)), h = 2.0 * k + 1.0, p = h * a;
+        const double d = fma(254.0, fabs(y), -p) - fma(h, a, -p);
         const int lo = (int)k;
         const int m = d > 0.0 ? lo + 1 : d < 0.0 ? lo : lo + (lo & 1);
         n = v < 0.0 ? -m : m;

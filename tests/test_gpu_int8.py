@@ -77,6 +77,51 @@ def test_quantize_rows_ties(dev, dtype):
     _check_rows(torch.ldexp(x, torch.tensor(-130, device=dev)))  # among the subnormals
 
 
+def _exact_rows(x, norm):
+    """q from the definition in whole fractions: 127 y / a to nearest, ties to even, for rows on the host."""
+    from fractions import Fraction
+    out = []
+    for row in x.tolist():
+        y = [Fraction(a) * Fraction(b) for a, b in zip(row, norm.tolist())]
+        a = max(map(abs, y))
+        out.append([round(127 * v / a) if a else 0 for v in y])
+    return torch.tensor(out, dtype=torch.int8)
+
+
+@pytest.mark.parametrize("K", [528, 16400])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+def test_quantize_rows_ties_under_a_norm(dev, dtype, K):
+    """Halves of rows with a norm whose weights have all of f32's bits: (2 k + 1) m against 254 m, m as long as the type
+    allows, their neighbours, and halves that two weights make. y and a are products of 48 bits, 127 y has 55."""
+    g = torch.Generator().manual_seed(17)
+    bits = {F32: 16, BF16: 1, F16: 4}[dtype]
+    x = torch.zeros(8, K, dtype=F32)
+    norm = torch.rand(K, generator=g) + 0.5
+    k = torch.arange(127, dtype=F32)
+    for i in range(8):
+        m = float(torch.randint(2 ** (bits - 1), 2 ** bits, (), generator=g)) if bits > 1 else 1.0
+        v = ((2 * k + 1) * m).to(dtype).float()
+        x[i, :127], x[i, 127:254] = v, -v
+        x[i, 254:381] = torch.nextafter(v.to(dtype), torch.zeros_like(v, dtype=dtype)).float()
+        x[i, 400] = 254 * m
+        # half the largest by the weight: the element is the largest one's
+        x[i, 401], x[i, K - 1] = 254 * m, -254 * m
+    w = float(norm[0])
+    norm[:401] = w
+    norm[401], norm[K - 1] = w / 2, w / 2
+    x = x.to(dtype)
+    from llmr_amd import int8
+    q, _ = int8.quantize_rows(x.to(dev), norm=norm.to(dev))
+    torch.cuda.synchronize()
+    want = _exact_rows(x.double()[:, :528], norm[:528].double())
+    if K > 528:
+        want[:, 401:] = 0
+        want[:, 401] = 64
+    got = q.cpu()[:, :528]
+    assert torch.equal(got, want), int((got != want).sum())
+    assert bool((want[:, 401] == 64).all()) and bool((q.cpu()[:, K - 1] == -64).all())
+
+
 @pytest.mark.parametrize("norm", [False, True], ids=["plain", "norm"])
 def test_quantize_rows_special_values(dev, norm):
     g = torch.Generator(device=dev).manual_seed(1)
