@@ -718,8 +718,8 @@ LLMR_API size_t llmr_paged_attention_scratch_bytes(llmr_context* ctx, const llmr
  * 2i + 1 in its high one; scales [n_pages, n_kv_heads, page_size, head_dim / 32]:
  * exponent + 127, 255 for a block that is NaN. Both 16-byte aligned. A key takes
  * head_dim * 17 / 32 bytes where F16 takes 2 * head_dim. llmr_qkv_tokens_mx4 writes
- * exponents in [-23, 13]; a larger one put there by other means may read as
- * infinite or NaN, a smaller one as rounded to the reader's type. */
+ * exponents in [-23, 13]; of others, put there by other means, the numbers are rounded
+ * to the reader's type (F16: infinite from 65520 on). */
 typedef struct llmr_mx4_cache {
     void* data;
     void* scales;
@@ -738,10 +738,10 @@ LLMR_API int llmr_qkv_tokens_mx4(llmr_context* ctx, const float* qkv, const floa
                                  const int32_t* slots, void* q, const llmr_mx4_cache* k, const llmr_mx4_cache* v,
                                  const llmr_qkv_tokens_params* params);
 
-/* llmr_paged_attention over such caches: the same requests, pages, rows and
- * scratch rules. q and out of type F16 or BF16; a key or value is what its block
- * stands for, in that type (as llmr_qkv_tokens_mx4 writes them: exactly). The
- * scratch is llmr_paged_attention_mx4_scratch_bytes'. */
+/* llmr_paged_attention over such caches: the same requests, pages, rows, scratch
+ * rules and arithmetic. q and out of type F16 or BF16; a key or value is what its block stands for, in that
+ * type (as llmr_qkv_tokens_mx4 writes them: exactly), wherever it lies in the
+ * context. The scratch is llmr_paged_attention_mx4_scratch_bytes'. */
 LLMR_API int llmr_paged_attention_mx4(llmr_context* ctx, const void* q, const llmr_mx4_cache* k,
                                       const llmr_mx4_cache* v, uint32_t type, void* out, const int32_t* seq_offsets,
                                       const int32_t* kv_len, const int32_t* block_table, void* scratch,

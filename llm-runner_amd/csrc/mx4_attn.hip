@@ -32,16 +32,28 @@ struct Mx4Keys : seqattn::PagedKeys<D / 2u> {
         }
         return x;
     }
-    __device__ __forceinline__ uint32_t nan_blocks(uint32_t j) const {
+    // the cache's row of key j < n_keys (-1: on no page)
+    __device__ __forceinline__ int64_t row_of(uint32_t j) const {
         const uint32_t at = this->key0 + j, p = (uint32_t)this->table[at >> this->log2];
-        uint32_t bits = 0;
-        if (p < this->n_pages) {
-            const uint8_t* const s = v_scales + ((((uint64_t)p * this->n_kv_heads + this->kvh) << this->log2) +
-                                                 (at & ((1u << this->log2) - 1u))) * (D / 32u);
+        return p < this->n_pages ? (int64_t)((((uint64_t)p * this->n_kv_heads + this->kvh) << this->log2) +
+                                             (at & ((1u << this->log2) - 1u)))
+                                 : -1;
+    }
+    __device__ __forceinline__ bool far_value(uint32_t j) const {
+        const int64_t row = row_of(j);
+        bool far = false;
+        if (row >= 0) {
 #pragma unroll
-            for (uint32_t i = 0; i < D / 32u; i++) bits |= s[i] > mx4attn::kTopPower ? 1u << i : 0u;
+            for (uint32_t i = 0; i < D / 32u; i++) far = far || v_scales[row * (D / 32u) + i] > mx4attn::kTopPower;
         }
-        return bits;
+        return far;
+    }
+    template <uint32_t T>
+    __device__ __forceinline__ u32x2 value4(const void* v, uint32_t j, uint32_t dim) const {
+        const int64_t row = row_of(j);
+        const u32x4 w = seqattn::values8<T>(*(const uint16_t*)((const uint8_t*)v + row * (D / 2u) + dim / 2u),
+                                            seqattn::power4(v_scales[row * (D / 32u) + dim / 32u]));
+        return u32x2{w.x, w.y};
     }
 };
 

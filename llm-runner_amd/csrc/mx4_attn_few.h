@@ -39,7 +39,7 @@ using namespace seqattn;
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 
 constexpr uint32_t kWaves = 4;         // of a worker
-constexpr uint32_t kTopPower = 127 + 13;  // of what llmr_qkv_tokens_mx4 writes; above it values may be infinite
+constexpr uint32_t kTopPower = 127 + 13;  // of what llmr_qkv_tokens_mx4 writes; above it values may be infinite, at 255 NaN
 // A pair's units on the line: those of its keys, the first of them kPairStart units more, for what a
 // pair costs a worker (its pages, queries and first rows waited for, its rows added up).
 constexpr uint32_t kPairStart = 12;
@@ -178,32 +178,24 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
                 x.power[h] = *(scales + at.row[h] * SROW + so);
             }
         };
+        bool any_far = false;  // (uniform)
         // unit i, in x; each of its registers is asked for again, for unit i + 2, as soon as it is free
         auto step = [&](Mx4Unit<D>& x, uint32_t i) {
             const uint32_t u = u0 + wave + kWaves * i;
             // keys past the last one, on no page, or unseen by a row: masked
             const bool on[2] = {x.on[0], x.on[1]};
             const bool masked = !on[0] || !on[1] || (int32_t)(u * kUnit + kUnit - 1u) > hi_min;
+            bool far = false;  // V's blocks may hold infinities or NaN
             if (masked) {
                 // a row's weight of a key it does not see is 0, and 0 times an infinity or NaN is NaN: V's rows
-                // of keys that there are not are set to 0, and so are blocks that are not all finite, whose
-                // rows that do see them become NaN at once
+                // of keys that there are not are set to 0 here, and what is not finite in others below; the rows
+                // that do see it get it after the part's last unit
                 const uint32_t last = rq.keys - u * kUnit;  // (of keys; this unit has some, or the part has none at all)
 #pragma unroll
                 for (uint32_t h = 0; h < 2u; h++) {
                     const bool is = on[h] && 16u * h + vrow < last;
-                    const bool bad = is && x.v.power[h] > kTopPower;
-                    for (uint64_t b = __builtin_amdgcn_ballot_w64(bad); b != 0; b &= b - 1u) {
-                        const uint32_t l = (uint32_t)__builtin_ctzll(b);
-                        const int32_t key = (int32_t)(u * kUnit + 16u * h + (l >> 2));
-                        const uint32_t block = D == 128u ? l & 3u : (l & 3u) >> 1;
-#pragma unroll
-                        for (int r = 0; r < (int)NR; r++)
-#pragma unroll
-                            for (int dt = 0; dt < DT; dt++)
-                                if (key <= hi[r] && (uint32_t)dt >> 1 == block) o[r][dt] += __uint_as_float(0x7fc00000u);
-                    }
-                    if (bad || !is) {
+                    far = far || __builtin_amdgcn_ballot_w64(is && x.v.power[h] > kTopPower) != 0;
+                    if (!is) {
                         x.v.power[h] = 0;
 #pragma unroll
                         for (int e = 0; e < ND; e++) x.v.n[h][e] = 0;
@@ -218,6 +210,19 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
 #pragma unroll
                 for (uint32_t h = 0; h < 2u; h++)
                     *(lds_u32x4*)(uintptr_t)(at + h * 16u * ROW) = values8<T>(x.v.n[h][e], power4(x.v.power[h]));
+            }
+            if (far) {
+                any_far = true;
+                uint32_t lo = 0xffffu;  // (opaque: hipcc would keep the masks in registers from the beginning on)
+                asm volatile("" : "+s"(lo));
+#pragma unroll 1
+                for (uint32_t e = 16u * lane; e < TILE; e += 1024u) {
+                    lds_u32x4* const at = (lds_u32x4*)(uintptr_t)(vt0 + e);
+                    u32x4 w = *at;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) w[k] = finite2<T>(w[k], lo);
+                    *at = w;
+                }
             }
             const bool more = i + 2u < count;
             if (more) {
@@ -329,6 +334,38 @@ __device__ __forceinline__ void few_rows(const Mx4Args& m4, uint8_t* lds, JoinRe
             f32x4* const ow = (f32x4*)vt;  // [16][D / 4], chunk q of row x at q ^ x
 #pragma unroll
             for (int dt = 0; dt < DT; dt++) ow[n16 * (D / 4u) + ((4u * dt + g) ^ n16)] = o[r][dt];
+            if (any_far) {  // what masked units hold that is not finite, to the rows that see it
+                uint32_t so = vso;  // (opaque, as above)
+                float inf = INFINITY;
+                asm volatile("" : "+v"(so), "+s"(inf));
+                Mx4Unit<D> z;
+#pragma unroll 1
+                for (uint32_t i = 0; i < count; i++) {
+                    place(z, i);
+                    const uint32_t k0 = (u0 + wave + kWaves * i) * kUnit;
+                    if (z.on[0] && z.on[1] && (int32_t)(k0 + kUnit - 1u) <= hi_min) continue;  // not masked
+#pragma unroll
+                    for (uint32_t h = 0; h < 2u; h++) {
+                        const bool is = z.on[h] && k0 + 16u * h + vrow < rq.keys;
+                        uint64_t b = __builtin_amdgcn_ballot_w64(is && m4.v_scales[z.row[h] * SROW + so] > kTopPower);
+#pragma unroll 1
+                        for (; b != 0; b &= b - 1u) {
+                            const uint32_t l = (uint32_t)__builtin_ctzll(b), d0 = D / 4u * (l & 3u);
+                            const uint64_t row = z.row[h] + (l >> 2);
+                            const float s = power4(m4.v_scales[row * SROW + d0 / 32u]);
+                            if ((int32_t)(k0 + 16u * h + (l >> 2)) > hi[r]) continue;
+#pragma unroll 1
+                            for (uint32_t d = d0 + 4u * g; d < d0 + D / 4u; d += 16u) {
+                                const u32x4 w = values8<T>(*(const uint16_t*)((const uint8_t*)a.v + row * ROW4 + d / 2u), s);
+                                f32x4 v{lo_f32<T>(w.x), hi_f32<T>(w.x), lo_f32<T>(w.y), hi_f32<T>(w.y)};
+#pragma unroll
+                                for (int e = 0; e < 4; e++) v[e] = !(fabsf(v[e]) < inf) ? v[e] : 0.0f;
+                                ow[n16 * (D / 4u) + (d / 4u ^ n16)] += v;
+                            }
+                        }
+                    }
+                }
+            }
             if (g == 0) {
                 ml[wave * 32u + n16] = (fresh >> r) & 1u ? -INFINITY : -nm[r].x;
                 ml[wave * 32u + 16u + n16] = sn ? l : -1.0f;

@@ -76,11 +76,11 @@ __device__ __forceinline__ float hi_f32(uint32_t w) {
     if constexpr (T == kGgmlBF16) return __uint_as_float(w & 0xffff0000u);
     else return (float)__builtin_bit_cast(f16x2, w).y;
 }
-// A dword's halves with 0 in the place of infinities and NaN.
+// A dword's halves with 0 in the place of infinities and NaN. (lo: 0xffff)
 template <uint32_t T>
-__device__ __forceinline__ uint32_t finite2(uint32_t w) {
+__device__ __forceinline__ uint32_t finite2(uint32_t w, uint32_t lo = 0xffffu) {
     constexpr uint32_t E = T == kGgmlBF16 ? 0x7f80u : 0x7c00u;
-    return w & (((w & E) == E ? 0u : 0xffffu) | ((w & (E << 16)) == (E << 16) ? 0u : 0xffff0000u));
+    return w & (((w & E) == E ? 0u : lo) | ((w & (E << 16)) == (E << 16) ? 0u : ~lo));
 }
 // Whether either half of a dword is an infinity or NaN.
 template <uint32_t T>
@@ -150,7 +150,8 @@ struct RowOfLane {
 //   const uint8_t* row(base, j): key j < n_keys's row (null: on no page).
 // kBlocks4: keys and values are blocks of 4-bit numbers; instead of tile, voffset and row
 //   Blocks4<D> fetch(base, scales, t, page, lane): the lane's piece of the wave's keys of tile t,
-//   k_scales, v_scales, and uint32_t nan_blocks(j): bit i: block i of key j < n_keys's value is NaN.
+//   k_scales, v_scales; bool far_value(j): key j < n_keys's value may hold infinities or NaN, and
+//   u32x2 value4<T>(base, j, dim): four of its numbers then, in 16 bits.
 // out_at(): element offset of the lane's row in `out`.
 //
 // A lane's piece of a tile of blocks: key 8 wave + lane / 8, dims D / 8 * (lane % 8) ..
@@ -404,41 +405,36 @@ __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, So
     };
     auto add_bad = [&](uint32_t t) {
         const uint32_t j = t * kKeys + lane;
-        if constexpr (B4) {
-            const uint32_t blocks = j < n_keys ? src.nan_blocks(j) : 0u;
-            for (uint64_t bad = __builtin_amdgcn_ballot_w64(blocks != 0); bad != 0; bad &= bad - 1u) {
-                const int l = __builtin_ctzll(bad), key = (int)(t * kKeys) + l;
-                const uint32_t of = (uint32_t)__builtin_amdgcn_readlane((int)blocks, l);
-                const bool in = key >= row.lo && key <= row.hi;
-#pragma unroll
-                for (int dt = 0; dt < CH; dt++)
-                    if (in && ((of >> dt) & 1u)) o[dt] += __uint_as_float(0x7fc00000u);
-            }
-            return;
-        } else {
         bool n = false;
         if (j < n_keys) {
-            const uint8_t* const vr = src.row(a.v, j);
-            for (uint32_t b = 0; vr && b < CPR; b++) {
-                const u32x4 w = *(const u32x4*)(vr + 16u * b);
-                n = n || nonfinite4<T>(w);
+            if constexpr (B4) {
+                n = src.far_value(j);
+            } else {
+                const uint8_t* const vr = src.row(a.v, j);
+                for (uint32_t b = 0; vr && b < CPR; b++) {
+                    const u32x4 w = *(const u32x4*)(vr + 16u * b);
+                    n = n || nonfinite4<T>(w);
+                }
             }
         }
         for (uint64_t bad = __builtin_amdgcn_ballot_w64(n); bad != 0; bad &= bad - 1u) {
             const uint32_t key = t * kKeys + (uint32_t)__builtin_ctzll(bad);  // < n_keys: a lane found it there
             const bool in = (int)key >= row.lo && (int)key <= row.hi;
-            const uint8_t* const vr = src.row(a.v, key);
+            const uint8_t* vr = nullptr;
+            if constexpr (!B4) vr = src.row(a.v, key);
 #pragma unroll
             for (int dt = 0; dt < CH; dt++)
 #pragma unroll
                 for (int g = 0; g < 4; g++) {
-                    const u32x2 v = *(const u32x2*)(vr + 64u * dt + 16u * g + 8u * kh);
+                    const uint32_t dim = 32u * dt + 8u * g + 4u * kh;
+                    u32x2 v;
+                    if constexpr (B4) v = src.template value4<T>(a.v, key, dim);
+                    else v = *(const u32x2*)(vr + 2u * dim);
                     const float x[4] = {lo_f32<T>(v.x), hi_f32<T>(v.x), lo_f32<T>(v.y), hi_f32<T>(v.y)};
 #pragma unroll
                     for (int e = 0; e < 4; e++)
                         o[dt][4 * g + e] += (int)in & (int)!(fabsf(x[e]) < INFINITY) ? x[e] : 0.0f;
                 }
-        }
         }
     };
 

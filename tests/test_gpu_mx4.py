@@ -479,6 +479,84 @@ def test_nan_values_that_rows_see(dev, D, new):
     _check(got, o, A, e, float(v.nan_to_num(0.0).abs().max()), kv[0], BF16, "beside NaN")
 
 
+# Powers above those that qkv_tokens_mx4 writes (a cache filled by other means): finite in bf16; in fp16 2^14 times 4
+# and 6, and 2^16 times anything but 0, are infinite.
+FAR_POWERS = [141, 143, 160, 200, 230, 255]
+
+
+def _check_infinite(got, out, A, e, v, keys, dtype, what):
+    """_check where values are infinite: those sums are infinite or NaN in the same places."""
+    got = got.double()
+    inf = out.isinf()
+    assert torch.equal(got.isinf(), inf) and torch.equal(got[inf], out[inf]), (what, "infinities in other places")
+    zero = torch.zeros_like(out)
+    _check(torch.where(inf, zero, got), torch.where(inf, zero, out), torch.where(A.isfinite(), A, zero), e,
+           float(v.nan_to_num(0, 0, 0).abs().max()), keys, dtype, what)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new", [1, 5, 20, 100])
+@pytest.mark.parametrize("power", FAR_POWERS)
+def test_values_of_powers_past_the_writers(dev, dtype, D, new, power):
+    """A value block of such a power is the same numbers wherever it lies: deep in the context, next to the last keys, in
+    a new token that some rows see and others do not, and by itself in a context of few keys."""
+    from llmr_amd import serve
+    for past, places in ((3000, (17, 2999, 3000 + new - 1)), (3000, (1234,)), (3000, (3000 + new // 2,)), (4, (2,))):
+        q, kc, vc, rows, at, off, kvl, table, kv = _paged_case(dev, dtype, D, 8, 2, 16, [past], [new], seed=power + new)
+        clean = serve.paged_attention_mx4(q, kc, vc, off, kvl, table, new).clone()
+        v = rows[0][1]
+        for i, row in enumerate(places):
+            head, block = i % 2, (i + 1) % (D // 32)
+            page = int(table[0, row // 16])
+            vc.scales[page, head, row % 16, block] = power
+            v[row, head] = _decode(vc.data[page, head, row % 16], vc.scales[page, head, row % 16])
+        v = v.to(dtype).double()  # the values that mx4_rows reads
+        out = serve.paged_attention_mx4(q, kc, vc, off, kvl, table, new)
+        torch.cuda.synchronize()
+        o, A, e = _definition(q, rows[0][0], v, 1 / math.sqrt(D), past)
+        _check_infinite(out.unflatten(1, (8, D)), o, A, e, v, kv[0], dtype, f"2^{power - 127} at {places} of {kv[0]}")
+        unseen = max(0, min(places) - past)  # rows before the first of them
+        assert torch.equal(out[:unseen], clean[:unseen])
+
+
+@pytest.mark.parametrize("e", [14, 40, 90])
+@pytest.mark.parametrize("new", [1, 3, 50])
+def test_keys_of_powers_past_the_writers(dev, e, new):
+    """Keys of larger powers in bf16, against a scale that leaves their scores as they are."""
+    from llmr_amd import serve
+    q, kc, vc, rows, at, off, kvl, table, kv = _paged_case(dev, BF16, 64, 4, 2, 16, [200], [new], seed=e, poison=False)
+    kc.scales.fill_(e + 127)
+    j = torch.arange(kv[0], device=dev)
+    pages = table[0].long()
+    k = _decode(kc.data[pages[j // 16], :, j % 16], kc.scales[pages[j // 16], :, j % 16])
+    out = serve.paged_attention_mx4(q, kc, vc, off, kvl, table, new, scale=2.0 ** -(e + 3))
+    torch.cuda.synchronize()
+    v = rows[0][1]
+    o, A, err = _definition(q[:new], k, v, 2.0 ** -(e + 3), 200)
+    _check(out[:new].unflatten(1, (4, 64)), o, A, err, float(v.abs().max()), kv[0], BF16, f"2^{e}")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+def test_mx4_rows_of_every_power(dev, dtype):
+    """Each code under each of the 256 powers: its value, rounded to the type (infinite past it)."""
+    from llmr_amd import serve
+    kc, vc = _caches(16, 1, 16, 64, dev)
+    code = torch.arange(64, device=dev) % 16
+    for c in (kc, vc):
+        c.data[:] = (code[::2] | code[1::2] << 4).to(torch.uint8)
+        c.scales[:] = torch.arange(256, device=dev).view(16, 1, 16, 1).to(torch.uint8)
+    ko, vo = (torch.empty(256, 1, 64, dtype=dtype, device=dev) for _ in range(2))
+    serve.mx4_rows(kc, vc, torch.arange(256, dtype=torch.int32, device=dev), ko, vo)
+    torch.cuda.synchronize()
+    n = torch.tensor(NUMBERS + [-x for x in NUMBERS], dtype=torch.float64)
+    s = torch.tensor([2.0 ** (i - 127) for i in range(255)] + [math.nan], dtype=torch.float64)
+    want = (s[:, None] * n).to(dtype)[:, code.cpu()]
+    for got in (ko[:, 0].cpu(), vo[:, 0].cpu()):
+        assert torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got.nan_to_num(0.0, math.inf, -math.inf), want.nan_to_num(0.0, math.inf, -math.inf))
+
+
 @pytest.mark.parametrize("new", [[1, 1, 1, 1], [20, 1, 70, 2]])
 def test_bad_tables_and_lengths(dev, new):
     """Pages outside the cache are seen by nobody, lengths past the table end with it, a row that sees no key is
