@@ -11,6 +11,7 @@
 // 4.9 TB/s), as many rows read back 10.5; 64 tokens 3.6 and 2.5, a launch each.
 #include "llmr_device.h"
 #include "llmr_internal.h"
+#include "mx4_values.h"
 
 // products and sums round where the formulas write them, as in the other glue
 #pragma clang fp contract(off)
@@ -184,19 +185,7 @@ __global__ void __launch_bounds__(256) mx4_rows_kernel(Mx4RowsArgs a) {
     const Mx4Pages& c = is_v ? a.v : a.k;
     const size_t row = (((size_t)page * a.n_kv_heads + kh) << a.page_log2) + ((uint32_t)slot & ((1u << a.page_log2) - 1u));
     const uint32_t w = *(const uint32_t*)(c.data + row * (D / 2u) + 4u * l);
-    const float s = __uint_as_float((uint32_t)c.scales[row * (D / 32u) + l / 4u] << 23);  // (255: NaN comes out)
-    u32x4 o;
-    if constexpr (OT == kGgmlF16) {
-        o.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 0));
-        o.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 1));
-        o.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 2));
-        o.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 3));
-    } else {
-        o.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0));
-        o.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1));
-        o.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2));
-        o.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3));
-    }
+    const u32x4 o = values8<OT>(w, power4(c.scales[row * (D / 32u) + l / 4u]));
     *(u32x4*)((uint16_t*)(is_v ? a.v_out : a.k_out) + (size_t)r * a.out_stride + (size_t)kh * D + 8u * l) = o;
 }
 

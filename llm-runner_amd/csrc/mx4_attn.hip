@@ -51,8 +51,8 @@ struct Mx4Keys : seqattn::PagedKeys<D / 2u> {
     template <uint32_t T>
     __device__ __forceinline__ u32x2 value4(const void* v, uint32_t j, uint32_t dim) const {
         const int64_t row = row_of(j);
-        const u32x4 w = seqattn::values8<T>(*(const uint16_t*)((const uint8_t*)v + row * (D / 2u) + dim / 2u),
-                                            seqattn::power4(v_scales[row * (D / 32u) + dim / 32u]));
+        const u32x4 w = values8<T>(*(const uint16_t*)((const uint8_t*)v + row * (D / 2u) + dim / 2u),
+                                   power4(v_scales[row * (D / 32u) + dim / 32u]));
         return u32x2{w.x, w.y};
     }
 };

@@ -40,6 +40,7 @@
 
 #include "llmr_device.h"
 #include "llmr_internal.h"
+#include "mx4_values.h"
 
 namespace llmr {
 namespace seqattn {
@@ -136,6 +137,13 @@ struct RowOfLane {
     bool live;         // the lane has a row
 };
 
+// A lane's piece of a tile of blocks of 4-bit numbers: key 8 wave + lane / 8, dims D / 8 * (lane % 8) ..
+template <uint32_t D>
+struct Blocks4 {
+    uint32_t n[D / 64];  // eight numbers each
+    uint32_t power;      // + 127
+};
+
 // One workgroup: its rows over n_keys keys, into `out`, or, where part is given, as a part
 // to be joined with others: O[32 NW][D] f32, then m, then l (l = -1: the row sees no key of
 // the part). Source: where keys come from,
@@ -153,32 +161,6 @@ struct RowOfLane {
 //   k_scales, v_scales; bool far_value(j): key j < n_keys's value may hold infinities or NaN, and
 //   u32x2 value4<T>(base, j, dim): four of its numbers then, in 16 bits.
 // out_at(): element offset of the lane's row in `out`.
-//
-// A lane's piece of a tile of blocks: key 8 wave + lane / 8, dims D / 8 * (lane % 8) ..
-template <uint32_t D>
-struct Blocks4 {
-    uint32_t n[D / 64];  // eight numbers each
-    uint32_t power;      // + 127
-};
-// Eight numbers (a dword) times a power of two, as 16-bit values: exact.
-template <uint32_t T>
-__device__ __forceinline__ u32x4 values8(uint32_t w, float s) {
-    u32x4 o;
-    if constexpr (T == kGgmlBF16) {
-        o.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0));
-        o.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1));
-        o.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2));
-        o.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3));
-    } else {
-        o.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 0));
-        o.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 1));
-        o.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 2));
-        o.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 3));
-    }
-    return o;
-}
-__device__ __forceinline__ float power4(uint32_t byte) { return __uint_as_float(byte << 23); }  // (255: NaN comes out)
-
 template <uint32_t T, uint32_t D, uint32_t NW, typename Source, typename OutAt>
 __device__ __forceinline__ void tile_rows(const SeqAttnArgs& a, uint8_t* lds, Source& src, uint32_t n_keys,
                                           const RowOfLane& row, float* part, const OutAt& out_at) {
