@@ -745,6 +745,65 @@ def test_unseen_keys_change_no_bit(dev, dtype, D, new):
         assert torch.equal(out[:first], clean[:first]), first
 
 
+@pytest.mark.parametrize("D,H,Hk", [(128, 8, 2), (64, 6, 3)])
+@pytest.mark.parametrize("new", [[1, 1, 1], [4, 1, 2], [70, 1, 33]])
+def test_strided_rows_and_shared_pages(dev, D, H, Hk, new):
+    """Queries among other columns and a result into columns of a wider buffer; requests with the same first pages."""
+    from llmr_amd import serve
+    q, kc, vc, rows, at, off, kvl, table, kv = _paged_case(dev, F16, D, H, Hk, 16, [900, 900, 333], new, 3, seed=21)
+    table[1, :40] = table[0, :40]
+    for i in (0, 1):
+        rows[1][i][:640] = rows[0][i][:640]
+    wide = torch.full((q.shape[0], H + 3, D), math.nan, dtype=F16, device=dev)
+    wide[:, 1:H + 1] = q
+    buf = torch.full((q.shape[0], H * D + 24), 7.0, dtype=F16, device=dev)
+    out = buf[:, 8:8 + H * D]
+    assert serve.paged_attention_mx4(wide[:, 1:H + 1], kc, vc, off, kvl, table, max(new), out=out) is out
+    ref = serve.paged_attention_mx4(q, kc, vc, off, kvl, table, max(new))
+    torch.cuda.synchronize()
+    _paged_check(q, rows, at, kv, out, 1 / math.sqrt(D), "strided")
+    assert torch.equal(out[:at[-1]], ref[:at[-1]])
+    out[:at[-1]] = 7.0
+    assert bool((buf == 7).all())
+
+
+@pytest.mark.parametrize("new", [1, 3])
+def test_as_many_requests_as_a_call_takes(dev, new):
+    from llmr_amd import capi, serve
+    n, D, H, Hk = capi.MAX_SEQS, 64, 4, 1
+    past = [(31 * i) % 90 for i in range(n)]
+    q, kc, vc, rows, at, off, kvl, table, kv = _paged_case(dev, BF16, D, H, Hk, 16, past, [new] * n, seed=n)
+    out = serve.paged_attention_mx4(q, kc, vc, off, kvl, table, new)
+    torch.cuda.synchronize()
+    for i in list(range(0, n, 257)) + [n - 1]:
+        o, A, e = _definition(q[at[i]:at[i + 1]], *rows[i], 1 / math.sqrt(D), past[i])
+        _check(out[at[i]:at[i + 1]].unflatten(1, (H, D)), o, A, e, float(rows[i][1].abs().max()), kv[i], BF16, f"request {i}")
+    # the same rows a request at a time lie within the bound of one definition
+    for i in (0, 1000, n - 1):
+        one = serve.paged_attention_mx4(q[at[i]:at[i + 1]].contiguous(), kc, vc, off[:2].contiguous(), kvl[i:i + 1].contiguous(),
+                                        table[i:i + 1].contiguous(), new)
+        torch.cuda.synchronize()
+        _beside(out[at[i]:at[i + 1]], one, rows[i][1], i)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("new", [[1, 1], [5, 2], [60, 30]])
+def test_a_query_of_no_number(dev, dtype, new):
+    """An infinity or NaN in one head of one row makes that row NaN and changes no bit of the others."""
+    from llmr_amd import serve
+    q, kc, vc, rows, at, off, kvl, table, kv = _paged_case(dev, dtype, 128, 8, 2, 16, [3000, 40], new, seed=3)
+    ref = serve.paged_attention_mx4(q, kc, vc, off, kvl, table, max(new)).view(-1, 8, 128)
+    row = at[1] - 1
+    for bad in (math.nan, math.inf, -math.inf):
+        other = q.clone()
+        other[row, 3, 5] = bad
+        out = serve.paged_attention_mx4(other, kc, vc, off, kvl, table, max(new)).view(-1, 8, 128)
+        torch.cuda.synchronize()
+        assert bool(out[row, 3].isnan().all())
+        out[row, 3] = ref[row, 3]
+        assert torch.equal(out, ref), bad
+
+
 @pytest.mark.parametrize("D,H,Hk", [(128, 8, 2), (64, 5, 1)])
 def test_out_may_be_q(dev, D, H, Hk):
     from llmr_amd import serve
