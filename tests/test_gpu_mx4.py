@@ -248,6 +248,33 @@ def test_mx4_rows(dev, dtype, D, Hk, page, n):
         assert bool((o[~live] == 7).all()) and bool((x[:, Hk] == 7).all())
 
 
+def test_more_rows_than_a_launch_has_along_x(dev):
+    """2^23 + 37 rows into a cache and back: the first, those around the border and the last as a call of their own."""
+    from llmr_amd import serve
+    T, D, page = (1 << 23) + 37, 64, 256
+    g = torch.Generator(device=dev).manual_seed(9)
+    n_pages = -(-T // page)
+    qkv = torch.empty(T, 3 * D, device=dev).normal_(generator=g)
+    q = torch.zeros(T, 1, D, dtype=F16, device=dev)
+    kc, vc = _caches(n_pages, 1, page, D, dev, 77)
+    slots = torch.arange(T, dtype=torch.int32, device=dev).flip(0)
+    slots[5::1000] = -1
+    serve.qkv_tokens_mx4(qkv, q, kc, vc, slots)
+    ko, vo = (torch.full((T, 1, D), 7.0, dtype=F16, device=dev) for _ in range(2))
+    serve.mx4_rows(kc, vc, slots, ko, vo)
+    torch.cuda.synchronize()
+    for a, b in ((0, 2000), ((1 << 23) - 1000, T)):
+        live = slots[a:b] >= 0
+        x = qkv[a:b].view(-1, 3, D)
+        assert torch.equal(q[a:b, 0], x[:, 0].half())
+        for got, y in ((ko, x[:, 1:2]), (vo, x[:, 2:])):
+            want = _decode(*_encode(y))
+            assert torch.equal(got[a:b][live].double(), want[live]) and bool((got[a:b][~live] == 7).all())
+    unused = torch.ones(n_pages * page, dtype=torch.bool, device=dev)
+    unused[slots[slots >= 0].long()] = False
+    assert bool((kc.data.view(-1, D // 2)[unused] == 77).all()) and bool((vc.scales.view(-1, 2)[unused] == 77).all())
+
+
 # ---- attention over the pages -------------------------------------------------------
 
 
