@@ -739,9 +739,10 @@ LLMR_API int llmr_qkv_tokens_mx4(llmr_context* ctx, const float* qkv, const floa
                                  const llmr_qkv_tokens_params* params);
 
 /* llmr_paged_attention over such caches: the same requests, pages, rows, scratch
- * rules and arithmetic. q and out of type F16 or BF16; a key or value is what its block stands for, in that
- * type (as llmr_qkv_tokens_mx4 writes them: exactly), wherever it lies in the
- * context. The scratch is llmr_paged_attention_mx4_scratch_bytes'. */
+ * rules and arithmetic (f32, the softmax weights rounded to `type` for the products
+ * with v). q and out of type F16 or BF16; a key or value is what its block stands
+ * for, in that type (as llmr_qkv_tokens_mx4 writes them: exactly), wherever it lies
+ * in the context. The scratch is llmr_paged_attention_mx4_scratch_bytes'. */
 LLMR_API int llmr_paged_attention_mx4(llmr_context* ctx, const void* q, const llmr_mx4_cache* k,
                                       const llmr_mx4_cache* v, uint32_t type, void* out, const int32_t* seq_offsets,
                                       const int32_t* kv_len, const int32_t* block_table, void* scratch,
@@ -783,7 +784,7 @@ typedef struct llmr_quantize_rows_params {
  *   scales[r] = a / 127, with norm times 1 / sqrt(sum x^2 / dim + eps)
  * so that scales[r] * q[r, k] stands for x, or for its RMS norm
  * (llmr_batch_rmsnorm's; the norm's size only enters the scale). 64-bit
- * arithmetic, scales rounded once (below 2^-149 to 0). A row with an infinity or NaN has q = 0 and
+ * arithmetic, scales rounded once (to 0 up to 2^-150). A row with an infinity or NaN has q = 0 and
  * scale NaN. Weights [out_dim, in_dim] get their scales a channel by the same call
  * without norm. q and scales overlap no other array. */
 LLMR_API int llmr_quantize_rows_i8(llmr_context* ctx, const void* x, const float* norm, int8_t* q, float* scales,

@@ -5,10 +5,13 @@
 // A row is read once and held in registers, as it lies, from its sums to the rounding;
 // rows past 16384 elements are read twice. The definition is in 64 bits, so that q does
 // not depend on an order or a contraction; f32 rounds where it provably gives the same
-// (round8). Bound by memory: 8192 x 3840 bf16 19.6 us (4.8 TB/s), 8192 x 4096 f32 with
-// the norm 31 (5.4), 8192 x 10240 f32 with the norm 103 (4.1: 16 waves a CU,
-// whose sums and roundings do not hide all of their loads); one row of 4096
-// 3.4 to 4.1, a launch and two dependent loads.
+// (round8). Bound by memory, a wave's loads waited for (76% of its cycles at 8192 x 3840). Over
+// inputs past the memory-side cache, us: 8192 x 3840 bf16 27.4 (3.4 TB/s), 8192 x 4096 f32 with
+// the norm 39 (4.3), 8192 x 10240 f32 with the norm 100 (4.2: 16 waves a CU, whose sums and
+// roundings do not hide all of their loads); with an input that it holds 26, 34, 103. Rows past
+// 16384: 2048 x 28672 bf16 59 (3.0; a large copy's rate would be 34), 8192 x 28672 190 (3.7),
+// 64 x 28672 22, one of 28672 13, one of 131056 55: 256 threads a row, each step waits for its
+// own load. One row of 4096 3.0 to 4.1, a launch and two dependent loads.
 #include "llmr_device.h"
 #include "llmr_internal.h"
 

@@ -23,9 +23,10 @@
 // as in paged_attn_few: scores, maxima, sums and O are f32; P is rounded to the values' type for
 // its product, as the MFMA takes it.
 // Measured in a graph, us, floors by bytes: 4 x 131000..40000 keys of 8 heads of 128, one token
-// each 79 (71.6 at a large copy's rate: 4.7 TB/s), eight 100; 64 x 100..12000 keys of 6 heads 37
+// each 78 (71.6 at a large copy's rate: 4.7 TB/s), eight 98; 64 x 100..12000 keys of 6 heads 37
 // (24.3); one of 1100 keys 10.7 (two launches and a pair's start). Bound by HBM at long contexts,
-// at short ones by the workers' starts, the last of them, and the join.
+// at short ones by the workers' starts, the last of them, and the join. (Counters, of a wave's
+// cycles: waits 41 to 49%, for its turn to issue 16 to 28%, VALU 17 to 24%.)
 #pragma once
 
 #include "seq_attn_few.h"

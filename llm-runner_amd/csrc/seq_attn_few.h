@@ -545,8 +545,10 @@ paged_attn_few(SeqAttnArgs a, JoinRecord* __restrict__ records, float* __restric
 // longest of five): 16 rows or shares at a time, eight parts' loads in flight a thread; 56 ->
 // 42 us for that call, 14.0 -> 12.6 for one request of 1100 keys. Larger parts are fewer and
 // have rows enough: with as many threads 24 mixed requests took 43 us for 39. Eight loads in
-// flight are worth it for parts of 32 rows too (16 x 4 tokens of 28 heads over a 4-bit cache
-// 32.3 -> 31.5).
+// flight are worth it for parts of 32 rows too, us: 16 x 4 tokens of 28 heads over a 4-bit cache
+// 32.3 -> 31.5; over a 16-bit one, with the kernel before it, one request of 1100 keys with 8 tokens
+// of four heads 27.8 -> 25.0, 8 x 5 tokens 25.8 -> 24.4, four of 40000 to 131000 keys 363 -> 360, 64 x 5
+// tokens 159 both, 16 x 4 tokens of 28/4 heads of 64 81.6 -> 83.7 (the join itself 11.4 -> 9.5 there).
 template <uint32_t D, uint32_t PR>
 constexpr uint32_t join_threads() { return PR == 16u ? 4u * D : 256u; }
 
